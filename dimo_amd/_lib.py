@@ -87,6 +87,21 @@ _SIGNATURES = {
                         + [c_ptr] * 7 + [C.POINTER(C.c_void_p)] * 2 + [c_ptr]),
     "dimo_ssim_image_loss": (C.c_int, [C.c_int] * 3 + [c_ptr] * 6 + [C.c_int, C.POINTER(C.c_float)] + [C.c_float] * 5
                              + [c_ptr] * 8 + [C.POINTER(C.c_void_p)] * 2 + [c_ptr]),
+    "dimo_route_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int]),
+    "dimo_route_topk_forward": (C.c_int, [C.c_int] * 4 + [c_ptr, C.c_int64, c_ptr, C.c_int] + [c_ptr] * 4
+                                + [C.c_size_t, c_ptr]),
+    "dimo_route_topk_backward": (C.c_int, [C.c_int] * 4 + [c_ptr, C.c_int64, c_ptr, C.c_int] + [c_ptr] * 6),
+    "dimo_group_rows_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int]),
+    "dimo_group_rows": (C.c_int, [C.c_int64, C.c_int] + [c_ptr] * 5 + [C.c_size_t, c_ptr]),
+    "dimo_grouped_linear_forward": (C.c_int, [C.c_int] * 5 + [c_ptr, C.c_int64, C.c_int] + [c_ptr] * 4 + [C.c_int]
+                                    + [c_ptr] * 3),
+    "dimo_grouped_linear_dgrad": (C.c_int, [C.c_int] * 5 + [c_ptr] * 5),
+    "dimo_grouped_linear_wgrad": (C.c_int, [C.c_int] * 5 + [c_ptr, c_ptr, C.c_int64, C.c_int] + [c_ptr] * 5),
+    "dimo_activation_backward": (C.c_int, [C.c_int, C.c_int, C.c_int64] + [c_ptr] * 4),
+    "dimo_combine_rows_forward": (C.c_int, [C.c_int] * 3 + [C.c_int64, C.c_int, c_ptr, C.c_int64] + [c_ptr] * 3
+                                  + [C.c_int64, c_ptr, c_ptr]),
+    "dimo_combine_rows_backward": (C.c_int, [C.c_int] * 3 + [C.c_int64, C.c_int, C.c_int, c_ptr, C.c_int64, c_ptr,
+                                                             C.c_int64] + [c_ptr] * 6),
 }
 
 ERRORS = {-1: "DIMO_E_ARG (bad argument)", -2: "DIMO_E_LAUNCH (HIP launch/runtime error)",

@@ -31,6 +31,8 @@ SOURCES = {
     "timenet.hip": [],
     "fps.hip": ["-ffp-contract=off"],
     "executor.hip": [],
+    "experts.hip": [],
+    "grouped.hip": [],
 }
 if os.environ.get("DIMO_BWD_TRACE") == "1":  # per-item trace of the blend backward (tools/bwd_trace.py)
     SOURCES["blend.hip"] = SOURCES["blend.hip"] + ["-DDIMO_BWD_TRACE"]

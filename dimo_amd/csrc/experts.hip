@@ -1,0 +1,604 @@
+// Routing of rows to experts: top-k softmax routing with its gradient, grouping of the places by expert (a stable
+// counting sort), and the weighted sum that brings the experts' rows back together, with its gradient.
+//
+//   route    p_t = softmax(z_t); the k largest z of a row (ties: the lowest expert; -inf never): experts, and
+//            w_tj = exp(z_t,ej - m) / sum over the chosen (or over all experts: `normalize` off); load_e = mean_t p_te
+//   group    offsets[e] = places with an expert < e; order[] = the places sorted by (expert, place); position[] its inverse
+//   combine  out_t = residual_t + sum_j w_tj y[position_tj]
+//
+// All of it is bound by memory at large sizes and by launches and dependent loads at small ones: the arithmetic of a
+// row is E exponentials and k selections.  Statistics, weights and sums are fp32; nothing is added with floating-point
+// atomics, so results do not depend on the schedule.
+#include <hip/hip_runtime.h>
+
+#include "numeric.hpp"
+
+using namespace dimo;
+
+namespace {
+
+constexpr int ROUTE_THREADS = 256;
+constexpr int ROUTE_MAX_E = DIMO_MAX_EXPERTS;
+constexpr int ROUTE_MAX_BLOCKS = 512;  // workgroups of a routing launch that also sums the load: one row of partial sums each
+
+// ---- routing ---------------------------------------------------------------------------------------------------
+// L lanes per row (a power of two, so that the butterflies stay inside the row's lanes), V values per lane: element
+// c * L + lane.  Rows with 4 E <= 256 take L = E / 4 lanes: the cost of a selection round is log2(L) exchanges, which
+// outweighs the V comparisons before it.
+struct RouteArgs {
+  int T, E, k, normalize;
+  const void *logits;
+  int64_t ld;
+  const uint8_t *row_mask;
+  float *weights;
+  int32_t *experts;
+  float *partial;  // [gridDim.x, E] sums of p over the workgroup's rows, or null
+  float load_scale;
+};
+
+template <int L>
+__device__ __forceinline__ float row_sum(float v) {
+#pragma unroll
+  for (int m = 1; m < L; m *= 2) v += __shfl_xor(v, m);
+  return v;
+}
+template <int L>
+__device__ __forceinline__ float row_max(float v) {
+#pragma unroll
+  for (int m = 1; m < L; m *= 2) v = fmaxf(v, __shfl_xor(v, m));
+  return v;
+}
+
+template <class T, int V>
+__device__ __forceinline__ void load_row(const void *logits, int64_t at, int E, int L, int lane, bool live, float (&z)[V]) {
+  const typename T::store *src = static_cast<const typename T::store *>(logits) + at;
+#pragma unroll
+  for (int c = 0; c < V; ++c) {
+    const int e = c * L + lane;
+    z[c] = (live && e < E) ? T::load(src[e]) : -INFINITY;
+  }
+}
+
+template <class T, int L, int V>
+__global__ __launch_bounds__(ROUTE_THREADS) void route_forward_kernel(RouteArgs a) {
+  constexpr int ROWS = ROUTE_THREADS / L;
+  const int lane = threadIdx.x % L, sub = threadIdx.x / L;
+  float mine[V];  // sums of p over this lane's rows
+#pragma unroll
+  for (int c = 0; c < V; ++c) mine[c] = 0.f;
+  const int rounds = (a.T + ROWS * (int)gridDim.x - 1) / (ROWS * (int)gridDim.x);
+  for (int it = 0; it < rounds; ++it) {  // (the same number of rounds for every lane: the exchanges need the whole wave)
+    const int64_t row = ((int64_t)it * gridDim.x + blockIdx.x) * ROWS + sub;
+    const bool in = row < a.T;
+    const bool live = in && (!a.row_mask || a.row_mask[in ? row : 0] != 0);
+    float z[V];
+    load_row<T, V>(a.logits, (in ? row : 0) * a.ld, a.E, L, lane, live, z);
+    bool nan = false;
+#pragma unroll
+    for (int c = 0; c < V; ++c) nan |= z[c] != z[c];
+    // a NaN is never chosen; the row's weights and probabilities are NaN by the formula
+    const float poison = row_max<L>(nan ? 1.f : 0.f) > 0.f ? NAN : 0.f;
+    int slot[V];
+    float top = 0.f;      // the row's largest logit
+    float chosen = 0.f;   // sum of exp over the chosen
+    int count = 0;
+#pragma unroll
+    for (int c = 0; c < V; ++c) slot[c] = -1;
+    for (int j = 0; j < a.k; ++j) {
+      float best = -INFINITY;
+      int at = ROUTE_MAX_E;
+#pragma unroll
+      for (int c = 0; c < V; ++c)  // (ascending index: the first of equals stays)
+        if (slot[c] < 0 && z[c] > best) best = z[c], at = c * L + lane;
+#pragma unroll
+      for (int m = 1; m < L; m *= 2) {
+        const float ob = __shfl_xor(best, m);
+        const int oa = __shfl_xor(at, m);
+        if (ob > best || (ob == best && oa < at)) best = ob, at = oa;
+      }
+      if (j == 0) top = best > -INFINITY ? best : 0.f;
+      if (best > -INFINITY) {
+        chosen += expf(best - top);
+        ++count;
+      }
+#pragma unroll
+      for (int c = 0; c < V; ++c)
+        if (at == c * L + lane && best > -INFINITY) slot[c] = j;
+    }
+    float all = 0.f, p[V];
+#pragma unroll
+    for (int c = 0; c < V; ++c) p[c] = expf(z[c] - top), all += z[c] == z[c] ? p[c] : 0.f;
+    all = row_sum<L>(all);
+    const float inv_all = (all > 0.f ? 1.f / all : 0.f) + poison;
+    const float inv = a.normalize ? (count ? 1.f / chosen : 0.f) + poison : inv_all;
+    if (in) {
+#pragma unroll
+      for (int c = 0; c < V; ++c)
+        if (slot[c] >= 0) {
+          a.weights[row * a.k + slot[c]] = p[c] * inv;
+          a.experts[row * a.k + slot[c]] = c * L + lane;
+        }
+      for (int j = count + lane; j < a.k; j += L) {
+        a.weights[row * a.k + j] = 0.f;
+        a.experts[row * a.k + j] = -1;
+      }
+      if (live)
+#pragma unroll
+        for (int c = 0; c < V; ++c) mine[c] += p[c] * inv_all;
+    }
+  }
+  if (!a.partial) return;
+  // the workgroup's rows one after the other, in a fixed order
+  __shared__ float sums[ROUTE_THREADS * V];
+#pragma unroll
+  for (int c = 0; c < V; ++c) sums[sub * (L * V) + c * L + lane] = mine[c];
+  __syncthreads();
+  for (int e = threadIdx.x; e < a.E; e += ROUTE_THREADS) {
+    float s = 0.f;
+    for (int r = 0; r < ROWS; ++r) s += sums[r * (L * V) + e];
+    a.partial[(size_t)blockIdx.x * a.E + e] = s * a.load_scale;
+  }
+}
+
+// load[e] = sum over the workgroups' partial sums, in their order
+__global__ __launch_bounds__(256) void route_load_kernel(int E, int blocks, const float *__restrict__ partial,
+                                                         float *__restrict__ load) {
+  __shared__ float s[4][64];
+  const int e = blockIdx.x * 64 + (threadIdx.x & 63), part = threadIdx.x >> 6;
+  float v = 0.f;
+  if (e < E)
+    for (int b = part; b < blocks; b += 4) v += partial[(size_t)b * E + e];
+  s[part][threadIdx.x & 63] = v;
+  __syncthreads();
+  if (part == 0 && e < E) load[e] = (s[0][threadIdx.x] + s[1][threadIdx.x]) + (s[2][threadIdx.x] + s[3][threadIdx.x]);
+}
+
+// Backward: the chosen experts' share arrives in LDS (one row of E per row of logits), the rest is per element.
+//   normalize:  g_ej = w_j (gw_j - sum_i w_i gw_i)         otherwise  p_e (g_e - sum p g), g_ej = gw_j
+//   load:       + p_e (gl_e - sum p gl) / T
+struct RouteBwdArgs {
+  int T, E, k, normalize;
+  const void *logits;
+  int64_t ld;
+  const uint8_t *row_mask;
+  const float *weights;
+  const int32_t *experts;
+  const float *g_weights, *g_load;
+  void *g_logits;
+  float load_scale;
+};
+
+template <class T, int L, int V>
+__global__ __launch_bounds__(ROUTE_THREADS) void route_backward_kernel(RouteBwdArgs a) {
+  constexpr int ROWS = ROUTE_THREADS / L;
+  __shared__ float sparse[ROUTE_THREADS * V];
+  const int lane = threadIdx.x % L, sub = threadIdx.x / L;
+  const int64_t row = (int64_t)blockIdx.x * ROWS + sub;
+  const bool in = row < a.T;
+  const bool live = in && (!a.row_mask || a.row_mask[in ? row : 0] != 0);
+  float *g_row = sparse + sub * (L * V);
+#pragma unroll
+  for (int c = 0; c < V; ++c) g_row[c * L + lane] = 0.f;
+  __syncthreads();
+  float inner = 0.f;
+  if (live && a.g_weights && a.normalize)
+    for (int j = lane; j < a.k; j += L)
+      if (a.experts[row * a.k + j] >= 0) inner += a.weights[row * a.k + j] * a.g_weights[row * a.k + j];
+  inner = row_sum<L>(inner);
+  if (live && a.g_weights)
+    for (int j = lane; j < a.k; j += L) {
+      const int e = a.experts[row * a.k + j];
+      if (e < 0 || e >= a.E) continue;
+      const float g = a.g_weights[row * a.k + j];
+      g_row[e] = a.normalize ? a.weights[row * a.k + j] * (g - inner) : g;
+    }
+  __syncthreads();
+  float out[V];
+#pragma unroll
+  for (int c = 0; c < V; ++c) out[c] = g_row[c * L + lane];
+  if (a.g_load || !a.normalize) {
+    float z[V], p[V], g[V];
+    load_row<T, V>(a.logits, (in ? row : 0) * a.ld, a.E, L, lane, live, z);
+    float m = -INFINITY, all = 0.f;
+#pragma unroll
+    for (int c = 0; c < V; ++c) m = fmaxf(m, z[c]);
+    m = row_max<L>(m);
+    if (!(m > -INFINITY)) m = 0.f;
+#pragma unroll
+    for (int c = 0; c < V; ++c) p[c] = expf(z[c] - m), all += p[c];
+    all = row_sum<L>(all);
+    const float inv = all > 0.f ? 1.f / all : (all == 0.f ? 0.f : all);  // (NaN stays NaN)
+    float dot = 0.f;
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+      const int e = c * L + lane;
+      p[c] *= inv;
+      g[c] = (a.g_load && e < a.E) ? a.g_load[e] * a.load_scale : 0.f;
+      if (!a.normalize) g[c] += out[c], out[c] = 0.f;
+      dot += e < a.E ? p[c] * g[c] : 0.f;
+    }
+    dot = row_sum<L>(dot);
+#pragma unroll
+    for (int c = 0; c < V; ++c) out[c] += p[c] * (g[c] - dot);
+  }
+  if (in) {
+    typename T::store *dst = static_cast<typename T::store *>(a.g_logits) + row * a.E;
+#pragma unroll
+    for (int c = 0; c < V; ++c)
+      if (c * L + lane < a.E) dst[c * L + lane] = T::save(live ? out[c] : 0.f);
+  }
+}
+
+// lanes per row and values per lane for E experts
+inline int route_lanes(int E) {
+  int L = 1;
+  while (L < 64 && 4 * L < E) L *= 2;
+  return L;
+}
+inline int route_blocks(int T, int E) {
+  const int rows = ROUTE_THREADS / route_lanes(E);
+  return (T + rows - 1) / rows;
+}
+
+template <class T>
+void launch_route_forward(const RouteArgs &a, int grid, hipStream_t s) {
+  switch (route_lanes(a.E)) {
+    case 1: hipLaunchKernelGGL((route_forward_kernel<T, 1, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a); break;
+    case 2: hipLaunchKernelGGL((route_forward_kernel<T, 2, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a); break;
+    case 4: hipLaunchKernelGGL((route_forward_kernel<T, 4, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a); break;
+    case 8: hipLaunchKernelGGL((route_forward_kernel<T, 8, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a); break;
+    case 16: hipLaunchKernelGGL((route_forward_kernel<T, 16, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a); break;
+    case 32: hipLaunchKernelGGL((route_forward_kernel<T, 32, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a); break;
+    default:
+      if (a.E <= 256)
+        hipLaunchKernelGGL((route_forward_kernel<T, 64, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a);
+      else
+        hipLaunchKernelGGL((route_forward_kernel<T, 64, 16>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a);
+  }
+}
+template <class T>
+void launch_route_backward(const RouteBwdArgs &a, int grid, hipStream_t s) {
+  switch (route_lanes(a.E)) {
+    case 1: hipLaunchKernelGGL((route_backward_kernel<T, 1, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a); break;
+    case 2: hipLaunchKernelGGL((route_backward_kernel<T, 2, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a); break;
+    case 4: hipLaunchKernelGGL((route_backward_kernel<T, 4, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a); break;
+    case 8: hipLaunchKernelGGL((route_backward_kernel<T, 8, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a); break;
+    case 16: hipLaunchKernelGGL((route_backward_kernel<T, 16, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a); break;
+    case 32: hipLaunchKernelGGL((route_backward_kernel<T, 32, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a); break;
+    default:
+      if (a.E <= 256)
+        hipLaunchKernelGGL((route_backward_kernel<T, 64, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a);
+      else
+        hipLaunchKernelGGL((route_backward_kernel<T, 64, 16>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a);
+  }
+}
+
+// ---- grouping --------------------------------------------------------------------------------------------------
+// A stable counting sort of the places by expert.  A workgroup owns GROUP_CHUNK consecutive places, a wave of it 256
+// of them (four rounds of 64): per-wave counts in LDS, an exclusive scan over (expert, workgroup, wave), then every
+// round ranks its 64 places among equals with one ballot per bit of the expert's number.  A place without an expert
+// (any value outside 0 .. E-1) is sorted behind the last group and gets order = -1 there, position = -1.
+constexpr int GROUP_THREADS = 1024, GROUP_WAVES = GROUP_THREADS / 64, GROUP_CHUNK = 4096;
+constexpr int GROUP_ROUNDS = GROUP_CHUNK / GROUP_THREADS;
+
+__device__ __forceinline__ int group_key(const int32_t *experts, int64_t S, int64_t at, int E) {
+  if (at >= S) return -1;
+  const int e = experts[at];
+  return (e >= 0 && e < E) ? e : E;
+}
+
+__global__ __launch_bounds__(GROUP_THREADS) void group_count_kernel(int64_t S, int E, const int32_t *__restrict__ experts,
+                                                                    int32_t *__restrict__ counts) {
+  __shared__ int hist[ROUTE_MAX_E + 1];
+  for (int e = threadIdx.x; e <= E; e += GROUP_THREADS) hist[e] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < GROUP_ROUNDS; ++r) {
+    const int key = group_key(experts, S, (int64_t)blockIdx.x * GROUP_CHUNK + r * GROUP_THREADS + threadIdx.x, E);
+    if (key >= 0) atomicAdd(&hist[key], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e <= E; e += GROUP_THREADS) counts[(size_t)blockIdx.x * (E + 1) + e] = hist[e];
+}
+
+__global__ __launch_bounds__(GROUP_THREADS) void group_place_kernel(int64_t S, int E, int bits,
+                                                                    const int32_t *__restrict__ experts,
+                                                                    const int32_t *__restrict__ counts, int blocks,
+                                                                    int32_t *__restrict__ offsets,
+                                                                    int32_t *__restrict__ order,
+                                                                    int32_t *__restrict__ position) {
+  HIP_DYNAMIC_SHARED(int, base)  // [GROUP_WAVES][E + 1]
+  __shared__ int wave_total[GROUP_WAVES];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, E1 = E + 1;
+  for (int i = t; i < GROUP_WAVES * E1; i += GROUP_THREADS) base[i] = 0;
+  __syncthreads();
+  int key[GROUP_ROUNDS];
+  const int64_t first = (int64_t)blockIdx.x * GROUP_CHUNK + wave * (64 * GROUP_ROUNDS) + lane;
+#pragma unroll
+  for (int r = 0; r < GROUP_ROUNDS; ++r) {
+    key[r] = group_key(experts, S, first + 64 * r, E);
+    if (key[r] >= 0) atomicAdd(&base[wave * E1 + key[r]], 1);
+  }
+  __syncthreads();
+  // exclusive scan over the experts: thread t owns expert t (the last thread's round also the places without one)
+  int running = 0;
+  for (int e0 = 0; e0 < E1; e0 += GROUP_THREADS) {
+    const int e = e0 + t;
+    int before = 0, total = 0;
+    if (e < E1) {
+      if (counts)
+        for (int b = 0; b < blocks; ++b) {
+          const int n = counts[(size_t)b * E1 + e];
+          if (b < (int)blockIdx.x) before += n;
+          total += n;
+        }
+      else
+        for (int w = 0; w < GROUP_WAVES; ++w) total += base[w * E1 + e];
+    }
+    int scan = total;  // inclusive over the wave
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int o = __shfl_up(scan, d);
+      if (lane >= d) scan += o;
+    }
+    if (lane == 63) wave_total[wave] = scan;
+    __syncthreads();
+    int ahead = running, sum = 0;
+    for (int w = 0; w < GROUP_WAVES; ++w) {
+      if (w < wave) ahead += wave_total[w];
+      sum += wave_total[w];
+    }
+    running += sum;
+    if (e < E1) {
+      const int start = ahead + scan - total;
+      if (blockIdx.x == 0) offsets[e] = start;  // offsets[E] = places that have an expert
+      int at = start + before;
+      for (int w = 0; w < GROUP_WAVES; ++w) {
+        const int n = base[w * E1 + e];
+        base[w * E1 + e] = at;
+        at += n;
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int r = 0; r < GROUP_ROUNDS; ++r) {
+    unsigned long long peers = __ballot(key[r] >= 0);
+    for (int b = 0; b < bits; ++b) {
+      const bool bit = (key[r] >> b) & 1;
+      const unsigned long long set = __ballot(bit && key[r] >= 0);
+      peers &= bit ? set : ~set;
+    }
+    // the first of the equals takes the places of all of them from the wave's counter
+    const int leader = (key[r] >= 0) ? __ffsll((long long)peers) - 1 : lane;
+    int start = 0;
+    if (key[r] >= 0 && leader == lane) {
+      start = base[wave * E1 + key[r]];
+      base[wave * E1 + key[r]] = start + __popcll(peers);
+    }
+    start = __shfl(start, leader);
+    const int64_t place = first + 64 * r;
+    if (key[r] >= 0) {
+      const int at = start + __popcll(peers & ((1ull << lane) - 1ull));
+      const bool has = key[r] < E;
+      order[at] = has ? (int32_t)place : -1;
+      position[place] = has ? at : -1;
+    }
+  }
+}
+
+// ---- bringing rows together ------------------------------------------------------------------------------------
+// out[t] = residual[t] + sum_j w[t, j] y[position[t, j]]: VEC consecutive elements per thread, the k loads of a thread
+// independent of each other.
+struct CombineArgs {
+  int T, k, N, chunks;  // chunks = N / VEC
+  int64_t S;
+  const void *y;
+  int64_t ldy;
+  const float *weights;      // [T, k] or null (all 1)
+  const int32_t *position;   // [T, k]
+  const void *residual;      // [T, N] rows at ld_res, or null
+  int64_t ld_res;
+  void *out;                 // [T, N]
+};
+template <class T, int VEC>
+__global__ __launch_bounds__(256) void combine_kernel(CombineArgs a) {
+  typedef typename T::store E;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (int64_t)a.T * a.chunks) return;
+  const int64_t t = i / a.chunks;
+  const int n = (int)(i % a.chunks) * VEC;
+  float acc[VEC];
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) acc[v] = 0.f;
+  if (a.residual) load_vec<T, VEC>(static_cast<const E *>(a.residual) + t * a.ld_res + n, acc);
+  for (int j = 0; j < a.k; ++j) {
+    const int32_t p = a.position[t * a.k + j];
+    if (p < 0 || p >= a.S) continue;
+    const float w = a.weights ? a.weights[t * a.k + j] : 1.f;
+    float y[VEC];
+    load_vec<T, VEC>(static_cast<const E *>(a.y) + (int64_t)p * a.ldy + n, y);
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) acc[v] += w * y[v];
+  }
+  store_vec<T, VEC>(static_cast<E *>(a.out) + t * a.N + n, acc);
+}
+
+// Backward, a wave per row: gy[position_tj] = w_tj g_t, gw_tj = <g_t, y[position_tj]>; the rows of gy behind the last
+// group, which no place points to, are cleared (wave t looks after rows t k .. t k + k - 1).
+struct CombineBwdArgs {
+  int T, k, N, E;
+  int64_t S;
+  const void *g, *y;
+  int64_t ldg, ldy;
+  const float *weights;
+  const int32_t *position, *offsets;
+  void *g_y;         // [S, N] or null
+  float *g_weights;  // [T, k] or null
+};
+template <class T, int VEC>
+__global__ __launch_bounds__(256) void combine_backward_kernel(CombineBwdArgs a) {
+  typedef typename T::store E;
+  const int lane = threadIdx.x & 63;
+  const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (t >= a.T) return;
+  for (int j = 0; j < a.k; ++j) {
+    const int32_t p = a.position[t * a.k + j];
+    const bool has = p >= 0 && p < a.S;
+    const float w = a.weights ? a.weights[t * a.k + j] : 1.f;
+    float dot = 0.f;
+    if (has)
+      for (int n = lane * VEC; n < a.N; n += 64 * VEC) {
+        float g[VEC], v[VEC];
+        load_vec<T, VEC>(static_cast<const E *>(a.g) + t * a.ldg + n, g);
+        if (a.g_weights) {
+          load_vec<T, VEC>(static_cast<const E *>(a.y) + (int64_t)p * a.ldy + n, v);
+#pragma unroll
+          for (int q = 0; q < VEC; ++q) dot += g[q] * v[q];
+        }
+        if (a.g_y) {
+#pragma unroll
+          for (int q = 0; q < VEC; ++q) v[q] = w * g[q];
+          store_vec<T, VEC>(static_cast<E *>(a.g_y) + (int64_t)p * a.N + n, v);
+        }
+      }
+    if (a.g_weights) {
+      dot = row_sum<64>(dot);
+      if (lane == 0) a.g_weights[t * a.k + j] = has ? dot : 0.f;
+    }
+  }
+  if (!a.g_y) return;
+  const int64_t used = a.offsets[a.E];
+  const float zero[VEC] = {};
+  for (int64_t r = t * a.k; r < (t + 1) * a.k; ++r)
+    if (r >= used)
+      for (int n = lane * VEC; n < a.N; n += 64 * VEC) store_vec<T, VEC>(static_cast<E *>(a.g_y) + r * a.N + n, zero);
+}
+
+}  // namespace
+
+extern "C" size_t dimo_route_workspace_bytes(int T, int E) {
+  if (T <= 0 || E <= 0) return 0;
+  const int blocks = route_blocks(T, E);
+  return align_up((size_t)(blocks < ROUTE_MAX_BLOCKS ? blocks : ROUTE_MAX_BLOCKS) * E * sizeof(float));
+}
+
+extern "C" int dimo_route_topk_forward(int T, int E, int k, int dtype, const void *logits, int64_t ld,
+                                       const uint8_t *row_mask, int normalize, float *weights, int32_t *experts,
+                                       float *load, void *workspace, size_t workspace_bytes, void *stream) {
+  if (T < 0 || E < 1 || E > ROUTE_MAX_E || k < 1 || k > E || !known_dtype(dtype) || ld < E) return DIMO_E_ARG;
+  if (T > 0 && (!logits || !weights || !experts)) return DIMO_E_ARG;
+  hipStream_t s = (hipStream_t)stream;
+  clear_errors();
+  ScopedTimer timer(T_ROUTE, s);
+  int grid = T > 0 ? route_blocks(T, E) : 0;
+  if (load) {
+    if (workspace_bytes < dimo_route_workspace_bytes(T, E) || (T > 0 && !workspace)) return DIMO_E_WORKSPACE;
+    if (grid > ROUTE_MAX_BLOCKS) grid = ROUTE_MAX_BLOCKS;
+  }
+  float *partial = static_cast<float *>(workspace);
+  if (T > 0) {
+    const RouteArgs a{T, E, k, normalize, logits, ld, row_mask, weights, experts,
+                      load ? (grid == 1 ? load : partial) : nullptr, 1.0f / (float)T};
+    with_dtype(dtype, [&](auto tag) { launch_route_forward<decltype(tag)>(a, grid, s); });
+  }
+  if (load && grid != 1)
+    hipLaunchKernelGGL(route_load_kernel, dim3((E + 63) / 64), dim3(256), 0, s, E, grid, partial, load);
+  return check_launch();
+}
+
+extern "C" int dimo_route_topk_backward(int T, int E, int k, int dtype, const void *logits, int64_t ld,
+                                        const uint8_t *row_mask, int normalize, const float *weights,
+                                        const int32_t *experts, const float *g_weights, const float *g_load,
+                                        void *g_logits, void *stream) {
+  if (T < 0 || E < 1 || E > ROUTE_MAX_E || k < 1 || k > E || !known_dtype(dtype) || ld < E) return DIMO_E_ARG;
+  if (T == 0) return DIMO_OK;
+  if (!logits || !weights || !experts || !g_logits) return DIMO_E_ARG;
+  hipStream_t s = (hipStream_t)stream;
+  clear_errors();
+  ScopedTimer timer(T_ROUTE, s);
+  const RouteBwdArgs a{T, E, k, normalize, logits, ld, row_mask, weights, experts, g_weights, g_load, g_logits, 1.0f / (float)T};
+  with_dtype(dtype, [&](auto tag) { launch_route_backward<decltype(tag)>(a, route_blocks(T, E), s); });
+  return check_launch();
+}
+
+extern "C" size_t dimo_group_rows_workspace_bytes(int64_t S, int E) {
+  if (S <= GROUP_CHUNK || E <= 0) return 0;
+  return align_up((size_t)((S + GROUP_CHUNK - 1) / GROUP_CHUNK) * (E + 1) * sizeof(int32_t));
+}
+
+extern "C" int dimo_group_rows(int64_t S, int E, const int32_t *experts, int32_t *offsets, int32_t *order,
+                               int32_t *position, void *workspace, size_t workspace_bytes, void *stream) {
+  if (S < 0 || S > 0x7fffffffLL || E < 1 || E > ROUTE_MAX_E || !offsets) return DIMO_E_ARG;
+  if (S > 0 && (!experts || !order || !position)) return DIMO_E_ARG;
+  if (workspace_bytes < dimo_group_rows_workspace_bytes(S, E) || (S > GROUP_CHUNK && !workspace)) return DIMO_E_WORKSPACE;
+  hipStream_t s = (hipStream_t)stream;
+  clear_errors();
+  ScopedTimer timer(T_ROUTE, s);
+  int bits = 1;
+  while ((1 << bits) <= E) ++bits;
+  const int blocks = S > 0 ? (int)((S + GROUP_CHUNK - 1) / GROUP_CHUNK) : 1;
+  int32_t *counts = blocks > 1 ? static_cast<int32_t *>(workspace) : nullptr;
+  if (counts)
+    hipLaunchKernelGGL(group_count_kernel, dim3(blocks), dim3(GROUP_THREADS), 0, s, S, E, experts, counts);
+  const size_t lds = (size_t)GROUP_WAVES * (E + 1) * sizeof(int);
+  if (lds > 65536 - 1024) {  // (1024 experts: 65 600 bytes; a workgroup has 160 KB)
+    if (hipFuncSetAttribute(reinterpret_cast<const void *>(group_place_kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                            (int)lds) != hipSuccess)
+      return check_launch();
+  }
+  hipLaunchKernelGGL(group_place_kernel, dim3(blocks), dim3(GROUP_THREADS), lds, s, S, E, bits, experts, counts, blocks,
+                     offsets, order, position);
+  return check_launch();
+}
+
+extern "C" int dimo_combine_rows_forward(int T, int k, int N, int64_t S, int dtype, const void *y, int64_t ldy,
+                                         const float *weights, const int32_t *position, const void *residual,
+                                         int64_t ld_residual, void *out, void *stream) {
+  if (T < 0 || k < 1 || N < 0 || S < 0 || !known_dtype(dtype) || ldy < N || (residual && ld_residual < N)) return DIMO_E_ARG;
+  if (T == 0 || N == 0) return DIMO_OK;
+  if ((S > 0 && !y) || !position || !out) return DIMO_E_ARG;
+  hipStream_t s = (hipStream_t)stream;
+  clear_errors();
+  ScopedTimer timer(T_COMBINE, s);
+  const int vec = 16 / (int)dtype_bytes(dtype);
+  const bool wide = N % vec == 0 && ldy % vec == 0 && aligned16(y) && aligned16(out) &&
+                    (!residual || (ld_residual % vec == 0 && aligned16(residual)));
+  CombineArgs a{T, k, N, wide ? N / vec : N, S, y, ldy, weights, position, residual, ld_residual, out};
+  const int64_t blocks = ((int64_t)T * a.chunks + 255) / 256;
+  if (blocks > 0x7fffffffLL) return DIMO_E_ARG;
+  with_dtype(dtype, [&](auto tag) {
+    typedef decltype(tag) Tag;
+    if (wide)
+      hipLaunchKernelGGL((combine_kernel<Tag, Vec16<Tag>::N>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+    else
+      hipLaunchKernelGGL((combine_kernel<Tag, 1>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+  });
+  return check_launch();
+}
+
+extern "C" int dimo_combine_rows_backward(int T, int k, int N, int64_t S, int E, int dtype, const void *g_out,
+                                          int64_t ldg, const void *y, int64_t ldy, const float *weights,
+                                          const int32_t *position, const int32_t *offsets, void *g_y,
+                                          float *g_weights, void *stream) {
+  if (T < 0 || k < 1 || N < 0 || E < 1 || S != (int64_t)T * k || !known_dtype(dtype) || ldg < N || (g_weights && ldy < N))
+    return DIMO_E_ARG;
+  if (T == 0) return DIMO_OK;
+  if ((N > 0 && (!g_out || (g_weights && !y))) || !position || !offsets) return DIMO_E_ARG;
+  hipStream_t s = (hipStream_t)stream;
+  clear_errors();
+  ScopedTimer timer(T_COMBINE, s);
+  const int vec = 16 / (int)dtype_bytes(dtype);
+  const bool wide = N % vec == 0 && ldg % vec == 0 && aligned16(g_out) && (!g_y || aligned16(g_y)) &&
+                    (!g_weights || (ldy % vec == 0 && aligned16(y)));
+  const CombineBwdArgs a{T, k, N, E, S, g_out, y, ldg, ldy, weights, position, offsets, g_y, g_weights};
+  const int blocks = (T + 3) / 4;
+  with_dtype(dtype, [&](auto tag) {
+    typedef decltype(tag) Tag;
+    if (wide)
+      hipLaunchKernelGGL((combine_backward_kernel<Tag, Vec16<Tag>::N>), dim3(blocks), dim3(256), 0, s, a);
+    else
+      hipLaunchKernelGGL((combine_backward_kernel<Tag, 1>), dim3(blocks), dim3(256), 0, s, a);
+  });
+  return check_launch();
+}

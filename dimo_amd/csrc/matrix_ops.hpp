@@ -1,0 +1,38 @@
+// 16-bit matrix instructions of the expert kernels (gfx950), and fp32 operands as sums of bf16 ones.
+#pragma once
+#include "numeric.hpp"
+
+namespace dimo {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// D = A B + C over 16 values of k.  Lane l holds A[i = l % 32][k = 8 (l / 32) ..+ 7] and B[k = 8 (l / 32) ..+ 7][j = l % 32]
+// (eight 16-bit values in ascending k); register r of lane l is D[i = 8 (r / 4) + 4 (l / 32) + r % 4][j = l % 32].
+__device__ __forceinline__ f32x16 mfma_32x32x16(BF16, uint4 a, uint4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma_32x32x16(F16, uint4 a, uint4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// fp32 = three bf16 pieces: the top eight significant bits (cut, so that no finite value becomes infinite), what is left
+// rounded to eight bits, and the rest, which eight bits hold exactly -- 24 bits in all.  Of the nine products of two
+// such sums the three smallest (below 2^-21 of the product, of random sign) are left out: the error of one product is
+// then of the size of one fp32 rounding, at 6 / 16 of an fp32 matrix instruction's issue time.
+// An infinite value leaves NaN (inf - inf) and so shows up as NaN in its row of outputs.
+struct Split3 {
+  uint16_t hi, mid, lo;
+};
+__device__ __forceinline__ Split3 split3(float v) {
+  Split3 s;
+  s.hi = (uint16_t)(__builtin_bit_cast(uint32_t, v) >> 16);
+  const float r = v - BF16::load(s.hi);
+  s.mid = BF16::save(r);
+  s.lo = BF16::save(r - BF16::load(s.mid));
+  return s;
+}
+
+}  // namespace dimo

@@ -1,0 +1,372 @@
+"""Expert blocks on the HIP library: top-k routing of rows, products grouped by expert, and the weighted sum that brings
+the experts' rows back together (dimo_amd/csrc/experts.hip, grouped.hip; include/dimo_hip.h).
+
+    weights, experts, load = route_topk(logits, k)            # [T, k], [T, k], [E]
+    groups = group_rows(experts, E)                           # the T k places, grouped by expert
+    h = grouped_linear(x, w1, groups, b1, "relu", gather=True)  # [T k, F]: rows of x, in the order of the groups
+    y = grouped_linear(h, w2, groups, b2)                     # [T k, N]
+    out = combine_rows(y, groups, weights, residual=x)        # [T, N]
+
+`expert_mlp` is this sequence as one call, `ExpertMLP` the module around it.  Nothing here has a counterpart in the
+reference, whose deformation network (renderer/latent_gs_renderer.py:184-245) is one dense MLP for all motions: an
+expert block gives that network capacity of which every row uses k parts (`deform.TimeNet(experts=...)`).
+
+Types: fp32, bf16, fp16 (all tensors of a call alike; routing weights, load and their gradients are fp32).  The sizes of
+the groups stay on the device: no call synchronises, every call may be captured into a graph.  All calls run on the
+current stream of the tensors' device.  GPU only.
+"""
+import torch
+from torch import nn
+
+from . import _lib
+
+MAX_EXPERTS = 1024
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_ACTIVATIONS = {None: 0, "relu": 1, "silu": 2}
+
+
+def _dtype(t, what):
+    if t.dtype not in _DTYPES:
+        raise ValueError(f"{what}: fp32, bf16 or fp16 expected, got {t.dtype}")
+    return _DTYPES[t.dtype]
+
+
+def _gpu(*tensors):
+    """The tensors' common device (a GPU), or an error."""
+    device = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"tensors on different devices ({device}, {t.device})")
+    if device.type != "cuda":
+        raise RuntimeError("the expert operators need GPU tensors (no CPU fallback in the product path)")
+    return device
+
+
+class _on:
+    """Makes a tensor's device current for a launch (nothing to do when it is)."""
+
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *_):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+
+
+def _rows(t):
+    """A matrix whose rows are contiguous (a view of a wider tensor is taken as it is)."""
+    if t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]):
+        return t
+    return t.contiguous()
+
+
+def _ld(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _tracked(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+# ------------------------------------------------------------------------------------------------ routing
+def _route_forward(logits, k, row_mask, normalize):
+    T, E = logits.shape
+    L = _lib.lib()
+    weights = torch.empty(T, k, dtype=torch.float32, device=logits.device)
+    experts = torch.empty(T, k, dtype=torch.int32, device=logits.device)
+    load = torch.empty(E, dtype=torch.float32, device=logits.device)
+    with _on(logits.device):
+        ws = torch.empty(L.dimo_route_workspace_bytes(T, E), dtype=torch.uint8, device=logits.device)
+        _lib.check(L.dimo_route_topk_forward(T, E, k, _DTYPES[logits.dtype], logits.data_ptr(), _ld(logits),
+                                             _lib.ptr(row_mask), int(normalize), weights.data_ptr(), experts.data_ptr(),
+                                             load.data_ptr(), ws.data_ptr(), ws.numel(), _lib.current_stream()),
+                   "dimo_route_topk_forward")
+    return weights, experts, load
+
+
+class _RouteTopk(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, k, row_mask, normalize):
+        weights, experts, load = _route_forward(logits, k, row_mask, normalize)
+        ctx.save_for_backward(logits, row_mask, weights, experts)
+        ctx.normalize = bool(normalize)
+        ctx.mark_non_differentiable(experts)
+        ctx.set_materialize_grads(False)
+        return weights, experts, load
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_weights, _, g_load):
+        logits, row_mask, weights, experts = ctx.saved_tensors
+        if g_weights is None and g_load is None:
+            return None, None, None, None
+        T, E = logits.shape
+        g = torch.empty(T, E, dtype=logits.dtype, device=logits.device)
+        g_weights = None if g_weights is None else g_weights.contiguous()
+        g_load = None if g_load is None else g_load.contiguous()
+        with _on(logits.device):
+            _lib.check(_lib.lib().dimo_route_topk_backward(
+                T, E, weights.shape[1], _DTYPES[logits.dtype], logits.data_ptr(), _ld(logits), _lib.ptr(row_mask),
+                int(ctx.normalize), weights.data_ptr(), experts.data_ptr(), _lib.ptr(g_weights), _lib.ptr(g_load),
+                g.data_ptr(), _lib.current_stream()), "dimo_route_topk_backward")
+        return g, None, None, None
+
+
+def route_topk(logits, k, row_mask=None, normalize=True):
+    """(weights [T, k] fp32, experts [T, k] int32, load [E] fp32) of logits [T, E].
+
+    experts: each row's k largest logits in descending order (ties: the lowest index; -inf and NaN are never chosen;
+    -1 with weight 0 where nothing is left, and in rows whose row_mask [T] is False).  weights: softmax over the chosen
+    (normalize=False: over all E).  load: the experts' mean softmax probability over the T rows (masked rows count as
+    0), for a balancing term.  A row with a NaN or +inf logit has NaN weights.  Differentiable in `logits` through
+    weights and load."""
+    if logits.dim() != 2:
+        raise ValueError("logits: [T, E] expected")
+    _gpu(logits, row_mask)
+    _dtype(logits, "logits")
+    if not 1 <= logits.shape[1] <= MAX_EXPERTS or not 1 <= k <= logits.shape[1]:
+        raise ValueError(f"1 <= k <= E <= {MAX_EXPERTS} expected, got k = {k}, E = {logits.shape[1]}")
+    if row_mask is not None:
+        if row_mask.dtype != torch.bool or row_mask.shape != logits.shape[:1]:
+            raise ValueError("row_mask: bool [T] expected")
+        row_mask = row_mask.contiguous()
+    logits = _rows(logits)
+    if _tracked(logits):
+        return _RouteTopk.apply(logits, k, row_mask, normalize)
+    return _route_forward(logits, k, row_mask, normalize)
+
+
+class RowGroups:
+    """Rows grouped by expert.  offsets [E + 1] int32: expert e owns rows offsets[e] .. offsets[e + 1] - 1 (offsets[0]
+    = 0); rows behind offsets[E] belong to nobody.  From `group_rows` also order [T k] (which place a row came from) and
+    position [T, k] (which row a place went to; -1: none)."""
+
+    __slots__ = ("offsets", "order", "position")
+
+    def __init__(self, offsets, order=None, position=None):
+        if offsets.dim() != 1 or offsets.dtype != torch.int32 or not offsets.is_contiguous():
+            raise ValueError("offsets: contiguous int32 [E + 1] expected")
+        if not 2 <= offsets.shape[0] <= MAX_EXPERTS + 1:
+            raise ValueError(f"1 to {MAX_EXPERTS} groups expected")
+        self.offsets, self.order, self.position = offsets, order, position
+
+    @property
+    def num_experts(self):
+        return self.offsets.shape[0] - 1
+
+    @property
+    def places(self):
+        """Places per row of what was routed (k), 0 without a routing."""
+        return 0 if self.position is None else self.position.shape[1]
+
+
+def group_rows(experts, num_experts):
+    """RowGroups of the places of experts [T, k] int32, stable: by expert, then by place.  A place whose value is outside
+    0 .. num_experts - 1 belongs to nobody."""
+    if experts.dim() != 2 or experts.dtype != torch.int32:
+        raise ValueError("experts: int32 [T, k] expected")
+    if not 1 <= num_experts <= MAX_EXPERTS or experts.shape[1] < 1:
+        raise ValueError(f"1 to {MAX_EXPERTS} experts and k >= 1 expected")
+    device = _gpu(experts)
+    experts = experts.contiguous()
+    S = experts.numel()
+    if S > 0x7FFFFFFF:
+        raise ValueError("more than 2^31 - 1 places")
+    L = _lib.lib()
+    offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=device)
+    order = torch.empty(S, dtype=torch.int32, device=device)
+    position = torch.empty(experts.shape, dtype=torch.int32, device=device)
+    with _on(device):
+        nbytes = L.dimo_group_rows_workspace_bytes(S, num_experts)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        _lib.check(L.dimo_group_rows(S, num_experts, experts.data_ptr(), offsets.data_ptr(), order.data_ptr(),
+                                     position.data_ptr(), _lib.ptr(ws), nbytes, _lib.current_stream()), "dimo_group_rows")
+    return RowGroups(offsets, order, position)
+
+
+# ------------------------------------------------------------------------------------------------ grouped products
+def _linear_forward(x, weight, bias, groups, act, gather, save_z):
+    E, N, K = weight.shape
+    R = groups.order.shape[0] if gather else x.shape[0]
+    y = torch.empty(R, N, dtype=x.dtype, device=x.device)
+    z = torch.empty_like(y) if save_z else None
+    with _on(x.device):
+        _lib.check(_lib.lib().dimo_grouped_linear_forward(
+            _DTYPES[x.dtype], R, E, K, N, x.data_ptr(), _ld(x), groups.places if gather else 0,
+            _lib.ptr(groups.order) if gather else None, groups.offsets.data_ptr(), weight.data_ptr(), _lib.ptr(bias), act,
+            y.data_ptr(), _lib.ptr(z), _lib.current_stream()), "dimo_grouped_linear_forward")
+    return y, z
+
+
+def _linear_dgrad(g, weight, groups):
+    E, N, K = weight.shape
+    gx = torch.empty(g.shape[0], K, dtype=g.dtype, device=g.device)
+    with _on(g.device):
+        _lib.check(_lib.lib().dimo_grouped_linear_dgrad(
+            _DTYPES[g.dtype], g.shape[0], E, K, N, g.data_ptr(), groups.offsets.data_ptr(), weight.data_ptr(), gx.data_ptr(),
+            _lib.current_stream()), "dimo_grouped_linear_dgrad")
+    return gx
+
+
+def _linear_wgrad(g, x, shape, groups, gather, need_bias):
+    E, N, K = shape
+    gw = torch.empty(E, N, K, dtype=g.dtype, device=g.device)
+    gb = torch.empty(E, N, dtype=g.dtype, device=g.device) if need_bias else None
+    with _on(g.device):
+        _lib.check(_lib.lib().dimo_grouped_linear_wgrad(
+            _DTYPES[g.dtype], g.shape[0], E, K, N, g.data_ptr(), x.data_ptr(), _ld(x), groups.places if gather else 0,
+            _lib.ptr(groups.order) if gather else None, groups.offsets.data_ptr(), gw.data_ptr(), _lib.ptr(gb),
+            _lib.current_stream()), "dimo_grouped_linear_wgrad")
+    return gw, gb
+
+
+def _activation_backward(g, saved, act):
+    out = torch.empty_like(g)
+    with _on(g.device):
+        _lib.check(_lib.lib().dimo_activation_backward(_DTYPES[g.dtype], act, g.numel(), g.data_ptr(), saved.data_ptr(),
+                                                       out.data_ptr(), _lib.current_stream()), "dimo_activation_backward")
+    return out
+
+
+def _combine_forward(y, weights, groups, residual):
+    T, k = groups.position.shape
+    out = torch.empty(T, y.shape[1], dtype=y.dtype, device=y.device)
+    with _on(y.device):
+        _lib.check(_lib.lib().dimo_combine_rows_forward(
+            T, k, y.shape[1], y.shape[0], _DTYPES[y.dtype], y.data_ptr(), _ld(y), _lib.ptr(weights),
+            groups.position.data_ptr(), _lib.ptr(residual), _ld(residual) if residual is not None else 0, out.data_ptr(),
+            _lib.current_stream()), "dimo_combine_rows_forward")
+    return out
+
+
+def _combine_backward(g, y, weights, groups, need_y, need_weights):
+    T, k = groups.position.shape
+    N = g.shape[1]
+    g_y = torch.empty(T * k, N, dtype=g.dtype, device=g.device) if need_y else None
+    g_w = torch.empty(T, k, dtype=torch.float32, device=g.device) if need_weights else None
+    with _on(g.device):
+        _lib.check(_lib.lib().dimo_combine_rows_backward(
+            T, k, N, T * k, groups.num_experts, _DTYPES[g.dtype], g.data_ptr(), _ld(g), _lib.ptr(y), _ld(y) if y is not None else 0,
+            _lib.ptr(weights), groups.position.data_ptr(), groups.offsets.data_ptr(), _lib.ptr(g_y), _lib.ptr(g_w),
+            _lib.current_stream()), "dimo_combine_rows_backward")
+    return g_y, g_w
+
+
+class _GroupedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, act, gather):
+        y, z = _linear_forward(x, weight, bias, groups, act, gather, act == 2)
+        ctx.save_for_backward(x, weight, z if act == 2 else y if act == 1 else None)
+        ctx.groups, ctx.act, ctx.gather, ctx.bias = groups, act, gather, bias is not None
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        x, weight, saved = ctx.saved_tensors
+        groups = ctx.groups
+        g = g.contiguous()
+        if ctx.act:
+            g = _activation_backward(g, saved, ctx.act)
+        gx = gw = gb = None
+        if ctx.needs_input_grad[0]:
+            gx = _linear_dgrad(g, weight, groups)
+            if ctx.gather:
+                gx = _combine_forward(gx, None, groups, None)
+        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
+            gw, gb = _linear_wgrad(g, x, weight.shape, groups, ctx.gather, ctx.bias)
+        return gx, gw, gb, None, None, None
+
+
+def _check_linear(x, weight, bias, groups, activation, gather):
+    if x.dim() != 2 or weight.dim() != 3:
+        raise ValueError("x: [rows, K] and weight: [E, N, K] expected")
+    _gpu(x, weight, bias, groups.offsets)
+    _dtype(x, "x")
+    if weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
+        raise ValueError("x, weight and bias must have one type")
+    E, N, K = weight.shape
+    if x.shape[1] != K or K < 1 or N < 1:
+        raise ValueError(f"x has {x.shape[1]} columns, weight takes {K}")
+    if E != groups.num_experts:
+        raise ValueError(f"{E} experts' weights for {groups.num_experts} groups")
+    if bias is not None and bias.shape != (E, N):
+        raise ValueError("bias: [E, N] expected")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"activation: one of {list(_ACTIVATIONS)} expected")
+    if gather:
+        if groups.position is None:
+            raise ValueError("gather=True needs groups made by group_rows")
+        if x.shape[0] != groups.position.shape[0]:
+            raise ValueError(f"{x.shape[0]} rows, {groups.position.shape[0]} were grouped")
+    elif groups.position is not None and x.shape[0] != groups.order.shape[0]:
+        raise ValueError(f"{x.shape[0]} rows in the order of the groups, {groups.order.shape[0]} expected")
+
+
+def grouped_linear(x, weight, groups, bias=None, activation=None, gather=False):
+    """y[r] = activation(weight[e] @ x[r] + bias[e]) for every row r of group e; zeros behind the last group.
+
+    x [R, K] in the order of the groups, or (gather=True) the [T, K] rows that were routed: row r then reads the row its
+    place came from, and x's gradient is the sum over a row's places.  weight [E, N, K], bias [E, N] or None,
+    activation None, "relu" or "silu".  Differentiable in x, weight and bias; an expert without rows gets zero
+    gradients."""
+    _check_linear(x, weight, bias, groups, activation, gather)
+    x, weight = _rows(x), weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    if _tracked(x, weight, bias):
+        return _GroupedLinear.apply(x, weight, bias, groups, _ACTIVATIONS[activation], gather)
+    return _linear_forward(x, weight, bias, groups, _ACTIVATIONS[activation], gather, False)[0]
+
+
+class _CombineRows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, weights, residual, groups):
+        ctx.save_for_backward(y if weights is not None and weights.requires_grad else None, weights)
+        ctx.groups = groups
+        return _combine_forward(y, weights, groups, residual)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        y, weights = ctx.saved_tensors
+        g_y = g_w = None
+        if ctx.needs_input_grad[0] or ctx.needs_input_grad[1]:
+            g_y, g_w = _combine_backward(_rows(g), y, weights, ctx.groups, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        return g_y, g_w, g if ctx.needs_input_grad[2] else None, None
+
+
+def combine_rows(y, groups, weights=None, residual=None):
+    """out[t] = residual[t] + sum_j weights[t, j] y[position[t, j]]: the rows y [T k, N] of the groups, back at their
+    places and summed over a row's k places (weights fp32 [T, k], None: 1; places of nobody add nothing).  Differentiable
+    in y, weights and residual."""
+    if groups.position is None:
+        raise ValueError("combine_rows needs groups made by group_rows")
+    if y.dim() != 2 or y.shape[0] != groups.order.shape[0]:
+        raise ValueError(f"y: [{groups.order.shape[0]}, N] expected")
+    _gpu(y, weights, residual, groups.offsets)
+    _dtype(y, "y")
+    if weights is not None and (weights.shape != groups.position.shape or weights.dtype != torch.float32):
+        raise ValueError("weights: fp32 [T, k] expected")
+    if residual is not None and (residual.dtype != y.dtype or residual.shape != (groups.position.shape[0], y.shape[1])):
+        raise ValueError("residual: [T, N] of y's type expected")
+    y = _rows(y)
+    weights = None if weights is None else weights.contiguous()
+    residual = None if residual is None else _rows(residual)
+    if _tracked(y, weights, residual):
+        return _CombineRows.apply(y, weights, residual, groups)
+    return _combine_forward(y, weights, groups, residual)
+
+
+def expert_mlp(x, logits, w1, b1, w2, b2, k, activation="relu", row_mask=None):
+    """x + sum over a row's k experts of weight * (w2 activation(w1 x + b1) + b2): routing, both products and the sum.
+    x [T, K], logits [T, E], w1 [E, F, K], b1 [E, F], w2 [E, K, F], b2 [E, K].  Differentiable in all of them."""
+    weights, experts, _ = route_topk(logits, k, row_mask)
+    groups = group_rows(experts, logits.shape[1])
+    h = grouped_linear(x, w1, groups, b1, activation, gather=True)
+    y = grouped_linear(h, w2, groups, b2)
+    return combine_rows(y, groups, weights, residual=x)

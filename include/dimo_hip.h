@@ -55,7 +55,8 @@ const char *dimo_last_error(void);
  * duration and launch count of one group: "preprocess_fwd" "scan" "emit" "sort" "ranges" "blend_fwd"
  * "blend_bwd" "preprocess_bwd" "knn" "dist2" "ssim_fwd" "ssim_bwd" "deform_fwd" "deform_bwd" "image_loss" "adam"
  * "timenet_fwd" "timenet_bwd" "place" (binning, dimo_amd/csrc/binning.hip: "scan" = offsets + level-1 entries,
- * "sort" = per-bucket LDS sort, "ranges" = level-2 count, "place" = level-2 fill; "emit" is no longer used).
+ * "sort" = per-bucket LDS sort, "ranges" = level-2 count, "place" = level-2 fill; "emit" is no longer used) "route"
+ * "grouped" "combine" "mx4" (the expert operators).
  * dimo_timing_enable(1) clears earlier records; returns the previous state.  dimo_timing_select restricts the
  * instrumentation to a comma-separated list of groups (NULL or "": all) -- two event records per launch are not
  * free, a throughput run that only needs one kernel's duration selects that kernel. */
@@ -440,6 +441,57 @@ int dimo_executor_backward_skinning_in_order(void *executor, const dimo_step_com
 /* ... and, on main_stream, per render: wait for it, g_f_dc += g_shs, skinning backward (accumulate) */
 int dimo_executor_backward_accumulate(void *executor, const dimo_step_common *common, int first, int count,
                                       const dimo_render_desc *renders, void *main_stream);
+
+/* ---- expert operators (no reference counterpart: the reference's deformation network is one dense MLP) ------------
+ * Element types: DIMO_F32, DIMO_BF16, DIMO_F16; statistics, weights and sums are fp32.  Up to DIMO_MAX_EXPERTS experts.
+ * Sizes of groups stay on the device; nothing synchronises, every launch may be captured. */
+#define DIMO_F32 0
+#define DIMO_BF16 1
+#define DIMO_F16 2
+#define DIMO_MAX_EXPERTS 1024
+#define DIMO_ACT_NONE 0
+#define DIMO_ACT_RELU 1
+#define DIMO_ACT_SILU 2
+
+/* Top-k softmax routing of T rows of E logits (row t at logits + t * ld).  experts[t, j] = the j-th largest logit's
+ * index (ties: the lowest; a logit of -inf or NaN is never chosen; -1 where nothing is left), weights[t, j] = its softmax
+ * probability among the chosen (normalize != 0) or among all E; a row with a NaN or +inf logit has NaN weights.
+ * row_mask [T] or NULL: rows with 0 choose nothing.  load [E] or NULL: sum_t p[t, e] / T (needs the workspace). */
+size_t dimo_route_workspace_bytes(int T, int E);
+int dimo_route_topk_forward(int T, int E, int k, int dtype, const void *logits, int64_t ld, const uint8_t *row_mask,
+                            int normalize, float *weights, int32_t *experts, float *load, void *workspace,
+                            size_t workspace_bytes, void *stream);
+/* g_logits [T, E] (dense) from g_weights [T, k] and g_load [E] (either may be NULL); weights, experts: the forward's */
+int dimo_route_topk_backward(int T, int E, int k, int dtype, const void *logits, int64_t ld, const uint8_t *row_mask,
+                             int normalize, const float *weights, const int32_t *experts, const float *g_weights,
+                             const float *g_load, void *g_logits, void *stream);
+/* Stable grouping of S places by expert: offsets [E + 1], order [S] (the places, group after group; -1 behind the last
+ * group), position [S] (its inverse; -1 for a place whose expert is outside 0 .. E-1). */
+size_t dimo_group_rows_workspace_bytes(int64_t S, int E);
+int dimo_group_rows(int64_t S, int E, const int32_t *experts, int32_t *offsets, int32_t *order, int32_t *position,
+                    void *workspace, size_t workspace_bytes, void *stream);
+/* y[r] = act(w[e] x[src(r)] + bias[e]) for rows r in [offsets[e], offsets[e + 1]), zeros behind the last group.
+ * x: rows at ldx; places > 0: src(r) = order[r] / places, otherwise r.  w [E, N, K], bias [E, N] or NULL, y [R, N];
+ * z [R, N] or NULL: the value before the activation. */
+int dimo_grouped_linear_forward(int dtype, int R, int E, int K, int N, const void *x, int64_t ldx, int places,
+                                const int32_t *order, const int32_t *offsets, const void *w, const void *bias, int act,
+                                void *y, void *z, void *stream);
+/* gx[r] = g[r] w[e] (g [R, N], gx [R, K] in the order of the groups) */
+int dimo_grouped_linear_dgrad(int dtype, int R, int E, int K, int N, const void *g, const int32_t *offsets, const void *w,
+                              void *gx, void *stream);
+/* gw[e] = sum of g[r]^T x[src(r)], gb[e] = sum of g[r] (gb may be NULL) over the rows of the group */
+int dimo_grouped_linear_wgrad(int dtype, int R, int E, int K, int N, const void *g, const void *x, int64_t ldx, int places,
+                              const int32_t *order, const int32_t *offsets, void *gw, void *gb, void *stream);
+/* out = g * act'(saved): saved = the activation's output for relu, its input for silu; n elements */
+int dimo_activation_backward(int dtype, int act, int64_t n, const void *g, const void *saved, void *out, void *stream);
+/* out[t] = residual[t] + sum_j weights[t, j] y[position[t, j]] (weights NULL: 1; position -1: nothing) */
+int dimo_combine_rows_forward(int T, int k, int N, int64_t S, int dtype, const void *y, int64_t ldy, const float *weights,
+                              const int32_t *position, const void *residual, int64_t ld_residual, void *out, void *stream);
+/* g_y[position[t, j]] = weights[t, j] g_out[t] (zeros behind offsets[E]; g_y may be NULL), g_weights[t, j] =
+ * <g_out[t], y[position[t, j]]> (may be NULL); S = T * k */
+int dimo_combine_rows_backward(int T, int k, int N, int64_t S, int E, int dtype, const void *g_out, int64_t ldg,
+                               const void *y, int64_t ldy, const float *weights, const int32_t *position,
+                               const int32_t *offsets, void *g_y, float *g_weights, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,321 @@
+"""Checks of the expert operators (dimo_amd/experts.py) against their definitions in float64, shared by the CPU-emulated
+and the GPU tests: every check takes the device its tensors live on.
+
+Tolerances are derived, element by element.  A sum of n products computed in fp32 is off by at most about n 2^-24 of the
+sum of the products' absolute values; fp32 operands go through three bf16 pieces each, of whose products those below
+2^-21 of the product are left out: n + 32 covers both.  Writing a result rounds it by at most half a step of its type."""
+import math
+
+import torch
+
+HALF_STEP = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TINY = {torch.float32: 2.0 ** -126, torch.bfloat16: 2.0 ** -126, torch.float16: 2.0 ** -24}  # where steps stop shrinking
+
+
+def near(got, ref, dtype, slack, what):
+    """|got - ref| <= half a step of dtype + slack (fp32 arithmetic's share, a tensor or a number); NaN and inf equal."""
+    got, ref = got.detach().double().cpu(), ref.double().cpu()
+    assert got.shape == ref.shape, (what, got.shape, ref.shape)
+    fine = torch.isfinite(ref)
+    assert torch.equal(torch.isnan(got), torch.isnan(ref)), f"{what}: NaN in other places"
+    assert torch.equal(got[~fine & ~torch.isnan(ref)], ref[~fine & ~torch.isnan(ref)]), f"{what}: infinities differ"
+    slack = slack.double().cpu().expand(ref.shape) if torch.is_tensor(slack) else torch.full(ref.shape, float(slack), dtype=torch.float64)
+    tol = HALF_STEP[dtype] * (ref.abs() + slack) + slack + TINY[dtype]
+    over = ((got - ref).abs() - tol)[fine]
+    assert over.numel() == 0 or float(over.max()) <= 0, f"{what}: {float(over.max()):.3e} over the tolerance"
+
+
+def product_slack(n, absolute):
+    return (n + 32) * 2.0 ** -24 * absolute
+
+
+# ---------------------------------------------------------------------------------------------------------- routing
+def route_reference(z, k, mask=None, normalize=True):
+    """(weights, experts, load) of logits z in float64 by the definition, differentiable (NaN-free logits)."""
+    if mask is not None:
+        z = z.masked_fill(~mask[:, None], -math.inf)
+    T, E = z.shape
+    order = torch.sort(z.detach(), dim=1, descending=True, stable=True)[1][:, :k]
+    top = torch.gather(z, 1, order)
+    live = top.detach() > -math.inf
+    m = torch.where(live[:, :1], top.detach()[:, :1], torch.zeros(T, 1, dtype=z.dtype))
+    p = torch.exp(z - m)
+    total = p.sum(1, keepdim=True)
+    p = torch.where(total > 0, p / torch.where(total > 0, total, 1.0), 0.0)
+    w = torch.where(live, torch.gather(p, 1, order), 0.0)
+    if normalize:
+        s = w.sum(1, keepdim=True)
+        w = torch.where(s > 0, w / torch.where(s > 0, s, 1.0), 0.0)
+    return w, torch.where(live, order, -1).to(torch.int32), p.sum(0) / max(T, 1)
+
+
+def make_logits(T, E, dtype, seed, kind="normal"):
+    g = torch.Generator().manual_seed(seed)
+    z = torch.randn(T, E, generator=g) * 2
+    if kind == "ties":
+        z = torch.randint(-2, 3, (T, E), generator=g).float()
+    if kind == "-inf":
+        z[torch.rand(T, E, generator=g) < 0.6] = -math.inf
+        z[0] = -math.inf
+    if kind == "lowest":
+        z[torch.rand(T, E, generator=g) < 0.6] = torch.finfo(dtype).min
+        z[0] = torch.finfo(dtype).min
+    return z.to(dtype)
+
+
+def check_route(ex, device, T, E, k, dtype, normalize=True, masked=False, kind="normal", pad=0, seed=0):
+    z = make_logits(T, E, dtype, seed, kind)
+    g = torch.Generator().manual_seed(seed + 1)
+    mask = torch.rand(T, generator=g) > 0.3 if masked else None
+    gw, gl = torch.randn(T, k, generator=g), torch.randn(E, generator=g)
+    z64 = z.double().requires_grad_(True)
+    w, e, load = route_reference(z64, k, mask, normalize)
+    wide = torch.full((T, E + pad), 7.0, dtype=dtype)
+    wide[:, :E] = z
+    zd = wide.to(device)[:, :E].detach().requires_grad_(True)
+    md = None if mask is None else mask.to(device)
+    weights, experts, got_load = ex.route_topk(zd, k, row_mask=md, normalize=normalize)
+    assert experts.dtype == torch.int32 and torch.equal(experts.cpu(), e), "experts"
+    # exp(z - m) with |z - m| <= 32 where it counts: 2^-24 of 32 from the argument, a few roundings, a sum over E
+    rel = (64 + E) * 2.0 ** -24
+    near(weights, w.detach(), torch.float32, rel * w.detach().abs(), "weights")
+    near(got_load, load.detach(), torch.float32, rel * load.detach() + (T + 16) * 2.0 ** -24 * load.detach(), "load")
+    plain = ex.route_topk(zd.detach(), k, row_mask=md, normalize=normalize)
+    assert torch.equal(plain[0], weights) and torch.equal(plain[1], experts) and torch.equal(plain[2], got_load)
+    if T == 0:
+        return
+    for with_w, with_l in ((True, True), (True, False), (False, True)):
+        outs = [t for t, on in ((weights, with_w), (got_load, with_l)) if on]
+        gs = [t.to(device) for t, on in ((gw, with_w), (gl, with_l)) if on]
+        got = torch.autograd.grad(outs, zd, gs, retain_graph=True)[0]
+        refs = [t for t, on in ((w, with_w), (load, with_l)) if on]
+        ref = torch.autograd.grad(refs, z64, [t.double() for t, on in ((gw, with_w), (gl, with_l)) if on], retain_graph=True)[0]
+        ref = torch.nan_to_num(ref, nan=0.0)  # (autograd of exp(-inf - m) is 0 * -inf; the formula's term is 0)
+        scale = 4 * gw.abs().sum(1, keepdim=True).double() * with_w + 4 * float(gl.abs().max()) / T * with_l
+        near(got, ref, dtype, rel * scale.expand_as(ref) if torch.is_tensor(scale) else rel * scale, f"g_logits {with_w} {with_l}")
+
+
+def check_route_special(ex, device, dtype):
+    """Rows with NaN or +inf: weights NaN, the choice goes by the other logits, nothing is out of range."""
+    z = torch.tensor([[1.0, math.nan, 3.0, 2.0, 0.0], [math.inf, 1.0, 2.0, 3.0, 4.0], [0.0, 1.0, 2.0, 3.0, 4.0],
+                      [math.nan] * 5, [-math.inf, 5.0, -math.inf, -math.inf, -math.inf]]).to(dtype).to(device)
+    w, e, load = ex.route_topk(z, 2)
+    assert e.cpu().tolist() == [[2, 3], [0, 4], [4, 3], [-1, -1], [1, -1]]
+    w = w.cpu()
+    assert torch.isnan(w[0]).all() and torch.isnan(w[1]).any() and w[4].tolist() == [1.0, 0.0] and w[3].tolist() == [0.0, 0.0]
+    assert torch.isfinite(w[2]).all() and torch.isnan(load.cpu()).any()
+    keep = torch.tensor([False, False, True, False, True], device=device)  # masked rows: whatever they hold counts as nothing
+    w, e, load = ex.route_topk(z, 2, row_mask=keep)
+    assert e.cpu().tolist() == [[-1, -1], [-1, -1], [4, 3], [-1, -1], [1, -1]]
+    assert torch.isfinite(w).all() and torch.isfinite(load).all() and float(w[0].abs().sum()) == 0
+    zg = z.clone().requires_grad_(True)
+    w, _, load = ex.route_topk(zg, 2, row_mask=keep)
+    g = torch.autograd.grad((w, load), zg, (torch.ones_like(w), torch.ones_like(load)))[0].cpu()
+    assert torch.isfinite(g).all() and float(g[~keep.cpu()].abs().sum()) == 0
+
+
+# --------------------------------------------------------------------------------------------------------- grouping
+def group_reference(experts, E):
+    flat = experts.flatten().tolist()
+    buckets = [[] for _ in range(E)]
+    for i, e in enumerate(flat):
+        if 0 <= e < E:
+            buckets[e].append(i)
+    order = [i for b in buckets for i in b]
+    offsets = [0]
+    for b in buckets:
+        offsets.append(offsets[-1] + len(b))
+    position = [-1] * len(flat)
+    for r, i in enumerate(order):
+        position[i] = r
+    order += [-1] * (len(flat) - len(order))
+    as_int = lambda v: torch.tensor(v, dtype=torch.int32)
+    return as_int(offsets), as_int(order), as_int(position).view(experts.shape)
+
+
+def check_group(ex, device, T, k, E, seed=0, skew=False, dropped=True):
+    g = torch.Generator().manual_seed(seed)
+    e = torch.randint(0, E, (T, k), generator=g, dtype=torch.int32)
+    if skew:
+        e = torch.where(torch.rand(T, k, generator=g) < 0.9, min(E - 1, 2), e).to(torch.int32)
+    if dropped and T:
+        bad = torch.tensor([-1, E, E + 5, -7, 2 ** 31 - 1, -2 ** 31], dtype=torch.int64).to(torch.int32)
+        e = torch.where(torch.rand(T, k, generator=g) < 0.2, bad[torch.randint(0, 6, (T, k), generator=g)], e)
+    offsets, order, position = group_reference(e, E)
+    got = ex.group_rows(e.to(device), E)
+    assert torch.equal(got.offsets.cpu(), offsets), "offsets"
+    assert torch.equal(got.order.cpu(), order), "order"
+    assert torch.equal(got.position.cpu(), position), "position"
+
+
+# ----------------------------------------------------------------------------------------------------- the products
+def activation64(z, act):
+    return z.clamp_min(0) if act == "relu" else z * torch.sigmoid(z) if act == "silu" else z
+
+
+def make_offsets(counts, device):
+    return torch.tensor([0] + torch.tensor(counts).cumsum(0).tolist(), dtype=torch.int32).to(device)
+
+
+def check_products(ex, device, counts, K, N, dtype, act=None, tail=0, pad=0, bias=True, seed=0, scale=1.0):
+    """grouped_linear on rows in the order of the groups, forward and backward, against float64."""
+    E, R = len(counts), sum(counts) + tail
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn(R, K, generator=g) * scale).to(dtype)
+    w = (torch.randn(E, N, K, generator=g) / math.sqrt(K)).to(dtype)
+    b = torch.randn(E, N, generator=g).to(dtype) if bias else None
+    gy = torch.randn(R, N, generator=g).to(dtype)
+    wide = torch.full((R, K + pad), math.nan, dtype=dtype)  # (what lies between the rows must not be read into results)
+    wide[:, :K] = x
+    xd = wide.to(device)[:, :K].detach().requires_grad_(True)
+    wd = w.to(device).requires_grad_(True)
+    bd = b.to(device).requires_grad_(True) if bias else None
+    groups = ex.RowGroups(make_offsets(counts, device))
+    y = ex.grouped_linear(xd, wd, groups, bias=bd, activation=act)
+    none = ex.grouped_linear(xd.detach(), wd.detach(), groups, bias=None if b is None else bd.detach(), activation=act)
+    assert torch.equal(none, y.detach()), "with and without gradients"
+    leaves = [xd, wd] + ([bd] if bias else [])
+    grads = torch.autograd.grad(y, leaves, gy.to(device))
+    X, W, G = x.double(), w.detach().double(), gy.double()
+    Y, GX, GW, GB = torch.zeros(R, N).double(), torch.zeros(R, K).double(), torch.zeros(E, N, K).double(), torch.zeros(E, N).double()
+    sY, sX, sW, sB = torch.zeros_like(Y), torch.zeros_like(GX), torch.zeros_like(GW), torch.zeros_like(GB)
+    lo = 0
+    for e, n in enumerate(counts):
+        r = slice(lo, lo + n)
+        lo += n
+        z = X[r] @ W[e].T + (b[e].detach().double() if bias else 0)
+        s = product_slack(K, X[r].abs() @ W[e].abs().T + (b[e].detach().double().abs() if bias else 0))
+        Y[r], sY[r] = activation64(z, act), 1.1 * s + 8 * 2.0 ** -24 * z.abs()  # (|silu'| <= 1.1; its own roundings)
+        gz, gs = G[r], torch.zeros_like(s)
+        if act:
+            # the slope is taken from what the forward kept in the inputs' type; relu: its output's sign, which may be
+            # either within the sum's own error of zero -- those elements are compared with a gradient of both signs allowed
+            d = (z > 0).double() if act == "relu" else torch.sigmoid(z) * (1 + z * (1 - torch.sigmoid(z)))
+            kept = HALF_STEP[dtype] * z.abs() + s
+            ds = (z.abs() <= kept).double() if act == "relu" else 0.5 * kept + 8 * 2.0 ** -24 * (1 + z.abs())  # |silu''| <= 1/2
+            gz = G[r] * d
+            gs = G[r].abs() * ds + HALF_STEP[dtype] * gz.abs() * (1 + 0) + HALF_STEP[dtype] * G[r].abs() * ds + TINY[dtype]
+        GX[r] = gz @ W[e]
+        sX[r] = product_slack(N, gz.abs() @ W[e].abs()) + gs @ W[e].abs() * 1.01
+        GW[e] = gz.T @ X[r]
+        sW[e] = product_slack(n, gz.abs().T @ X[r].abs()) + gs.T @ X[r].abs() * 1.01
+        GB[e] = gz.sum(0)
+        sB[e] = product_slack(n, gz.abs().sum(0)) + gs.sum(0) * 1.01
+    near(y, Y, dtype, sY, "y")
+    near(grads[0], GX, dtype, sX, "g_x")
+    near(grads[1], GW, dtype, sW, "g_w")
+    if bias:
+        near(grads[2], GB, dtype, sB, "g_b")
+    if tail:
+        assert float(y[R - tail:].detach().float().abs().sum()) == 0 and float(grads[0][R - tail:].float().abs().sum()) == 0
+
+
+def check_gather(ex, device, T, k, E, K, N, dtype, seed=0, pad=0):
+    """The products reading x through the grouping, places without an expert among them; x's gradient is the sum over
+    a row's places."""
+    g = torch.Generator().manual_seed(seed)
+    e = torch.randint(-1, E, (T, k), generator=g, dtype=torch.int32)
+    x = torch.randn(T, K, generator=g).to(dtype)
+    w = (torch.randn(E, N, K, generator=g) / math.sqrt(K)).to(dtype)
+    wide = torch.full((T, K + pad), math.nan, dtype=dtype)
+    wide[:, :K] = x
+    xd, wd = wide.to(device)[:, :K].detach().requires_grad_(True), w.to(device).requires_grad_(True)
+    groups = ex.group_rows(e.to(device), E)
+    y = ex.grouped_linear(xd, wd, groups, gather=True)
+    gy = torch.randn(T * k, N, generator=g).to(dtype)
+    gx, gw = torch.autograd.grad(y, (xd, wd), gy.to(device))
+    offsets, order, position = group_reference(e, E)
+    X, W, G = x.double(), w.detach().double(), gy.double()
+    Y, sY = torch.zeros(T * k, N).double(), torch.zeros(T * k, N).double()
+    GX, sX = torch.zeros(T, K).double(), torch.zeros(T, K).double()
+    GW, sW = torch.zeros(E, N, K).double(), torch.zeros(E, N, K).double()
+    for r, place in enumerate(order.tolist()):
+        if place < 0:
+            continue
+        t, q = place // k, int(e.flatten()[place])
+        Y[r], sY[r] = W[q] @ X[t], product_slack(K, W[q].abs() @ X[t].abs())
+        row = G[r] @ W[q]
+        GX[t] += row
+        sX[t] += product_slack(N, G[r].abs() @ W[q].abs()) + HALF_STEP[dtype] * row.abs() + TINY[dtype] + k * 2.0 ** -24 * row.abs()
+        GW[q] += G[r][:, None] * X[t][None]
+        sW[q] += (G[r].abs()[:, None] * X[t].abs()[None])
+    near(y, Y, dtype, sY, "y")
+    near(gx, GX, dtype, 1.01 * sX, "g_x")
+    near(gw, GW, dtype, product_slack(T * k, sW), "g_w")
+
+
+# ---------------------------------------------------------------------------------------------------- bringing together
+def check_combine(ex, device, T, k, E, N, dtype, weighted=True, residual=True, pad=0, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    e = torch.randint(-1, E, (T, k), generator=g, dtype=torch.int32)
+    groups = ex.group_rows(e.to(device), E)
+    _, _, position = group_reference(e, E)
+    y = torch.randn(T * k, N, generator=g).to(dtype)
+    w = torch.rand(T, k, generator=g) if weighted else None
+    res = torch.randn(T, N, generator=g).to(dtype) if residual else None
+    go = torch.randn(T, N, generator=g).to(dtype)
+    wide = torch.full((T * k, N + pad), math.nan, dtype=dtype)
+    wide[:, :N] = y
+    yd = wide.to(device)[:, :N].detach().requires_grad_(True)
+    leaves = [yd] + [t.to(device).requires_grad_(True) for t in (w, res) if t is not None]
+    out = ex.combine_rows(yd, groups, leaves[1] if weighted else None, leaves[-1] if residual else None)
+    grads = torch.autograd.grad(out, leaves, go.to(device))
+    at = position.long().clamp_min(0)
+    ys = y.double()[at] * (position >= 0)[..., None]
+    W = w.double() if weighted else torch.ones(T, k).double()
+    ref = (W[..., None] * ys).sum(1) + (res.double() if residual else 0)
+    mag = (W[..., None] * ys.abs()).sum(1) + (res.double().abs() if residual else 0)
+    near(out, ref, dtype, (k + 2) * 2.0 ** -24 * mag, "out")
+    gy = torch.zeros(T * k, N).double()
+    live = position >= 0
+    gy[position[live].long()] = (W[..., None] * go.double()[:, None])[live]
+    near(grads[0], gy, dtype, 2.0 ** -24 * gy.abs(), "g_y")
+    if weighted:
+        near(grads[1], (ys * go.double()[:, None]).sum(-1), torch.float32,
+             (N + 8) * 2.0 ** -24 * (ys.abs() * go.double()[:, None].abs()).sum(-1), "g_weights")
+    if residual:
+        assert torch.equal(grads[-1].cpu(), go)
+
+
+# ------------------------------------------------------------------------------------------------------ used together
+def check_layer(ex, device, T, K, F, E, k, act, seed=0):
+    """expert_mlp in fp32, masked rows among them: output and every gradient against float64 autograd, and the gradient
+    against differences of the float64 form along a random direction."""
+    g = torch.Generator().manual_seed(seed)
+    names = ("x", "logits", "w1", "b1", "w2", "b2")
+    leaf = [torch.randn(T, K, generator=g), torch.randn(T, E, generator=g), torch.randn(E, F, K, generator=g) / math.sqrt(K),
+            0.3 * torch.randn(E, F, generator=g), torch.randn(E, K, F, generator=g) / math.sqrt(F), 0.3 * torch.randn(E, K, generator=g)]
+    mask = torch.rand(T, generator=g) > 0.2
+    go = torch.randn(T, K, generator=g)
+
+    def reference(x, z, w1, b1, w2, b2):
+        w, e, _ = route_reference(z, k, mask)
+        out = x
+        for j in range(k):
+            i = e[:, j].long().clamp_min(0)
+            h = activation64(torch.einsum("tfk,tk->tf", w1[i], x) + b1[i], act)
+            out = out + (w[:, j] * (e[:, j] >= 0))[:, None] * (torch.einsum("tkf,tf->tk", w2[i], h) + b2[i])
+        return out
+
+    l64 = [t.double().requires_grad_(True) for t in leaf]
+    out64 = reference(*l64)
+    g64 = torch.autograd.grad(out64, l64, go.double())
+    ld = [t.to(device).requires_grad_(True) for t in leaf]
+    out = ex.expert_mlp(*ld, k=k, activation=act, row_mask=mask.to(device))
+    grads = torch.autograd.grad(out, ld, go.to(device))
+    # two products of K and F terms each way, each within (n + 32) 2^-24 of its terms' sizes: the terms of a sum of n
+    # unit-variance products are sqrt(n) times larger than the sum, three such sums follow one another
+    tol = 4 * (max(K, F, T) + 32) * math.sqrt(max(K, F)) * 2.0 ** -24
+    for name, got, ref in zip(("out",) + names, (out,) + grads, (out64.detach(),) + g64):
+        ref = torch.nan_to_num(ref, nan=0.0)
+        assert float((got.detach().double().cpu() - ref).abs().max()) <= tol * max(1.0, float(ref.abs().max())), name
+    step = 1e-6
+    ways = [torch.randn(t.shape, generator=g).double() for t in leaf]
+    ways[1] *= mask[:, None]
+    with torch.no_grad():
+        hi = reference(*[t.detach() + step * d for t, d in zip(l64, ways)])
+        lo = reference(*[t.detach() - step * d for t, d in zip(l64, ways)])
+    slope = float(((hi - lo) * go.double()).sum()) / (2 * step)
+    along = sum(float((gr.double().cpu() * d).sum()) for gr, d in zip(grads, ways))
+    size = sum(float((gr.double().cpu() * d).abs().sum()) for gr, d in zip(grads, ways))
+    assert abs(along - slope) <= (tol + 1e-5) * size, (along, slope)

@@ -134,7 +134,33 @@ SUBST["wave_ops.hpp"] = [
     ('asm volatile("s_nop 1\\n\\t" DIMO_RA(0, 8) DIMO_RA(1, 9) DIMO_RA1(2) DIMO_RA1(3) DIMO_RA1(4) DIMO_RA1(5) DIMO_RA1(6)\n'
      '                 DIMO_RA1(7) DIMO_RTAIL DIMO_ROPS);', "simt_wave_reduce16<10>(v);"),
 ]
-HEADERS = ["common.hpp", "proj_math.hpp", "wave_ops.hpp", "deform_body.hpp", "loss_terms.hpp"]  # copied beside the sources (substitutions applied)
+# the expert operators: routing, grouping, grouped products
+TARGETS["experts"] = (["experts.hip", "grouped.hip"], "experts_emu.cpp")
+SEPARATE.add("experts")
+SUBST["experts.hip"] = []
+SUBST["grouped.hip"] = []
+SUBST["row_tiles.hpp"] = []
+SUBST["numeric.hpp"] = [  # gcc 11 has neither 16-bit floating type on x86-64, nor std::bit_cast's builtin
+    ("__builtin_bit_cast(float, (uint32_t)v << 16)", "simt_from_bf16(v)"),
+    ("__builtin_bit_cast(uint16_t, (__bf16)v)", "simt_to_bf16(v)"),
+    ("(float)__builtin_bit_cast(_Float16, v)", "simt_from_f16(v)"),
+    ("__builtin_bit_cast(uint16_t, (_Float16)v)", "simt_to_f16(v)"),
+    ("__builtin_bit_cast(float, w[i % 4])", "__uint_as_float(w[i % 4])"),
+    ("__builtin_bit_cast(uint32_t, v[i % N])", "__float_as_uint(v[i % N])"),
+]
+SUBST["matrix_ops.hpp"] = [
+    ("typedef float f32x4 __attribute__((ext_vector_type(4)));", "typedef float f32x4 __attribute__((vector_size(16)));"),
+    ("typedef float f32x16 __attribute__((ext_vector_type(16)));", "typedef float f32x16 __attribute__((vector_size(64)));"),
+    ("typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));", ""),
+    ("typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));", ""),
+    ("__builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0)",
+     "simt_mfma_32x32x16(a, b, c, simt_from_bf16)"),
+    ("__builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0)",
+     "simt_mfma_32x32x16(a, b, c, simt_from_f16)"),
+    ("(uint16_t)(__builtin_bit_cast(uint32_t, v) >> 16)", "(uint16_t)(__float_as_uint(v) >> 16)"),
+]
+HEADERS = ["common.hpp", "proj_math.hpp", "wave_ops.hpp", "deform_body.hpp", "loss_terms.hpp", "numeric.hpp",
+           "matrix_ops.hpp", "row_tiles.hpp"]  # copied beside the sources (substitutions applied)
 
 
 def build(force=False, target="binning"):

@@ -327,6 +327,54 @@ static inline simt_f32x4 simt_mfma_4x4x1(float a, float b, simt_f32x4 c, int, in
 }
 #undef SIMT_A
 #undef SIMT_B
+// 16-bit conversions (round to nearest, ties to even) and the 16-bit matrix instructions of the expert kernels.
+static inline uint16_t simt_to_bf16(float f) {
+  uint32_t u = __float_as_uint(f);
+  if (f != f) return (uint16_t)((u >> 16) | 0x40);
+  return (uint16_t)((u + 0x7fff + ((u >> 16) & 1)) >> 16);
+}
+static inline float simt_from_bf16(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
+static inline uint16_t simt_to_f16(float f) {
+  const uint32_t u = __float_as_uint(f), sign = (u >> 16) & 0x8000u;
+  const float a = fabsf(f);
+  if (f != f) return (uint16_t)(sign | 0x7e00u);
+  if (a >= 65520.f) return (uint16_t)(sign | 0x7c00u);
+  const float step = a < 6.103515625e-05f ? 5.9604644775390625e-08f : ldexpf(1.f, ilogbf(a) - 10);
+  const float q = nearbyintf(a / step);  // (exact: step is a power of two; the default rounding is to nearest even)
+  if (a < 6.103515625e-05f) return (uint16_t)(sign | (uint32_t)q);
+  return (uint16_t)(sign | (((uint32_t)(ilogbf(a) + 15) << 10) + (uint32_t)q - 1024u));
+}
+static inline float simt_from_f16(uint16_t h) {
+  const int e = (h >> 10) & 31, m = h & 1023;
+  const float v = e == 31 ? (m ? NAN : INFINITY) : e ? ldexpf((float)(1024 + m), e - 25) : ldexpf((float)m, -24);
+  return h & 0x8000 ? -v : v;
+}
+// the 16-byte operands of all 64 lanes
+struct SimtOperands {
+  uint16_t a[64][8], b[64][8];
+  SimtOperands(uint4 x, uint4 y) {
+    const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    for (int q = 0; q < 4; ++q) {
+      const uint64_t *v = simt::wave_exchange(((uint64_t)w[2 * q + 1] << 32) | w[2 * q]);
+      for (int l = 0; l < 64; ++l)
+        for (int h = 0; h < 4; ++h) (q < 2 ? a : b)[l][4 * (q & 1) + h] = (uint16_t)(v[l] >> (16 * h));
+    }
+  }
+};
+// v_mfma_f32_32x32x16_{bf16,f16}: lane l holds A[i = l % 32][k = 8 (l / 32) ..+ 7], B[the same k][j = l % 32]; D as
+// v_mfma_f32_32x32x2_f32's
+template <class Load>
+static inline simt_f32x16 simt_mfma_32x32x16(uint4 x, uint4 y, simt_f32x16 c, Load load) {
+  const SimtOperands o(x, y);
+  const int l = simt::lane_id(), j = l & 31;
+  for (int r = 0; r < 16; ++r) {
+    const int i = 8 * (r >> 2) + 4 * (l >> 5) + (r & 3);
+    float s = c[r];
+    for (int k = 0; k < 16; ++k) s = fmaf(load(o.a[32 * (k >> 3) + i][k & 7]), load(o.b[32 * (k >> 3) + j][k & 7]), s);
+    c[r] = s;
+  }
+  return c;
+}
 #define __builtin_amdgcn_mfma_f32_16x16x4f32 simt_mfma_16x16x4
 #define __builtin_amdgcn_mfma_f32_32x32x2f32 simt_mfma_32x32x2
 #define __builtin_amdgcn_mfma_f32_4x4x1f32 simt_mfma_4x4x1

@@ -1,0 +1,152 @@
+"""The expert kernels (dimo_amd/csrc/experts.hip, grouped.hip, as hipcc compiles them) on the CPU SIMT emulation, through
+dimo_amd/experts.py, against float64 definitions (tests/expert_cases.py); and what the entry points refuse."""
+import math
+
+import pytest
+import torch
+
+from dimo_amd import experts as ex
+from tests import expert_cases as cases
+from tests import expert_emulation
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+@pytest.fixture
+def emulated(monkeypatch):
+    expert_emulation.use(monkeypatch, ex)
+
+
+@pytest.mark.parametrize("T,E,k,dtype,normalize,masked,kind,pad", [
+    (1, 1, 1, F32, True, False, "normal", 0),
+    (0, 4, 2, F32, True, False, "normal", 0),
+    (5, 3, 3, BF16, True, True, "normal", 1),
+    (70, 8, 2, F32, True, False, "normal", 0),
+    (70, 8, 2, F32, False, True, "normal", 0),
+    (33, 64, 8, F16, True, False, "ties", 0),
+    (33, 17, 5, F32, True, True, "-inf", 3),
+    (33, 17, 5, F32, False, False, "-inf", 0),
+    (9, 130, 5, F32, False, False, "normal", 0),
+    (9, 33, 4, BF16, True, False, "lowest", 0),
+    (9, 33, 4, F32, True, False, "lowest", 0),
+    (7, 257, 9, BF16, True, True, "ties", 0),
+    (3, 1024, 6, F32, True, False, "normal", 0),
+])
+def test_route(emulated, T, E, k, dtype, normalize, masked, kind, pad):
+    cases.check_route(ex, "cpu", T, E, k, dtype, normalize, masked, kind, pad, seed=T + E)
+
+
+def test_route_nan_and_infinities(emulated):
+    cases.check_route_special(ex, "cpu", F32)
+
+
+@pytest.mark.parametrize("T,k,E,skew", [(0, 2, 3, False), (1, 1, 1, False), (1, 8, 64, False), (63, 1, 5, False),
+                                        (4096, 1, 7, True), (2049, 2, 64, False), (5000, 2, 3, True), (700, 2, 1024, False)])
+def test_group(emulated, T, k, E, skew):
+    cases.check_group(ex, "cpu", T, k, E, seed=T + E, skew=skew)
+
+
+@pytest.mark.parametrize("counts,K,N,dtype,act,tail,pad", [
+    ([1], 1, 1, F32, None, 0, 0),
+    ([0, 3, 0], 8, 5, F32, "silu", 2, 0),
+    ([70, 0, 5, 64], 40, 66, BF16, None, 3, 8),
+    ([70, 0, 5, 64], 37, 65, F16, "relu", 0, 3),
+    ([33, 130], 72, 64, F32, "silu", 1, 0),
+    ([0, 0], 16, 16, BF16, None, 5, 0),
+    ([65], 129, 33, BF16, "silu", 0, 0),
+])
+def test_products(emulated, counts, K, N, dtype, act, tail, pad):
+    cases.check_products(ex, "cpu", counts, K, N, dtype, act, tail, pad, seed=K)
+
+
+@pytest.mark.parametrize("T,k,E,K,N,dtype,pad", [(1, 1, 1, 3, 2, F32, 0), (37, 2, 4, 24, 40, BF16, 4), (20, 3, 5, 33, 17, F32, 1)])
+def test_products_gathered(emulated, T, k, E, K, N, dtype, pad):
+    cases.check_gather(ex, "cpu", T, k, E, K, N, dtype, seed=K, pad=pad)
+
+
+@pytest.mark.parametrize("T,k,E,N,dtype,weighted,residual,pad", [
+    (1, 1, 1, 1, F32, True, True, 0), (21, 2, 5, 64, BF16, True, True, 8), (21, 3, 5, 33, F32, False, False, 1),
+    (9, 2, 2, 520, F16, True, False, 0)])
+def test_combine(emulated, T, k, E, N, dtype, weighted, residual, pad):
+    cases.check_combine(ex, "cpu", T, k, E, N, dtype, weighted, residual, pad, seed=N)
+
+
+@pytest.mark.parametrize("T,K,F,E,k,act", [(1, 8, 8, 2, 1, "silu"), (26, 24, 40, 5, 2, "silu")])
+def test_layer(emulated, T, K, F, E, k, act):
+    cases.check_layer(ex, "cpu", T, K, F, E, k, act)
+
+
+def test_bad_offsets_stay_inside(emulated):
+    """Offsets that the caller got wrong give wrong rows, never an address outside (run under AddressSanitizer too)."""
+    x, w = torch.randn(40, 8), torch.randn(3, 4, 8)
+    for bad in ([0, 100, -5, 40], [0, 40, 10, 1000], [7, 2 ** 31 - 1, -2 ** 31, 3]):
+        groups = ex.RowGroups(torch.tensor(bad, dtype=torch.int32))
+        xg = x.clone().requires_grad_(True)
+        y = ex.grouped_linear(xg, w, groups)
+        torch.autograd.grad(y.sum(), xg)
+
+
+def test_refusals():
+    z = torch.zeros(4, 6)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        ex.route_topk(z, 2)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        ex.group_rows(torch.zeros(4, 2, dtype=torch.int32), 6)
+
+
+@pytest.mark.parametrize("call", [
+    lambda: ex.route_topk(torch.zeros(4, 6), 0),
+    lambda: ex.route_topk(torch.zeros(4, 6), 7),
+    lambda: ex.route_topk(torch.zeros(4, 1025), 2),
+    lambda: ex.route_topk(torch.zeros(4, 6, dtype=torch.float64), 2),
+    lambda: ex.route_topk(torch.zeros(6), 2),
+    lambda: ex.route_topk(torch.zeros(4, 6), 2, row_mask=torch.ones(4)),
+    lambda: ex.route_topk(torch.zeros(4, 6), 2, row_mask=torch.ones(5, dtype=torch.bool)),
+    lambda: ex.group_rows(torch.zeros(4, 2, dtype=torch.int64), 6),
+    lambda: ex.group_rows(torch.zeros(4, 2, dtype=torch.int32), 0),
+    lambda: ex.RowGroups(torch.zeros(4, dtype=torch.int64)),
+    lambda: ex.RowGroups(torch.zeros(1, dtype=torch.int32)),
+    lambda: ex.grouped_linear(torch.zeros(4, 8), torch.zeros(3, 5, 9), ex.RowGroups(torch.zeros(4, dtype=torch.int32))),
+    lambda: ex.grouped_linear(torch.zeros(4, 8), torch.zeros(2, 5, 8), ex.RowGroups(torch.zeros(4, dtype=torch.int32))),
+    lambda: ex.grouped_linear(torch.zeros(4, 8), torch.zeros(3, 5, 8).half(), ex.RowGroups(torch.zeros(4, dtype=torch.int32))),
+    lambda: ex.grouped_linear(torch.zeros(4, 8), torch.zeros(3, 5, 8), ex.RowGroups(torch.zeros(4, dtype=torch.int32)),
+                              bias=torch.zeros(3, 4)),
+    lambda: ex.grouped_linear(torch.zeros(4, 8), torch.zeros(3, 5, 8), ex.RowGroups(torch.zeros(4, dtype=torch.int32)),
+                              activation="gelu"),
+    lambda: ex.grouped_linear(torch.zeros(4, 8), torch.zeros(3, 5, 8), ex.RowGroups(torch.zeros(4, dtype=torch.int32)),
+                              gather=True),
+    lambda: ex.grouped_linear(torch.zeros(4, 8), torch.zeros(6, 5, 8), ex.group_rows(torch.zeros(3, 2, dtype=torch.int32), 6),
+                              gather=True),
+    lambda: ex.grouped_linear(torch.zeros(4, 8), torch.zeros(6, 5, 8), ex.group_rows(torch.zeros(4, 2, dtype=torch.int32), 6)),
+    lambda: ex.combine_rows(torch.zeros(4, 8), ex.RowGroups(torch.zeros(4, dtype=torch.int32))),
+    lambda: ex.combine_rows(torch.zeros(4, 8), ex.group_rows(torch.zeros(4, 2, dtype=torch.int32), 6)),
+    lambda: ex.combine_rows(torch.zeros(8, 8), ex.group_rows(torch.zeros(4, 2, dtype=torch.int32), 6),
+                            weights=torch.zeros(4, 2, dtype=torch.float64)),
+    lambda: ex.combine_rows(torch.zeros(8, 8), ex.group_rows(torch.zeros(4, 2, dtype=torch.int32), 6),
+                            residual=torch.zeros(4, 7)),
+])
+def test_bad_arguments(emulated, call):
+    with pytest.raises(ValueError):
+        call()
+
+
+def test_c_entry_points_refuse():
+    """The C ABI returns an error for what its header does not allow, before it launches anything."""
+    L = expert_emulation.emulated_library()
+    assert L.dimo_route_topk_forward(4, 6, 7, 0, 1, 6, None, 1, 1, 1, None, None, 0, None) == -1
+    assert L.dimo_route_topk_forward(4, 6, 2, 3, 1, 6, None, 1, 1, 1, None, None, 0, None) == -1
+    assert L.dimo_route_topk_forward(4, 6, 2, 0, 1, 5, None, 1, 1, 1, None, None, 0, None) == -1
+    assert L.dimo_route_topk_forward(4, 6, 2, 0, 1, 6, None, 1, 1, 1, 1, None, 0, None) == -3
+    assert L.dimo_route_topk_forward(4, 6, 2, 0, None, 6, None, 1, 1, 1, None, None, 0, None) == -1
+    assert L.dimo_group_rows(10000, 6, 1, 1, 1, 1, None, 0, None) == -3
+    assert L.dimo_group_rows(-1, 6, 1, 1, 1, 1, None, 0, None) == -1
+    assert L.dimo_group_rows(4, 1025, 1, 1, 1, 1, None, 0, None) == -1
+    assert L.dimo_grouped_linear_forward(0, 4, 3, 8, 5, 1, 7, 0, None, 1, 1, None, 0, 1, None, None) == -1
+    assert L.dimo_grouped_linear_forward(0, 4, 3, 8, 5, 1, 8, 2, None, 1, 1, None, 0, 1, None, None) == -1
+    assert L.dimo_grouped_linear_forward(0, 4, 3, 8, 5, 1, 8, 0, None, 1, 1, None, 3, 1, None, None) == -1
+    assert L.dimo_grouped_linear_dgrad(0, 4, 0, 8, 5, 1, 1, 1, 1, None) == -1
+    assert L.dimo_grouped_linear_wgrad(0, 4, 3, 8, 5, 1, 1, 8, 0, None, None, 1, None, None) == -1
+    assert L.dimo_activation_backward(0, 0, 8, 1, 1, 1, None) == -1
+    assert L.dimo_combine_rows_forward(4, 2, 8, 8, 0, 1, 7, None, 1, None, 0, 1, None) == -1
+    assert L.dimo_combine_rows_backward(4, 2, 8, 9, 3, 0, 1, 8, 1, 8, 1, 1, 1, 1, 1, None) == -1
+    assert L.dimo_route_topk_forward(0, 6, 2, 0, None, 6, None, 1, None, None, None, None, 0, None) == 0

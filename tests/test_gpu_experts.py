@@ -1,0 +1,146 @@
+"""The expert operators (dimo_amd/experts.py) on the GPU against their float64 definitions (tests/expert_cases.py has the
+checks and derives the tolerances), and how they are used: strides, streams, captured graphs, together."""
+import math
+
+import pytest
+import torch
+
+from tests import expert_cases as cases
+
+pytestmark = pytest.mark.gpu
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module")
+def ex():
+    from dimo_amd import experts
+    return experts
+
+
+@pytest.mark.parametrize("T,E,k,dtype,normalize,masked,kind,pad", [
+    (1, 1, 1, F32, True, False, "normal", 0),
+    (0, 4, 2, F32, True, False, "normal", 0),
+    (1, 64, 8, F32, True, False, "normal", 0),
+    (5, 3, 3, BF16, True, True, "normal", 1),
+    (4096, 8, 2, F32, True, False, "normal", 0),
+    (4097, 8, 2, F32, False, True, "normal", 0),
+    (333, 64, 8, F16, True, False, "ties", 0),
+    (333, 17, 5, F32, True, True, "-inf", 3),
+    (333, 17, 5, F32, False, False, "-inf", 0),
+    (333, 33, 4, BF16, True, False, "lowest", 0),
+    (333, 33, 4, F32, True, False, "lowest", 0),
+    (9000, 128, 8, BF16, True, True, "ties", 0),
+    (257, 256, 256, F32, False, False, "normal", 0),
+    (130, 257, 9, BF16, True, True, "ties", 0),
+    (77, 1024, 6, F32, True, False, "normal", 0),
+    (200000, 4, 1, F32, True, False, "normal", 0),
+])
+def test_route(ex, T, E, k, dtype, normalize, masked, kind, pad):
+    cases.check_route(ex, "cuda", T, E, k, dtype, normalize, masked, kind, pad, seed=T + E)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_route_nan_and_infinities(ex, dtype):
+    cases.check_route_special(ex, "cuda", dtype)
+
+
+@pytest.mark.parametrize("T,k,E,skew", [(0, 2, 3, False), (1, 1, 1, False), (1, 8, 64, False), (63, 1, 5, False),
+                                        (4096, 1, 7, True), (2049, 2, 64, False), (50000, 2, 3, True), (7001, 2, 1024, False),
+                                        (131072, 4, 128, False)])
+def test_group(ex, T, k, E, skew):
+    cases.check_group(ex, "cuda", T, k, E, seed=T + E, skew=skew)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("counts,K,N,act,tail,pad", [
+    ([1], 1, 1, None, 0, 0),
+    ([0, 3, 0], 8, 5, "silu", 2, 0),
+    ([1, 0, 1, 2], 256, 64, "relu", 0, 0),
+    ([70, 0, 5, 64], 40, 66, None, 3, 8),
+    ([70, 0, 5, 64], 37, 65, "relu", 0, 3),
+    ([130, 300], 256, 256, "silu", 1, 0),
+    ([513, 0, 1, 255, 128], 360, 257, None, 0, 8),
+    ([0, 0], 16, 16, None, 5, 0),
+    ([65], 129, 33, "silu", 0, 0),
+    ([700], 512, 136, "relu", 60, 8),
+    ([3] * 150, 72, 96, "silu", 0, 0),
+])
+def test_products(ex, counts, K, N, dtype, act, tail, pad):
+    cases.check_products(ex, "cuda", counts, K, N, dtype, act, tail, pad, seed=K)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("T,k,E,K,N,pad", [(1, 1, 1, 3, 2, 0), (1, 2, 8, 512, 256, 0), (200, 2, 4, 256, 128, 8), (150, 3, 5, 33, 17, 1)])
+def test_products_gathered(ex, T, k, E, K, N, dtype, pad):
+    cases.check_gather(ex, "cuda", T, k, E, K, N, dtype, seed=K, pad=pad)
+
+
+@pytest.mark.parametrize("T,k,E,N,dtype,weighted,residual,pad", [
+    (1, 1, 1, 1, F32, True, True, 0), (500, 2, 5, 64, BF16, True, True, 8), (211, 3, 5, 33, F32, False, False, 1),
+    (99, 2, 2, 520, F16, True, False, 0), (301, 8, 16, 1024, F32, True, True, 0)])
+def test_combine(ex, T, k, E, N, dtype, weighted, residual, pad):
+    cases.check_combine(ex, "cuda", T, k, E, N, dtype, weighted, residual, pad, seed=N)
+
+
+@pytest.mark.parametrize("T,K,F,E,k,act", [(1, 8, 8, 2, 1, "silu"), (126, 24, 40, 5, 2, "silu"), (600, 256, 128, 8, 2, "silu")])
+def test_layer(ex, T, K, F, E, k, act):
+    cases.check_layer(ex, "cuda", T, K, F, E, k, act)
+
+
+def _layer_leaves(T, K, F, E, dtype, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    return [t.to(dtype).requires_grad_(True) for t in (r(T, K), r(T, E), r(E, F, K) / math.sqrt(K), r(E, F), r(E, K, F) / math.sqrt(F), r(E, K))]
+
+
+def test_same_results_every_time_and_on_another_stream(ex):
+    """No result depends on the schedule: a second call, and one on another stream, give the same bits."""
+    leaves = _layer_leaves(1000, 256, 128, 8, BF16, 3)
+    go = torch.ones_like(leaves[0])
+
+    def step():
+        out = ex.expert_mlp(*leaves, k=2, activation="silu")
+        return (out,) + torch.autograd.grad(out, leaves, go)
+    first = step()
+    again = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        there = step()
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b, c in zip(first, again, there):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_captured_steps(ex):
+    """Two captured training steps (their workspaces are the graphs' own) replayed in turns, new inputs every time, the
+    eager step between them."""
+    graphs = []
+    for seed in (1, 2):
+        leaves = _layer_leaves(700, 128, 64, 4, F32, seed)
+        go = torch.randn_like(leaves[0])
+
+        def step(leaves=leaves, go=go):
+            out = ex.expert_mlp(*leaves, k=2, activation="silu")
+            return (out,) + torch.autograd.grad(out, leaves, go)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step()
+        graphs.append((graph, leaves, step, outs))
+    for it in range(3):
+        for n, (graph, leaves, step, outs) in enumerate(graphs):
+            g = torch.Generator(device="cuda").manual_seed(10 * it + n)
+            with torch.no_grad():
+                leaves[0].copy_(torch.randn(leaves[0].shape, generator=g, device="cuda"))
+                leaves[1].copy_(torch.randn(leaves[1].shape, generator=g, device="cuda"))
+        for graph, _, _, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, _, step, outs in graphs:
+            for got, ref in zip(outs, step()):
+                assert torch.equal(got, ref)
