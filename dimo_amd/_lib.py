@@ -102,6 +102,9 @@ _SIGNATURES = {
                                   + [C.c_int64, c_ptr, c_ptr]),
     "dimo_combine_rows_backward": (C.c_int, [C.c_int] * 3 + [C.c_int64, C.c_int, C.c_int, c_ptr, C.c_int64, c_ptr,
                                                              C.c_int64] + [c_ptr] * 6),
+    "dimo_mx4_quantize": (C.c_int, [C.c_int, C.c_int64, C.c_int, c_ptr, C.c_int64, C.c_int] + [c_ptr] * 4),
+    "dimo_mx4_dequantize": (C.c_int, [C.c_int, C.c_int64, C.c_int] + [c_ptr] * 4),
+    "dimo_mx4_linear": (C.c_int, [C.c_int] * 5 + [c_ptr] * 6 + [C.c_int, c_ptr, c_ptr]),
 }
 
 ERRORS = {-1: "DIMO_E_ARG (bad argument)", -2: "DIMO_E_LAUNCH (HIP launch/runtime error)",

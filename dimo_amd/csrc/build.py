@@ -13,6 +13,8 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB = os.path.join(HERE, "libdimo_hip.so")
 ARCH = "gfx950"
+# no packed fp32 instructions: some forms of v_pk_{add,mul,fma}_f32 have given wrong results now and then
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 SOURCES = {
     "api.hip": [],
     # (no SLP packing: the projection backward needs 90 VGPRs instead of 110 -- five waves per SIMD -- and runs 67.9
@@ -31,8 +33,9 @@ SOURCES = {
     "timenet.hip": [],
     "fps.hip": ["-ffp-contract=off"],
     "executor.hip": [],
-    "experts.hip": [],
-    "grouped.hip": [],
+    "experts.hip": NO_PACKED_FP32,
+    "grouped.hip": NO_PACKED_FP32,
+    "mx4.hip": NO_PACKED_FP32,
 }
 if os.environ.get("DIMO_BWD_TRACE") == "1":  # per-item trace of the blend backward (tools/bwd_trace.py)
     SOURCES["blend.hip"] = SOURCES["blend.hip"] + ["-DDIMO_BWD_TRACE"]

@@ -52,12 +52,6 @@ __device__ __forceinline__ int64_t source_row(const GroupedArgs &a, int r) {
   return a.places > 0 ? a.order[r] / a.places : r;
 }
 
-__device__ __forceinline__ float activate(float v, int act) {
-  if (act == DIMO_ACT_RELU) return v > 0.f ? v : (v != v ? v : 0.f);
-  if (act == DIMO_ACT_SILU) return v / (1.f + expf(-v));
-  return v;
-}
-
 // eight elements of an operand's stage as fp32, `ok` of them inside
 template <class T>
 __device__ __forceinline__ void stage_elements(const typename T::store *p, int ok, bool wide, typename T::store (&v)[8]) {

@@ -91,6 +91,13 @@ __device__ __forceinline__ void store_vec(typename T::store *dst, const float (&
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// (relu keeps a NaN)
+__device__ __forceinline__ float activate(float v, int act) {
+  if (act == DIMO_ACT_RELU) return v > 0.f ? v : (v != v ? v : 0.f);
+  if (act == DIMO_ACT_SILU) return v / (1.f + expf(-v));
+  return v;
+}
+
 // slope of an activation: from its output for relu (positive exactly where its input is), from its input for silu
 __device__ __forceinline__ float activation_slope(float s, int act) {
   if (act == DIMO_ACT_RELU) return s > 0.f ? 1.f : (s != s ? s : 0.f);

@@ -283,6 +283,13 @@ class _GroupedLinear(torch.autograd.Function):
         return gx, gw, gb, None, None, None
 
 
+def _check_linear_groups(E, rows, groups):
+    if E != groups.num_experts:
+        raise ValueError(f"{E} experts' weights for {groups.num_experts} groups")
+    if rows is not None and groups.position is not None and rows != groups.order.shape[0]:
+        raise ValueError(f"{rows} rows in the order of the groups, {groups.order.shape[0]} expected")
+
+
 def _check_linear(x, weight, bias, groups, activation, gather):
     if x.dim() != 2 or weight.dim() != 3:
         raise ValueError("x: [rows, K] and weight: [E, N, K] expected")
@@ -293,8 +300,6 @@ def _check_linear(x, weight, bias, groups, activation, gather):
     E, N, K = weight.shape
     if x.shape[1] != K or K < 1 or N < 1:
         raise ValueError(f"x has {x.shape[1]} columns, weight takes {K}")
-    if E != groups.num_experts:
-        raise ValueError(f"{E} experts' weights for {groups.num_experts} groups")
     if bias is not None and bias.shape != (E, N):
         raise ValueError("bias: [E, N] expected")
     if activation not in _ACTIVATIONS:
@@ -304,8 +309,7 @@ def _check_linear(x, weight, bias, groups, activation, gather):
             raise ValueError("gather=True needs groups made by group_rows")
         if x.shape[0] != groups.position.shape[0]:
             raise ValueError(f"{x.shape[0]} rows, {groups.position.shape[0]} were grouped")
-    elif groups.position is not None and x.shape[0] != groups.order.shape[0]:
-        raise ValueError(f"{x.shape[0]} rows in the order of the groups, {groups.order.shape[0]} expected")
+    _check_linear_groups(E, None if gather else x.shape[0], groups)
 
 
 def grouped_linear(x, weight, groups, bias=None, activation=None, gather=False):

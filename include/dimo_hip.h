@@ -492,6 +492,17 @@ int dimo_combine_rows_forward(int T, int k, int N, int64_t S, int dtype, const v
 int dimo_combine_rows_backward(int T, int k, int N, int64_t S, int E, int dtype, const void *g_out, int64_t ldg,
                                const void *y, int64_t ldy, const float *weights, const int32_t *position,
                                const int32_t *offsets, void *g_y, float *g_weights, void *stream);
+/* Microscaled 4-bit floating point: e2m1 elements in blocks of 32 along a row, one scale byte (2^(byte - 127), 255 = NaN)
+ * per block.  codes [rows, 16 ceil(K / 32)] (two to a byte, low four bits first), scales [rows, ceil(K / 32)].
+ * x: rows at ldx; places > 0: row r is order[r] / places of x, zeros where order[r] is negative. */
+int dimo_mx4_quantize(int dtype, int64_t rows, int K, const void *x, int64_t ldx, int places, const int32_t *order,
+                      uint8_t *codes, uint8_t *scales, void *stream);
+int dimo_mx4_dequantize(int dtype, int64_t rows, int K, const uint8_t *codes, const uint8_t *scales, void *out, void *stream);
+/* y[r] = act(w[e] x[r] + bias[e]) of quantised x [R, K] and w [E, N, K]; offsets as in dimo_grouped_linear_forward, or NULL
+ * with E = 1; dtype: of y and bias.  Both code arrays on 16-byte boundaries. */
+int dimo_mx4_linear(int dtype, int R, int E, int K, int N, const uint8_t *x_codes, const uint8_t *x_scales,
+                    const int32_t *offsets, const uint8_t *w_codes, const uint8_t *w_scales, const void *bias, int act,
+                    void *y, void *stream);
 
 #ifdef __cplusplus
 }

@@ -261,10 +261,10 @@ def check_combine(ex, device, T, k, E, N, dtype, weighted=True, residual=True, p
     out = ex.combine_rows(yd, groups, leaves[1] if weighted else None, leaves[-1] if residual else None)
     grads = torch.autograd.grad(out, leaves, go.to(device))
     at = position.long().clamp_min(0)
-    ys = y.double()[at] * (position >= 0)[..., None]
-    W = w.double() if weighted else torch.ones(T, k).double()
-    ref = (W[..., None] * ys).sum(1) + (res.double() if residual else 0)
-    mag = (W[..., None] * ys.abs()).sum(1) + (res.double().abs() if residual else 0)
+    ys = y.detach().double()[at] * (position >= 0)[..., None]
+    W = w.detach().double() if weighted else torch.ones(T, k).double()
+    ref = (W[..., None] * ys).sum(1) + (res.detach().double() if residual else 0)
+    mag = (W[..., None] * ys.abs()).sum(1) + (res.detach().double().abs() if residual else 0)
     near(out, ref, dtype, (k + 2) * 2.0 ** -24 * mag, "out")
     gy = torch.zeros(T * k, N).double()
     live = position >= 0
@@ -319,3 +319,134 @@ def check_layer(ex, device, T, K, F, E, k, act, seed=0):
     along = sum(float((gr.double().cpu() * d).sum()) for gr, d in zip(grads, ways))
     size = sum(float((gr.double().cpu() * d).abs().sum()) for gr, d in zip(grads, ways))
     assert abs(along - slope) <= (tol + 1e-5) * size, (along, slope)
+
+
+# ------------------------------------------------------------------------------------------- microscaled 4-bit values
+E2M1 = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], dtype=torch.float64)
+
+
+def quantize_reference(x):
+    """(codes [R, 32 B], scale bytes [R, B], values [R, K]) of x [R, K] in float64, one element at a time by distance."""
+    x = x.double().cpu()
+    R, K = x.shape
+    B = -(-K // 32)
+    v = torch.nn.functional.pad(x, (0, 32 * B - K)).view(R, B, 32)
+    big = v.abs().amax(-1)
+    finite = torch.isfinite(v).all(-1)
+    byte = torch.full((R, B), 255, dtype=torch.int64)
+    exponent = torch.frexp(torch.where(finite & (big > 0), big, 1.0))[1].long() - 1
+    byte = torch.where(finite, torch.where(big > 0, (exponent - 2 + 127).clamp_min(0), 0), byte)
+    scale = torch.ldexp(torch.ones(R, B, dtype=torch.float64), (byte - 127).int())
+    a = torch.where(finite[..., None], v / scale[..., None], 0.0).abs().clamp_max(6.0)
+    off = (a[..., None] - E2M1).abs()
+    best = off.amin(-1, keepdim=True)
+    tied = off == best
+    even = tied & (torch.arange(8) % 2 == 0)
+    code = torch.where(even.any(-1), even.to(torch.uint8).argmax(-1), tied.to(torch.uint8).argmax(-1))
+    sign = torch.signbit(v).long()
+    values = torch.where(finite[..., None], E2M1[code] * torch.where(sign > 0, -1.0, 1.0) * scale[..., None], math.nan)
+    return code | (sign << 3), byte, values.reshape(R, -1)[:, :K], finite
+
+
+def unpacked(codes):
+    codes = codes.cpu().long()
+    return torch.stack([codes & 15, codes >> 4], -1).flatten(-2)
+
+
+def quantize_inputs(R, K, dtype, seed, kind="normal"):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(R, K, generator=g) * torch.exp(2 * torch.randn(1, K, generator=g))
+    if kind == "borders":  # every value on or next to a rounding border, the block's largest 4
+        borders = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 7.0, 0.0, -0.0, 4.0])
+        x = borders[torch.randint(0, 12, (R, K), generator=g)] * torch.where(torch.rand(R, K, generator=g) < 0.5, -1.0, 1.0)
+        x = x * torch.exp2(torch.randint(-6, 7, (R, 1), generator=g).float())
+        if dtype == torch.float32:
+            x = x * (1 + (torch.randint(-1, 2, (R, K), generator=g)).float() * 2.0 ** -23)
+    if kind == "range":  # from the smallest magnitudes to the largest of the type
+        top = {torch.float32: 127, torch.bfloat16: 127, torch.float16: 15}[dtype]
+        low = {torch.float32: -149, torch.bfloat16: -133, torch.float16: -24}[dtype]
+        x = torch.ldexp(1 + torch.rand(R, K, generator=g) * 0.99, torch.randint(low, top + 1, (R, 1), generator=g).int())
+        x[0] = 0
+    if kind == "special":
+        x[0, 0], x[1, K // 2], x[2, K - 1] = math.inf, -math.inf, math.nan
+    return x.to(dtype)
+
+
+def check_quantize(mx4, device, R, K, dtype, kind="normal", pad=0, seed=0):
+    x = quantize_inputs(R, K, dtype, seed, kind)
+    code, byte, values, finite = quantize_reference(x)
+    wide = torch.full((R, K + pad), math.nan, dtype=dtype)
+    wide[:, :K] = x
+    q = mx4.quantize_mx4(wide.to(device)[:, :K])
+    assert tuple(q.shape) == (R, K)
+    assert torch.equal(q.scales.cpu().long(), byte), "scales"
+    got = unpacked(q.codes).view(R, -1, 32)
+    assert torch.equal(got[finite], code[finite]), "codes"
+    for out in (torch.float32, torch.bfloat16, torch.float16):
+        d = q.dequantize(out).cpu()
+        assert d.dtype == out and torch.equal(torch.isnan(d), torch.isnan(values))
+        ref = values.to(torch.float32).to(out)
+        assert torch.equal(torch.nan_to_num(d, nan=0.0, posinf=1.0, neginf=-1.0), torch.nan_to_num(ref, nan=0.0, posinf=1.0, neginf=-1.0)), out
+
+
+def check_mx4_linear(mx4, ex, device, counts, K, N, dtype, act=None, bias=True, tail=0, grouped=True, seed=0):
+    E, R = len(counts), sum(counts) + tail
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(R, K, generator=g) * torch.exp(torch.randn(1, K, generator=g))
+    w = torch.randn(E, N, K, generator=g) / math.sqrt(K)
+    b = torch.randn(E, N, generator=g).to(dtype) if bias else None
+    xq, wq = mx4.quantize_mx4(x.to(device)), mx4.quantize_mx4(w.to(device))
+    assert tuple(wq.shape) == (E, N, K)
+    X = quantize_reference(x)[2]
+    W = quantize_reference(w.view(E * N, K))[2].view(E, N, K)
+    if grouped:
+        groups = ex.RowGroups(make_offsets(counts, device))
+        y = mx4.mx4_linear(xq, wq, None if b is None else b.to(device), groups, act, dtype)
+    else:
+        y = mx4.mx4_linear(xq, mx4.MX4(wq.codes[0], wq.scales[0], K), None if b is None else b[0].to(device), None, act, dtype)
+    Y, s = torch.zeros(R, N).double(), torch.zeros(R, N).double()
+    lo = 0
+    for e, n in enumerate(counts):
+        r = slice(lo, lo + n)
+        lo += n
+        z = X[r] @ W[e].T + (b[e].double() if bias else 0)
+        Y[r] = activation64(z, act)
+        s[r] = 1.1 * product_slack(K, X[r].abs() @ W[e].abs().T + (b[e].double().abs() if bias else 0)) + 8 * 2.0 ** -24 * z.abs()
+    near(y, Y, dtype, s, "y")
+    if tail:
+        assert float(y[R - tail:].float().abs().sum()) == 0
+
+
+def check_mx4_layer(mx4, ex, device, T, k, E, K, F, seed=0):
+    """Routing, grouping, quantisation through the grouping, two grouped 4-bit products, the weighted sum: as they are
+    used together, places without an expert among them."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(T, K, generator=g)
+    z = torch.randn(T, E, generator=g)
+    mask = torch.rand(T, generator=g) > 0.3
+    w1, w2 = torch.randn(E, F, K, generator=g) / math.sqrt(K), torch.randn(E, K, F, generator=g) / math.sqrt(F)
+    w, e, _ = ex.route_topk(z.to(device), k, row_mask=mask.to(device))
+    groups = ex.group_rows(e, E)
+    xq = mx4.quantize_mx4(x.to(device), groups)
+    assert tuple(xq.shape) == (T * k, K)
+    h = mx4.mx4_linear(xq, mx4.quantize_mx4(w1.to(device)), None, groups, "relu", torch.float32)
+    y = mx4.mx4_linear(mx4.quantize_mx4(h), mx4.quantize_mx4(w2.to(device)), None, groups, None, torch.float32)
+    out = ex.combine_rows(y, groups, w, x.to(device)).cpu().double()
+    W, C, _ = route_reference(z.double(), k, mask)
+    X = quantize_reference(x)[2]
+    W1 = quantize_reference(w1.view(E * F, K))[2].view(E, F, K)
+    W2 = quantize_reference(w2.view(E * K, F))[2].view(E, K, F)
+    H = h.cpu().double()
+    order = groups.order.cpu().tolist()
+    ref, slack = x.double().clone(), torch.zeros(T, K).double()
+    for r, place in enumerate(order):
+        if place < 0:
+            assert float(H[r].abs().sum()) == 0 and float(xq.dequantize().cpu()[r].abs().sum()) == 0
+            continue
+        t, q = place // k, int(C.flatten()[place])
+        hr = (W1[q] @ X[t]).clamp_min(0)
+        assert float((H[r] - hr).abs().max()) <= float((product_slack(K, W1[q].abs() @ X[t].abs()) + 2.0 ** -23 * hr).max())
+        hq = quantize_reference(h[r:r + 1].cpu())[2][0]  # (a hidden value next to a border may round either way: the kernel's own)
+        ref[t] += W[t, place % k] * (W2[q] @ hq)
+        slack[t] += W[t, place % k] * product_slack(F, W2[q].abs() @ hq.abs()) * 2 + 2.0 ** -20 * (W2[q] @ hq).abs() * W[t, place % k]
+    near(out, ref, torch.float32, slack + 2.0 ** -22 * ref.abs(), "out")

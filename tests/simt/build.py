@@ -134,11 +134,12 @@ SUBST["wave_ops.hpp"] = [
     ('asm volatile("s_nop 1\\n\\t" DIMO_RA(0, 8) DIMO_RA(1, 9) DIMO_RA1(2) DIMO_RA1(3) DIMO_RA1(4) DIMO_RA1(5) DIMO_RA1(6)\n'
      '                 DIMO_RA1(7) DIMO_RTAIL DIMO_ROPS);', "simt_wave_reduce16<10>(v);"),
 ]
-# the expert operators: routing, grouping, grouped products
-TARGETS["experts"] = (["experts.hip", "grouped.hip"], "experts_emu.cpp")
+# the expert operators: routing, grouping, grouped products, 4-bit products
+TARGETS["experts"] = (["experts.hip", "grouped.hip", "mx4.hip"], "experts_emu.cpp")
 SEPARATE.add("experts")
 SUBST["experts.hip"] = []
 SUBST["grouped.hip"] = []
+SUBST["mx4.hip"] = []
 SUBST["row_tiles.hpp"] = []
 SUBST["numeric.hpp"] = [  # gcc 11 has neither 16-bit floating type on x86-64, nor std::bit_cast's builtin
     ("__builtin_bit_cast(float, (uint32_t)v << 16)", "simt_from_bf16(v)"),
@@ -157,6 +158,9 @@ SUBST["matrix_ops.hpp"] = [
      "simt_mfma_32x32x16(a, b, c, simt_from_bf16)"),
     ("__builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0)",
      "simt_mfma_32x32x16(a, b, c, simt_from_f16)"),
+    ("typedef int i32x8 __attribute__((ext_vector_type(8)));", "typedef int i32x8 __attribute__((vector_size(32)));"),
+    ("__builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c, 4, 4, 0, scale_a, 0, scale_b)",
+     "simt_mfma_mx4_32x32x64(a, scale_a, b, scale_b, c)"),
     ("(uint16_t)(__builtin_bit_cast(uint32_t, v) >> 16)", "(uint16_t)(__float_as_uint(v) >> 16)"),
 ]
 HEADERS = ["common.hpp", "proj_math.hpp", "wave_ops.hpp", "deform_body.hpp", "loss_terms.hpp", "numeric.hpp",

@@ -361,6 +361,31 @@ struct SimtOperands {
     }
   }
 };
+// e2m1 code times 2^(byte - 127)
+static inline double simt_mx4_value(uint32_t code, uint32_t byte) {
+  code &= 15;
+  static const double mag[8] = {0., .5, 1., 1.5, 2., 3., 4., 6.};
+  if (byte == 255) return NAN;
+  return (code & 8 ? -1. : 1.) * ldexp(mag[code & 7], (int)byte - 127);
+}
+// v_mfma_scale_f32_32x32x64_f8f6f4 on e2m1 operands: lane l holds A[i = l % 32][k = 32 (l / 32) ..+ 31] and its scale, B
+// likewise
+static inline simt_f32x16 simt_mfma_mx4_32x32x64(uint4 x, int sx, uint4 y, int sy, simt_f32x16 c) {
+  const SimtOperands o(x, y);
+  const uint64_t *sv = simt::wave_exchange(((uint64_t)(uint32_t)(sx & 255) << 32) | (uint32_t)(sy & 255));
+  const int l = simt::lane_id(), j = l & 31;
+  for (int r = 0; r < 16; ++r) {
+    const int i = 8 * (r >> 2) + 4 * (l >> 5) + (r & 3);
+    double s = c[r];
+    for (int k = 0; k < 64; ++k) {
+      const int la = 32 * (k >> 5) + i, lb = 32 * (k >> 5) + j, q = k & 31;
+      s += simt_mx4_value(o.a[la][q >> 2] >> (4 * (q & 3)), (uint32_t)(sv[la] >> 32)) *
+           simt_mx4_value(o.b[lb][q >> 2] >> (4 * (q & 3)), (uint32_t)sv[lb]);
+    }
+    c[r] = (float)s;
+  }
+  return c;
+}
 // v_mfma_f32_32x32x16_{bf16,f16}: lane l holds A[i = l % 32][k = 8 (l / 32) ..+ 7], B[the same k][j = l % 32]; D as
 // v_mfma_f32_32x32x2_f32's
 template <class Load>

@@ -100,7 +100,7 @@ def test_same_results_every_time_and_on_another_stream(ex):
 
     def step():
         out = ex.expert_mlp(*leaves, k=2, activation="silu")
-        return (out,) + torch.autograd.grad(out, leaves, go)
+        return (out.detach(),) + torch.autograd.grad(out, leaves, go)
     first = step()
     again = step()
     side = torch.cuda.Stream()
@@ -122,7 +122,7 @@ def test_captured_steps(ex):
 
         def step(leaves=leaves, go=go):
             out = ex.expert_mlp(*leaves, k=2, activation="silu")
-            return (out,) + torch.autograd.grad(out, leaves, go)
+            return (out.detach(),) + torch.autograd.grad(out, leaves, go)
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):

@@ -1,0 +1,52 @@
+"""The microscaled 4-bit operators (dimo_amd/mx4.py) on the GPU against a float64 definition (tests/expert_cases.py has the
+checks and derives the tolerances)."""
+import pytest
+import torch
+
+from tests import expert_cases as cases
+
+pytestmark = pytest.mark.gpu
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from dimo_amd import experts, mx4
+    return mx4, experts
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("R,K,kind,pad", [(1, 1, "normal", 0), (5, 32, "normal", 0), (700, 100, "normal", 4), (901, 77, "borders", 3),
+                                          (4000, 64, "range", 0), (4, 96, "special", 0), (1001, 1000, "normal", 0),
+                                          (300, 2048, "borders", 8)])
+def test_quantize(ops, R, K, dtype, kind, pad):
+    cases.check_quantize(ops[0], "cuda", R, K, dtype, kind, pad, seed=R + K)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("counts,K,N,act,bias,tail,grouped", [
+    ([1], 1, 1, None, True, 0, False),
+    ([70], 96, 65, "relu", True, 0, False),
+    ([33, 0, 66], 64, 40, "silu", True, 3, True),
+    ([0, 0], 32, 8, None, False, 4, True),
+    ([5, 130], 200, 72, None, False, 0, True),
+    ([1, 0, 2, 1, 0, 4], 2048, 512, None, True, 0, True),
+    ([300, 513, 0, 129], 512, 257, None, True, 5, True),
+    ([1000], 1024, 640, "silu", True, 0, False),
+    ([3], 4096, 1000, None, True, 0, False),
+])
+def test_linear(ops, counts, K, N, dtype, act, bias, tail, grouped):
+    cases.check_mx4_linear(*ops, "cuda", counts, K, N, dtype, act, bias, tail, grouped, seed=K)
+
+
+@pytest.mark.parametrize("T,k,E,K,F", [(1, 2, 8, 512, 256), (300, 2, 4, 72, 40), (200, 4, 16, 256, 512)])
+def test_layer(ops, T, k, E, K, F):
+    cases.check_mx4_layer(*ops, "cuda", T, k, E, K, F)
+
+
+def test_nan_block_makes_its_row_nan(ops):
+    mx4, _ = ops
+    x = torch.randn(300, 256, device="cuda")
+    x[1, 40] = float("inf")
+    y = mx4.mx4_linear(mx4.quantize_mx4(x), mx4.quantize_mx4(torch.randn(136, 256, device="cuda")), out_dtype=F32)
+    assert torch.isnan(y[1]).all() and torch.isfinite(y[0]).all() and torch.isfinite(y[2:]).all()
