@@ -337,7 +337,8 @@ class _TimeNetFn(torch.autograd.Function):
 
 
 def timenet_fusable(net, pts):
-    return pts.is_cuda and len(getattr(net, "skips", [0, 0])) <= 1 and pts.dtype == torch.float32
+    return (pts.is_cuda and len(getattr(net, "skips", [0, 0])) <= 1 and pts.dtype == torch.float32
+            and getattr(net, "experts", None) is None)  # (expert blocks run through the module: dimo_amd/experts.py)
 
 
 def timenet_apply(net, pts, latent_table, times, rows=None):

@@ -43,7 +43,9 @@ def _xavier(m):
 class TimeNet(nn.Module):
     """(control point, time, latent code) -> (delta xyz [.,3], delta quaternion [.,4])."""
 
-    def __init__(self, D=8, W=256, skips=(4,), latent_code_dim=32, device=None):
+    def __init__(self, D=8, W=256, skips=(4,), latent_code_dim=32, device=None, experts=0, top_k=2):
+        """experts > 0 (no reference counterpart): a block of that many expert MLPs behind the hidden layers, of which
+        every row uses `top_k` (dimo_amd/experts.py; GPU only).  The block starts as the identity."""
         super().__init__()
         self.pts_ch, self.times_ch = 10, 6
         self.pts_emb_fn, pts_dims = get_embedder(self.pts_ch, 3)
@@ -56,6 +58,10 @@ class TimeNet(nn.Module):
         self.pts_layers = nn.Sequential(nn.Linear(W, W), nn.ReLU(), nn.Linear(W, 3))
         self.rot_layers = nn.Sequential(nn.Linear(W, W), nn.ReLU(), nn.Linear(W, 4))
         self.apply(_xavier)
+        self.experts = None
+        if experts:
+            from .experts import ExpertMLP
+            self.experts = ExpertMLP(W, experts, top_k)
         with torch.no_grad():  # zero motion / identity rotation at initialisation
             self.pts_layers[-1].weight.zero_()
             self.pts_layers[-1].bias.zero_()
@@ -81,6 +87,8 @@ class TimeNet(nn.Module):
             h = F.relu(layer(h))
             if i in self.skips:
                 h = torch.cat([emb, h], dim=-1)
+        if self.experts is not None:
+            h = self.experts(h)
         pts_t, rot_t = self.pts_layers(h), self.rot_layers(h)
         if nobatch:
             pts_t, rot_t = pts_t[0], rot_t[0]

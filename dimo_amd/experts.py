@@ -374,3 +374,61 @@ def expert_mlp(x, logits, w1, b1, w2, b2, k, activation="relu", row_mask=None):
     h = grouped_linear(x, w1, groups, b1, activation, gather=True)
     y = grouped_linear(h, w2, groups, b2)
     return combine_rows(y, groups, weights, residual=x)
+
+
+class ExpertMLP(nn.Module):
+    """h + the weighted sum of a row's k experts (each width -> hidden -> width), h [..., width].  The second products
+    start at zero, so a network that gets such a block starts as it was.  `quantized()`: the same block for evaluation
+    only, its products in microscaled 4-bit form (dimo_amd/mx4.py)."""
+
+    def __init__(self, width, num_experts, k=2, hidden=None, activation="relu", device=None):
+        super().__init__()
+        hidden = width if hidden is None else hidden
+        if not 1 <= k <= num_experts <= MAX_EXPERTS:
+            raise ValueError(f"1 <= k <= num_experts <= {MAX_EXPERTS} expected")
+        if activation not in _ACTIVATIONS:
+            raise ValueError(f"activation: one of {list(_ACTIVATIONS)} expected")
+        self.k, self.activation = k, activation
+        self.router = nn.Linear(width, num_experts, bias=False)
+        self.w1 = nn.Parameter(torch.empty(num_experts, hidden, width))
+        self.b1 = nn.Parameter(torch.zeros(num_experts, hidden))
+        self.w2 = nn.Parameter(torch.zeros(num_experts, width, hidden))
+        self.b2 = nn.Parameter(torch.zeros(num_experts, width))
+        for w in self.w1:
+            nn.init.xavier_uniform_(w)
+        if device is not None:
+            self.to(device)
+
+    def forward(self, h):
+        rows = h.reshape(-1, h.shape[-1])
+        out = expert_mlp(rows, self.router(rows), self.w1, self.b1, self.w2, self.b2, self.k, self.activation)
+        return out.view(h.shape)
+
+    def quantized(self):
+        return QuantizedExpertMLP(self)
+
+
+class QuantizedExpertMLP(nn.Module):
+    """An ExpertMLP's weights of this moment in 4-bit form, for evaluation: no parameters, no gradients; the router stays
+    as it is."""
+
+    def __init__(self, block):
+        super().__init__()
+        from .mx4 import quantize_mx4
+        self.k, self.activation, self.hidden = block.k, block.activation, block.w1.shape[1]
+        q1, q2 = quantize_mx4(block.w1), quantize_mx4(block.w2)
+        for name, t in (("router", block.router.weight.detach().clone()), ("b1", block.b1.detach().clone()),
+                        ("b2", block.b2.detach().clone()), ("w1_codes", q1.codes), ("w1_scales", q1.scales),
+                        ("w2_codes", q2.codes), ("w2_scales", q2.scales)):
+            self.register_buffer(name, t)
+
+    @torch.no_grad()
+    def forward(self, h):
+        from .mx4 import MX4, mx4_linear, quantize_mx4
+        rows = h.reshape(-1, h.shape[-1])
+        weights, experts, _ = route_topk(rows @ self.router.T, self.k)
+        groups = group_rows(experts, self.router.shape[0])
+        y = mx4_linear(quantize_mx4(rows, groups), MX4(self.w1_codes, self.w1_scales, rows.shape[1]), self.b1, groups,
+                       self.activation, rows.dtype)
+        y = mx4_linear(quantize_mx4(y), MX4(self.w2_codes, self.w2_scales, self.hidden), self.b2, groups, None, rows.dtype)
+        return combine_rows(y, groups, weights, residual=rows).view(h.shape)

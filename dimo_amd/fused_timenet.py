@@ -33,6 +33,8 @@ class FusedTimeNet:
             raise RuntimeError("FusedTimeNet needs a GPU (no CPU fallback in the product path)")
         if len(net.skips) > 1:
             raise ValueError("one skip connection supported (the reference uses skips=[4])")
+        if getattr(net, "experts", None) is not None:
+            raise ValueError("a TimeNet with experts runs through its module (dimo_amd/experts.py)")
         self.net, self.device, self.L = net, p.device, _lib.lib()
         self.layers = linear_layers(net)
         if len(self.layers) > MAX_LAYERS:

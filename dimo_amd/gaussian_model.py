@@ -69,7 +69,7 @@ class BasicPointCloud(NamedTuple):
 
 class GaussianModel(DensifyMixin, PlyMixin):
     def __init__(self, sh_degree: int, num_latent_code: int = 1, latent_code_dim: int = 32, vae_latent: bool = False,
-                 device=None, dist2_fn=None):
+                 device=None, dist2_fn=None, timenet_experts: int = 0, timenet_top_k: int = 2):
         self.device = torch.device(device if device is not None else ("cuda" if torch.cuda.is_available() else "cpu"))
         self.active_sh_degree = 0
         self.max_sh_degree = sh_degree
@@ -87,7 +87,8 @@ class GaussianModel(DensifyMixin, PlyMixin):
             self._log_var = nn.Parameter(torch.zeros(num_latent_code, latent_code_dim, device=self.device))
         else:
             self._latent_codes = nn.Parameter(torch.randn(num_latent_code, latent_code_dim, device=self.device))
-        self._timenet = TimeNet(latent_code_dim=latent_code_dim, device=self.device)
+        self._timenet = TimeNet(latent_code_dim=latent_code_dim, device=self.device, experts=timenet_experts,
+                                top_k=timenet_top_k)
         self.neighbor_dists = self.neighbor_indices = None
         self.flat_params = self.flat_grads = None
         self._dist2_fn = dist2_fn  # defaults to the HIP distCUDA2 drop-in (no CPU fallback)

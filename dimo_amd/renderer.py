@@ -38,13 +38,14 @@ def _ball_points(n, radius, rng):
 class Renderer:
     def __init__(self, sh_degree=3, white_background=True, radius=1, delta_t=1 / 32, num_latent_code=1,
                  latent_code_dim=32, add_normal=False, vae_latent=False, device=None, rasterizer_factory=None,
-                 capacity=None, dist2_fn=None, batch_renders=True):
+                 capacity=None, dist2_fn=None, batch_renders=True, timenet_experts=0, timenet_top_k=2):
         self.sh_degree = sh_degree
         self.white_background = white_background
         self.radius = radius
         self.gaussians = GaussianModel(sh_degree=sh_degree, num_latent_code=num_latent_code,
                                        latent_code_dim=latent_code_dim, vae_latent=vae_latent, device=device,
-                                       dist2_fn=dist2_fn)
+                                       dist2_fn=dist2_fn, timenet_experts=timenet_experts,
+                                       timenet_top_k=timenet_top_k)
         self.device = self.gaussians.device
         self.bg_color = torch.tensor([1, 1, 1] if white_background else [0, 0, 0], dtype=torch.float32,
                                      device=self.device)

@@ -686,9 +686,9 @@ class Trainer:
                 self.find_knn(k=4)
         ex.set_common(g, self.renderer.bg_color, self.renderer.add_normal, stage1=s1)
         self._mark("start")
-        fused_tn = (self.fused_timenet or s1) and len(g._timenet.skips) <= 1
+        fused_tn = (self.fused_timenet or s1) and len(g._timenet.skips) <= 1 and g._timenet.experts is None
         if s1 and not fused_tn:
-            raise RuntimeError("the stage-s1 direct pipeline needs the fused TimeNet (one skip connection)")
+            raise RuntimeError("the stage-s1 direct pipeline needs the fused TimeNet (one skip connection, no experts)")
         if fused_tn:
             dxyz_c, dquat_c, pair_of, lat = self._fused_deform(mine)
         else:

@@ -450,3 +450,76 @@ def check_mx4_layer(mx4, ex, device, T, k, E, K, F, seed=0):
         ref[t] += W[t, place % k] * (W2[q] @ hq)
         slack[t] += W[t, place % k] * product_slack(F, W2[q].abs() @ hq.abs()) * 2 + 2.0 ** -20 * (W2[q] @ hq).abs() * W[t, place % k]
     near(out, ref, torch.float32, slack + 2.0 ** -22 * ref.abs(), "out")
+
+
+def expert_block_reference(block, h):
+    """ExpertMLP in float64 on the CPU: h + the weighted experts' rows."""
+    w, e, _ = route_reference(h @ block["router.weight"].T, block["k"])
+    out = h
+    for j in range(block["k"]):
+        i = e[:, j].long().clamp_min(0)
+        a = activation64(torch.einsum("tfk,tk->tf", block["w1"][i], h) + block["b1"][i], block["activation"])
+        out = out + w[:, j:j + 1] * (torch.einsum("tkf,tf->tk", block["w2"][i], a) + block["b2"][i])
+    return out
+
+
+def check_timenet_with_experts(device, W, P, M, E, k, seed=0):
+    """deform.TimeNet(experts=E) against its own module in float64 with the block spelled out: outputs and the gradients
+    of every parameter.  silu instead of relu inside the block and no relu kinks from it; the rows whose hidden relu
+    inputs lie next to zero are left out of the comparison, as in tests/test_gpu_timenet.py."""
+    import copy
+
+    from dimo_amd.deform import TimeNet
+    torch.manual_seed(seed)
+    net = TimeNet(D=3, W=W, skips=(1,), latent_code_dim=8, experts=E, top_k=k)
+    net.experts.activation = "silu"
+    g = torch.Generator().manual_seed(seed + 1)
+    with torch.no_grad():
+        for p in (net.experts.w2, net.experts.b1, net.experts.b2):
+            p.copy_(torch.randn(p.shape, generator=g) * 0.1)
+        for lin in (net.pts_layers[2], net.rot_layers[2]):
+            lin.weight.copy_(0.1 * torch.randn(lin.weight.shape, generator=g))
+    n64 = copy.deepcopy(net).double()
+    block = dict(n64.experts.named_parameters(), k=k, activation="silu")
+    n64.experts.forward = lambda h: expert_block_reference(block, h.reshape(-1, W)).view(h.shape)
+    pts, t = torch.rand(M, 3, generator=g) - 0.5, torch.rand(P, 1, 1, generator=g).expand(P, M, 1)
+    lat = torch.randn(P, 1, 8, generator=g).expand(P, M, 8)
+    gx, gr = torch.randn(P, M, 3, generator=g), torch.randn(P, M, 4, generator=g)
+    small = []
+    hooks = [lin.register_forward_hook(lambda _m, _i, out: small.append(out.detach().abs().amin(-1)))
+             for lin in list(n64.deformnet) + [n64.pts_layers[0], n64.rot_layers[0]]]
+    dx64, dr64 = n64(pts[None].double(), t.double(), lat.double(), t_apply=True)
+    for h in hooks:
+        h.remove()
+    keep = (torch.stack(small).amin(0) > 2e-5)[..., None]
+    gx, gr = gx * keep, gr * keep
+    ((dx64 * gx.double()).sum() + (dr64 * gr.double()).sum()).backward()
+    net = net.to(device)
+    dx, dr = net(pts[None].to(device), t.to(device), lat.to(device), t_apply=True)
+    ((dx * gx.to(device)).sum() + (dr * gr.to(device)).sum()).backward()
+    assert torch.allclose(dx.detach().cpu().double(), dx64.detach(), rtol=0, atol=1e-4 * float(dx64.abs().max()))
+    assert torch.allclose(dr.detach().cpu().double(), dr64.detach(), rtol=0, atol=1e-4 * float(dr64.abs().max()))
+    ref = dict(n64.named_parameters())
+    for name, p in net.named_parameters():
+        r = ref[name].grad
+        assert torch.allclose(p.grad.cpu().double(), r, rtol=0, atol=1e-4 * max(float(r.abs().max()), 1e-6)), name
+
+
+def check_quantized_block(ex, mx4, device, T, W, E, k, seed=0):
+    """ExpertMLP.quantized(): what its own 4-bit operators give, and near the block it was made from (each product's
+    operands rounded by at most 2^-2 relative: the block's contribution stays within half of its size)."""
+    torch.manual_seed(seed)
+    block = ex.ExpertMLP(W, E, k, device=device)
+    with torch.no_grad():
+        block.w2.copy_(torch.randn(block.w2.shape) / math.sqrt(W))
+    h = torch.randn(T, W).to(device)
+    with torch.no_grad():
+        full, q = block(h), block.quantized()
+        out = q(h)
+        weights, experts, _ = ex.route_topk(block.router(h), k)
+        groups = ex.group_rows(experts, E)
+        y = mx4.mx4_linear(mx4.quantize_mx4(h, groups), mx4.quantize_mx4(block.w1), block.b1, groups, "relu", torch.float32)
+        y = mx4.mx4_linear(mx4.quantize_mx4(y), mx4.quantize_mx4(block.w2), block.b2, groups, None, torch.float32)
+        assert torch.equal(out, ex.combine_rows(y, groups, weights, h))
+    assert not list(q.parameters())
+    assert float((out - full).norm()) <= 0.5 * float((full - h).norm())

@@ -150,3 +150,31 @@ def test_c_entry_points_refuse():
     assert L.dimo_combine_rows_forward(4, 2, 8, 8, 0, 1, 7, None, 1, None, 0, 1, None) == -1
     assert L.dimo_combine_rows_backward(4, 2, 8, 9, 3, 0, 1, 8, 1, 8, 1, 1, 1, 1, 1, None) == -1
     assert L.dimo_route_topk_forward(0, 6, 2, 0, None, 6, None, 1, None, None, None, None, 0, None) == 0
+
+
+def test_timenet_with_experts(emulated):
+    cases.check_timenet_with_experts("cpu", 32, 2, 9, 4, 2)
+
+
+def test_quantized_block(emulated, monkeypatch):
+    from dimo_amd import mx4
+    expert_emulation.use(monkeypatch, mx4)
+    cases.check_quantized_block(ex, mx4, "cpu", 40, 64, 4, 2)
+
+
+def test_timenet_keeps_its_state_dict_without_experts():
+    from dimo_amd.deform import TimeNet
+    assert not [k for k in TimeNet(D=2, W=8).state_dict() if "experts" in k]
+    assert [k for k in TimeNet(D=2, W=8, experts=2, top_k=1).state_dict() if "experts" in k]
+
+
+def test_fused_timenet_refuses_experts():
+    from dimo_amd.batched_render import timenet_fusable
+    from dimo_amd.deform import TimeNet
+    net = TimeNet(D=2, W=8, skips=(), experts=2, top_k=1)
+
+    class OnGpu:
+        is_cuda, dtype = True, F32
+    assert not timenet_fusable(net, OnGpu)
+    net.experts = None
+    assert timenet_fusable(net, OnGpu)

@@ -144,3 +144,37 @@ def test_captured_steps(ex):
         for _, _, step, outs in graphs:
             for got, ref in zip(outs, step()):
                 assert torch.equal(got, ref)
+
+
+@pytest.mark.parametrize("W,P,M,E,k", [(64, 2, 70, 4, 2), (256, 4, 128, 8, 2)])
+def test_timenet_with_experts(W, P, M, E, k):
+    cases.check_timenet_with_experts("cuda", W, P, M, E, k)
+
+
+def test_quantized_block(ex):
+    from dimo_amd import mx4
+    cases.check_quantized_block(ex, mx4, "cuda", 300, 256, 8, 2)
+
+
+@pytest.mark.parametrize("direct", [True, False])
+def test_train_step_with_experts(direct):
+    """The trainer's own step with an expert block in the deformation network: every parameter of the block moves once
+    its second products have left zero."""
+    from dimo_amd.rasterizer import CapacityPolicy
+    from dimo_amd.renderer import Renderer
+    from dimo_amd.synth import init_synthetic_model
+    from dimo_amd.trainer import TrainConfig, Trainer
+    cfg = TrainConfig(num_pts=2000, num_cpts=64, num_motions=4, resolution=128, motions_per_step=2, views_per_step=1,
+                      frames_per_step=2)
+    rd = Renderer(sh_degree=0, num_latent_code=4, add_normal=True, device="cuda", capacity=CapacityPolicy(initial=1 << 18),
+                  timenet_experts=4, timenet_top_k=2)
+    init_synthetic_model(rd, cfg.num_pts, cfg.num_cpts, seed=0, num_latent=4)
+    tr = Trainer(cfg, rd, direct=direct)
+    block = rd.gaussians._timenet.experts
+    before = {n: p.detach().clone() for n, p in block.named_parameters()}
+    for _ in range(3):
+        tr.train_step()
+    torch.cuda.synchronize()
+    assert torch.isfinite(rd.gaussians.flat_params).all()
+    for n, p in block.named_parameters():
+        assert not torch.equal(before[n], p.detach()), n
