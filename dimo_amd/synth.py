@@ -65,10 +65,15 @@ def init_synthetic_model(renderer, num_pts, num_cpts, seed=0, regime="trained", 
             if isinstance(m, nn.Linear):
                 w = torch.empty(m.weight.shape)
                 nn.init.xavier_uniform_(w, gain=1, generator=tg)
-                bound = 1.0 / math.sqrt(m.in_features)
-                b = (torch.rand(m.bias.shape, generator=tg) * 2 - 1) * bound
                 m.weight.copy_(w)
-                m.bias.copy_(b)
+                if m.bias is not None:
+                    bound = 1.0 / math.sqrt(m.in_features)
+                    m.bias.copy_((torch.rand(m.bias.shape, generator=tg) * 2 - 1) * bound)
+        if g._timenet.experts is not None:  # (first products; the second ones start at zero)
+            w1 = torch.empty(g._timenet.experts.w1.shape)
+            for w in w1:
+                nn.init.xavier_uniform_(w, generator=tg)
+            g._timenet.experts.w1.copy_(w1)
         g._timenet.pts_layers[-1].bias.zero_()
         g._timenet.rot_layers[-1].bias.copy_(torch.tensor([1.0, 0.0, 0.0, 0.0]))
         # the reference zero-inits the heads (no motion); use small random heads so deformation is non-trivial
