@@ -96,7 +96,9 @@ _SIGNATURES = {
     "dimo_grouped_linear_forward": (C.c_int, [C.c_int] * 5 + [c_ptr, C.c_int64, C.c_int] + [c_ptr] * 4 + [C.c_int]
                                     + [c_ptr] * 3),
     "dimo_grouped_linear_dgrad": (C.c_int, [C.c_int] * 5 + [c_ptr] * 5),
-    "dimo_grouped_linear_wgrad": (C.c_int, [C.c_int] * 5 + [c_ptr, c_ptr, C.c_int64, C.c_int] + [c_ptr] * 5),
+    "dimo_grouped_linear_wgrad_workspace_bytes": (C.c_size_t, [C.c_int] * 5),
+    "dimo_grouped_linear_wgrad": (C.c_int, [C.c_int] * 5 + [c_ptr, c_ptr, C.c_int64, C.c_int] + [c_ptr] * 5
+                                  + [C.c_size_t, c_ptr]),
     "dimo_activation_backward": (C.c_int, [C.c_int, C.c_int, C.c_int64] + [c_ptr] * 4),
     "dimo_combine_rows_forward": (C.c_int, [C.c_int] * 3 + [C.c_int64, C.c_int, c_ptr, C.c_int64] + [c_ptr] * 3
                                   + [C.c_int64, c_ptr, c_ptr]),

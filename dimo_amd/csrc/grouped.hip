@@ -10,28 +10,12 @@
 // products (matrix_ops.hpp).
 #include <hip/hip_runtime.h>
 
-#include "matrix_ops.hpp"
 #include "row_tiles.hpp"
+#include "tile_product.hpp"
 
 using namespace dimo;
 
 namespace {
-
-// ---- the general kernel: any size, stride and alignment ----------------------------------------------------------
-// 64 x 64 outputs per workgroup, 32 x 32 per wave, 32 deep stages through registers into LDS as [row][k] (40 elements
-// apart: sixteen-byte reads of 32 consecutive rows then spread over all banks).
-constexpr int GM = 64, GN = 64, GK = 32, GLD = 40;
-
-template <class T>
-struct Planes {
-  static constexpr int N = 1;
-  typedef T Tag;
-};
-template <>
-struct Planes<F32> {
-  static constexpr int N = 3;
-  typedef BF16 Tag;
-};
 
 struct GroupedArgs {
   int R, E, K, N;          // rows, experts, width of x, width of y
@@ -46,169 +30,252 @@ struct GroupedArgs {
   const void *g;           // [R, N] (dgrad, wgrad)
   void *gx;                // [R, K]
   void *gw, *gb;           // [E, N, K], [E, N] or null
+  int wide;                // four neighbouring outputs of a row may be written at once
+  int split_rows, chunks;  // wgrad: > 0: partial sums over that many rows at a time, `chunks` of them at most
+  float *partial;          // [chunks, N, K], then [chunks, N]
 };
 
 __device__ __forceinline__ int64_t source_row(const GroupedArgs &a, int r) {
   return a.places > 0 ? a.order[r] / a.places : r;
 }
 
-// eight elements of an operand's stage as fp32, `ok` of them inside
-template <class T>
-__device__ __forceinline__ void stage_elements(const typename T::store *p, int ok, bool wide, typename T::store (&v)[8]) {
-  if (wide && ok >= 8) {
-    constexpr int Q = sizeof(typename T::store) == 4 ? 2 : 1;
-    uint4 q[Q];
-#pragma unroll
-    for (int i = 0; i < Q; ++i) q[i] = reinterpret_cast<const uint4 *>(p)[i];
-    __builtin_memcpy(v, q, sizeof(v));
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = i < ok ? p[i] : typename T::store(0);
-}
-
-template <class T>
-__device__ __forceinline__ void split_store(uint16_t (*S)[GM][GLD], int i, int k, typename T::store v) {
-  if constexpr (Planes<T>::N == 3) {
-    const Split3 s = split3(v);
-    S[0][i][k] = s.hi, S[1][i][k] = s.mid, S[2][i][k] = s.lo;
-  } else {
-    S[0][i][k] = v;
-  }
-}
-
-// k contiguous: thread t brings row t / 4, eight k from 8 (t % 4);  row contiguous (transposed on its way into LDS):
-// k = t / 8, eight rows from 8 (t % 8)
-template <class T, bool KC>
-__device__ __forceinline__ void stage_store(uint16_t (*S)[GM][GLD], const typename T::store (&v)[8]) {
-  const int t = threadIdx.x;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (KC)
-      split_store<T>(S, t >> 2, 8 * (t & 3) + i, v[i]);
-    else
-      split_store<T>(S, 8 * (t & 7) + i, t >> 3, v[i]);
-  }
-}
-
-template <class T>
-__device__ __forceinline__ void stage_multiply(uint16_t (*A)[GM][GLD], uint16_t (*B)[GN][GLD], f32x16 &acc, f32x16 *ones_acc) {
-  constexpr int P = Planes<T>::N;
-  typedef typename Planes<T>::Tag Tag;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int i = (wave >> 1) * 32 + (lane & 31), j = (wave & 1) * 32 + (lane & 31);
-#pragma unroll
-  for (int ks = 0; ks < GK; ks += 16) {
-    const int k = ks + 8 * (lane >> 5);
-    uint4 a[P], b[P];
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-      a[p] = *reinterpret_cast<const uint4 *>(&A[p][i][k]);
-      b[p] = *reinterpret_cast<const uint4 *>(&B[p][j][k]);
-    }
-#pragma unroll
-    for (int d = P - 1; d >= 0; --d)  // the smallest products first
-#pragma unroll
-      for (int p = 0; p <= d; ++p) acc = mfma_32x32x16(Tag{}, a[p], b[d - p], acc);
-    if (ones_acc) {
-      const uint32_t w = (uint32_t)Tag::save(1.0f) * 0x10001u;
-      const uint4 ones = make_uint4(w, w, w, w);
-#pragma unroll
-      for (int p = P - 1; p >= 0; --p) *ones_acc = mfma_32x32x16(Tag{}, a[p], ones, *ones_acc);
-    }
-  }
-}
-
 enum { FORWARD = 0, DGRAD = 1 };
 
-template <class T, int MODE>
-__global__ __launch_bounds__(256) void grouped_rows_general_kernel(GroupedArgs a, bool wide_a, bool wide_b) {
+// TJ rows x TI columns per workgroup, WJ x WI waves.
+template <int TJ_, int TI_, int WJ_, int WI_>
+struct Tile {
+  static constexpr int TJ = TJ_, TI = TI_, WJ = WJ_, WI = WI_, THREADS = 64 * WJ * WI;
+  static constexpr int NJ = TJ / WJ / 32, NI = TI / WI / 32;
+};
+
+// The stages of a product, one after the other.  DIRECT: two LDS buffers, the next stage's loads go straight into the one
+// while the other is multiplied, one barrier per stage.  Otherwise (fp32, odd ends, odd alignment): the next stage waits in
+// registers, one buffer, two barriers.
+template <class T, class C, bool ORDER_J, bool ORDER_I, bool DIRECT, bool SUMS, class RowJ, class RowI>
+__device__ __forceinline__ void run_stages(const Staging<T, ORDER_J, C::TJ, Planes<T>::DEPTH, C::THREADS> &sj,
+                                           const Staging<T, ORDER_I, C::TI, Planes<T>::DEPTH, C::THREADS> &si, int begin,
+                                           int end, RowJ &&row_j, RowI &&row_i, Accumulators<C::NJ, C::NI> &acc,
+                                           bool with_sums) {
+  constexpr int BK = Planes<T>::DEPTH, P = Planes<T>::N;
+  const int wave = threadIdx.x >> 6;
+  const int j0 = (wave / C::WI) * 32 * C::NJ, i0 = (wave % C::WI) * 32 * C::NI;
+  if constexpr (DIRECT) {
+    // (separate arrays: the compiler then knows that what is on its way into one is not what is read from the other)
+    __shared__ __attribute__((aligned(1024))) uint16_t SJ0[C::TJ * BK], SI0[C::TI * BK], SJ1[C::TJ * BK], SI1[C::TI * BK];
+    sj.load_direct(SJ0, begin, end, row_j);
+    si.load_direct(SI0, begin, end, row_i);
+    for (int k0 = begin;; k0 += 2 * BK) {
+      __syncthreads();  // this stage is there, and everyone is done with the other buffer
+      if (k0 + BK < end) {
+        sj.load_direct(SJ1, k0 + BK, end, row_j);
+        si.load_direct(SI1, k0 + BK, end, row_i);
+      }
+      __builtin_amdgcn_sched_barrier(0);  // (the loads first: they have this stage's products to arrive under)
+      multiply_stage<T, ORDER_J, ORDER_I, C::TJ, C::TI, BK, C::NJ, C::NI, SUMS>(SJ0, SI0, j0, i0, acc, with_sums);
+      if (k0 + BK >= end) break;
+      __syncthreads();
+      if (k0 + 2 * BK < end) {
+        sj.load_direct(SJ0, k0 + 2 * BK, end, row_j);
+        si.load_direct(SI0, k0 + 2 * BK, end, row_i);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      multiply_stage<T, ORDER_J, ORDER_I, C::TJ, C::TI, BK, C::NJ, C::NI, SUMS>(SJ1, SI1, j0, i0, acc, with_sums);
+      if (k0 + 2 * BK >= end) break;
+    }
+  } else {
+    typedef Staging<T, ORDER_J, C::TJ, BK, C::THREADS> LJ;
+    typedef Staging<T, ORDER_I, C::TI, BK, C::THREADS> LI;
+    __shared__ __attribute__((aligned(1024))) uint16_t SJ[P * C::TJ * BK], SI[P * C::TI * BK];
+    typename LJ::Chunk vj[LJ::CHUNKS];
+    typename LI::Chunk vi[LI::CHUNKS];
+    sj.load(vj, begin, end, row_j);
+    si.load(vi, begin, end, row_i);
+    for (int k0 = begin; k0 < end; k0 += BK) {
+      __syncthreads();  // everyone is done with the last stage
+      sj.store(vj, SJ, C::TJ * BK);
+      si.store(vi, SI, C::TI * BK);
+      __syncthreads();
+      if (k0 + BK < end) {
+        sj.load(vj, k0 + BK, end, row_j);
+        si.load(vi, k0 + BK, end, row_i);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      multiply_stage<T, ORDER_J, ORDER_I, C::TJ, C::TI, BK, C::NJ, C::NI, SUMS>(SJ, SI, j0, i0, acc, with_sums);
+    }
+  }
+}
+
+// For every quad of the wave's outputs: column(c) once per quad of columns, then f(row of the tile, column of the tile, the
+// quad's sums, what column(c) gave) for its rows.
+template <class C, class G, class F>
+__device__ __forceinline__ void for_quads(const Accumulators<C::NJ, C::NI> &acc, G &&column, F &&f) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int j0 = (wave / C::WI) * 32 * C::NJ + (lane & 31), i0 = (wave % C::WI) * 32 * C::NI + 4 * (lane >> 5);
+#pragma unroll
+  for (int i = 0; i < C::NI; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float4 more = column(i0 + 32 * i + 8 * q);
+#pragma unroll
+      for (int j = 0; j < C::NJ; ++j) {
+        const float v[4] = {acc.v[j][i][4 * q] + more.x, acc.v[j][i][4 * q + 1] + more.y, acc.v[j][i][4 * q + 2] + more.z,
+                            acc.v[j][i][4 * q + 3] + more.w};
+        f(j0 + 32 * j, i0 + 32 * i + 8 * q, v);
+      }
+      __builtin_amdgcn_sched_barrier(0);  // (quad by quad: all of them at once would not fit the registers)
+    }
+}
+
+// four elements of a row from column c on, `columns` exist
+template <class T>
+__device__ __forceinline__ void store_quad(typename T::store *row, int c, int columns, bool wide, const float (&v)[4]) {
   typedef typename T::store E;
-  __shared__ __attribute__((aligned(16))) uint16_t As[Planes<T>::N][GM][GLD], Bs[Planes<T>::N][GN][GLD];
-  const RowTile tile = find_row_tile(a.offsets, a.E, a.R, GM, (int)blockIdx.x);
+  if (wide && c + 4 <= columns) {
+    if constexpr (sizeof(E) == 4)
+      *reinterpret_cast<float4 *>(row + c) = make_float4(v[0], v[1], v[2], v[3]);
+    else
+      *reinterpret_cast<uint2 *>(row + c) = make_uint2((uint32_t)T::save(v[0]) | (uint32_t)T::save(v[1]) << 16,
+                                                       (uint32_t)T::save(v[2]) | (uint32_t)T::save(v[3]) << 16);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (c + e < columns) row[c + e] = T::save(v[e]);
+  }
+}
+
+template <class T, int MODE, bool DIRECT, class C>
+__global__ __launch_bounds__(C::THREADS, 2) void grouped_rows_kernel(GroupedArgs a) {
+  typedef typename T::store E;
+  constexpr int BK = Planes<T>::DEPTH;
+  const int columns = MODE == FORWARD ? a.N : a.K, reduction = MODE == FORWARD ? a.K : a.N;
+  int ct = 0;
+  const RowTile tile = find_row_tile(a.offsets, a.E, a.R, C::TJ, (columns + C::TI - 1) / C::TI, (int)blockIdx.x, &ct);
   if (tile.expert < 0) return;
-  const int cols = MODE == FORWARD ? a.N : a.K, red = MODE == FORWARD ? a.K : a.N;
-  const int n0 = blockIdx.y * GN, t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int c0 = ct * C::TI;
   E *out = static_cast<E *>(MODE == FORWARD ? a.y : a.gx);
   if (tile.expert == a.E) {  // behind the last group
-    for (int i = t; i < GM * GN; i += 256) {
-      const int r = tile.begin + i / GN, c = n0 + i % GN;
-      if (r < tile.end && c < cols) {
-        out[(int64_t)r * cols + c] = E(0);
-        if (MODE == FORWARD && a.z) static_cast<E *>(a.z)[(int64_t)r * cols + c] = E(0);
+    for (int i = threadIdx.x; i < C::TJ * C::TI; i += C::THREADS) {
+      const int r = tile.begin + i / C::TI, c = c0 + i % C::TI;
+      if (r < tile.end && c < columns) {
+        out[(int64_t)r * columns + c] = E(0);
+        if (MODE == FORWARD && a.z) static_cast<E *>(a.z)[(int64_t)r * columns + c] = E(0);
       }
     }
     return;
   }
   const E *W = static_cast<const E *>(a.w) + (int64_t)tile.expert * a.N * a.K;
-  // this thread's row of A (k contiguous)
-  const int ra = min(tile.begin + (t >> 2), tile.end - 1);
-  const E *A = MODE == FORWARD ? static_cast<const E *>(a.x) + source_row(a, ra) * a.ldx
-                               : static_cast<const E *>(a.g) + (int64_t)ra * a.N;
-  const int ka = 8 * (t & 3);
-  f32x16 acc;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-  for (int k0 = 0; k0 < red; k0 += GK) {
-    E va[8], vb[8];
-    stage_elements<T>(A + min(k0 + ka, red), red - k0 - ka, wide_a, va);
-    if (MODE == FORWARD) {  // row n0 + t / 4 of W
-      const int n = n0 + (t >> 2);
-      stage_elements<T>(W + (int64_t)min(n, a.N - 1) * a.K + min(k0 + ka, red), n < a.N ? red - k0 - ka : 0, wide_b, vb);
-    } else {  // row k0 + t / 8 of W, eight columns
-      const int n = k0 + (t >> 3), c = n0 + 8 * (t & 7);
-      stage_elements<T>(W + (int64_t)min(n, a.N - 1) * a.K + min(c, a.K), n < a.N ? a.K - c : 0, wide_b, vb);
+  Staging<T, LINES, C::TJ, BK, C::THREADS> sj;
+  sj.init_lines([&](int i) {
+    const int r = min(tile.begin + i, tile.end - 1);
+    return MODE == FORWARD ? static_cast<const E *>(a.x) + source_row(a, r) * a.ldx
+                           : static_cast<const E *>(a.g) + (int64_t)r * a.N;
+  });
+  Staging<T, MODE == FORWARD ? LINES : COLUMNS, C::TI, BK, C::THREADS> si;
+  if constexpr (MODE == FORWARD)
+    si.init_lines([&](int i) { return W + (int64_t)min(c0 + i, a.N - 1) * a.K; });
+  else
+    si.init_columns(W + c0, a.K, a.K - c0);
+  Accumulators<C::NJ, C::NI> acc;
+  acc.clear();
+  const auto same = [](int r) { return (int64_t)r; };
+  run_stages<T, C, LINES, MODE == FORWARD ? LINES : COLUMNS, DIRECT, false>(sj, si, 0, reduction, same, same, acc, false);
+  const E *bias = MODE == FORWARD && a.bias ? static_cast<const E *>(a.bias) + (int64_t)tile.expert * a.N : nullptr;
+  const auto columns_bias = [&](int i) {
+    const int c = c0 + i;
+    if (!bias || c >= columns) return make_float4(0.f, 0.f, 0.f, 0.f);
+    return make_float4(T::load(bias[c]), T::load(bias[min(c + 1, columns - 1)]), T::load(bias[min(c + 2, columns - 1)]),
+                       T::load(bias[min(c + 3, columns - 1)]));
+  };
+  for_quads<C>(acc, columns_bias, [&](int j, int i, const float (&s)[4]) {
+    const int r = tile.begin + j, c = c0 + i;
+    if (r >= tile.end || c >= columns) return;
+    if constexpr (MODE == FORWARD) {
+      if (a.z) store_quad<T>(static_cast<E *>(a.z) + (int64_t)r * columns, c, columns, a.wide, s);
+      const float v[4] = {activate(s[0], a.act), activate(s[1], a.act), activate(s[2], a.act), activate(s[3], a.act)};
+      store_quad<T>(out + (int64_t)r * columns, c, columns, a.wide, v);
+    } else {
+      store_quad<T>(out + (int64_t)r * columns, c, columns, a.wide, s);
     }
-    __syncthreads();
-    stage_store<T, true>(As, va);
-    stage_store<T, MODE == FORWARD>(Bs, vb);
-    __syncthreads();
-    stage_multiply<T>(As, Bs, acc, nullptr);
+  });
+}
+
+// gW[e]: rows n (from g) x columns k (from x), summed over the group's rows -- all of them, or split_rows of them into a
+// slice of `partial` (few experts with narrow weights would leave most of the chip idle otherwise; the slices are summed
+// in their order by the next kernel, so the result does not depend on the schedule)
+template <class T, bool DIRECT, class C>
+__global__ __launch_bounds__(C::THREADS, 2) void grouped_wgrad_kernel(GroupedArgs a) {
+  typedef typename T::store E;
+  constexpr int BK = Planes<T>::DEPTH;
+  const int tiles_k = (a.K + C::TI - 1) / C::TI, tiles_n = (a.N + C::TJ - 1) / C::TJ;
+  int expert, begin, end, chunk = 0, block;
+  if (a.split_rows) {
+    int column = 0;
+    const RowTile t = find_row_tile(a.offsets, a.E, a.R, a.split_rows, tiles_k * tiles_n, (int)blockIdx.x, &column);
+    if (t.expert < 0 || t.expert == a.E || t.number >= a.chunks) return;
+    expert = t.expert, begin = t.begin, end = t.end, chunk = t.number, block = column;
+  } else {
+    expert = blockIdx.x / (tiles_k * tiles_n), block = blockIdx.x % (tiles_k * tiles_n);
+    begin = clamp_offset(a.offsets, expert, a.R), end = max(begin, clamp_offset(a.offsets, expert + 1, a.R));
   }
-  const int c = n0 + (wave & 1) * 32 + (lane & 31);
-  if (c >= cols) return;
-  const float bias = MODE == FORWARD && a.bias ? T::load(static_cast<const E *>(a.bias)[(int64_t)tile.expert * a.N + c]) : 0.f;
+  const int n0 = block / tiles_k * C::TJ, k0 = block % tiles_k * C::TI;
+  Staging<T, COLUMNS, C::TJ, BK, C::THREADS> sj;
+  Staging<T, COLUMNS, C::TI, BK, C::THREADS> si;
+  sj.init_columns(static_cast<const E *>(a.g) + n0, a.N, a.N - n0);
+  si.init_columns(static_cast<const E *>(a.x) + k0, a.ldx, a.K - k0);
+  Accumulators<C::NJ, C::NI> acc;
+  acc.clear();
+  const bool sums = a.gb && k0 == 0 && (int)(threadIdx.x >> 6) % C::WI == 0;  // (one of the waves that read a row)
+  if (begin < end)
+    run_stages<T, C, COLUMNS, COLUMNS, DIRECT, true>(sj, si, begin, end, [](int r) { return (int64_t)r; },
+                                                     [&](int r) { return source_row(a, r); }, acc, sums);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float *pw = a.partial + (int64_t)chunk * a.N * a.K, *pb = a.partial + (int64_t)a.chunks * a.N * a.K + (int64_t)chunk * a.N;
+  E *gw = static_cast<E *>(a.gw) + (int64_t)expert * a.N * a.K, *gb = static_cast<E *>(a.gb) + (int64_t)expert * a.N;
+  for_quads<C>(acc, [](int) { return make_float4(0.f, 0.f, 0.f, 0.f); }, [&](int j, int i, const float (&v)[4]) {
+    const int n = n0 + j, k = k0 + i;
+    if (n >= a.N || k >= a.K) return;
+    if (a.split_rows)
+      store_quad<F32>(pw + (int64_t)n * a.K, k, a.K, a.wide, v);
+    else
+      store_quad<T>(gw + (int64_t)n * a.K, k, a.K, a.wide, v);
+  });
+  if (sums) {
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int row = tile.begin + (wave >> 1) * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-    if (row >= tile.end) continue;
-    const float v = acc[r] + bias;
-    if (MODE == FORWARD && a.z) static_cast<E *>(a.z)[(int64_t)row * cols + c] = T::save(v);
-    out[(int64_t)row * cols + c] = T::save(MODE == FORWARD ? activate(v, a.act) : v);
+    for (int j = 0; j < C::NJ; ++j) {
+      const float v = acc.sums[j] + __shfl_xor(acc.sums[j], 32);
+      const int n = n0 + (wave / C::WI) * 32 * C::NJ + 32 * j + lane;
+      if (lane >= 32 || n >= a.N) continue;
+      if (a.split_rows)
+        pb[n] = v;
+      else
+        gb[n] = T::save(v);
+    }
   }
 }
 
-// one workgroup per 64 x 64 block of an expert's gradient, the rows of the group one stage after the other
+// gW[e], gb[e] = the sums of the expert's slices, in their order (zeros without any)
 template <class T>
-__global__ __launch_bounds__(256) void grouped_wgrad_general_kernel(GroupedArgs a, bool wide_a, bool wide_b) {
+__global__ __launch_bounds__(256) void grouped_wgrad_sum_kernel(GroupedArgs a) {
   typedef typename T::store E;
-  __shared__ __attribute__((aligned(16))) uint16_t As[Planes<T>::N][GM][GLD], Bs[Planes<T>::N][GN][GLD];
-  const int e = blockIdx.y, tiles_k = (a.K + GN - 1) / GN;
-  const int n0 = (blockIdx.x / tiles_k) * GM, k0 = (blockIdx.x % tiles_k) * GN;
-  const int begin = clamp_offset(a.offsets, e, a.R), end = max(begin, clamp_offset(a.offsets, e + 1, a.R));
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  f32x16 acc, sums;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) acc[i] = 0.f, sums[i] = 0.f;
-  const bool with_bias = a.gb && k0 == 0;
-  for (int r0 = begin; r0 < end; r0 += GK) {
-    const int r = r0 + (t >> 3), c = 8 * (t & 7), rc = min(r, end - 1);
-    E va[8], vb[8];
-    stage_elements<T>(static_cast<const E *>(a.g) + (int64_t)rc * a.N + min(n0 + c, a.N), r < end ? a.N - n0 - c : 0, wide_a, va);
-    stage_elements<T>(static_cast<const E *>(a.x) + source_row(a, rc) * a.ldx + min(k0 + c, a.K), r < end ? a.K - k0 - c : 0, wide_b, vb);
-    __syncthreads();
-    stage_store<T, false>(As, va);
-    stage_store<T, false>(Bs, vb);
-    __syncthreads();
-    stage_multiply<T>(As, Bs, acc, with_bias ? &sums : nullptr);
+  const int e = blockIdx.y;
+  int first = 0, count = 0;  // the expert's chunks: those of the experts before it come first
+  for (int i = 0; i <= e; ++i) {
+    const int lo = clamp_offset(a.offsets, i, a.R), hi = max(lo, clamp_offset(a.offsets, i + 1, a.R));
+    first += count;
+    count = (hi - lo + a.split_rows - 1) / a.split_rows;
   }
-  const int k = k0 + (wave & 1) * 32 + (lane & 31);
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int n = n0 + (wave >> 1) * 32 + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
-    if (n >= a.N) continue;
-    if (k < a.K) static_cast<E *>(a.gw)[((int64_t)e * a.N + n) * a.K + k] = T::save(acc[i]);
-    if (with_bias && (wave & 1) == 0 && (lane & 31) == 0) static_cast<E *>(a.gb)[(int64_t)e * a.N + n] = T::save(sums[i]);
+  count = min(count, max(0, a.chunks - first));
+  const int64_t size = (int64_t)a.N * a.K, all = size + (a.gb ? a.N : 0);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const float *p = i < size ? a.partial + (int64_t)first * size + i
+                              : a.partial + (int64_t)a.chunks * size + (int64_t)first * a.N + (i - size);
+    const int64_t step = i < size ? size : a.N;
+    float s = 0.f;
+    for (int c = 0; c < count; ++c) s += p[c * step];
+    if (i < size)
+      static_cast<E *>(a.gw)[(int64_t)e * size + i] = T::save(s);
+    else
+      static_cast<E *>(a.gb)[(int64_t)e * a.N + (i - size)] = T::save(s);
   }
 }
 
@@ -227,13 +294,87 @@ __global__ __launch_bounds__(256) void activation_backward_kernel(int64_t n, int
   store_vec<T, VEC>(out + i, gv);
 }
 
-template <class T>
-bool aligned_rows(const void *p, int64_t ld) {
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * (int64_t)sizeof(typename T::store) % 16 == 0;
-}
-
 bool bad_shape(int dtype, int R, int E, int K, int N) {
   return !known_dtype(dtype) || R < 0 || E < 1 || E > DIMO_MAX_EXPERTS || K < 1 || N < 1;
+}
+
+typedef Tile<64, 64, 2, 2> Small;
+typedef Tile<128, 128, 2, 2> Medium;
+typedef Tile<256, 256, 2, 4> Large;
+
+// rows on 16-byte boundaries whose ends are too
+bool whole_chunks(int dtype, const void *p, int64_t ld, int64_t width) {
+  const int64_t per = 16 / (int64_t)dtype_bytes(dtype);
+  return dtype != DIMO_F32 && aligned16(p) && ld % per == 0 && width % per == 0;
+}
+bool wide_output(int dtype, const void *p, int64_t columns) {
+  return columns % 4 == 0 && (reinterpret_cast<uintptr_t>(p) & (4 * dtype_bytes(dtype) - 1)) == 0;
+}
+
+template <class T, int MODE, bool DIRECT, class C>
+int launch_rows(const GroupedArgs &a, hipStream_t s) {
+  const int64_t groups = row_tile_workgroups(row_tile_count(a.R, a.E, C::TJ), ((MODE == FORWARD ? a.N : a.K) + C::TI - 1) / C::TI);
+  if (groups > 0x7fffffffLL) return DIMO_E_ARG;
+  hipLaunchKernelGGL((grouped_rows_kernel<T, MODE, DIRECT, C>), dim3((unsigned)groups), dim3(C::THREADS), 0, s, a);
+  return check_launch();
+}
+template <class T, bool DIRECT, class C>
+int launch_wgrad(const GroupedArgs &a, hipStream_t s) {
+  const int64_t tiles = (int64_t)((a.N + C::TJ - 1) / C::TJ) * ((a.K + C::TI - 1) / C::TI);
+  const int64_t groups = a.split_rows ? row_tile_workgroups(row_tile_count(a.R, a.E, a.split_rows), tiles) : tiles * a.E;
+  if (groups > 0x7fffffffLL || tiles > 0x7fffffffLL) return DIMO_E_ARG;
+  hipLaunchKernelGGL((grouped_wgrad_kernel<T, DIRECT, C>), dim3((unsigned)groups), dim3(C::THREADS), 0, s, a);
+  return check_launch();
+}
+
+// Which tile: a workgroup's tile is worth its size only where there are enough of them.
+enum { SMALL = 0, MEDIUM = 1, LARGE = 2 };
+int choose_tile(int64_t rows_per_group, int64_t groups, int64_t columns, bool direct) {
+  const auto blocks = [&](int64_t t) { return groups * ((rows_per_group + t - 1) / t) * ((columns + t - 1) / t); };
+  if (direct && rows_per_group >= 192 && columns >= 192 && blocks(256) >= 224) return LARGE;
+  if (rows_per_group >= 48 && columns >= 96 && blocks(128) >= 128) return MEDIUM;
+  return SMALL;
+}
+
+template <int MODE>
+int run_rows(int dtype, const GroupedArgs &a, bool direct, hipStream_t s) {
+  const int64_t per_group = (a.R + a.E - 1) / a.E;
+  const int tile = choose_tile(per_group, (a.R + per_group - 1) / per_group, MODE == FORWARD ? a.N : a.K, direct);
+  int rc = DIMO_OK;
+  with_dtype(dtype, [&](auto tag) {
+    typedef decltype(tag) T;
+    if constexpr (sizeof(typename T::store) == 2) {
+      if (direct) {
+        rc = tile == LARGE ? launch_rows<T, MODE, true, Large>(a, s) : tile == MEDIUM ? launch_rows<T, MODE, true, Medium>(a, s)
+                                                                               : launch_rows<T, MODE, true, Small>(a, s);
+        return;
+      }
+    }
+    rc = tile == SMALL ? launch_rows<T, MODE, false, Small>(a, s) : launch_rows<T, MODE, false, Medium>(a, s);
+  });
+  return rc;
+}
+
+// wgrad: the tile, and rows per slice (0: no split): enough workgroups for two on every CU
+struct WgradPlan {
+  int tile, split_rows, chunks;
+  size_t bytes;
+};
+WgradPlan wgrad_plan(int dtype, int R, int E, int K, int N) {
+  WgradPlan p{SMALL, 0, 0, 0};
+  const int64_t per_group = R > 0 ? (R + E - 1) / E : 1;
+  const auto blocks = [&](int64_t t) { return (int64_t)E * ((N + t - 1) / t) * ((K + t - 1) / t); };
+  const bool narrow = dtype == DIMO_F32;
+  p.tile = !narrow && blocks(256) >= 224 ? LARGE : N >= 96 && K >= 96 ? MEDIUM : SMALL;
+  const int64_t have = blocks(p.tile == LARGE ? 256 : p.tile == MEDIUM ? 128 : 64);
+  if (have < 512 && per_group >= 256) {
+    const int64_t splits = (512 + have - 1) / have;
+    int64_t rows = (per_group + splits - 1) / splits;
+    rows = rows < 128 ? 128 : (rows + 63) / 64 * 64;
+    p.split_rows = (int)rows, p.chunks = row_tile_count(R, E, (int)rows);
+    p.bytes = align_up((size_t)p.chunks * ((size_t)N * K + N) * sizeof(float));
+  }
+  return p;
 }
 
 }  // namespace
@@ -250,14 +391,8 @@ extern "C" int dimo_grouped_linear_forward(int dtype, int R, int E, int K, int N
   GroupedArgs a{};
   a.R = R, a.E = E, a.K = K, a.N = N, a.places = places, a.x = x, a.ldx = ldx, a.order = order, a.offsets = offsets;
   a.w = w, a.bias = bias, a.act = act, a.y = y, a.z = z;
-  const dim3 grid(row_tile_count(R, E, GM), (N + GN - 1) / GN);
-  if (grid.y > 65535) return DIMO_E_ARG;
-  with_dtype(dtype, [&](auto tag) {
-    typedef decltype(tag) Tag;
-    hipLaunchKernelGGL((grouped_rows_general_kernel<Tag, FORWARD>), grid, dim3(256), 0, s, a, aligned_rows<Tag>(x, ldx),
-                       aligned_rows<Tag>(w, K));
-  });
-  return check_launch();
+  a.wide = wide_output(dtype, y, N) && (!z || wide_output(dtype, z, N));
+  return run_rows<FORWARD>(dtype, a, whole_chunks(dtype, x, ldx, K) && whole_chunks(dtype, w, K, K), s);
 }
 
 extern "C" int dimo_grouped_linear_dgrad(int dtype, int R, int E, int K, int N, const void *g, const int32_t *offsets,
@@ -270,35 +405,48 @@ extern "C" int dimo_grouped_linear_dgrad(int dtype, int R, int E, int K, int N, 
   ScopedTimer timer(T_GROUPED, s);
   GroupedArgs a{};
   a.R = R, a.E = E, a.K = K, a.N = N, a.offsets = offsets, a.w = w, a.g = g, a.gx = gx;
-  const dim3 grid(row_tile_count(R, E, GM), (K + GN - 1) / GN);
-  if (grid.y > 65535) return DIMO_E_ARG;
-  with_dtype(dtype, [&](auto tag) {
-    typedef decltype(tag) Tag;
-    hipLaunchKernelGGL((grouped_rows_general_kernel<Tag, DGRAD>), grid, dim3(256), 0, s, a, aligned_rows<Tag>(g, N),
-                       aligned_rows<Tag>(w, K));
-  });
-  return check_launch();
+  a.wide = wide_output(dtype, gx, K);
+  return run_rows<DGRAD>(dtype, a, whole_chunks(dtype, g, N, N) && whole_chunks(dtype, w, K, K), s);
+}
+
+extern "C" size_t dimo_grouped_linear_wgrad_workspace_bytes(int dtype, int R, int E, int K, int N) {
+  return bad_shape(dtype, R, E, K, N) ? 0 : wgrad_plan(dtype, R, E, K, N).bytes;
 }
 
 extern "C" int dimo_grouped_linear_wgrad(int dtype, int R, int E, int K, int N, const void *g, const void *x, int64_t ldx,
                                          int places, const int32_t *order, const int32_t *offsets, void *gw, void *gb,
-                                         void *stream) {
+                                         void *workspace, size_t workspace_bytes, void *stream) {
   if (bad_shape(dtype, R, E, K, N) || ldx < K || places < 0 || !offsets || !gw) return DIMO_E_ARG;
   if (R > 0 && (!g || !x || (places > 0 && !order))) return DIMO_E_ARG;
+  const WgradPlan plan = wgrad_plan(dtype, R, E, K, N);
+  if (workspace_bytes < plan.bytes || (plan.bytes && (!workspace || !aligned16(workspace)))) return DIMO_E_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
   clear_errors();
   ScopedTimer timer(T_GROUPED, s);
   GroupedArgs a{};
   a.R = R, a.E = E, a.K = K, a.N = N, a.places = places, a.x = x, a.ldx = ldx, a.order = order, a.offsets = offsets;
-  a.g = g, a.gw = gw, a.gb = gb;
-  const int64_t tiles = (int64_t)((N + GM - 1) / GM) * ((K + GN - 1) / GN);
-  if (tiles > 0x7fffffffLL) return DIMO_E_ARG;
+  a.g = g, a.gw = gw, a.gb = gb, a.wide = wide_output(dtype, gw, K);
+  a.split_rows = plan.split_rows, a.chunks = plan.chunks, a.partial = static_cast<float *>(workspace);
+  const bool direct = whole_chunks(dtype, g, N, N) && whole_chunks(dtype, x, ldx, K);
+  int rc = DIMO_OK;
   with_dtype(dtype, [&](auto tag) {
-    typedef decltype(tag) Tag;
-    hipLaunchKernelGGL((grouped_wgrad_general_kernel<Tag>), dim3((unsigned)tiles, E), dim3(256), 0, s, a,
-                       aligned_rows<Tag>(g, N), aligned_rows<Tag>(x, ldx));
+    typedef decltype(tag) T;
+    bool done = false;
+    if constexpr (sizeof(typename T::store) == 2) {
+      if (direct) {
+        rc = plan.tile == LARGE ? launch_wgrad<T, true, Large>(a, s) : plan.tile == MEDIUM ? launch_wgrad<T, true, Medium>(a, s)
+                                                                                   : launch_wgrad<T, true, Small>(a, s);
+        done = true;
+      }
+    }
+    if (!done) rc = plan.tile == SMALL ? launch_wgrad<T, false, Small>(a, s) : launch_wgrad<T, false, Medium>(a, s);
+    if (!rc && a.split_rows) {
+      const int64_t blocks = ((int64_t)N * K + (gb ? N : 0) + 255) / 256;
+      hipLaunchKernelGGL((grouped_wgrad_sum_kernel<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096), E), dim3(256), 0, s, a);
+      rc = check_launch();
+    }
   });
-  return check_launch();
+  return rc;
 }
 
 extern "C" int dimo_activation_backward(int dtype, int act, int64_t n, const void *g, const void *saved, void *out,

@@ -18,7 +18,20 @@ __device__ __forceinline__ f32x16 mfma_32x32x16(F16, uint4 a, uint4 b, f32x16 c)
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// The same over 64 values of k in microscaled 4-bit form: lane l holds the block of 32 codes of A's row i = l % 32 at
+// Sixteen bytes per lane from memory straight into LDS: lane l's land at S + 16 l bytes (S: the wave's, the same in every
+// lane).  Done when vmcnt has counted it down, as for any load.
+__device__ __forceinline__ void load_to_lds(const void *from, uint16_t *S) {
+  __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void *)from,
+                                   (__attribute__((address_space(3))) void *)S, 16, 0, 0);
+}
+// Eight bytes per lane from LDS, transposed among 16 lanes: lane j of them names four 16-bit values of row j / 4 (columns
+// 4 (j % 4) ..+ 3 of a 4 x 16 block) and gets column j of the block, rows 0 .. 3.
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ uint2 read_transposed(const uint16_t *S) {
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)S));
+}
+
+// D = A B + C over 64 values of k in microscaled 4-bit form: lane l holds the block of 32 codes of A's row i = l % 32 at
 // k = 32 (l / 32) ..+ 31 (sixteen bytes, ascending k, low four bits first) with its scale byte, B's column j = l % 32
 // likewise.  D as above.
 typedef int i32x8 __attribute__((ext_vector_type(8)));

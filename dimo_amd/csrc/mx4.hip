@@ -135,16 +135,11 @@ struct Mx4Args {
 template <class T>
 __global__ __launch_bounds__(256) void mx4_rows_general_kernel(Mx4Args a) {
   typedef typename T::store E;
-  RowTile tile;
-  if (a.offsets) {
-    tile = find_row_tile(a.offsets, a.E, a.R, 64, (int)blockIdx.x);
-  } else {
-    tile.expert = 0, tile.begin = 64 * (int)blockIdx.x, tile.end = min(tile.begin + 64, a.R);
-    if (tile.begin >= a.R) return;
-  }
+  int ct = 0;
+  const RowTile tile = find_row_tile(a.offsets, a.E, a.R, 64, (a.N + 63) / 64, (int)blockIdx.x, &ct);
   if (tile.expert < 0) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-  const int n0 = blockIdx.y * 64 + (wave & 1) * 32, r0 = tile.begin + (wave >> 1) * 32;
+  const int n0 = ct * 64 + (wave & 1) * 32, r0 = tile.begin + (wave >> 1) * 32;
   E *out = static_cast<E *>(a.y);
   const int n = n0 + (lane & 31);
   if (tile.expert == a.E) {
@@ -233,10 +228,10 @@ extern "C" int dimo_mx4_linear(int dtype, int R, int E, int K, int N, const uint
   clear_errors();
   ScopedTimer timer(T_MX4, s);
   const Mx4Args a{R, E, K, N, (K + 31) / 32, x_codes, x_scales, w_codes, w_scales, offsets, bias, act, y};
-  const dim3 grid(offsets ? row_tile_count(R, E, 64) : (R + 63) / 64, (N + 63) / 64);
-  if (grid.y > 65535) return DIMO_E_ARG;
+  const int64_t grid = row_tile_workgroups(row_tile_count(R, E, 64), (N + 63) / 64);
+  if (grid > 0x7fffffffLL) return DIMO_E_ARG;
   with_dtype(dtype, [&](auto tag) {
-    hipLaunchKernelGGL((mx4_rows_general_kernel<decltype(tag)>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((mx4_rows_general_kernel<decltype(tag)>), dim3((unsigned)grid), dim3(256), 0, s, a);
   });
   return check_launch();
 }

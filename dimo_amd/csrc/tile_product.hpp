@@ -1,0 +1,225 @@
+// One output tile of a product on the 16-bit matrix instructions: out[row][col] = sum over the reduction of
+// ROW[row][.] COL[col][.], ROW and COL being any mix of
+//   LINES    the operand's lines lie along the reduction in memory (x, weights [N, K] of the forward)
+//   COLUMNS  its lines lie across it (the weights of dgrad, both operands of wgrad): reduction step r is one row of
+//            memory, the tile's lines are neighbours in it
+// A workgroup owns TJ x TI outputs, a wave WJ x WI of them as 32 x 32 blocks of v_mfma_f32_32x32x16 with the ROW operand
+// in the instruction's j (lane) and the COL operand in its i (register) dimension: a lane then holds four consecutive
+// columns of one output row.
+//
+// A stage is BK steps of the reduction.  In LDS it lies as it lies in memory -- LINES: [line][BK], COLUMNS: [step][TILE]
+// --, cut into chunks of 16 bytes whose place inside a row is permuted so that the operand reads (ds_read_b128 for
+// LINES, the transposing ds_read_b64_tr_b16 for COLUMNS) spread over all banks (`lines_place`, `columns_place`).
+#pragma once
+#include "matrix_ops.hpp"
+
+namespace dimo {
+
+constexpr bool LINES = true, COLUMNS = false;
+
+// sixteen zero bytes: what lies behind the end of the reduction is read from here
+__device__ const uint4 zero_chunk = {0u, 0u, 0u, 0u};
+
+// Place (in chunks) of logical chunk c of LDS row `row`; `per_row` chunks in a row.  Eight neighbouring rows' chunk c
+// fall on eight different 16-byte columns of the banks, sixteen on sixteen of a bank row twice as wide.
+template <int PER_ROW>
+__device__ __forceinline__ int lines_place(int row, int c) {
+  static_assert(PER_ROW == 8 || PER_ROW == 4, "stages are 64 or 32 deep");
+  return PER_ROW == 8 ? c ^ ((row & 7) ^ ((row >> 3) & 1)) : c ^ (((row >> 1) & 3) ^ ((row >> 3) & 1));
+}
+// ... of a COLUMNS row: a transposing read takes 32 bytes of each of four neighbouring rows per 16 lanes.
+template <int PER_ROW>
+__device__ __forceinline__ int columns_place(int row, int c) {
+  return c ^ (((row & 3) << 1) | (PER_ROW >= 16 ? (row & 1) << 3 : 0));
+}
+
+// ---- operand reads -----------------------------------------------------------------------------------------------
+// the eight values of the reduction that lane l of the matrix instruction holds for line (line0 + l % 32), from step
+// `step` (a multiple of 16) of the stage on
+template <bool ORDER, int TILE, int BK>
+__device__ __forceinline__ uint4 read_operand(const uint16_t *S, int line0, int step) {
+  const int lane = threadIdx.x & 63;
+  if constexpr (ORDER == LINES) {
+    const int row = line0 + (lane & 31), c = (step >> 3) + (lane >> 5);
+    return *reinterpret_cast<const uint4 *>(S + (row * (BK / 8) + lines_place<BK / 8>(row, c)) * 8);
+  } else {
+    // 16 lanes read four steps of 16 lines and get, lane by lane, one line's four steps
+    const int g = lane >> 4, j = lane & 15;
+    const int line = line0 + 16 * (g & 1) + 4 * (j & 3), row = step + 8 * (g >> 1) + (j >> 2);
+    const int c = line >> 3, in = line & 7;
+    const uint2 lo = read_transposed(S + (row * (TILE / 8) + columns_place<TILE / 8>(row, c)) * 8 + in);
+    const uint2 hi = read_transposed(S + ((row + 4) * (TILE / 8) + columns_place<TILE / 8>(row + 4, c)) * 8 + in);
+    return make_uint4(lo.x, lo.y, hi.x, hi.y);
+  }
+}
+
+// ---- staging -----------------------------------------------------------------------------------------------------
+// A thread brings CHUNKS chunks of 8 elements of an operand per stage.  Chunk q of thread t is number q * THREADS + t of the
+// stage in LDS order, so that the 64 lanes of a wave write 1024 consecutive bytes (what a load straight into LDS does).
+// For LINES a thread keeps its lines (and their addresses) from stage to stage, for COLUMNS its column.
+template <class T, bool ORDER, int TILE, int BK, int THREADS>
+struct Staging {
+  typedef typename T::store E;
+  static constexpr int CHUNKS = TILE * BK / 8 / THREADS;
+  static constexpr int PER_ROW = ORDER == LINES ? BK / 8 : TILE / 8;
+  static constexpr int ROW_STEP = THREADS / PER_ROW;  // LDS rows between two chunks of a thread
+  static_assert(CHUNKS >= 1 && THREADS % PER_ROW == 0, "whole chunks");
+  static_assert(ORDER == LINES ? ROW_STEP % 16 == 0 : ROW_STEP % 4 == 0, "a thread's chunks share their permutation");
+  const E *base[ORDER == LINES ? CHUNKS : 1];  // LINES: each line's first element of this thread's chunk
+  int64_t ld;                                  // COLUMNS: elements between two steps
+  int col;                                     // this thread's first element: LINES along the reduction, COLUMNS across
+  int limit;                                   // COLUMNS: elements of a row from `col` on that exist (<= 0: none)
+
+  static __device__ __forceinline__ int lds_row(int q) { return (int)threadIdx.x / PER_ROW + q * ROW_STEP; }
+  // (the permutations are their own inverse: the logical chunk at this thread's place)
+  static __device__ __forceinline__ int logical_chunk() {
+    const int place = (int)threadIdx.x % PER_ROW;
+    if constexpr (ORDER == LINES)
+      return lines_place<PER_ROW>((int)threadIdx.x / PER_ROW, place);
+    else
+      return columns_place<PER_ROW>((int)threadIdx.x / PER_ROW, place);
+  }
+  // line(i) -> pointer to the first element of line i of the tile (always a readable line)
+  template <class F>
+  __device__ __forceinline__ void init_lines(F &&line) {
+    col = 8 * logical_chunk();
+#pragma unroll
+    for (int q = 0; q < CHUNKS; ++q) base[q] = line(lds_row(q)) + col;
+  }
+  // p: the matrix's first element of the tile's first column, `columns` of them exist
+  __device__ __forceinline__ void init_columns(const E *p, int64_t ld_, int columns) {
+    col = 8 * logical_chunk();
+    ld = ld_, limit = columns - col;
+    base[0] = p + (limit > 0 ? col : 0);
+  }
+  // address of chunk q of the stage that begins at step k0 (the reduction ends at `end`), row(r) -> memory row of step r;
+  // what lies behind the end comes from the zero chunk
+  template <class F>
+  __device__ __forceinline__ const E *address(int q, int k0, int end, F &&row) const {
+    if constexpr (ORDER == LINES) {
+      return k0 + col < end ? base[q] + k0 : reinterpret_cast<const E *>(&zero_chunk);
+    } else {
+      const int r = k0 + lds_row(q);
+      return r < end ? base[0] + row(r) * ld : reinterpret_cast<const E *>(&zero_chunk);
+    }
+  }
+  // straight into LDS (16-bit elements, everything on 16-byte boundaries and the rows' ends too)
+  template <class F>
+  __device__ __forceinline__ void load_direct(uint16_t *S, int k0, int end, F &&row) const {
+#pragma unroll
+    for (int q = 0; q < CHUNKS; ++q)
+      load_to_lds(address(q, k0, end, row), S + (q * THREADS + ((int)threadIdx.x & ~63)) * 8);
+  }
+  // through registers: any alignment, any end
+  typedef E Chunk[8];
+  template <class F>
+  __device__ __forceinline__ void load(Chunk (&v)[CHUNKS], int k0, int end, F &&row) const {
+#pragma unroll
+    for (int q = 0; q < CHUNKS; ++q) {
+      const E *p;
+      int ok;
+      if constexpr (ORDER == LINES) {
+        ok = end - k0 - col, p = base[q] + (ok > 0 ? k0 : 0);
+      } else {
+        const int r = k0 + lds_row(q);
+        ok = r < end ? limit : 0, p = base[0] + (r < end ? row(r) : 0) * ld;
+      }
+      if (ok >= 8) {
+        __builtin_memcpy(v[q], p, sizeof(Chunk));  // (one or two 16-byte loads; the hardware takes any alignment)
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[q][e] = e < ok ? p[e] : E(0);
+      }
+    }
+  }
+  // into the planes of LDS (three for fp32, one otherwise), `plane` elements apart
+  __device__ __forceinline__ void store(const Chunk (&v)[CHUNKS], uint16_t *S, int plane) const {
+#pragma unroll
+    for (int q = 0; q < CHUNKS; ++q) {
+      uint16_t *dst = S + (q * THREADS + (int)threadIdx.x) * 8;
+      if constexpr (sizeof(E) == 4) {
+        uint32_t h[4], m[4], l[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const Split3 a = split3(v[q][2 * e]), b = split3(v[q][2 * e + 1]);
+          h[e] = a.hi | (uint32_t)b.hi << 16, m[e] = a.mid | (uint32_t)b.mid << 16, l[e] = a.lo | (uint32_t)b.lo << 16;
+        }
+        *reinterpret_cast<uint4 *>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4 *>(dst + plane) = make_uint4(m[0], m[1], m[2], m[3]);
+        *reinterpret_cast<uint4 *>(dst + 2 * plane) = make_uint4(l[0], l[1], l[2], l[3]);
+      } else {
+        uint4 w;
+        __builtin_memcpy(&w, v[q], 16);
+        *reinterpret_cast<uint4 *>(dst) = w;
+      }
+    }
+  }
+};
+
+template <class T>
+struct Planes {
+  static constexpr int N = 1, DEPTH = 64;
+  typedef T Tag;
+};
+template <>
+struct Planes<F32> {  // (three planes: half the depth keeps a stage of 128 + 128 lines at 48 KB)
+  static constexpr int N = 3, DEPTH = 32;
+  typedef BF16 Tag;
+};
+
+// ---- a wave's share ------------------------------------------------------------------------------------------------
+template <int NJ, int NI>
+struct Accumulators {
+  f32x16 v[NJ][NI];
+  float sums[NJ];  // with_sums: the ROW operand's sums along the reduction, this lane's share of line l % 32
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) v[j][i][r] = 0.f;
+      sums[j] = 0.f;
+    }
+  }
+};
+
+// one stage: J lines from j0, I lines from i0 (32 NJ and 32 NI of them)
+template <class T, bool ORDER_J, bool ORDER_I, int TJ, int TI, int BK, int NJ, int NI, bool SUMS>
+__device__ __forceinline__ void multiply_stage(const uint16_t *SJ, const uint16_t *SI, int j0, int i0, Accumulators<NJ, NI> &acc,
+                                               bool with_sums) {
+  constexpr int P = Planes<T>::N;
+  typedef typename Planes<T>::Tag Tag;
+#pragma unroll
+  for (int step = 0; step < BK; step += 16) {
+    uint4 a[P][NI], b[P][NJ];
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) a[p][i] = read_operand<ORDER_I, TI, BK>(SI + p * TI * BK, i0 + 32 * i, step);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) b[p][j] = read_operand<ORDER_J, TJ, BK>(SJ + p * TJ * BK, j0 + 32 * j, step);
+    }
+#pragma unroll
+    for (int d = P - 1; d >= 0; --d)  // (fp32: the smallest products first)
+#pragma unroll
+      for (int p = 0; p <= d; ++p)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int i = 0; i < NI; ++i) acc.v[j][i] = mfma_32x32x16(Tag{}, a[p][i], b[d - p][j], acc.v[j][i]);
+    if constexpr (SUMS)
+      if (with_sums) {
+#pragma unroll
+        for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) {
+            const uint32_t w[4] = {b[p][j].x, b[p][j].y, b[p][j].z, b[p][j].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc.sums[j] += Tag::load((uint16_t)w[e]) + Tag::load((uint16_t)(w[e] >> 16));
+          }
+      }
+  }
+}
+
+}  // namespace dimo

@@ -218,10 +218,13 @@ def _linear_wgrad(g, x, shape, groups, gather, need_bias):
     gw = torch.empty(E, N, K, dtype=g.dtype, device=g.device)
     gb = torch.empty(E, N, dtype=g.dtype, device=g.device) if need_bias else None
     with _on(g.device):
-        _lib.check(_lib.lib().dimo_grouped_linear_wgrad(
+        L = _lib.lib()
+        nbytes = L.dimo_grouped_linear_wgrad_workspace_bytes(_DTYPES[g.dtype], g.shape[0], E, K, N)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=g.device) if nbytes else None
+        _lib.check(L.dimo_grouped_linear_wgrad(
             _DTYPES[g.dtype], g.shape[0], E, K, N, g.data_ptr(), x.data_ptr(), _ld(x), groups.places if gather else 0,
             _lib.ptr(groups.order) if gather else None, groups.offsets.data_ptr(), gw.data_ptr(), _lib.ptr(gb),
-            _lib.current_stream()), "dimo_grouped_linear_wgrad")
+            _lib.ptr(ws), nbytes, _lib.current_stream()), "dimo_grouped_linear_wgrad")
     return gw, gb
 
 

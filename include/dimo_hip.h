@@ -480,8 +480,10 @@ int dimo_grouped_linear_forward(int dtype, int R, int E, int K, int N, const voi
 int dimo_grouped_linear_dgrad(int dtype, int R, int E, int K, int N, const void *g, const int32_t *offsets, const void *w,
                               void *gx, void *stream);
 /* gw[e] = sum of g[r]^T x[src(r)], gb[e] = sum of g[r] (gb may be NULL) over the rows of the group */
+size_t dimo_grouped_linear_wgrad_workspace_bytes(int dtype, int R, int E, int K, int N);
 int dimo_grouped_linear_wgrad(int dtype, int R, int E, int K, int N, const void *g, const void *x, int64_t ldx, int places,
-                              const int32_t *order, const int32_t *offsets, void *gw, void *gb, void *stream);
+                              const int32_t *order, const int32_t *offsets, void *gw, void *gb, void *workspace,
+                              size_t workspace_bytes, void *stream);
 /* out = g * act'(saved): saved = the activation's output for relu, its input for silu; n elements */
 int dimo_activation_backward(int dtype, int act, int64_t n, const void *g, const void *saved, void *out, void *stream);
 /* out[t] = residual[t] + sum_j weights[t, j] y[position[t, j]] (weights NULL: 1; position -1: nothing) */

@@ -141,6 +141,7 @@ SUBST["experts.hip"] = []
 SUBST["grouped.hip"] = []
 SUBST["mx4.hip"] = []
 SUBST["row_tiles.hpp"] = []
+SUBST["tile_product.hpp"] = []
 SUBST["numeric.hpp"] = [  # gcc 11 has neither 16-bit floating type on x86-64, nor std::bit_cast's builtin
     ("__builtin_bit_cast(float, (uint32_t)v << 16)", "simt_from_bf16(v)"),
     ("__builtin_bit_cast(uint16_t, (__bf16)v)", "simt_to_bf16(v)"),
@@ -158,13 +159,18 @@ SUBST["matrix_ops.hpp"] = [
      "simt_mfma_32x32x16(a, b, c, simt_from_bf16)"),
     ("__builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0)",
      "simt_mfma_32x32x16(a, b, c, simt_from_f16)"),
+    ("typedef short s16x4 __attribute__((ext_vector_type(4)));", ""),
+    ("""__builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void *)from,
+                                   (__attribute__((address_space(3))) void *)S, 16, 0, 0);""", "simt_load_to_lds(from, S);"),
+    ("__builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)S))",
+     "simt_read_transposed(S)"),
     ("typedef int i32x8 __attribute__((ext_vector_type(8)));", "typedef int i32x8 __attribute__((vector_size(32)));"),
     ("__builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c, 4, 4, 0, scale_a, 0, scale_b)",
      "simt_mfma_mx4_32x32x64(a, scale_a, b, scale_b, c)"),
     ("(uint16_t)(__builtin_bit_cast(uint32_t, v) >> 16)", "(uint16_t)(__float_as_uint(v) >> 16)"),
 ]
 HEADERS = ["common.hpp", "proj_math.hpp", "wave_ops.hpp", "deform_body.hpp", "loss_terms.hpp", "numeric.hpp",
-           "matrix_ops.hpp", "row_tiles.hpp"]  # copied beside the sources (substitutions applied)
+           "matrix_ops.hpp", "row_tiles.hpp", "tile_product.hpp"]  # copied beside the sources (substitutions applied)
 
 
 def build(force=False, target="binning"):

@@ -361,6 +361,18 @@ struct SimtOperands {
     }
   }
 };
+// global_load_lds_dwordx4: lane l's sixteen bytes land at S + 16 l
+static inline void simt_load_to_lds(const void *from, uint16_t *S) { memcpy(S + 8 * simt::lane_id(), from, 16); }
+// ds_read_b64_tr_b16: among 16 lanes, lane j names row j / 4, columns 4 (j % 4) ..+ 3 and gets column j
+static inline uint2 simt_read_transposed(const uint16_t *S) {
+  uint64_t mine;
+  memcpy(&mine, S, 8);
+  const uint64_t *v = simt::wave_exchange(mine);
+  const int l = simt::lane_id(), g = l & ~15, j = l & 15;
+  uint16_t out[4];
+  for (int r = 0; r < 4; ++r) out[r] = (uint16_t)(v[g + 4 * r + (j >> 2)] >> (16 * (j & 3)));
+  return uint2{(uint32_t)out[0] | (uint32_t)out[1] << 16, (uint32_t)out[2] | (uint32_t)out[3] << 16};
+}
 // e2m1 code times 2^(byte - 127)
 static inline double simt_mx4_value(uint32_t code, uint32_t byte) {
   code &= 15;

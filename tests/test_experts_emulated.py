@@ -54,6 +54,9 @@ def test_group(emulated, T, k, E, skew):
     ([33, 130], 72, 64, F32, "silu", 1, 0),
     ([0, 0], 16, 16, BF16, None, 5, 0),
     ([65], 129, 33, BF16, "silu", 0, 0),
+    ([300, 0, 600], 24, 40, BF16, None, 0, 0),     # weight gradients from slices of the rows
+    ([300, 0, 600], 23, 41, F32, None, 7, 0),
+    ([48 + i % 7 for i in range(128)], 40, 104, BF16, None, 3, 8),  # 128 x 128 tiles
 ])
 def test_products(emulated, counts, K, N, dtype, act, tail, pad):
     cases.check_products(ex, "cpu", counts, K, N, dtype, act, tail, pad, seed=K)
@@ -145,7 +148,8 @@ def test_c_entry_points_refuse():
     assert L.dimo_grouped_linear_forward(0, 4, 3, 8, 5, 1, 8, 2, None, 1, 1, None, 0, 1, None, None) == -1
     assert L.dimo_grouped_linear_forward(0, 4, 3, 8, 5, 1, 8, 0, None, 1, 1, None, 3, 1, None, None) == -1
     assert L.dimo_grouped_linear_dgrad(0, 4, 0, 8, 5, 1, 1, 1, 1, None) == -1
-    assert L.dimo_grouped_linear_wgrad(0, 4, 3, 8, 5, 1, 1, 8, 0, None, None, 1, None, None) == -1
+    assert L.dimo_grouped_linear_wgrad(0, 4, 3, 8, 5, 1, 1, 8, 0, None, None, 1, None, None, 0, None) == -1
+    assert L.dimo_grouped_linear_wgrad(1, 4096, 2, 64, 64, 1, 1, 64, 0, None, 1, 1, None, None, 0, None) == -3
     assert L.dimo_activation_backward(0, 0, 8, 1, 1, 1, None) == -1
     assert L.dimo_combine_rows_forward(4, 2, 8, 8, 0, 1, 7, None, 1, None, 0, 1, None) == -1
     assert L.dimo_combine_rows_backward(4, 2, 8, 9, 3, 0, 1, 8, 1, 8, 1, 1, 1, 1, 1, None) == -1

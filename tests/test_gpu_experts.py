@@ -64,6 +64,10 @@ def test_group(ex, T, k, E, skew):
     ([65], 129, 33, "silu", 0, 0),
     ([700], 512, 136, "relu", 60, 8),
     ([3] * 150, 72, 96, "silu", 0, 0),
+    ([300, 0, 600], 24, 40, None, 0, 0),
+    ([2000, 3, 1500], 264, 136, "silu", 9, 0),
+    ([48 + i % 7 for i in range(128)], 40, 104, None, 3, 8),
+    ([200 + i % 5 for i in range(225)], 200, 200, None, 0, 0),  # 256 x 256 tiles
 ])
 def test_products(ex, counts, K, N, dtype, act, tail, pad):
     cases.check_products(ex, "cuda", counts, K, N, dtype, act, tail, pad, seed=K)
