@@ -41,108 +41,6 @@ __device__ __forceinline__ int64_t source_row(const GroupedArgs &a, int r) {
 
 enum { FORWARD = 0, DGRAD = 1 };
 
-// TJ rows x TI columns per workgroup, WJ x WI waves.
-template <int TJ_, int TI_, int WJ_, int WI_>
-struct Tile {
-  static constexpr int TJ = TJ_, TI = TI_, WJ = WJ_, WI = WI_, THREADS = 64 * WJ * WI;
-  static constexpr int NJ = TJ / WJ / 32, NI = TI / WI / 32;
-};
-
-// The stages of a product, one after the other.  DIRECT: two LDS buffers, the next stage's loads go straight into the one
-// while the other is multiplied, one barrier per stage.  Otherwise (fp32, odd ends, odd alignment): the next stage waits in
-// registers, one buffer, two barriers.
-template <class T, class C, bool ORDER_J, bool ORDER_I, bool DIRECT, bool SUMS, class RowJ, class RowI>
-__device__ __forceinline__ void run_stages(const Staging<T, ORDER_J, C::TJ, Planes<T>::DEPTH, C::THREADS> &sj,
-                                           const Staging<T, ORDER_I, C::TI, Planes<T>::DEPTH, C::THREADS> &si, int begin,
-                                           int end, RowJ &&row_j, RowI &&row_i, Accumulators<C::NJ, C::NI> &acc,
-                                           bool with_sums) {
-  constexpr int BK = Planes<T>::DEPTH, P = Planes<T>::N;
-  const int wave = threadIdx.x >> 6;
-  const int j0 = (wave / C::WI) * 32 * C::NJ, i0 = (wave % C::WI) * 32 * C::NI;
-  if constexpr (DIRECT) {
-    // (separate arrays: the compiler then knows that what is on its way into one is not what is read from the other)
-    __shared__ __attribute__((aligned(1024))) uint16_t SJ0[C::TJ * BK], SI0[C::TI * BK], SJ1[C::TJ * BK], SI1[C::TI * BK];
-    sj.load_direct(SJ0, begin, end, row_j);
-    si.load_direct(SI0, begin, end, row_i);
-    for (int k0 = begin;; k0 += 2 * BK) {
-      __syncthreads();  // this stage is there, and everyone is done with the other buffer
-      if (k0 + BK < end) {
-        sj.load_direct(SJ1, k0 + BK, end, row_j);
-        si.load_direct(SI1, k0 + BK, end, row_i);
-      }
-      __builtin_amdgcn_sched_barrier(0);  // (the loads first: they have this stage's products to arrive under)
-      multiply_stage<T, ORDER_J, ORDER_I, C::TJ, C::TI, BK, C::NJ, C::NI, SUMS>(SJ0, SI0, j0, i0, acc, with_sums);
-      if (k0 + BK >= end) break;
-      __syncthreads();
-      if (k0 + 2 * BK < end) {
-        sj.load_direct(SJ0, k0 + 2 * BK, end, row_j);
-        si.load_direct(SI0, k0 + 2 * BK, end, row_i);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      multiply_stage<T, ORDER_J, ORDER_I, C::TJ, C::TI, BK, C::NJ, C::NI, SUMS>(SJ1, SI1, j0, i0, acc, with_sums);
-      if (k0 + 2 * BK >= end) break;
-    }
-  } else {
-    typedef Staging<T, ORDER_J, C::TJ, BK, C::THREADS> LJ;
-    typedef Staging<T, ORDER_I, C::TI, BK, C::THREADS> LI;
-    __shared__ __attribute__((aligned(1024))) uint16_t SJ[P * C::TJ * BK], SI[P * C::TI * BK];
-    typename LJ::Chunk vj[LJ::CHUNKS];
-    typename LI::Chunk vi[LI::CHUNKS];
-    sj.load(vj, begin, end, row_j);
-    si.load(vi, begin, end, row_i);
-    for (int k0 = begin; k0 < end; k0 += BK) {
-      __syncthreads();  // everyone is done with the last stage
-      sj.store(vj, SJ, C::TJ * BK);
-      si.store(vi, SI, C::TI * BK);
-      __syncthreads();
-      if (k0 + BK < end) {
-        sj.load(vj, k0 + BK, end, row_j);
-        si.load(vi, k0 + BK, end, row_i);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      multiply_stage<T, ORDER_J, ORDER_I, C::TJ, C::TI, BK, C::NJ, C::NI, SUMS>(SJ, SI, j0, i0, acc, with_sums);
-    }
-  }
-}
-
-// For every quad of the wave's outputs: column(c) once per quad of columns, then f(row of the tile, column of the tile, the
-// quad's sums, what column(c) gave) for its rows.
-template <class C, class G, class F>
-__device__ __forceinline__ void for_quads(const Accumulators<C::NJ, C::NI> &acc, G &&column, F &&f) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int j0 = (wave / C::WI) * 32 * C::NJ + (lane & 31), i0 = (wave % C::WI) * 32 * C::NI + 4 * (lane >> 5);
-#pragma unroll
-  for (int i = 0; i < C::NI; ++i)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float4 more = column(i0 + 32 * i + 8 * q);
-#pragma unroll
-      for (int j = 0; j < C::NJ; ++j) {
-        const float v[4] = {acc.v[j][i][4 * q] + more.x, acc.v[j][i][4 * q + 1] + more.y, acc.v[j][i][4 * q + 2] + more.z,
-                            acc.v[j][i][4 * q + 3] + more.w};
-        f(j0 + 32 * j, i0 + 32 * i + 8 * q, v);
-      }
-      __builtin_amdgcn_sched_barrier(0);  // (quad by quad: all of them at once would not fit the registers)
-    }
-}
-
-// four elements of a row from column c on, `columns` exist
-template <class T>
-__device__ __forceinline__ void store_quad(typename T::store *row, int c, int columns, bool wide, const float (&v)[4]) {
-  typedef typename T::store E;
-  if (wide && c + 4 <= columns) {
-    if constexpr (sizeof(E) == 4)
-      *reinterpret_cast<float4 *>(row + c) = make_float4(v[0], v[1], v[2], v[3]);
-    else
-      *reinterpret_cast<uint2 *>(row + c) = make_uint2((uint32_t)T::save(v[0]) | (uint32_t)T::save(v[1]) << 16,
-                                                       (uint32_t)T::save(v[2]) | (uint32_t)T::save(v[3]) << 16);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (c + e < columns) row[c + e] = T::save(v[e]);
-  }
-}
-
 template <class T, int MODE, bool DIRECT, class C>
 __global__ __launch_bounds__(C::THREADS, 2) void grouped_rows_kernel(GroupedArgs a) {
   typedef typename T::store E;
@@ -325,15 +223,6 @@ int launch_wgrad(const GroupedArgs &a, hipStream_t s) {
   if (groups > 0x7fffffffLL || tiles > 0x7fffffffLL) return DIMO_E_ARG;
   hipLaunchKernelGGL((grouped_wgrad_kernel<T, DIRECT, C>), dim3((unsigned)groups), dim3(C::THREADS), 0, s, a);
   return check_launch();
-}
-
-// Which tile: a workgroup's tile is worth its size only where there are enough of them.
-enum { SMALL = 0, MEDIUM = 1, LARGE = 2 };
-int choose_tile(int64_t rows_per_group, int64_t groups, int64_t columns, bool direct) {
-  const auto blocks = [&](int64_t t) { return groups * ((rows_per_group + t - 1) / t) * ((columns + t - 1) / t); };
-  if (direct && rows_per_group >= 192 && columns >= 192 && blocks(256) >= 224) return LARGE;
-  if (rows_per_group >= 48 && columns >= 96 && blocks(128) >= 128) return MEDIUM;
-  return SMALL;
 }
 
 template <int MODE>

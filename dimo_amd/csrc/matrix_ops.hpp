@@ -34,10 +34,12 @@ __device__ __forceinline__ uint2 read_transposed(const uint16_t *S) {
 // D = A B + C over 64 values of k in microscaled 4-bit form: lane l holds the block of 32 codes of A's row i = l % 32 at
 // k = 32 (l / 32) ..+ 31 (sixteen bytes, ascending k, low four bits first) with its scale byte, B's column j = l % 32
 // likewise.  D as above.
+// BYTE: which byte of the lane's scale words counts.
 typedef int i32x8 __attribute__((ext_vector_type(8)));
-__device__ __forceinline__ f32x16 mfma_mx4_32x32x64(uint4 a, int scale_a, uint4 b, int scale_b, f32x16 c) {
+template <int BYTE>
+__device__ __forceinline__ f32x16 mfma_mx4_32x32x64(uint4 a, uint32_t scale_a, uint4 b, uint32_t scale_b, f32x16 c) {
   const i32x8 av = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0}, bv = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c, 4, 4, 0, scale_a, 0, scale_b);  // (4: e2m1)
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c, 4, 4, BYTE, (int)scale_a, BYTE, (int)scale_b);  // (4: e2m1)
 }
 
 // fp32 = three bf16 pieces: the top eight significant bits (cut, so that no finite value becomes infinite), what is left

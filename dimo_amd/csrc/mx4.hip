@@ -7,8 +7,10 @@
 // The rounding to 4 bits is the only loss, and it happens in `quantise`, where the caller asked for it.
 #include <hip/hip_runtime.h>
 
-#include "matrix_ops.hpp"
+#include <type_traits>
+
 #include "row_tiles.hpp"
+#include "tile_product.hpp"
 
 using namespace dimo;
 
@@ -121,56 +123,150 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(int64_t rows, int K
   }
 }
 
-// ---- the product, general form: 64 x 64 outputs per workgroup, 32 x 32 per wave, operands straight from memory (16
-// bytes of codes per lane are exactly one block of 32) ---------------------------------------------------------------
+// ---- the product -------------------------------------------------------------------------------------------------
+// The tiles and LDS stages of tile_product.hpp with codes as elements: a stage of 64 16-bit words per line is 256 values of
+// k, eight blocks, and a lane's sixteen bytes are exactly one block.  The eight scale bytes of a lane's lines come a
+// stage ahead into registers; a byte permutation leaves those of its half of the wave (blocks 2 s + l / 32), one per
+// instruction.
 struct Mx4Args {
   int R, E, K, N, blocks;
   const uint8_t *xc, *xs, *wc, *ws;
   const int32_t *offsets;  // null: one group of all rows
   const void *bias;
-  int act;
+  int act, wide;
   void *y;
 };
 
-template <class T>
-__global__ __launch_bounds__(256) void mx4_rows_general_kernel(Mx4Args a) {
-  typedef typename T::store E;
-  int ct = 0;
-  const RowTile tile = find_row_tile(a.offsets, a.E, a.R, 64, (a.N + 63) / 64, (int)blockIdx.x, &ct);
-  if (tile.expert < 0) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-  const int n0 = ct * 64 + (wave & 1) * 32, r0 = tile.begin + (wave >> 1) * 32;
-  E *out = static_cast<E *>(a.y);
-  const int n = n0 + (lane & 31);
-  if (tile.expert == a.E) {
+// scale bytes of blocks b0 .. b0 + 7 of a line; what is behind its end counts as 2^0 (its codes are zero: a NaN scale must
+// not meet them)
+__device__ __forceinline__ uint2 load_scales(const uint8_t *line, int b0, int blocks) {
+  uint2 v;
+  if (b0 + 8 <= blocks) {
+    __builtin_memcpy(&v, line + b0, 8);
+    return v;
+  }
+  uint32_t w[2] = {0x7f7f7f7fu, 0x7f7f7f7fu};
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int row = r0 + 2 * i + half;
-      if (row < tile.end && n < a.N) out[(int64_t)row * a.N + n] = E(0);
+  for (int e = 0; e < 8; ++e)
+    if (b0 + e < blocks) w[e >> 2] = (w[e >> 2] & ~(255u << (8 * (e & 3)))) | (uint32_t)line[b0 + e] << (8 * (e & 3));
+  return make_uint2(w[0], w[1]);
+}
+// bytes half, half + 2, half + 4, half + 6
+__device__ __forceinline__ uint32_t own_scales(uint2 v, int half) {
+  return __builtin_amdgcn_perm(v.y, v.x, half ? 0x07050301u : 0x06040200u);
+}
+
+template <class C>
+__device__ __forceinline__ void multiply_codes(const uint16_t *SJ, const uint16_t *SI, int j0, int i0,
+                                               const uint32_t (&sj)[C::NJ], const uint32_t (&si)[C::NI],
+                                               Accumulators<C::NJ, C::NI> &acc) {
+  const auto step = [&](auto byte) {
+    constexpr int S = decltype(byte)::value;
+    uint4 a[C::NI], b[C::NJ];
+#pragma unroll
+    for (int i = 0; i < C::NI; ++i) a[i] = read_operand<LINES, C::TI, 64>(SI, i0 + 32 * i, 16 * S);
+#pragma unroll
+    for (int j = 0; j < C::NJ; ++j) b[j] = read_operand<LINES, C::TJ, 64>(SJ, j0 + 32 * j, 16 * S);
+#pragma unroll
+    for (int j = 0; j < C::NJ; ++j)
+#pragma unroll
+      for (int i = 0; i < C::NI; ++i) acc.v[j][i] = mfma_mx4_32x32x64<S>(a[i], si[i], b[j], sj[j], acc.v[j][i]);
+  };
+  step(std::integral_constant<int, 0>{});
+  step(std::integral_constant<int, 1>{});
+  step(std::integral_constant<int, 2>{});
+  step(std::integral_constant<int, 3>{});
+}
+
+template <class T, class C>
+__global__ __launch_bounds__(C::THREADS, 2) void mx4_rows_kernel(Mx4Args a) {
+  typedef typename T::store E;
+  constexpr int BK = 64;  // 16-bit words of codes per stage
+  __shared__ __attribute__((aligned(1024))) uint16_t SJ0[C::TJ * BK], SI0[C::TI * BK], SJ1[C::TJ * BK], SI1[C::TI * BK];
+  int ct = 0;
+  const RowTile tile = find_row_tile(a.offsets, a.E, a.R, C::TJ, (a.N + C::TI - 1) / C::TI, (int)blockIdx.x, &ct);
+  if (tile.expert < 0) return;
+  const int c0 = ct * C::TI;
+  E *out = static_cast<E *>(a.y);
+  if (tile.expert == a.E) {  // behind the last group
+    for (int i = threadIdx.x; i < C::TJ * C::TI; i += C::THREADS) {
+      const int r = tile.begin + i / C::TI, c = c0 + i % C::TI;
+      if (r < tile.end && c < a.N) out[(int64_t)r * a.N + c] = E(0);
     }
     return;
   }
-  const int64_t xr = min(r0 + (lane & 31), tile.end - 1), wr = (int64_t)tile.expert * a.N + min(n, a.N - 1);
-  const uint4 *xc = reinterpret_cast<const uint4 *>(a.xc) + xr * a.blocks, *wc = reinterpret_cast<const uint4 *>(a.wc) + wr * a.blocks;
-  const uint8_t *xs = a.xs + xr * a.blocks, *ws = a.ws + wr * a.blocks;
-  f32x16 acc;
+  const int end = 8 * a.blocks, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int j0 = (wave / C::WI) * 32 * C::NJ, i0 = (wave % C::WI) * 32 * C::NI;
+  const auto x_line = [&](int i) { return (int64_t)min(tile.begin + i, tile.end - 1); };
+  const auto w_line = [&](int i) { return (int64_t)tile.expert * a.N + min(c0 + i, a.N - 1); };
+  Staging<BF16, LINES, C::TJ, BK, C::THREADS> sj;  // (any 16-bit type: words of codes)
+  Staging<BF16, LINES, C::TI, BK, C::THREADS> si;
+  sj.init_lines([&](int i) { return reinterpret_cast<const uint16_t *>(a.xc) + x_line(i) * end; });
+  si.init_lines([&](int i) { return reinterpret_cast<const uint16_t *>(a.wc) + w_line(i) * end; });
+  const uint8_t *lj[C::NJ], *li[C::NI];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-  for (int b0 = 0; b0 < a.blocks; b0 += 2) {
-    const int b = min(b0 + half, a.blocks - 1);
-    const bool in = b0 + half < a.blocks;
-    uint4 x = xc[b], w = wc[b];
-    const int sx = xs[b], sw = ws[b];
-    if (!in) x = make_uint4(0, 0, 0, 0), w = x;  // (both zero under the scales of the last block, a NaN scale among them)
-    acc = mfma_mx4_32x32x64(x, sx, w, sw, acc);
-  }
-  if (n >= a.N) return;
-  const float bias = a.bias ? T::load(static_cast<const E *>(a.bias)[(int64_t)tile.expert * a.N + n]) : 0.f;
+  for (int j = 0; j < C::NJ; ++j) lj[j] = a.xs + x_line(j0 + 32 * j + (lane & 31)) * a.blocks;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int row = r0 + 8 * (i >> 2) + 4 * half + (i & 3);
-    if (row < tile.end) out[(int64_t)row * a.N + n] = T::save(activate(acc[i] + bias, a.act));
+  for (int i = 0; i < C::NI; ++i) li[i] = a.ws + w_line(i0 + 32 * i + (lane & 31)) * a.blocks;
+  Accumulators<C::NJ, C::NI> acc;
+  acc.clear();
+  uint2 nj[C::NJ], ni[C::NI];  // the next stage's scales
+  uint32_t cj[C::NJ], ci[C::NI];
+  const auto same = [](int r) { return (int64_t)r; };
+  const auto request = [&](uint16_t *SJ, uint16_t *SI, int k0) {
+    sj.load_direct(SJ, k0, end, same);
+    si.load_direct(SI, k0, end, same);
+#pragma unroll
+    for (int j = 0; j < C::NJ; ++j) nj[j] = load_scales(lj[j], k0 / 8, a.blocks);
+#pragma unroll
+    for (int i = 0; i < C::NI; ++i) ni[i] = load_scales(li[i], k0 / 8, a.blocks);
+  };
+  const auto take = [&]() {
+#pragma unroll
+    for (int j = 0; j < C::NJ; ++j) cj[j] = own_scales(nj[j], lane >> 5);
+#pragma unroll
+    for (int i = 0; i < C::NI; ++i) ci[i] = own_scales(ni[i], lane >> 5);
+  };
+  request(SJ0, SI0, 0);
+  for (int k0 = 0;; k0 += 2 * BK) {
+    __syncthreads();  // this stage is there, and everyone is done with the other buffer
+    take();
+    if (k0 + BK < end) request(SJ1, SI1, k0 + BK);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply_codes<C>(SJ0, SI0, j0, i0, cj, ci, acc);
+    if (k0 + BK >= end) break;
+    __syncthreads();
+    take();
+    if (k0 + 2 * BK < end) request(SJ0, SI0, k0 + 2 * BK);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply_codes<C>(SJ1, SI1, j0, i0, cj, ci, acc);
+    if (k0 + 2 * BK >= end) break;
   }
+  const E *bias = a.bias ? static_cast<const E *>(a.bias) + (int64_t)tile.expert * a.N : nullptr;
+  const auto columns_bias = [&](int i) {
+    const int c = c0 + i;
+    if (!bias || c >= a.N) return make_float4(0.f, 0.f, 0.f, 0.f);
+    return make_float4(T::load(bias[c]), T::load(bias[min(c + 1, a.N - 1)]), T::load(bias[min(c + 2, a.N - 1)]),
+                       T::load(bias[min(c + 3, a.N - 1)]));
+  };
+  for_quads<C>(acc, columns_bias, [&](int j, int i, const float (&s)[4]) {
+    const int r = tile.begin + j, c = c0 + i;
+    if (r >= tile.end || c >= a.N) return;
+    const float v[4] = {activate(s[0], a.act), activate(s[1], a.act), activate(s[2], a.act), activate(s[3], a.act)};
+    store_quad<T>(out + (int64_t)r * a.N, c, a.N, a.wide, v);
+  });
+}
+
+typedef Tile<64, 64, 2, 2> Small;
+typedef Tile<128, 128, 2, 2> Medium;
+typedef Tile<256, 256, 2, 4> Large;
+
+template <class T, class C>
+int launch_mx4(const Mx4Args &a, hipStream_t s) {
+  const int64_t groups = row_tile_workgroups(row_tile_count(a.R, a.E, C::TJ), (a.N + C::TI - 1) / C::TI);
+  if (groups > 0x7fffffffLL) return DIMO_E_ARG;
+  hipLaunchKernelGGL((mx4_rows_kernel<T, C>), dim3((unsigned)groups), dim3(C::THREADS), 0, s, a);
+  return check_launch();
 }
 
 }  // namespace
@@ -227,11 +323,14 @@ extern "C" int dimo_mx4_linear(int dtype, int R, int E, int K, int N, const uint
   hipStream_t s = (hipStream_t)stream;
   clear_errors();
   ScopedTimer timer(T_MX4, s);
-  const Mx4Args a{R, E, K, N, (K + 31) / 32, x_codes, x_scales, w_codes, w_scales, offsets, bias, act, y};
-  const int64_t grid = row_tile_workgroups(row_tile_count(R, E, 64), (N + 63) / 64);
-  if (grid > 0x7fffffffLL) return DIMO_E_ARG;
+  const bool wide = N % 4 == 0 && (reinterpret_cast<uintptr_t>(y) & (4 * dtype_bytes(dtype) - 1)) == 0;
+  const Mx4Args a{R, E, K, N, (K + 31) / 32, x_codes, x_scales, w_codes, w_scales, offsets, bias, act, wide, y};
+  const int64_t per_group = (R + E - 1) / E;
+  const int tile = choose_tile(per_group, (R + per_group - 1) / per_group, N, true);
+  int rc = DIMO_OK;
   with_dtype(dtype, [&](auto tag) {
-    hipLaunchKernelGGL((mx4_rows_general_kernel<decltype(tag)>), dim3((unsigned)grid), dim3(256), 0, s, a);
+    typedef decltype(tag) T;
+    rc = tile == LARGE ? launch_mx4<T, Large>(a, s) : tile == MEDIUM ? launch_mx4<T, Medium>(a, s) : launch_mx4<T, Small>(a, s);
   });
-  return check_launch();
+  return rc;
 }

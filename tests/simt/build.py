@@ -165,8 +165,8 @@ SUBST["matrix_ops.hpp"] = [
     ("__builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)S))",
      "simt_read_transposed(S)"),
     ("typedef int i32x8 __attribute__((ext_vector_type(8)));", "typedef int i32x8 __attribute__((vector_size(32)));"),
-    ("__builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c, 4, 4, 0, scale_a, 0, scale_b)",
-     "simt_mfma_mx4_32x32x64(a, scale_a, b, scale_b, c)"),
+    ("__builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c, 4, 4, BYTE, (int)scale_a, BYTE, (int)scale_b)",
+     "simt_mfma_mx4_32x32x64(a, (int)(scale_a >> (8 * BYTE)), b, (int)(scale_b >> (8 * BYTE)), c)"),
     ("(uint16_t)(__builtin_bit_cast(uint32_t, v) >> 16)", "(uint16_t)(__float_as_uint(v) >> 16)"),
 ]
 HEADERS = ["common.hpp", "proj_math.hpp", "wave_ops.hpp", "deform_body.hpp", "loss_terms.hpp", "numeric.hpp",

@@ -361,6 +361,14 @@ struct SimtOperands {
     }
   }
 };
+// v_perm_b32: byte i of the result = byte (sel >> 8 i) & 7 of the eight bytes lo, hi
+static inline uint32_t simt_perm(uint32_t hi, uint32_t lo, uint32_t sel) {
+  const uint64_t v = ((uint64_t)hi << 32) | lo;
+  uint32_t out = 0;
+  for (int i = 0; i < 4; ++i) out |= (uint32_t)((v >> (8 * ((sel >> (8 * i)) & 7))) & 255) << (8 * i);
+  return out;
+}
+#define __builtin_amdgcn_perm simt_perm
 // global_load_lds_dwordx4: lane l's sixteen bytes land at S + 16 l
 static inline void simt_load_to_lds(const void *from, uint16_t *S) { memcpy(S + 8 * simt::lane_id(), from, 16); }
 // ds_read_b64_tr_b16: among 16 lanes, lane j names row j / 4, columns 4 (j % 4) ..+ 3 and gets column j
