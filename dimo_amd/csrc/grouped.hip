@@ -30,7 +30,7 @@ struct GroupedArgs {
   const void *g;           // [R, N] (dgrad, wgrad)
   void *gx;                // [R, K]
   void *gw, *gb;           // [E, N, K], [E, N] or null
-  int wide;                // four neighbouring outputs of a row may be written at once
+  int wide;                // sixteen bytes of an output row may be written at once
   int split_rows, chunks;  // wgrad: > 0: partial sums over that many rows at a time, `chunks` of them at most
   float *partial;          // [chunks, N, K], then [chunks, N]
 };
@@ -76,24 +76,26 @@ __global__ __launch_bounds__(C::THREADS, 2) void grouped_rows_kernel(GroupedArgs
   Accumulators<C::NJ, C::NI> acc;
   acc.clear();
   const auto same = [](int r) { return (int64_t)r; };
-  run_stages<T, C, LINES, MODE == FORWARD ? LINES : COLUMNS, DIRECT, false>(sj, si, 0, reduction, same, same, acc, false);
+  DIMO_STAGE_BUFFERS(T, C, DIRECT);
+  run_stages<T, C, LINES, MODE == FORWARD ? LINES : COLUMNS, DIRECT, false>(sj, si, 0, reduction, same, same, acc, false, SJ0,
+                                                                            SI0, SJ1, SI1);
+  __syncthreads();
   const E *bias = MODE == FORWARD && a.bias ? static_cast<const E *>(a.bias) + (int64_t)tile.expert * a.N : nullptr;
-  const auto columns_bias = [&](int i) {
-    const int c = c0 + i;
-    if (!bias || c >= columns) return make_float4(0.f, 0.f, 0.f, 0.f);
-    return make_float4(T::load(bias[c]), T::load(bias[min(c + 1, columns - 1)]), T::load(bias[min(c + 2, columns - 1)]),
-                       T::load(bias[min(c + 3, columns - 1)]));
+  const auto add_bias = [&](int i, float (&v)[4]) {
+    if (MODE != FORWARD || !bias) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += T::load(bias[min(c0 + i + e, columns - 1)]);
   };
-  for_quads<C>(acc, columns_bias, [&](int j, int i, const float (&s)[4]) {
-    const int r = tile.begin + j, c = c0 + i;
-    if (r >= tile.end || c >= columns) return;
-    if constexpr (MODE == FORWARD) {
-      if (a.z) store_quad<T>(static_cast<E *>(a.z) + (int64_t)r * columns, c, columns, a.wide, s);
-      const float v[4] = {activate(s[0], a.act), activate(s[1], a.act), activate(s[2], a.act), activate(s[3], a.act)};
-      store_quad<T>(out + (int64_t)r * columns, c, columns, a.wide, v);
-    } else {
-      store_quad<T>(out + (int64_t)r * columns, c, columns, a.wide, s);
-    }
+  const auto out_row = [&](E *matrix) {
+    return [=](int j) { return tile.begin + j < tile.end ? matrix + (int64_t)(tile.begin + j) * columns : nullptr; };
+  };
+  if (MODE == FORWARD && a.z)
+    write_outputs<T, C, (int)sizeof(SJ0)>(acc, SJ0, c0, columns, a.wide, out_row(static_cast<E *>(a.z)), add_bias);
+  write_outputs<T, C, (int)sizeof(SJ0)>(acc, SJ0, c0, columns, a.wide, out_row(out), [&](int i, float (&v)[4]) {
+    add_bias(i, v);
+    if (MODE == FORWARD && a.act != DIMO_ACT_NONE)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = activate(v[e], a.act);
   });
 }
 
@@ -123,20 +125,21 @@ __global__ __launch_bounds__(C::THREADS, 2) void grouped_wgrad_kernel(GroupedArg
   Accumulators<C::NJ, C::NI> acc;
   acc.clear();
   const bool sums = a.gb && k0 == 0 && (int)(threadIdx.x >> 6) % C::WI == 0;  // (one of the waves that read a row)
+  DIMO_STAGE_BUFFERS(T, C, DIRECT);
   if (begin < end)
     run_stages<T, C, COLUMNS, COLUMNS, DIRECT, true>(sj, si, begin, end, [](int r) { return (int64_t)r; },
-                                                     [&](int r) { return source_row(a, r); }, acc, sums);
+                                                     [&](int r) { return source_row(a, r); }, acc, sums, SJ0, SI0, SJ1, SI1);
+  __syncthreads();
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   float *pw = a.partial + (int64_t)chunk * a.N * a.K, *pb = a.partial + (int64_t)a.chunks * a.N * a.K + (int64_t)chunk * a.N;
   E *gw = static_cast<E *>(a.gw) + (int64_t)expert * a.N * a.K, *gb = static_cast<E *>(a.gb) + (int64_t)expert * a.N;
-  for_quads<C>(acc, [](int) { return make_float4(0.f, 0.f, 0.f, 0.f); }, [&](int j, int i, const float (&v)[4]) {
-    const int n = n0 + j, k = k0 + i;
-    if (n >= a.N || k >= a.K) return;
-    if (a.split_rows)
-      store_quad<F32>(pw + (int64_t)n * a.K, k, a.K, a.wide, v);
-    else
-      store_quad<T>(gw + (int64_t)n * a.K, k, a.K, a.wide, v);
-  });
+  const auto as_it_is = [](int, float (&)[4]) {};
+  if (a.split_rows)
+    write_outputs<F32, C, (int)sizeof(SJ0)>(acc, SJ0, k0, a.K, a.wide,
+                                            [&](int j) { return n0 + j < a.N ? pw + (int64_t)(n0 + j) * a.K : nullptr; }, as_it_is);
+  else
+    write_outputs<T, C, (int)sizeof(SJ0)>(acc, SJ0, k0, a.K, a.wide,
+                                          [&](int j) { return n0 + j < a.N ? gw + (int64_t)(n0 + j) * a.K : nullptr; }, as_it_is);
   if (sums) {
 #pragma unroll
     for (int j = 0; j < C::NJ; ++j) {
@@ -206,7 +209,7 @@ bool whole_chunks(int dtype, const void *p, int64_t ld, int64_t width) {
   return dtype != DIMO_F32 && aligned16(p) && ld % per == 0 && width % per == 0;
 }
 bool wide_output(int dtype, const void *p, int64_t columns) {
-  return columns % 4 == 0 && (reinterpret_cast<uintptr_t>(p) & (4 * dtype_bytes(dtype) - 1)) == 0;
+  return columns % (16 / (int64_t)dtype_bytes(dtype)) == 0 && aligned16(p);
 }
 
 template <class T, int MODE, bool DIRECT, class C>

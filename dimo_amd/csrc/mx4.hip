@@ -157,21 +157,34 @@ __device__ __forceinline__ uint32_t own_scales(uint2 v, int half) {
 }
 
 template <class C>
-__device__ __forceinline__ void multiply_codes(const uint16_t *SJ, const uint16_t *SI, int j0, int i0,
+__device__ __forceinline__ void multiply_codes(const uint16_t *SJ, const uint16_t *SI,
+                                               const Reader<LINES, C::TJ, 64, C::NJ> &rj, const Reader<LINES, C::TI, 64, C::NI> &ri,
                                                const uint32_t (&sj)[C::NJ], const uint32_t (&si)[C::NI],
                                                Accumulators<C::NJ, C::NI> &acc) {
+  // (the next step's operands ahead of time, as in multiply_stage, where the registers allow it: with 128 sums, the scales
+  // and the addresses a 256 x 256 tile's wave has none left -- spilling it took 1476 us where this takes 698)
+  constexpr bool AHEAD = C::NI * C::NJ <= 4;
+  uint4 a[2][C::NI], b[2][C::NJ];
+  const auto read = [&](int s) {
+#pragma unroll
+    for (int i = 0; i < C::NI; ++i) a[s & 1][i] = ri.read(SI, i, s);
+#pragma unroll
+    for (int j = 0; j < C::NJ; ++j) b[s & 1][j] = rj.read(SJ, j, s);
+  };
   const auto step = [&](auto byte) {
     constexpr int S = decltype(byte)::value;
-    uint4 a[C::NI], b[C::NJ];
-#pragma unroll
-    for (int i = 0; i < C::NI; ++i) a[i] = read_operand<LINES, C::TI, 64>(SI, i0 + 32 * i, 16 * S);
-#pragma unroll
-    for (int j = 0; j < C::NJ; ++j) b[j] = read_operand<LINES, C::TJ, 64>(SJ, j0 + 32 * j, 16 * S);
+    if (AHEAD && S < 3) read(S + 1);
+    if (!AHEAD) read(S);
 #pragma unroll
     for (int j = 0; j < C::NJ; ++j)
 #pragma unroll
-      for (int i = 0; i < C::NI; ++i) acc.v[j][i] = mfma_mx4_32x32x64<S>(a[i], si[i], b[j], sj[j], acc.v[j][i]);
+      for (int i = 0; i < C::NI; ++i) acc.v[j][i] = mfma_mx4_32x32x64<S>(a[S & 1][i], si[i], b[S & 1][j], sj[j], acc.v[j][i]);
+    if constexpr (AHEAD) interleave<C::NI + C::NJ, C::NI * C::NJ>(S < 3);
   };
+  if constexpr (AHEAD) {
+    read(0);
+    __builtin_amdgcn_sched_group_barrier(0x100, C::NI + C::NJ, 0);
+  }
   step(std::integral_constant<int, 0>{});
   step(std::integral_constant<int, 1>{});
   step(std::integral_constant<int, 2>{});
@@ -203,11 +216,15 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx4_rows_kernel(Mx4Args a) {
   Staging<BF16, LINES, C::TI, BK, C::THREADS> si;
   sj.init_lines([&](int i) { return reinterpret_cast<const uint16_t *>(a.xc) + x_line(i) * end; });
   si.init_lines([&](int i) { return reinterpret_cast<const uint16_t *>(a.wc) + w_line(i) * end; });
-  const uint8_t *lj[C::NJ], *li[C::NI];
+  // scale bytes of this lane's lines: 32-bit offsets from the tile's first line (at most 256 lines of a row's blocks)
+  const uint8_t *xs = a.xs + x_line(0) * a.blocks, *ws = a.ws + w_line(0) * a.blocks;
+  uint32_t lj[C::NJ], li[C::NI];
 #pragma unroll
-  for (int j = 0; j < C::NJ; ++j) lj[j] = a.xs + x_line(j0 + 32 * j + (lane & 31)) * a.blocks;
+  for (int j = 0; j < C::NJ; ++j) lj[j] = (uint32_t)(x_line(j0 + 32 * j + (lane & 31)) - x_line(0)) * a.blocks;
 #pragma unroll
-  for (int i = 0; i < C::NI; ++i) li[i] = a.ws + w_line(i0 + 32 * i + (lane & 31)) * a.blocks;
+  for (int i = 0; i < C::NI; ++i) li[i] = (uint32_t)(w_line(i0 + 32 * i + (lane & 31)) - w_line(0)) * a.blocks;
+  const Reader<LINES, C::TJ, BK, C::NJ> rj(j0);
+  const Reader<LINES, C::TI, BK, C::NI> ri(i0);
   Accumulators<C::NJ, C::NI> acc;
   acc.clear();
   uint2 nj[C::NJ], ni[C::NI];  // the next stage's scales
@@ -217,9 +234,9 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx4_rows_kernel(Mx4Args a) {
     sj.load_direct(SJ, k0, end, same);
     si.load_direct(SI, k0, end, same);
 #pragma unroll
-    for (int j = 0; j < C::NJ; ++j) nj[j] = load_scales(lj[j], k0 / 8, a.blocks);
+    for (int j = 0; j < C::NJ; ++j) nj[j] = load_scales(xs + lj[j], k0 / 8, a.blocks);
 #pragma unroll
-    for (int i = 0; i < C::NI; ++i) ni[i] = load_scales(li[i], k0 / 8, a.blocks);
+    for (int i = 0; i < C::NI; ++i) ni[i] = load_scales(ws + li[i], k0 / 8, a.blocks);
   };
   const auto take = [&]() {
 #pragma unroll
@@ -227,34 +244,34 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx4_rows_kernel(Mx4Args a) {
 #pragma unroll
     for (int i = 0; i < C::NI; ++i) ci[i] = own_scales(ni[i], lane >> 5);
   };
+  const int stages = (end + BK - 1) / BK;
   request(SJ0, SI0, 0);
-  for (int k0 = 0;; k0 += 2 * BK) {
+  int k0 = 0;
+  for (int n = 1; n < stages; n += 2, k0 += 2 * BK) {
     __syncthreads();  // this stage is there, and everyone is done with the other buffer
     take();
-    if (k0 + BK < end) request(SJ1, SI1, k0 + BK);
+    request(SJ1, SI1, k0 + BK);
     __builtin_amdgcn_sched_barrier(0);
-    multiply_codes<C>(SJ0, SI0, j0, i0, cj, ci, acc);
-    if (k0 + BK >= end) break;
+    multiply_codes<C>(SJ0, SI0, rj, ri, cj, ci, acc);
     __syncthreads();
     take();
-    if (k0 + 2 * BK < end) request(SJ0, SI0, k0 + 2 * BK);
+    if (n + 1 < stages) request(SJ0, SI0, k0 + 2 * BK);
     __builtin_amdgcn_sched_barrier(0);
-    multiply_codes<C>(SJ1, SI1, j0, i0, cj, ci, acc);
-    if (k0 + 2 * BK >= end) break;
+    multiply_codes<C>(SJ1, SI1, rj, ri, cj, ci, acc);
+  }
+  if (stages & 1) {
+    __syncthreads();
+    take();
+    multiply_codes<C>(SJ0, SI0, rj, ri, cj, ci, acc);
   }
   const E *bias = a.bias ? static_cast<const E *>(a.bias) + (int64_t)tile.expert * a.N : nullptr;
-  const auto columns_bias = [&](int i) {
-    const int c = c0 + i;
-    if (!bias || c >= a.N) return make_float4(0.f, 0.f, 0.f, 0.f);
-    return make_float4(T::load(bias[c]), T::load(bias[min(c + 1, a.N - 1)]), T::load(bias[min(c + 2, a.N - 1)]),
-                       T::load(bias[min(c + 3, a.N - 1)]));
-  };
-  for_quads<C>(acc, columns_bias, [&](int j, int i, const float (&s)[4]) {
-    const int r = tile.begin + j, c = c0 + i;
-    if (r >= tile.end || c >= a.N) return;
-    const float v[4] = {activate(s[0], a.act), activate(s[1], a.act), activate(s[2], a.act), activate(s[3], a.act)};
-    store_quad<T>(out + (int64_t)r * a.N, c, a.N, a.wide, v);
-  });
+  __syncthreads();
+  write_outputs<T, C, (int)sizeof(SJ0)>(
+      acc, SJ0, c0, a.N, a.wide, [&](int j) { return tile.begin + j < tile.end ? out + (int64_t)(tile.begin + j) * a.N : nullptr; },
+      [&](int i, float (&v)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = activate(v[e] + (bias ? T::load(bias[min(c0 + i + e, a.N - 1)]) : 0.f), a.act);
+      });
 }
 
 typedef Tile<64, 64, 2, 2> Small;
@@ -323,7 +340,7 @@ extern "C" int dimo_mx4_linear(int dtype, int R, int E, int K, int N, const uint
   hipStream_t s = (hipStream_t)stream;
   clear_errors();
   ScopedTimer timer(T_MX4, s);
-  const bool wide = N % 4 == 0 && (reinterpret_cast<uintptr_t>(y) & (4 * dtype_bytes(dtype) - 1)) == 0;
+  const bool wide = N % (16 / (int)dtype_bytes(dtype)) == 0 && aligned16(y);
   const Mx4Args a{R, E, K, N, (K + 31) / 32, x_codes, x_scales, w_codes, w_scales, offsets, bias, act, wide, y};
   const int64_t per_group = (R + E - 1) / E;
   const int tile = choose_tile(per_group, (R + per_group - 1) / per_group, N, true);

@@ -34,24 +34,39 @@ __device__ __forceinline__ int columns_place(int row, int c) {
 }
 
 // ---- operand reads -----------------------------------------------------------------------------------------------
-// the eight values of the reduction that lane l of the matrix instruction holds for line (line0 + l % 32), from step
-// `step` (a multiple of 16) of the stage on
-template <bool ORDER, int TILE, int BK>
-__device__ __forceinline__ uint4 read_operand(const uint16_t *S, int line0, int step) {
-  const int lane = threadIdx.x & 63;
-  if constexpr (ORDER == LINES) {
-    const int row = line0 + (lane & 31), c = (step >> 3) + (lane >> 5);
-    return *reinterpret_cast<const uint4 *>(S + (row * (BK / 8) + lines_place<BK / 8>(row, c)) * 8);
-  } else {
-    // 16 lanes read four steps of 16 lines and get, lane by lane, one line's four steps
-    const int g = lane >> 4, j = lane & 15;
-    const int line = line0 + 16 * (g & 1) + 4 * (j & 3), row = step + 8 * (g >> 1) + (j >> 2);
-    const int c = line >> 3, in = line & 7;
-    const uint2 lo = read_transposed(S + (row * (TILE / 8) + columns_place<TILE / 8>(row, c)) * 8 + in);
-    const uint2 hi = read_transposed(S + ((row + 4) * (TILE / 8) + columns_place<TILE / 8>(row + 4, c)) * 8 + in);
-    return make_uint4(lo.x, lo.y, hi.x, hi.y);
+// Where in a stage lane l of the matrix instruction finds its eight values of the reduction, for NB blocks of 32 lines: the
+// permutation of a lane's row does not change from block to block (LINES) or from step to step (COLUMNS), so a few
+// offsets serve all reads, the rest is the instructions' constant offset.
+template <bool ORDER, int TILE, int BK, int NB>
+struct Reader {
+  static constexpr int READS = ORDER == LINES ? 1 : 2;  // instructions per read()
+  int at[ORDER == LINES ? BK / 16 : NB];
+  __device__ __forceinline__ explicit Reader(int line0) {
+    const int lane = threadIdx.x & 63;
+    if constexpr (ORDER == LINES) {
+      const int row = line0 + (lane & 31);
+#pragma unroll
+      for (int s = 0; s < BK / 16; ++s) at[s] = row * BK + lines_place<BK / 8>(row, 2 * s + (lane >> 5)) * 8;
+    } else {
+      // 16 lanes read four steps of 16 lines and get, lane by lane, one line's four steps
+      const int g = lane >> 4, j = lane & 15, row = 8 * (g >> 1) + (j >> 2);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const int line = line0 + 32 * b + 16 * (g & 1) + 4 * (j & 3);
+        at[b] = row * TILE + columns_place<TILE / 8>(row, line >> 3) * 8 + (line & 7);
+      }
+    }
   }
-}
+  // block b, steps 16 s ..+ 15 of the stage
+  __device__ __forceinline__ uint4 read(const uint16_t *S, int b, int s) const {
+    if constexpr (ORDER == LINES) {
+      return *reinterpret_cast<const uint4 *>(S + at[s] + 32 * b * BK);
+    } else {
+      const uint2 lo = read_transposed(S + at[b] + 16 * s * TILE), hi = read_transposed(S + at[b] + (16 * s + 4) * TILE);
+      return make_uint4(lo.x, lo.y, hi.x, hi.y);
+    }
+  }
+};
 
 // ---- staging -----------------------------------------------------------------------------------------------------
 // A thread brings CHUNKS chunks of 8 elements of an operand per stage.  Chunk q of thread t is number q * THREADS + t of the
@@ -100,7 +115,8 @@ struct Staging {
       return k0 + col < end ? base[q] + k0 : reinterpret_cast<const E *>(&zero_chunk);
     } else {
       const int r = k0 + lds_row(q);
-      return r < end ? base[0] + row(r) * ld : reinterpret_cast<const E *>(&zero_chunk);
+      const E *p = base[0] + row(min(r, end - 1)) * ld;
+      return r < end ? p : reinterpret_cast<const E *>(&zero_chunk);
     }
   }
   // straight into LDS (16-bit elements, everything on 16-byte boundaries and the rows' ends too)
@@ -167,6 +183,13 @@ struct Planes<F32> {  // (three planes: half the depth keeps a stage of 128 + 12
   typedef BF16 Tag;
 };
 
+// TJ rows x TI columns per workgroup, WJ x WI waves.
+template <int TJ_, int TI_, int WJ_, int WI_>
+struct Tile {
+  static constexpr int TJ = TJ_, TI = TI_, WJ = WJ_, WI = WI_, THREADS = 64 * WJ * WI;
+  static constexpr int NJ = TJ / WJ / 32, NI = TI / WI / 32;
+};
+
 // ---- a wave's share ------------------------------------------------------------------------------------------------
 template <int NJ, int NI>
 struct Accumulators {
@@ -184,22 +207,40 @@ struct Accumulators {
   }
 };
 
-// one stage: J lines from j0, I lines from i0 (32 NJ and 32 NI of them)
-template <class T, bool ORDER_J, bool ORDER_I, int TJ, int TI, int BK, int NJ, int NI, bool SUMS>
-__device__ __forceinline__ void multiply_stage(const uint16_t *SJ, const uint16_t *SI, int j0, int i0, Accumulators<NJ, NI> &acc,
-                                               bool with_sums) {
-  constexpr int P = Planes<T>::N;
-  typedef typename Planes<T>::Tag Tag;
+// Asks the scheduler for one LDS read behind each matrix instruction while there are any (READS of them for PRODUCTS
+// instructions).
+template <int READS, int PRODUCTS>
+__device__ __forceinline__ void interleave(bool reads) {
 #pragma unroll
-  for (int step = 0; step < BK; step += 16) {
-    uint4 a[P][NI], b[P][NJ];
+  for (int p = 0; p < PRODUCTS; ++p) {
+    constexpr int EACH = (READS + PRODUCTS - 1) / PRODUCTS;
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    if (reads && p * EACH < READS) __builtin_amdgcn_sched_group_barrier(0x100, EACH, 0);
+  }
+}
+
+// One stage of a wave's 32 NJ x 32 NI outputs: the operands of the next sixteen steps are read while these are multiplied
+// (a read between two matrix instructions: issued all at once they would leave the matrix pipe waiting for them).
+template <class T, class C, int BK, bool SUMS, class RJ, class RI>
+__device__ __forceinline__ void multiply_stage(const uint16_t *SJ, const uint16_t *SI, const RJ &rj, const RI &ri,
+                                               Accumulators<C::NJ, C::NI> &acc, bool with_sums) {
+  constexpr int P = Planes<T>::N, NJ = C::NJ, NI = C::NI, STEPS = BK / 16;
+  typedef typename Planes<T>::Tag Tag;
+  uint4 a[2][P][NI], b[2][P][NJ];
+  const auto read = [&](int s) {
 #pragma unroll
     for (int p = 0; p < P; ++p) {
 #pragma unroll
-      for (int i = 0; i < NI; ++i) a[p][i] = read_operand<ORDER_I, TI, BK>(SI + p * TI * BK, i0 + 32 * i, step);
+      for (int i = 0; i < NI; ++i) a[s & 1][p][i] = ri.read(SI + p * C::TI * BK, i, s);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) b[p][j] = read_operand<ORDER_J, TJ, BK>(SJ + p * TJ * BK, j0 + 32 * j, step);
+      for (int j = 0; j < NJ; ++j) b[s & 1][p][j] = rj.read(SJ + p * C::TJ * BK, j, s);
     }
+  };
+  read(0);
+  if constexpr (!SUMS) __builtin_amdgcn_sched_group_barrier(0x100, P * (NI * RI::READS + NJ * RJ::READS), 0);
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    if (s + 1 < STEPS) read(s + 1);
 #pragma unroll
     for (int d = P - 1; d >= 0; --d)  // (fp32: the smallest products first)
 #pragma unroll
@@ -207,27 +248,29 @@ __device__ __forceinline__ void multiply_stage(const uint16_t *SJ, const uint16_
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
-          for (int i = 0; i < NI; ++i) acc.v[j][i] = mfma_32x32x16(Tag{}, a[p][i], b[d - p][j], acc.v[j][i]);
+          for (int i = 0; i < NI; ++i) acc.v[j][i] = mfma_32x32x16(Tag{}, a[s & 1][p][i], b[s & 1][d - p][j], acc.v[j][i]);
     if constexpr (SUMS)
       if (with_sums) {
 #pragma unroll
         for (int p = P - 1; p >= 0; --p)
 #pragma unroll
           for (int j = 0; j < NJ; ++j) {
-            const uint32_t w[4] = {b[p][j].x, b[p][j].y, b[p][j].z, b[p][j].w};
+            const uint4 v = b[s & 1][p][j];
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc.sums[j] += Tag::load((uint16_t)w[e]) + Tag::load((uint16_t)(w[e] >> 16));
           }
       }
+    if constexpr (!SUMS) interleave<P * (NI * RI::READS + NJ * RJ::READS), NJ * NI * P * (P + 1) / 2>(s + 1 < STEPS);
   }
 }
 
-// TJ rows x TI columns per workgroup, WJ x WI waves.
-template <int TJ_, int TI_, int WJ_, int WI_>
-struct Tile {
-  static constexpr int TJ = TJ_, TI = TI_, WJ = WJ_, WI = WI_, THREADS = 64 * WJ * WI;
-  static constexpr int NJ = TJ / WJ / 32, NI = TI / WI / 32;
-};
+// The LDS of a product's stages: separate arrays, so that the compiler knows that what is on its way into one is not what is
+// read from another (it would wait for every load in flight before each read otherwise).
+#define DIMO_STAGE_BUFFERS(T, C, DIRECT)                                                                                       \
+  __shared__ __attribute__((aligned(1024))) uint16_t SJ0[Planes<T>::N * C::TJ * Planes<T>::DEPTH],                             \
+      SI0[Planes<T>::N * C::TI * Planes<T>::DEPTH], SJ1[DIRECT ? C::TJ * Planes<T>::DEPTH : 8],                                \
+      SI1[DIRECT ? C::TI * Planes<T>::DEPTH : 8]
 
 // The stages of a product, one after the other.  DIRECT: two LDS buffers, the next stage's loads go straight into the one
 // while the other is multiplied, one barrier per stage.  Otherwise (fp32, odd ends, odd alignment): the next stage waits in
@@ -236,75 +279,54 @@ template <class T, class C, bool ORDER_J, bool ORDER_I, bool DIRECT, bool SUMS, 
 __device__ __forceinline__ void run_stages(const Staging<T, ORDER_J, C::TJ, Planes<T>::DEPTH, C::THREADS> &sj,
                                            const Staging<T, ORDER_I, C::TI, Planes<T>::DEPTH, C::THREADS> &si, int begin,
                                            int end, RowJ &&row_j, RowI &&row_i, Accumulators<C::NJ, C::NI> &acc,
-                                           bool with_sums) {
-  constexpr int BK = Planes<T>::DEPTH, P = Planes<T>::N;
+                                           bool with_sums, uint16_t *SJ0, uint16_t *SI0, uint16_t *SJ1, uint16_t *SI1) {
+  constexpr int BK = Planes<T>::DEPTH;
   const int wave = threadIdx.x >> 6;
-  const int j0 = (wave / C::WI) * 32 * C::NJ, i0 = (wave % C::WI) * 32 * C::NI;
+  const Reader<ORDER_J, C::TJ, BK, C::NJ> rj((wave / C::WI) * 32 * C::NJ);
+  const Reader<ORDER_I, C::TI, BK, C::NI> ri((wave % C::WI) * 32 * C::NI);
   if constexpr (DIRECT) {
-    // (separate arrays: the compiler then knows that what is on its way into one is not what is read from the other)
-    __shared__ __attribute__((aligned(1024))) uint16_t SJ0[C::TJ * BK], SI0[C::TI * BK], SJ1[C::TJ * BK], SI1[C::TI * BK];
+    const int stages = (end - begin + BK - 1) / BK;
     sj.load_direct(SJ0, begin, end, row_j);
     si.load_direct(SI0, begin, end, row_i);
-    for (int k0 = begin;; k0 += 2 * BK) {
+    int k0 = begin;
+    for (int n = 1; n < stages; n += 2, k0 += 2 * BK) {
       __syncthreads();  // this stage is there, and everyone is done with the other buffer
-      if (k0 + BK < end) {
-        sj.load_direct(SJ1, k0 + BK, end, row_j);
-        si.load_direct(SI1, k0 + BK, end, row_i);
-      }
+      sj.load_direct(SJ1, k0 + BK, end, row_j);
+      si.load_direct(SI1, k0 + BK, end, row_i);
       __builtin_amdgcn_sched_barrier(0);  // (the loads first: they have this stage's products to arrive under)
-      multiply_stage<T, ORDER_J, ORDER_I, C::TJ, C::TI, BK, C::NJ, C::NI, SUMS>(SJ0, SI0, j0, i0, acc, with_sums);
-      if (k0 + BK >= end) break;
+      multiply_stage<T, C, BK, SUMS>(SJ0, SI0, rj, ri, acc, with_sums);
       __syncthreads();
-      if (k0 + 2 * BK < end) {
+      if (n + 1 < stages) {
         sj.load_direct(SJ0, k0 + 2 * BK, end, row_j);
         si.load_direct(SI0, k0 + 2 * BK, end, row_i);
       }
       __builtin_amdgcn_sched_barrier(0);
-      multiply_stage<T, ORDER_J, ORDER_I, C::TJ, C::TI, BK, C::NJ, C::NI, SUMS>(SJ1, SI1, j0, i0, acc, with_sums);
-      if (k0 + 2 * BK >= end) break;
+      multiply_stage<T, C, BK, SUMS>(SJ1, SI1, rj, ri, acc, with_sums);
+    }
+    if (stages & 1) {
+      __syncthreads();
+      multiply_stage<T, C, BK, SUMS>(SJ0, SI0, rj, ri, acc, with_sums);
     }
   } else {
     typedef Staging<T, ORDER_J, C::TJ, BK, C::THREADS> LJ;
     typedef Staging<T, ORDER_I, C::TI, BK, C::THREADS> LI;
-    __shared__ __attribute__((aligned(1024))) uint16_t SJ[P * C::TJ * BK], SI[P * C::TI * BK];
     typename LJ::Chunk vj[LJ::CHUNKS];
     typename LI::Chunk vi[LI::CHUNKS];
     sj.load(vj, begin, end, row_j);
     si.load(vi, begin, end, row_i);
     for (int k0 = begin; k0 < end; k0 += BK) {
       __syncthreads();  // everyone is done with the last stage
-      sj.store(vj, SJ, C::TJ * BK);
-      si.store(vi, SI, C::TI * BK);
+      sj.store(vj, SJ0, C::TJ * BK);
+      si.store(vi, SI0, C::TI * BK);
       __syncthreads();
       if (k0 + BK < end) {
         sj.load(vj, k0 + BK, end, row_j);
         si.load(vi, k0 + BK, end, row_i);
       }
       __builtin_amdgcn_sched_barrier(0);
-      multiply_stage<T, ORDER_J, ORDER_I, C::TJ, C::TI, BK, C::NJ, C::NI, SUMS>(SJ, SI, j0, i0, acc, with_sums);
+      multiply_stage<T, C, BK, SUMS>(SJ0, SI0, rj, ri, acc, with_sums);
     }
   }
-}
-
-// For every quad of the wave's outputs: column(c) once per quad of columns, then f(row of the tile, column of the tile, the
-// quad's sums, what column(c) gave) for its rows.
-template <class C, class G, class F>
-__device__ __forceinline__ void for_quads(const Accumulators<C::NJ, C::NI> &acc, G &&column, F &&f) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int j0 = (wave / C::WI) * 32 * C::NJ + (lane & 31), i0 = (wave % C::WI) * 32 * C::NI + 4 * (lane >> 5);
-#pragma unroll
-  for (int i = 0; i < C::NI; ++i)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float4 more = column(i0 + 32 * i + 8 * q);
-#pragma unroll
-      for (int j = 0; j < C::NJ; ++j) {
-        const float v[4] = {acc.v[j][i][4 * q] + more.x, acc.v[j][i][4 * q + 1] + more.y, acc.v[j][i][4 * q + 2] + more.z,
-                            acc.v[j][i][4 * q + 3] + more.w};
-        f(j0 + 32 * j, i0 + 32 * i + 8 * q, v);
-      }
-      __builtin_amdgcn_sched_barrier(0);  // (quad by quad: all of them at once would not fit the registers)
-    }
 }
 
 // four elements of a row from column c on, `columns` exist
@@ -321,6 +343,73 @@ __device__ __forceinline__ void store_quad(typename T::store *row, int c, int co
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (c + e < columns) row[c + e] = T::save(v[e]);
+  }
+}
+
+// Writes a wave's outputs.  A lane holds quads of 32 different rows: written as they are, an instruction would touch 32 lines
+// of memory for 16 bytes each (measured: 22 us for a 256 x 256 tile, a third of its time at a reduction of 2048).  So
+// blocks of 32 rows go through LDS -- 4 KB of the wave's own, chunks permuted as in a stage -- and leave as whole lines.
+//   at(row of the tile) -> the output row, or null;  value(quad's column of the tile, its four sums) changes them in place
+// The caller has passed a barrier behind the last stage; `buffer` holds 4 KB per wave.
+template <class T, class C, int BYTES, class At, class Value>
+__device__ __forceinline__ void write_outputs(const Accumulators<C::NJ, C::NI> &acc, uint16_t *buffer, int first_column,
+                                              int columns, bool wide, At &&at, Value &&value) {
+  typedef typename T::store E;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int j0 = (wave / C::WI) * 32 * C::NJ, i0 = (wave % C::WI) * 32 * C::NI;
+  constexpr int SLAB_ROW = sizeof(E) * 32 * C::NI < 128 ? sizeof(E) * 32 * C::NI : 128;  // bytes of a row that go together
+  constexpr int CHUNKS = SLAB_ROW / 16, PER = 16 / (int)sizeof(E), SLABS = (int)sizeof(E) * 32 * C::NI / SLAB_ROW;
+  constexpr int BLOCKS = C::NI / SLABS;  // 32-column blocks per slab
+  if constexpr (C::WJ * C::WI * 32 * SLAB_ROW > BYTES) {
+#pragma unroll
+    for (int i = 0; i < C::NI; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int j = 0; j < C::NJ; ++j) {
+          const int c = i0 + 32 * i + 8 * q + 4 * (lane >> 5);
+          float v[4] = {acc.v[j][i][4 * q], acc.v[j][i][4 * q + 1], acc.v[j][i][4 * q + 2], acc.v[j][i][4 * q + 3]};
+          value(c, v);
+          E *row = at(j0 + 32 * j + (lane & 31));
+          if (row && first_column + c < columns) store_quad<T>(row, first_column + c, columns, wide, v);
+        }
+  } else {
+    char *own = reinterpret_cast<char *>(buffer) + wave * 32 * SLAB_ROW;
+#pragma unroll
+    for (int j = 0; j < C::NJ; ++j)
+#pragma unroll
+      for (int s = 0; s < SLABS; ++s) {
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < BLOCKS; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int in = 32 * i + 8 * q + 4 * (lane >> 5), b = s * BLOCKS + i;  // column inside the slab
+            float v[4] = {acc.v[j][b][4 * q], acc.v[j][b][4 * q + 1], acc.v[j][b][4 * q + 2], acc.v[j][b][4 * q + 3]};
+            value(i0 + 32 * b + 8 * q + 4 * (lane >> 5), v);
+            const int place = (in / PER) ^ (lane & (CHUNKS - 1));
+            store_quad<T>(reinterpret_cast<E *>(own + (lane & 31) * SLAB_ROW + 16 * place) + in % PER, 0, 4, true, v);
+          }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int r = 0; r < 32; r += 64 / CHUNKS) {
+          const int row = r + lane / CHUNKS, chunk = lane % CHUNKS;
+          const uint4 v = *reinterpret_cast<const uint4 *>(own + row * SLAB_ROW + 16 * (chunk ^ (row & (CHUNKS - 1))));
+          E *dst = at(j0 + 32 * j + row);
+          const int c = first_column + i0 + 32 * BLOCKS * s + PER * chunk;
+          if (!dst || c >= columns) continue;
+          if (wide && c + PER <= columns) {
+            *reinterpret_cast<uint4 *>(dst + c) = v;
+          } else {
+            E e[PER];
+            __builtin_memcpy(e, &v, 16);
+#pragma unroll
+            for (int k = 0; k < PER; ++k)
+              if (c + k < columns) dst[c + k] = e[k];
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);  // (block by block: all of them at once would not fit the registers)
+      }
   }
 }
 

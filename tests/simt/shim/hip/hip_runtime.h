@@ -278,6 +278,8 @@ static inline int simt_readfirstlane(int x) {
 }
 #define __builtin_amdgcn_readfirstlane simt_readfirstlane
 #define __builtin_amdgcn_sched_barrier(x) ((void)0)
+#define __builtin_amdgcn_wave_barrier() ((void)simt::wave_ballot(true))  // (the lanes of a wave are fibers here)
+#define __builtin_amdgcn_sched_group_barrier(mask, size, id) ((void)0)
 #define __builtin_amdgcn_exp2f exp2f  // (v_exp_f32 / v_rcp_f32 are 1 ulp: tolerances, not bits)
 #define __builtin_amdgcn_rcpf(x) (1.0f / (x))
 #define __builtin_amdgcn_rsqf(x) (1.0f / sqrtf(x))
