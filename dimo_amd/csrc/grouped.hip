@@ -124,13 +124,13 @@ __global__ __launch_bounds__(C::THREADS, 2) void grouped_wgrad_kernel(GroupedArg
   si.init_columns(static_cast<const E *>(a.x) + k0, a.ldx, a.K - k0);
   Accumulators<C::NJ, C::NI> acc;
   acc.clear();
-  const bool sums = a.gb && k0 == 0 && (int)(threadIdx.x >> 6) % C::WI == 0;  // (one of the waves that read a row)
+  const bool sums = a.gb && k0 == 0 && wave_number() % C::WI == 0;  // (one of the waves that read a row)
   DIMO_STAGE_BUFFERS(T, C, DIRECT);
   if (begin < end)
     run_stages<T, C, COLUMNS, COLUMNS, DIRECT, true>(sj, si, begin, end, [](int r) { return (int64_t)r; },
                                                      [&](int r) { return source_row(a, r); }, acc, sums, SJ0, SI0, SJ1, SI1);
   __syncthreads();
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = wave_number();
   float *pw = a.partial + (int64_t)chunk * a.N * a.K, *pb = a.partial + (int64_t)a.chunks * a.N * a.K + (int64_t)chunk * a.N;
   E *gw = static_cast<E *>(a.gw) + (int64_t)expert * a.N * a.K, *gb = static_cast<E *>(a.gb) + (int64_t)expert * a.N;
   const auto as_it_is = [](int, float (&)[4]) {};

@@ -125,9 +125,8 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(int64_t rows, int K
 
 // ---- the product -------------------------------------------------------------------------------------------------
 // The tiles and LDS stages of tile_product.hpp with codes as elements: a stage of 64 16-bit words per line is 256 values of
-// k, eight blocks, and a lane's sixteen bytes are exactly one block.  The eight scale bytes of a lane's lines come a
-// stage ahead into registers; a byte permutation leaves those of its half of the wave (blocks 2 s + l / 32), one per
-// instruction.
+// k, eight blocks, and a lane's sixteen bytes are exactly one block.  The scale bytes come
+// through LDS too; a byte permutation leaves those of a lane's half of the wave (blocks 2 s + l / 32), one per instruction.
 struct Mx4Args {
   int R, E, K, N, blocks;
   const uint8_t *xc, *xs, *wc, *ws;
@@ -137,19 +136,28 @@ struct Mx4Args {
   void *y;
 };
 
-// scale bytes of blocks b0 .. b0 + 7 of a line; what is behind its end counts as 2^0 (its codes are zero: a NaN scale must
-// not meet them)
+// Scale bytes of blocks b0 .. b0 + 7 of a line; what is behind its end counts as 2^0 (its codes are zero: a NaN scale must
+// not meet them).  Without a branch: the eight bytes are read from where the line still has eight and shifted down (a
+// branch here would split the stage, and the compiler then moves the stage's matrix instructions behind the next barrier,
+// its operands into scratch).  SHORT: lines of fewer than eight blocks.
+template <bool SHORT>
 __device__ __forceinline__ uint2 load_scales(const uint8_t *line, int b0, int blocks) {
-  uint2 v;
-  if (b0 + 8 <= blocks) {
-    __builtin_memcpy(&v, line + b0, 8);
-    return v;
-  }
-  uint32_t w[2] = {0x7f7f7f7fu, 0x7f7f7f7fu};
+  if constexpr (!SHORT) {
+    const int from = min(b0, blocks - 8), bytes = b0 - from;
+    uint64_t w;
+    __builtin_memcpy(&w, line + from, 8);
+    const uint64_t ones = 0x7f7f7f7f7f7f7f7full;
+    w = bytes >= 8 ? ones : w >> (8 * bytes) | (ones << 1 << (63 - 8 * bytes));
+    return make_uint2((uint32_t)w, (uint32_t)(w >> 32));
+  } else {
+    uint32_t w[2] = {0u, 0u};
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (b0 + e < blocks) w[e >> 2] = (w[e >> 2] & ~(255u << (8 * (e & 3)))) | (uint32_t)line[b0 + e] << (8 * (e & 3));
-  return make_uint2(w[0], w[1]);
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t byte = line[min(b0 + e, blocks - 1)];
+      w[e >> 2] |= (b0 + e < blocks ? byte : 0x7fu) << (8 * (e & 3));
+    }
+    return make_uint2(w[0], w[1]);
+  }
 }
 // bytes half, half + 2, half + 4, half + 6
 __device__ __forceinline__ uint32_t own_scales(uint2 v, int half) {
@@ -161,9 +169,6 @@ __device__ __forceinline__ void multiply_codes(const uint16_t *SJ, const uint16_
                                                const Reader<LINES, C::TJ, 64, C::NJ> &rj, const Reader<LINES, C::TI, 64, C::NI> &ri,
                                                const uint32_t (&sj)[C::NJ], const uint32_t (&si)[C::NI],
                                                Accumulators<C::NJ, C::NI> &acc) {
-  // (the next step's operands ahead of time, as in multiply_stage, where the registers allow it: with 128 sums, the scales
-  // and the addresses a 256 x 256 tile's wave has none left -- spilling it took 1476 us where this takes 698)
-  constexpr bool AHEAD = C::NI * C::NJ <= 4;
   uint4 a[2][C::NI], b[2][C::NJ];
   const auto read = [&](int s) {
 #pragma unroll
@@ -173,29 +178,28 @@ __device__ __forceinline__ void multiply_codes(const uint16_t *SJ, const uint16_
   };
   const auto step = [&](auto byte) {
     constexpr int S = decltype(byte)::value;
-    if (AHEAD && S < 3) read(S + 1);
-    if (!AHEAD) read(S);
+    if (S < 3) read(S + 1);
 #pragma unroll
     for (int j = 0; j < C::NJ; ++j)
 #pragma unroll
       for (int i = 0; i < C::NI; ++i) acc.v[j][i] = mfma_mx4_32x32x64<S>(a[S & 1][i], si[i], b[S & 1][j], sj[j], acc.v[j][i]);
-    if constexpr (AHEAD) interleave<C::NI + C::NJ, C::NI * C::NJ>(S < 3);
+    interleave<C::NI + C::NJ, C::NI * C::NJ>(S < 3);
+    __builtin_amdgcn_sched_barrier(0);  // (or the compiler reads the whole stage first, into registers that are not there)
   };
-  if constexpr (AHEAD) {
-    read(0);
-    __builtin_amdgcn_sched_group_barrier(0x100, C::NI + C::NJ, 0);
-  }
+  read(0);
+  __builtin_amdgcn_sched_barrier(0);
   step(std::integral_constant<int, 0>{});
   step(std::integral_constant<int, 1>{});
   step(std::integral_constant<int, 2>{});
   step(std::integral_constant<int, 3>{});
 }
 
-template <class T, class C>
+template <class T, class C, bool SHORT>
 __global__ __launch_bounds__(C::THREADS, 2) void mx4_rows_kernel(Mx4Args a) {
   typedef typename T::store E;
   constexpr int BK = 64;  // 16-bit words of codes per stage
   __shared__ __attribute__((aligned(1024))) uint16_t SJ0[C::TJ * BK], SI0[C::TI * BK], SJ1[C::TJ * BK], SI1[C::TI * BK];
+  __shared__ uint2 scales[2][C::TJ + C::TI][2];  // [pairs of stages in turn][line][stage of the pair]
   int ct = 0;
   const RowTile tile = find_row_tile(a.offsets, a.E, a.R, C::TJ, (a.N + C::TI - 1) / C::TI, (int)blockIdx.x, &ct);
   if (tile.expert < 0) return;
@@ -208,7 +212,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx4_rows_kernel(Mx4Args a) {
     }
     return;
   }
-  const int end = 8 * a.blocks, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int end = 8 * a.blocks, lane = threadIdx.x & 63, wave = wave_number();
   const int j0 = (wave / C::WI) * 32 * C::NJ, i0 = (wave % C::WI) * 32 * C::NI;
   const auto x_line = [&](int i) { return (int64_t)min(tile.begin + i, tile.end - 1); };
   const auto w_line = [&](int i) { return (int64_t)tile.expert * a.N + min(c0 + i, a.N - 1); };
@@ -216,52 +220,57 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx4_rows_kernel(Mx4Args a) {
   Staging<BF16, LINES, C::TI, BK, C::THREADS> si;
   sj.init_lines([&](int i) { return reinterpret_cast<const uint16_t *>(a.xc) + x_line(i) * end; });
   si.init_lines([&](int i) { return reinterpret_cast<const uint16_t *>(a.wc) + w_line(i) * end; });
-  // scale bytes of this lane's lines: 32-bit offsets from the tile's first line (at most 256 lines of a row's blocks)
-  const uint8_t *xs = a.xs + x_line(0) * a.blocks, *ws = a.ws + w_line(0) * a.blocks;
-  uint32_t lj[C::NJ], li[C::NI];
-#pragma unroll
-  for (int j = 0; j < C::NJ; ++j) lj[j] = (uint32_t)(x_line(j0 + 32 * j + (lane & 31)) - x_line(0)) * a.blocks;
-#pragma unroll
-  for (int i = 0; i < C::NI; ++i) li[i] = (uint32_t)(w_line(i0 + 32 * i + (lane & 31)) - w_line(0)) * a.blocks;
+  // a thread brings one line's scales, two stages of them at a time, into LDS (each wave reading those of its lines from
+  // memory took three times the requests of the codes themselves)
+  const int mine = threadIdx.x % (C::TJ + C::TI);
+  const uint8_t *line = mine < C::TJ ? a.xs + x_line(mine) * a.blocks : a.ws + w_line(mine - C::TJ) * a.blocks;
+  const auto fetch = [&](int b0) {
+    const uint2 lo = load_scales<SHORT>(line, b0, a.blocks), hi = load_scales<SHORT>(line, b0 + 8, a.blocks);
+    return make_uint4(lo.x, lo.y, hi.x, hi.y);
+  };
   const Reader<LINES, C::TJ, BK, C::NJ> rj(j0);
   const Reader<LINES, C::TI, BK, C::NI> ri(i0);
   Accumulators<C::NJ, C::NI> acc;
   acc.clear();
-  uint2 nj[C::NJ], ni[C::NI];  // the next stage's scales
   uint32_t cj[C::NJ], ci[C::NI];
   const auto same = [](int r) { return (int64_t)r; };
   const auto request = [&](uint16_t *SJ, uint16_t *SI, int k0) {
     sj.load_direct(SJ, k0, end, same);
     si.load_direct(SI, k0, end, same);
-#pragma unroll
-    for (int j = 0; j < C::NJ; ++j) nj[j] = load_scales(xs + lj[j], k0 / 8, a.blocks);
-#pragma unroll
-    for (int i = 0; i < C::NI; ++i) ni[i] = load_scales(ws + li[i], k0 / 8, a.blocks);
   };
-  const auto take = [&]() {
+  const auto take = [&](const uint2 (*S)[2], int which) {
 #pragma unroll
-    for (int j = 0; j < C::NJ; ++j) cj[j] = own_scales(nj[j], lane >> 5);
+    for (int j = 0; j < C::NJ; ++j) cj[j] = own_scales(S[j0 + 32 * j + (lane & 31)][which], lane >> 5);
 #pragma unroll
-    for (int i = 0; i < C::NI; ++i) ci[i] = own_scales(ni[i], lane >> 5);
+    for (int i = 0; i < C::NI; ++i) ci[i] = own_scales(S[C::TJ + i0 + 32 * i + (lane & 31)][which], lane >> 5);
+  };
+  const auto put = [&](uint2 (*S)[2], uint4 v) {
+    S[mine][0] = make_uint2(v.x, v.y), S[mine][1] = make_uint2(v.z, v.w);
   };
   const int stages = (end + BK - 1) / BK;
   request(SJ0, SI0, 0);
+  put(scales[0], fetch(0));
+  uint4 next = fetch(16);
   int k0 = 0;
   for (int n = 1; n < stages; n += 2, k0 += 2 * BK) {
     __syncthreads();  // this stage is there, and everyone is done with the other buffer
-    take();
+    take(scales[(n >> 1) & 1], 0);
     request(SJ1, SI1, k0 + BK);
     __builtin_amdgcn_sched_barrier(0);
     multiply_codes<C>(SJ0, SI0, rj, ri, cj, ci, acc);
+    acc.hold();
     __syncthreads();
-    take();
-    if (n + 1 < stages) request(SJ0, SI0, k0 + 2 * BK);
+    take(scales[(n >> 1) & 1], 1);
+    put(scales[((n >> 1) + 1) & 1], next);
+    next = fetch((k0 + 4 * BK) / 8);
+    request(SJ0, SI0, k0 + 2 * BK);  // (behind the end: zeros)
     __builtin_amdgcn_sched_barrier(0);
     multiply_codes<C>(SJ1, SI1, rj, ri, cj, ci, acc);
+    acc.hold();
   }
   if (stages & 1) {
     __syncthreads();
-    take();
+    take(scales[(stages >> 1) & 1], 0);
     multiply_codes<C>(SJ0, SI0, rj, ri, cj, ci, acc);
   }
   const E *bias = a.bias ? static_cast<const E *>(a.bias) + (int64_t)tile.expert * a.N : nullptr;
@@ -278,11 +287,11 @@ typedef Tile<64, 64, 2, 2> Small;
 typedef Tile<128, 128, 2, 2> Medium;
 typedef Tile<256, 256, 2, 4> Large;
 
-template <class T, class C>
+template <class T, class C, bool SHORT>
 int launch_mx4(const Mx4Args &a, hipStream_t s) {
   const int64_t groups = row_tile_workgroups(row_tile_count(a.R, a.E, C::TJ), (a.N + C::TI - 1) / C::TI);
   if (groups > 0x7fffffffLL) return DIMO_E_ARG;
-  hipLaunchKernelGGL((mx4_rows_kernel<T, C>), dim3((unsigned)groups), dim3(C::THREADS), 0, s, a);
+  hipLaunchKernelGGL((mx4_rows_kernel<T, C, SHORT>), dim3((unsigned)groups), dim3(C::THREADS), 0, s, a);
   return check_launch();
 }
 
@@ -347,7 +356,11 @@ extern "C" int dimo_mx4_linear(int dtype, int R, int E, int K, int N, const uint
   int rc = DIMO_OK;
   with_dtype(dtype, [&](auto tag) {
     typedef decltype(tag) T;
-    rc = tile == LARGE ? launch_mx4<T, Large>(a, s) : tile == MEDIUM ? launch_mx4<T, Medium>(a, s) : launch_mx4<T, Small>(a, s);
+    if (a.blocks < 8)
+      rc = tile == SMALL ? launch_mx4<T, Small, true>(a, s) : launch_mx4<T, Medium, true>(a, s);
+    else
+      rc = tile == LARGE ? launch_mx4<T, Large, false>(a, s) : tile == MEDIUM ? launch_mx4<T, Medium, false>(a, s)
+                                                                        : launch_mx4<T, Small, false>(a, s);
   });
   return rc;
 }

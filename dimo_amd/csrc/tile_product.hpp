@@ -17,6 +17,9 @@ namespace dimo {
 
 constexpr bool LINES = true, COLUMNS = false;
 
+// (a scalar: what it leads to stays out of the vector registers)
+__device__ __forceinline__ int wave_number() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
+
 // sixteen zero bytes: what lies behind the end of the reduction is read from here
 __device__ const uint4 zero_chunk = {0u, 0u, 0u, 0u};
 
@@ -124,7 +127,7 @@ struct Staging {
   __device__ __forceinline__ void load_direct(uint16_t *S, int k0, int end, F &&row) const {
 #pragma unroll
     for (int q = 0; q < CHUNKS; ++q)
-      load_to_lds(address(q, k0, end, row), S + (q * THREADS + ((int)threadIdx.x & ~63)) * 8);
+      load_to_lds(address(q, k0, end, row), S + (q * THREADS + 64 * wave_number()) * 8);
   }
   // through registers: any alignment, any end
   typedef E Chunk[8];
@@ -205,6 +208,14 @@ struct Accumulators {
       sums[j] = 0.f;
     }
   }
+  // Ends a stage: the sums are taken to be used here, so the compiler cannot move the stage's matrix instructions (pure to
+  // it) behind the next barrier, where their operands would have to wait in registers that are not there.
+  __device__ __forceinline__ void hold() {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int i = 0; i < NI; ++i) asm volatile("" : "+v"(v[j][i]));
+  }
 };
 
 // Asks the scheduler for one LDS read behind each matrix instruction while there are any (READS of them for PRODUCTS
@@ -281,7 +292,7 @@ __device__ __forceinline__ void run_stages(const Staging<T, ORDER_J, C::TJ, Plan
                                            int end, RowJ &&row_j, RowI &&row_i, Accumulators<C::NJ, C::NI> &acc,
                                            bool with_sums, uint16_t *SJ0, uint16_t *SI0, uint16_t *SJ1, uint16_t *SI1) {
   constexpr int BK = Planes<T>::DEPTH;
-  const int wave = threadIdx.x >> 6;
+  const int wave = wave_number();
   const Reader<ORDER_J, C::TJ, BK, C::NJ> rj((wave / C::WI) * 32 * C::NJ);
   const Reader<ORDER_I, C::TI, BK, C::NI> ri((wave % C::WI) * 32 * C::NI);
   if constexpr (DIRECT) {
@@ -295,13 +306,13 @@ __device__ __forceinline__ void run_stages(const Staging<T, ORDER_J, C::TJ, Plan
       si.load_direct(SI1, k0 + BK, end, row_i);
       __builtin_amdgcn_sched_barrier(0);  // (the loads first: they have this stage's products to arrive under)
       multiply_stage<T, C, BK, SUMS>(SJ0, SI0, rj, ri, acc, with_sums);
+      acc.hold();
       __syncthreads();
-      if (n + 1 < stages) {
-        sj.load_direct(SJ0, k0 + 2 * BK, end, row_j);
-        si.load_direct(SI0, k0 + 2 * BK, end, row_i);
-      }
+      sj.load_direct(SJ0, k0 + 2 * BK, end, row_j);  // (behind the end: zeros; a branch would split the stage)
+      si.load_direct(SI0, k0 + 2 * BK, end, row_i);
       __builtin_amdgcn_sched_barrier(0);
       multiply_stage<T, C, BK, SUMS>(SJ1, SI1, rj, ri, acc, with_sums);
+      acc.hold();
     }
     if (stages & 1) {
       __syncthreads();
@@ -355,7 +366,7 @@ template <class T, class C, int BYTES, class At, class Value>
 __device__ __forceinline__ void write_outputs(const Accumulators<C::NJ, C::NI> &acc, uint16_t *buffer, int first_column,
                                               int columns, bool wide, At &&at, Value &&value) {
   typedef typename T::store E;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = wave_number();
   const int j0 = (wave / C::WI) * 32 * C::NJ, i0 = (wave % C::WI) * 32 * C::NI;
   constexpr int SLAB_ROW = sizeof(E) * 32 * C::NI < 128 ? sizeof(E) * 32 * C::NI : 128;  // bytes of a row that go together
   constexpr int CHUNKS = SLAB_ROW / 16, PER = 16 / (int)sizeof(E), SLABS = (int)sizeof(E) * 32 * C::NI / SLAB_ROW;

@@ -141,7 +141,9 @@ SUBST["experts.hip"] = []
 SUBST["grouped.hip"] = []
 SUBST["mx4.hip"] = []
 SUBST["row_tiles.hpp"] = []
-SUBST["tile_product.hpp"] = []
+SUBST["tile_product.hpp"] = [  # (an empty statement that pins registers)
+    ('asm volatile("" : "+v"(v[j][i]));', ";"),
+]
 SUBST["numeric.hpp"] = [  # gcc 11 has neither 16-bit floating type on x86-64, nor std::bit_cast's builtin
     ("__builtin_bit_cast(float, (uint32_t)v << 16)", "simt_from_bf16(v)"),
     ("__builtin_bit_cast(uint16_t, (__bf16)v)", "simt_to_bf16(v)"),
