@@ -92,19 +92,23 @@ _SIGNATURES = {
                                 + [C.c_size_t, c_ptr]),
     "dimo_route_topk_backward": (C.c_int, [C.c_int] * 4 + [c_ptr, C.c_int64, c_ptr, C.c_int] + [c_ptr] * 6),
     "dimo_group_rows_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int]),
-    "dimo_group_rows": (C.c_int, [C.c_int64, C.c_int] + [c_ptr] * 5 + [C.c_size_t, c_ptr]),
-    "dimo_grouped_linear_forward": (C.c_int, [C.c_int] * 5 + [c_ptr, C.c_int64, C.c_int] + [c_ptr] * 4 + [C.c_int]
+    "dimo_group_rows": (C.c_int, [C.c_int64, C.c_int, C.c_int] + [c_ptr] * 6 + [C.c_size_t, c_ptr]),
+    "dimo_grouped_linear_forward": (C.c_int, [C.c_int] * 5 + [c_ptr, C.c_int64] + [c_ptr] * 4 + [C.c_int]
                                     + [c_ptr] * 3),
-    "dimo_grouped_linear_dgrad": (C.c_int, [C.c_int] * 5 + [c_ptr] * 5),
+    "dimo_grouped_linear_dgrad": (C.c_int, [C.c_int] * 5 + [c_ptr] * 3 + [C.c_int] + [c_ptr] * 3),
     "dimo_grouped_linear_wgrad_workspace_bytes": (C.c_size_t, [C.c_int] * 5),
-    "dimo_grouped_linear_wgrad": (C.c_int, [C.c_int] * 5 + [c_ptr, c_ptr, C.c_int64, C.c_int] + [c_ptr] * 5
+    "dimo_grouped_linear_wgrad": (C.c_int, [C.c_int] * 5 + [c_ptr, c_ptr, C.c_int64] + [c_ptr] * 5
                                   + [C.c_size_t, c_ptr]),
     "dimo_activation_backward": (C.c_int, [C.c_int, C.c_int, C.c_int64] + [c_ptr] * 4),
     "dimo_combine_rows_forward": (C.c_int, [C.c_int] * 3 + [C.c_int64, C.c_int, c_ptr, C.c_int64] + [c_ptr] * 3
                                   + [C.c_int64, c_ptr, c_ptr]),
     "dimo_combine_rows_backward": (C.c_int, [C.c_int] * 3 + [C.c_int64, C.c_int, C.c_int, c_ptr, C.c_int64, c_ptr,
                                                              C.c_int64] + [c_ptr] * 6),
-    "dimo_mx4_quantize": (C.c_int, [C.c_int, C.c_int64, C.c_int, c_ptr, C.c_int64, C.c_int] + [c_ptr] * 4),
+    "dimo_expert_mlp_workspace_bytes": (C.c_size_t, [C.c_void_p, C.c_int]),
+    "dimo_expert_mlp_scratch_bytes": (C.c_size_t, [C.c_void_p]),
+    "dimo_expert_mlp_forward": (C.c_int, [C.c_void_p, C.c_int, c_ptr, c_ptr, C.c_size_t, c_ptr]),
+    "dimo_expert_mlp_backward": (C.c_int, [C.c_void_p, c_ptr, C.c_int64, c_ptr, c_ptr, C.c_size_t] + [c_ptr] * 7),
+    "dimo_mx4_quantize": (C.c_int, [C.c_int, C.c_int64, C.c_int, c_ptr, C.c_int64] + [c_ptr] * 4),
     "dimo_mx4_dequantize": (C.c_int, [C.c_int, C.c_int64, C.c_int] + [c_ptr] * 4),
     "dimo_mx4_linear": (C.c_int, [C.c_int] * 5 + [c_ptr] * 6 + [C.c_int, c_ptr, c_ptr]),
 }

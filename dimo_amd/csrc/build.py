@@ -35,6 +35,7 @@ SOURCES = {
     "executor.hip": [],
     "experts.hip": NO_PACKED_FP32,
     "grouped.hip": NO_PACKED_FP32,
+    "expert_mlp.hip": NO_PACKED_FP32,
     "mx4.hip": NO_PACKED_FP32,
 }
 if os.environ.get("DIMO_BWD_TRACE") == "1":  # per-item trace of the blend backward (tools/bwd_trace.py)

@@ -306,7 +306,8 @@ __global__ __launch_bounds__(GROUP_THREADS) void group_place_kernel(int64_t S, i
                                                                     const int32_t *__restrict__ counts, int blocks,
                                                                     int32_t *__restrict__ offsets,
                                                                     int32_t *__restrict__ order,
-                                                                    int32_t *__restrict__ position) {
+                                                                    int32_t *__restrict__ position, int places,
+                                                                    int32_t *__restrict__ rows) {
   HIP_DYNAMIC_SHARED(int, base)  // [GROUP_WAVES][E + 1]
   __shared__ int wave_total[GROUP_WAVES];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, E1 = E + 1;
@@ -382,6 +383,7 @@ __global__ __launch_bounds__(GROUP_THREADS) void group_place_kernel(int64_t S, i
       const int at = start + __popcll(peers & ((1ull << lane) - 1ull));
       const bool has = key[r] < E;
       order[at] = has ? (int32_t)place : -1;
+      if (rows) rows[at] = has ? (int32_t)place / places : -1;
       position[place] = has ? at : -1;
     }
   }
@@ -527,9 +529,9 @@ extern "C" size_t dimo_group_rows_workspace_bytes(int64_t S, int E) {
   return align_up((size_t)((S + GROUP_CHUNK - 1) / GROUP_CHUNK) * (E + 1) * sizeof(int32_t));
 }
 
-extern "C" int dimo_group_rows(int64_t S, int E, const int32_t *experts, int32_t *offsets, int32_t *order,
-                               int32_t *position, void *workspace, size_t workspace_bytes, void *stream) {
-  if (S < 0 || S > 0x7fffffffLL || E < 1 || E > ROUTE_MAX_E || !offsets) return DIMO_E_ARG;
+extern "C" int dimo_group_rows(int64_t S, int E, int places, const int32_t *experts, int32_t *offsets, int32_t *order,
+                               int32_t *position, int32_t *rows, void *workspace, size_t workspace_bytes, void *stream) {
+  if (S < 0 || S > 0x7fffffffLL || E < 1 || E > ROUTE_MAX_E || places < 1 || !offsets) return DIMO_E_ARG;
   if (S > 0 && (!experts || !order || !position)) return DIMO_E_ARG;
   if (workspace_bytes < dimo_group_rows_workspace_bytes(S, E) || (S > GROUP_CHUNK && !workspace)) return DIMO_E_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
@@ -548,7 +550,7 @@ extern "C" int dimo_group_rows(int64_t S, int E, const int32_t *experts, int32_t
       return check_launch();
   }
   hipLaunchKernelGGL(group_place_kernel, dim3(blocks), dim3(GROUP_THREADS), lds, s, S, E, bits, experts, counts, blocks,
-                     offsets, order, position);
+                     offsets, order, position, places, rows);
   return check_launch();
 }
 

@@ -1,8 +1,8 @@
 // Matrix products grouped by expert, with groups of any size:
 //   forward  y_r = act(W_e x_src(r) + b_e)             rows r of [offsets[e], offsets[e + 1])
-//   dgrad    gx_r = gz_r W_e
+//   dgrad    gx_r = (gz_r W_e) act'(saved_r)           (the slope of the activation that made this product's input)
 //   wgrad    gW_e = sum_r gz_r x_src(r)^T, gb_e = sum_r gz_r
-// x may be read through the grouping's order (src(r) = order[r] / places: the gather of the rows is free), the sizes of
+// x may be read through the grouping (src(r) = rows[r]: the gather of the rows is free), the sizes of
 // the groups stay on the device: a launch has one workgroup per possible tile, and a workgroup finds its (expert, rows)
 // by a scan over the offsets.  Rows behind the last group are written as zeros.
 //
@@ -19,15 +19,15 @@ namespace {
 
 struct GroupedArgs {
   int R, E, K, N;          // rows, experts, width of x, width of y
-  int places;              // > 0: x rows are order[r] / places
   const void *x;           // [., K] rows at ldx
   int64_t ldx;
-  const int32_t *order, *offsets;
+  const int32_t *rows, *offsets;  // rows: x's row of row r, or null
   const void *w;           // [E, N, K]
   const void *bias;        // [E, N] or null
   int act;                 // DIMO_ACT_*
   void *y, *z;             // [R, N]; z: before the activation, or null
   const void *g;           // [R, N] (dgrad, wgrad)
+  const void *saved;       // [R, K] (dgrad, with act): output (relu) or input (silu) of the activation
   void *gx;                // [R, K]
   void *gw, *gb;           // [E, N, K], [E, N] or null
   int wide;                // sixteen bytes of an output row may be written at once
@@ -36,7 +36,7 @@ struct GroupedArgs {
 };
 
 __device__ __forceinline__ int64_t source_row(const GroupedArgs &a, int r) {
-  return a.places > 0 ? a.order[r] / a.places : r;
+  return a.rows ? max(a.rows[r], 0) : r;  // (no row stands behind the last group: offsets that reach there read row 0)
 }
 
 enum { FORWARD = 0, DGRAD = 1 };
@@ -89,14 +89,20 @@ __global__ __launch_bounds__(C::THREADS, 2) void grouped_rows_kernel(GroupedArgs
   const auto out_row = [&](E *matrix) {
     return [=](int j) { return tile.begin + j < tile.end ? matrix + (int64_t)(tile.begin + j) * columns : nullptr; };
   };
-  if (MODE == FORWARD && a.z)
-    write_outputs<T, C, (int)sizeof(SJ0)>(acc, SJ0, c0, columns, a.wide, out_row(static_cast<E *>(a.z)), add_bias);
-  write_outputs<T, C, (int)sizeof(SJ0)>(acc, SJ0, c0, columns, a.wide, out_row(out), [&](int i, float (&v)[4]) {
-    add_bias(i, v);
-    if (MODE == FORWARD && a.act != DIMO_ACT_NONE)
+  if constexpr (MODE == FORWARD) {
+    if (a.z) write_outputs<T, C, (int)sizeof(SJ0)>(acc, SJ0, c0, columns, a.wide, out_row(static_cast<E *>(a.z)), add_bias, NoSlope{});
+    write_outputs<T, C, (int)sizeof(SJ0)>(acc, SJ0, c0, columns, a.wide, out_row(out), [&](int i, float (&v)[4]) {
+      add_bias(i, v);
+      if (a.act != DIMO_ACT_NONE)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = activate(v[e], a.act);
-  });
+        for (int e = 0; e < 4; ++e) v[e] = activate(v[e], a.act);
+    }, NoSlope{});
+  } else if (a.act == DIMO_ACT_NONE) {
+    write_outputs<T, C, (int)sizeof(SJ0)>(acc, SJ0, c0, columns, a.wide, out_row(out), add_bias, NoSlope{});
+  } else {
+    const int64_t away = static_cast<const E *>(a.saved) - out;  // (both [R, K])
+    write_outputs<T, C, (int)sizeof(SJ0)>(acc, SJ0, c0, columns, a.wide, out_row(out), add_bias, Slope{a.act, away});
+  }
 }
 
 // gW[e]: rows n (from g) x columns k (from x), summed over the group's rows -- all of them, or split_rows of them into a
@@ -136,10 +142,10 @@ __global__ __launch_bounds__(C::THREADS, 2) void grouped_wgrad_kernel(GroupedArg
   const auto as_it_is = [](int, float (&)[4]) {};
   if (a.split_rows)
     write_outputs<F32, C, (int)sizeof(SJ0)>(acc, SJ0, k0, a.K, a.wide,
-                                            [&](int j) { return n0 + j < a.N ? pw + (int64_t)(n0 + j) * a.K : nullptr; }, as_it_is);
+                                            [&](int j) { return n0 + j < a.N ? pw + (int64_t)(n0 + j) * a.K : nullptr; }, as_it_is, NoSlope{});
   else
     write_outputs<T, C, (int)sizeof(SJ0)>(acc, SJ0, k0, a.K, a.wide,
-                                          [&](int j) { return n0 + j < a.N ? gw + (int64_t)(n0 + j) * a.K : nullptr; }, as_it_is);
+                                          [&](int j) { return n0 + j < a.N ? gw + (int64_t)(n0 + j) * a.K : nullptr; }, as_it_is, NoSlope{});
   if (sums) {
 #pragma unroll
     for (int j = 0; j < C::NJ; ++j) {
@@ -271,33 +277,33 @@ WgradPlan wgrad_plan(int dtype, int R, int E, int K, int N) {
 
 }  // namespace
 
-extern "C" int dimo_grouped_linear_forward(int dtype, int R, int E, int K, int N, const void *x, int64_t ldx, int places,
-                                           const int32_t *order, const int32_t *offsets, const void *w,
-                                           const void *bias, int act, void *y, void *z, void *stream) {
-  if (bad_shape(dtype, R, E, K, N) || ldx < K || places < 0 || act < DIMO_ACT_NONE || act > DIMO_ACT_SILU) return DIMO_E_ARG;
+extern "C" int dimo_grouped_linear_forward(int dtype, int R, int E, int K, int N, const void *x, int64_t ldx,
+                                           const int32_t *rows, const int32_t *offsets, const void *w, const void *bias, int act, void *y, void *z, void *stream) {
+  if (bad_shape(dtype, R, E, K, N) || ldx < K || act < DIMO_ACT_NONE || act > DIMO_ACT_SILU) return DIMO_E_ARG;
   if (R == 0) return DIMO_OK;
-  if (!x || !offsets || !w || !y || (places > 0 && !order)) return DIMO_E_ARG;
+  if (!x || !offsets || !w || !y) return DIMO_E_ARG;
   hipStream_t s = (hipStream_t)stream;
   clear_errors();
   ScopedTimer timer(T_GROUPED, s);
   GroupedArgs a{};
-  a.R = R, a.E = E, a.K = K, a.N = N, a.places = places, a.x = x, a.ldx = ldx, a.order = order, a.offsets = offsets;
+  a.R = R, a.E = E, a.K = K, a.N = N, a.x = x, a.ldx = ldx, a.rows = rows, a.offsets = offsets;
   a.w = w, a.bias = bias, a.act = act, a.y = y, a.z = z;
   a.wide = wide_output(dtype, y, N) && (!z || wide_output(dtype, z, N));
   return run_rows<FORWARD>(dtype, a, whole_chunks(dtype, x, ldx, K) && whole_chunks(dtype, w, K, K), s);
 }
 
 extern "C" int dimo_grouped_linear_dgrad(int dtype, int R, int E, int K, int N, const void *g, const int32_t *offsets,
-                                         const void *w, void *gx, void *stream) {
-  if (bad_shape(dtype, R, E, K, N)) return DIMO_E_ARG;
+                                         const void *w, int act, const void *saved, void *gx, void *stream) {
+  if (bad_shape(dtype, R, E, K, N) || act < DIMO_ACT_NONE || act > DIMO_ACT_SILU) return DIMO_E_ARG;
   if (R == 0) return DIMO_OK;
-  if (!g || !offsets || !w || !gx) return DIMO_E_ARG;
+  if (!g || !offsets || !w || !gx || (act != DIMO_ACT_NONE && !saved)) return DIMO_E_ARG;
   hipStream_t s = (hipStream_t)stream;
   clear_errors();
   ScopedTimer timer(T_GROUPED, s);
   GroupedArgs a{};
   a.R = R, a.E = E, a.K = K, a.N = N, a.offsets = offsets, a.w = w, a.g = g, a.gx = gx;
-  a.wide = wide_output(dtype, gx, K);
+  a.act = act, a.saved = saved;
+  a.wide = wide_output(dtype, gx, K) && (act == DIMO_ACT_NONE || wide_output(dtype, saved, K));
   return run_rows<DGRAD>(dtype, a, whole_chunks(dtype, g, N, N) && whole_chunks(dtype, w, K, K), s);
 }
 
@@ -306,17 +312,17 @@ extern "C" size_t dimo_grouped_linear_wgrad_workspace_bytes(int dtype, int R, in
 }
 
 extern "C" int dimo_grouped_linear_wgrad(int dtype, int R, int E, int K, int N, const void *g, const void *x, int64_t ldx,
-                                         int places, const int32_t *order, const int32_t *offsets, void *gw, void *gb,
+                                         const int32_t *rows, const int32_t *offsets, void *gw, void *gb,
                                          void *workspace, size_t workspace_bytes, void *stream) {
-  if (bad_shape(dtype, R, E, K, N) || ldx < K || places < 0 || !offsets || !gw) return DIMO_E_ARG;
-  if (R > 0 && (!g || !x || (places > 0 && !order))) return DIMO_E_ARG;
+  if (bad_shape(dtype, R, E, K, N) || ldx < K || !offsets || !gw) return DIMO_E_ARG;
+  if (R > 0 && (!g || !x)) return DIMO_E_ARG;
   const WgradPlan plan = wgrad_plan(dtype, R, E, K, N);
   if (workspace_bytes < plan.bytes || (plan.bytes && (!workspace || !aligned16(workspace)))) return DIMO_E_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
   clear_errors();
   ScopedTimer timer(T_GROUPED, s);
   GroupedArgs a{};
-  a.R = R, a.E = E, a.K = K, a.N = N, a.places = places, a.x = x, a.ldx = ldx, a.order = order, a.offsets = offsets;
+  a.R = R, a.E = E, a.K = K, a.N = N, a.x = x, a.ldx = ldx, a.rows = rows, a.offsets = offsets;
   a.g = g, a.gw = gw, a.gb = gb, a.wide = wide_output(dtype, gw, K);
   a.split_rows = plan.split_rows, a.chunks = plan.chunks, a.partial = static_cast<float *>(workspace);
   const bool direct = whole_chunks(dtype, g, N, N) && whole_chunks(dtype, x, ldx, K);

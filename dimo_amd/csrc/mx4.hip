@@ -34,10 +34,10 @@ __device__ __forceinline__ float e8m0_value(uint32_t byte) {
 // wave reads and writes whole lines; the block's largest magnitude takes two exchanges.
 struct QuantArgs {
   int64_t rows;
-  int K, blocks, places;   // blocks of 32 per row; places > 0: row r is order[r] / places of x (-1: zeros)
+  int K, blocks;           // blocks of 32 per row
   const void *x;
   int64_t ldx;
-  const int32_t *order;
+  const int32_t *from;     // x's row of row r (negative: zeros), or null
   uint8_t *codes, *scales; // [rows, 16 blocks], [rows, blocks]
 };
 template <class T, bool WIDE>
@@ -48,11 +48,7 @@ __global__ __launch_bounds__(256) void mx4_quantize_kernel(QuantArgs a) {
   const bool in = i < total;
   const int64_t row = in ? i / (4 * a.blocks) : 0;
   const int col = in ? 8 * (int)(i % (4 * a.blocks)) : 0;
-  int64_t src = row;
-  if (a.places > 0) {
-    const int32_t o = in ? a.order[row] : -1;
-    src = o < 0 ? -1 : o / a.places;
-  }
+  const int64_t src = a.from ? (in ? a.from[row] : -1) : row;
   float v[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = 0.f;
@@ -280,7 +276,8 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx4_rows_kernel(Mx4Args a) {
       [&](int i, float (&v)[4]) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = activate(v[e] + (bias ? T::load(bias[min(c0 + i + e, a.N - 1)]) : 0.f), a.act);
-      });
+      },
+      NoSlope{});
 }
 
 typedef Tile<64, 64, 2, 2> Small;
@@ -297,15 +294,15 @@ int launch_mx4(const Mx4Args &a, hipStream_t s) {
 
 }  // namespace
 
-extern "C" int dimo_mx4_quantize(int dtype, int64_t rows, int K, const void *x, int64_t ldx, int places,
-                                 const int32_t *order, uint8_t *codes, uint8_t *scales, void *stream) {
-  if (!known_dtype(dtype) || rows < 0 || K < 1 || ldx < K || places < 0) return DIMO_E_ARG;
+extern "C" int dimo_mx4_quantize(int dtype, int64_t rows, int K, const void *x, int64_t ldx,
+                                 const int32_t *from, uint8_t *codes, uint8_t *scales, void *stream) {
+  if (!known_dtype(dtype) || rows < 0 || K < 1 || ldx < K) return DIMO_E_ARG;
   if (rows == 0) return DIMO_OK;
-  if (!x || !codes || !scales || (places > 0 && !order) || (reinterpret_cast<uintptr_t>(codes) & 3)) return DIMO_E_ARG;
+  if (!x || !codes || !scales || (reinterpret_cast<uintptr_t>(codes) & 3)) return DIMO_E_ARG;
   hipStream_t s = (hipStream_t)stream;
   clear_errors();
   ScopedTimer timer(T_MX4, s);
-  const QuantArgs a{rows, K, (K + 31) / 32, places, x, ldx, order, codes, scales};
+  const QuantArgs a{rows, K, (K + 31) / 32, x, ldx, from, codes, scales};
   const int64_t grid = (rows * a.blocks * 4 + 255) / 256;
   if (grid > 0x7fffffffLL) return DIMO_E_ARG;
   with_dtype(dtype, [&](auto tag) {

@@ -357,14 +357,25 @@ __device__ __forceinline__ void store_quad(typename T::store *row, int c, int co
   }
 }
 
+// What happens to an output on its way out, behind the rounding to its type: nothing, or the multiplication by the slope of
+// an activation whose saved values lie `away` elements from the outputs.
+struct NoSlope {
+  static constexpr bool ON = false;
+};
+struct Slope {
+  static constexpr bool ON = true;
+  int act;
+  int64_t away;
+};
+
 // Writes a wave's outputs.  A lane holds quads of 32 different rows: written as they are, an instruction would touch 32 lines
 // of memory for 16 bytes each (measured: 22 us for a 256 x 256 tile, a third of its time at a reduction of 2048).  So
 // blocks of 32 rows go through LDS -- 4 KB of the wave's own, chunks permuted as in a stage -- and leave as whole lines.
 //   at(row of the tile) -> the output row, or null;  value(quad's column of the tile, its four sums) changes them in place
 // The caller has passed a barrier behind the last stage; `buffer` holds 4 KB per wave.
-template <class T, class C, int BYTES, class At, class Value>
+template <class T, class C, int BYTES, class At, class Value, class Out>
 __device__ __forceinline__ void write_outputs(const Accumulators<C::NJ, C::NI> &acc, uint16_t *buffer, int first_column,
-                                              int columns, bool wide, At &&at, Value &&value) {
+                                              int columns, bool wide, At &&at, Value &&value, Out slope) {
   typedef typename T::store E;
   const int lane = threadIdx.x & 63, wave = wave_number();
   const int j0 = (wave / C::WI) * 32 * C::NJ, i0 = (wave % C::WI) * 32 * C::NI;
@@ -382,7 +393,12 @@ __device__ __forceinline__ void write_outputs(const Accumulators<C::NJ, C::NI> &
           float v[4] = {acc.v[j][i][4 * q], acc.v[j][i][4 * q + 1], acc.v[j][i][4 * q + 2], acc.v[j][i][4 * q + 3]};
           value(c, v);
           E *row = at(j0 + 32 * j + (lane & 31));
-          if (row && first_column + c < columns) store_quad<T>(row, first_column + c, columns, wide, v);
+          if (!row || first_column + c >= columns) continue;
+          if constexpr (Out::ON)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (first_column + c + e < columns) v[e] *= activation_slope(T::load(row[first_column + c + e + slope.away]), slope.act);
+          store_quad<T>(row, first_column + c, columns, wide, v);
         }
   } else {
     char *own = reinterpret_cast<char *>(buffer) + wave * 32 * SLAB_ROW;
@@ -410,13 +426,28 @@ __device__ __forceinline__ void write_outputs(const Accumulators<C::NJ, C::NI> &
           const int c = first_column + i0 + 32 * BLOCKS * s + PER * chunk;
           if (!dst || c >= columns) continue;
           if (wide && c + PER <= columns) {
-            *reinterpret_cast<uint4 *>(dst + c) = v;
+            if constexpr (Out::ON) {
+              float f[PER], at_saved[PER];
+              Vec16<T> q{v};
+              q.get(f);
+              load_vec<T, PER>(dst + c + slope.away, at_saved);
+#pragma unroll
+              for (int k = 0; k < PER; ++k) f[k] *= activation_slope(at_saved[k], slope.act);
+              store_vec<T, PER>(dst + c, f);
+            } else {
+              *reinterpret_cast<uint4 *>(dst + c) = v;
+            }
           } else {
             E e[PER];
             __builtin_memcpy(e, &v, 16);
 #pragma unroll
-            for (int k = 0; k < PER; ++k)
-              if (c + k < columns) dst[c + k] = e[k];
+            for (int k = 0; k < PER; ++k) {
+              if (c + k >= columns) continue;
+              if constexpr (Out::ON)
+                dst[c + k] = T::save(T::load(e[k]) * activation_slope(T::load(dst[c + k + slope.away]), slope.act));
+              else
+                dst[c + k] = e[k];
+            }
           }
         }
         __builtin_amdgcn_sched_barrier(0);  // (block by block: all of them at once would not fit the registers)

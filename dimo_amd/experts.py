@@ -15,6 +15,8 @@ Types: fp32, bf16, fp16 (all tensors of a call alike; routing weights, load and 
 the groups stay on the device: no call synchronises, every call may be captured into a graph.  All calls run on the
 current stream of the tensors' device.  GPU only.
 """
+import ctypes as C
+
 import torch
 from torch import nn
 
@@ -144,25 +146,20 @@ def route_topk(logits, k, row_mask=None, normalize=True):
 class RowGroups:
     """Rows grouped by expert.  offsets [E + 1] int32: expert e owns rows offsets[e] .. offsets[e + 1] - 1 (offsets[0]
     = 0); rows behind offsets[E] belong to nobody.  From `group_rows` also order [T k] (which place a row came from) and
-    position [T, k] (which row a place went to; -1: none)."""
+    position [T, k] (which row a place went to; -1: none); rows [T k] = order / k."""
 
-    __slots__ = ("offsets", "order", "position")
+    __slots__ = ("offsets", "order", "position", "rows")
 
-    def __init__(self, offsets, order=None, position=None):
+    def __init__(self, offsets):
         if offsets.dim() != 1 or offsets.dtype != torch.int32 or not offsets.is_contiguous():
             raise ValueError("offsets: contiguous int32 [E + 1] expected")
         if not 2 <= offsets.shape[0] <= MAX_EXPERTS + 1:
             raise ValueError(f"1 to {MAX_EXPERTS} groups expected")
-        self.offsets, self.order, self.position = offsets, order, position
+        self.offsets, self.order, self.position, self.rows = offsets, None, None, None
 
     @property
     def num_experts(self):
         return self.offsets.shape[0] - 1
-
-    @property
-    def places(self):
-        """Places per row of what was routed (k), 0 without a routing."""
-        return 0 if self.position is None else self.position.shape[1]
 
 
 def group_rows(experts, num_experts):
@@ -178,15 +175,16 @@ def group_rows(experts, num_experts):
     if S > 0x7FFFFFFF:
         raise ValueError("more than 2^31 - 1 places")
     L = _lib.lib()
-    offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=device)
-    order = torch.empty(S, dtype=torch.int32, device=device)
-    position = torch.empty(experts.shape, dtype=torch.int32, device=device)
+    groups = RowGroups(torch.empty(num_experts + 1, dtype=torch.int32, device=device))
+    groups.order, groups.rows = torch.empty(2, S, dtype=torch.int32, device=device)
+    groups.position = torch.empty(experts.shape, dtype=torch.int32, device=device)
     with _on(device):
         nbytes = L.dimo_group_rows_workspace_bytes(S, num_experts)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-        _lib.check(L.dimo_group_rows(S, num_experts, experts.data_ptr(), offsets.data_ptr(), order.data_ptr(),
-                                     position.data_ptr(), _lib.ptr(ws), nbytes, _lib.current_stream()), "dimo_group_rows")
-    return RowGroups(offsets, order, position)
+        _lib.check(L.dimo_group_rows(S, num_experts, experts.shape[1], experts.data_ptr(), groups.offsets.data_ptr(),
+                                     groups.order.data_ptr(), groups.position.data_ptr(), groups.rows.data_ptr(),
+                                     _lib.ptr(ws), nbytes, _lib.current_stream()), "dimo_group_rows")
+    return groups
 
 
 # ------------------------------------------------------------------------------------------------ grouped products
@@ -197,9 +195,8 @@ def _linear_forward(x, weight, bias, groups, act, gather, save_z):
     z = torch.empty_like(y) if save_z else None
     with _on(x.device):
         _lib.check(_lib.lib().dimo_grouped_linear_forward(
-            _DTYPES[x.dtype], R, E, K, N, x.data_ptr(), _ld(x), groups.places if gather else 0,
-            _lib.ptr(groups.order) if gather else None, groups.offsets.data_ptr(), weight.data_ptr(), _lib.ptr(bias), act,
-            y.data_ptr(), _lib.ptr(z), _lib.current_stream()), "dimo_grouped_linear_forward")
+            _DTYPES[x.dtype], R, E, K, N, x.data_ptr(), _ld(x), groups.rows.data_ptr() if gather else None,
+            groups.offsets.data_ptr(), weight.data_ptr(), _lib.ptr(bias), act, y.data_ptr(), _lib.ptr(z), _lib.current_stream()), "dimo_grouped_linear_forward")
     return y, z
 
 
@@ -208,8 +205,8 @@ def _linear_dgrad(g, weight, groups):
     gx = torch.empty(g.shape[0], K, dtype=g.dtype, device=g.device)
     with _on(g.device):
         _lib.check(_lib.lib().dimo_grouped_linear_dgrad(
-            _DTYPES[g.dtype], g.shape[0], E, K, N, g.data_ptr(), groups.offsets.data_ptr(), weight.data_ptr(), gx.data_ptr(),
-            _lib.current_stream()), "dimo_grouped_linear_dgrad")
+            _DTYPES[g.dtype], g.shape[0], E, K, N, g.data_ptr(), groups.offsets.data_ptr(), weight.data_ptr(), 0, None,
+            gx.data_ptr(), _lib.current_stream()), "dimo_grouped_linear_dgrad")
     return gx
 
 
@@ -222,8 +219,8 @@ def _linear_wgrad(g, x, shape, groups, gather, need_bias):
         nbytes = L.dimo_grouped_linear_wgrad_workspace_bytes(_DTYPES[g.dtype], g.shape[0], E, K, N)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=g.device) if nbytes else None
         _lib.check(L.dimo_grouped_linear_wgrad(
-            _DTYPES[g.dtype], g.shape[0], E, K, N, g.data_ptr(), x.data_ptr(), _ld(x), groups.places if gather else 0,
-            _lib.ptr(groups.order) if gather else None, groups.offsets.data_ptr(), gw.data_ptr(), _lib.ptr(gb),
+            _DTYPES[g.dtype], g.shape[0], E, K, N, g.data_ptr(), x.data_ptr(), _ld(x),
+            groups.rows.data_ptr() if gather else None, groups.offsets.data_ptr(), gw.data_ptr(), _lib.ptr(gb),
             _lib.ptr(ws), nbytes, _lib.current_stream()), "dimo_grouped_linear_wgrad")
     return gw, gb
 
@@ -369,14 +366,85 @@ def combine_rows(y, groups, weights=None, residual=None):
     return _combine_forward(y, weights, groups, residual)
 
 
+class _ExpertMlpDesc(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("dtype", "T", "K", "F", "E", "k", "act")] + [("ld_x", C.c_int64), ("ld_logits", C.c_int64)] \
+        + [(n, C.c_void_p) for n in ("x", "logits", "w1", "b1", "w2", "b2", "row_mask")]
+
+
+def _expert_mlp_desc(x, logits, w1, b1, w2, b2, row_mask, k, act):
+    return _ExpertMlpDesc(_DTYPES[x.dtype], x.shape[0], x.shape[1], w1.shape[1], w1.shape[0], k, act, _ld(x), _ld(logits),
+                          x.data_ptr(), logits.data_ptr(), w1.data_ptr(), _lib.ptr(b1), w2.data_ptr(), _lib.ptr(b2),
+                          _lib.ptr(row_mask))
+
+
+def _expert_mlp_forward(x, logits, w1, b1, w2, b2, row_mask, k, act, keep):
+    L, d = _lib.lib(), _expert_mlp_desc(x, logits, w1, b1, w2, b2, row_mask, k, act)
+    at = C.addressof(d)
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    with _on(x.device):
+        nbytes = L.dimo_expert_mlp_workspace_bytes(at, keep)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        _lib.check(L.dimo_expert_mlp_forward(at, keep, out.data_ptr(), ws.data_ptr(), nbytes, _lib.current_stream()),
+                   "dimo_expert_mlp_forward")
+    return out, ws
+
+
+class _ExpertMlp(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, logits, w1, b1, w2, b2, row_mask, k, act):
+        out, ws = _expert_mlp_forward(x, logits, w1, b1, w2, b2, row_mask, k, act, True)
+        ctx.save_for_backward(x, logits, w1, b1, w2, b2, row_mask, ws)
+        ctx.k, ctx.act = k, act
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        *tensors, ws = ctx.saved_tensors
+        x, logits, w1, b1, w2, b2, _ = tensors
+        L, d = _lib.lib(), _expert_mlp_desc(*tensors, ctx.k, ctx.act)
+        at, need = C.addressof(d), ctx.needs_input_grad
+        g = _rows(g)
+        # (a bias gradient comes with its weight's)
+        wanted = [need[0], need[1], need[2] or need[3], need[3], need[4] or need[5], need[5]]
+        grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if on else None
+                 for t, on in zip((x, logits, w1, b1, w2, b2), wanted)]
+        with _on(x.device):
+            nbytes = L.dimo_expert_mlp_scratch_bytes(at)
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+            _lib.check(L.dimo_expert_mlp_backward(at, g.data_ptr(), _ld(g), ws.data_ptr(), scratch.data_ptr(), nbytes,
+                                                  *[_lib.ptr(t) for t in grads], _lib.current_stream()),
+                       "dimo_expert_mlp_backward")
+        return (*[t if on else None for t, on in zip(grads, need)], None, None, None)
+
+
 def expert_mlp(x, logits, w1, b1, w2, b2, k, activation="relu", row_mask=None):
-    """x + sum over a row's k experts of weight * (w2 activation(w1 x + b1) + b2): routing, both products and the sum.
-    x [T, K], logits [T, E], w1 [E, F, K], b1 [E, F], w2 [E, K, F], b2 [E, K].  Differentiable in all of them."""
-    weights, experts, _ = route_topk(logits, k, row_mask)
-    groups = group_rows(experts, logits.shape[1])
-    h = grouped_linear(x, w1, groups, b1, activation, gather=True)
-    y = grouped_linear(h, w2, groups, b2)
-    return combine_rows(y, groups, weights, residual=x)
+    """x + sum over a row's k experts of weight * (w2 activation(w1 x + b1) + b2): routing (weights normalised over the
+    chosen), both products and the sum as one call per direction -- what route_topk, group_rows, grouped_linear (gathering,
+    then plain) and combine_rows give one by one.  x [T, K], logits [T, E], w1 [E, F, K], b1 [E, F] or None, w2 [E, K, F],
+    b2 [E, K] or None; row_mask [T]: rows with False come back as they are.  Differentiable in x, logits and the weights."""
+    if x.dim() != 2 or logits.dim() != 2 or w1.dim() != 3:
+        raise ValueError("x: [T, K], logits: [T, E] and w1: [E, F, K] expected")
+    _gpu(x, logits, w1, b1, w2, b2, row_mask)
+    _dtype(x, "x")
+    (T, K), (E, F, _) = x.shape, w1.shape
+    for t, shape, what in ((logits, (T, E), "logits: [T, E]"), (w1, (E, F, K), "w1: [E, F, K]"), (w2, (E, K, F), "w2: [E, K, F]"),
+                           (b1, (E, F), "b1: [E, F]"), (b2, (E, K), "b2: [E, K]")):
+        if t is not None and (t.shape != shape or t.dtype != x.dtype):
+            raise ValueError(f"{what} of x's type expected")
+    if not 1 <= k <= E <= MAX_EXPERTS or K < 1 or F < 1 or T * k > 0x7FFFFFFF:
+        raise ValueError(f"1 <= k <= E <= {MAX_EXPERTS} and fewer than 2^31 places expected")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"activation: one of {list(_ACTIVATIONS)} expected")
+    if row_mask is not None:
+        if row_mask.dtype != torch.bool or row_mask.shape != (T,):
+            raise ValueError("row_mask: bool [T] expected")
+        row_mask = row_mask.contiguous()
+    x, logits, w1, w2 = _rows(x), _rows(logits), w1.contiguous(), w2.contiguous()
+    b1, b2 = None if b1 is None else b1.contiguous(), None if b2 is None else b2.contiguous()
+    if _tracked(x, logits, w1, b1, w2, b2):
+        return _ExpertMlp.apply(x, logits, w1, b1, w2, b2, row_mask, k, _ACTIVATIONS[activation])
+    return _expert_mlp_forward(x, logits, w1, b1, w2, b2, row_mask, k, _ACTIVATIONS[activation], False)[0]
 
 
 class ExpertMLP(nn.Module):

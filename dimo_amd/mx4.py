@@ -64,18 +64,18 @@ def quantize_mx4(x, groups=None):
     x = x.detach()
     K, lead = x.shape[-1], x.shape[:-1]
     flat = _rows(x) if x.dim() == 2 else x.contiguous().view(-1, K)
-    rows, places, order = flat.shape[0], 0, None
+    rows, source = flat.shape[0], None
     if groups is not None:
         if groups.position is None or x.dim() != 2 or x.shape[0] != groups.position.shape[0]:
             raise ValueError("groups of these rows, made by group_rows, expected")
         _gpu(x, groups.order)
-        rows, places, order = groups.order.shape[0], groups.places, groups.order
+        rows, source = groups.rows.shape[0], groups.rows
         lead = (rows,)
     blocks = -(-K // 32)
     codes = torch.empty(*lead, 16 * blocks, dtype=torch.uint8, device=x.device)
     scales = torch.empty(*lead, blocks, dtype=torch.uint8, device=x.device)
     with _on(x.device):
-        _lib.check(_lib.lib().dimo_mx4_quantize(dtype, rows, K, flat.data_ptr(), _ld(flat), places, _lib.ptr(order),
+        _lib.check(_lib.lib().dimo_mx4_quantize(dtype, rows, K, flat.data_ptr(), _ld(flat), _lib.ptr(source),
                                                 codes.data_ptr(), scales.data_ptr(), _lib.current_stream()),
                    "dimo_mx4_quantize")
     return MX4(codes, scales, K)

@@ -466,23 +466,24 @@ int dimo_route_topk_backward(int T, int E, int k, int dtype, const void *logits,
                              int normalize, const float *weights, const int32_t *experts, const float *g_weights,
                              const float *g_load, void *g_logits, void *stream);
 /* Stable grouping of S places by expert: offsets [E + 1], order [S] (the places, group after group; -1 behind the last
- * group), position [S] (its inverse; -1 for a place whose expert is outside 0 .. E-1). */
+ * group), position [S] (its inverse; -1 for a place whose expert is outside 0 .. E-1), rows [S] or NULL: order / places. */
 size_t dimo_group_rows_workspace_bytes(int64_t S, int E);
-int dimo_group_rows(int64_t S, int E, const int32_t *experts, int32_t *offsets, int32_t *order, int32_t *position,
-                    void *workspace, size_t workspace_bytes, void *stream);
+int dimo_group_rows(int64_t S, int E, int places, const int32_t *experts, int32_t *offsets, int32_t *order,
+                    int32_t *position, int32_t *rows, void *workspace, size_t workspace_bytes, void *stream);
 /* y[r] = act(w[e] x[src(r)] + bias[e]) for rows r in [offsets[e], offsets[e + 1]), zeros behind the last group.
- * x: rows at ldx; places > 0: src(r) = order[r] / places, otherwise r.  w [E, N, K], bias [E, N] or NULL, y [R, N];
+ * x: rows at ldx; src(r) = rows[r], or r without rows.  w [E, N, K], bias [E, N] or NULL, y [R, N];
  * z [R, N] or NULL: the value before the activation. */
-int dimo_grouped_linear_forward(int dtype, int R, int E, int K, int N, const void *x, int64_t ldx, int places,
-                                const int32_t *order, const int32_t *offsets, const void *w, const void *bias, int act,
+int dimo_grouped_linear_forward(int dtype, int R, int E, int K, int N, const void *x, int64_t ldx,
+                                const int32_t *rows, const int32_t *offsets, const void *w, const void *bias, int act,
                                 void *y, void *z, void *stream);
-/* gx[r] = g[r] w[e] (g [R, N], gx [R, K] in the order of the groups) */
+/* gx[r] = g[r] w[e] (g [R, N], gx [R, K] in the order of the groups); act: times the slope of the activation that made
+ * this product's input, from saved [R, K] (its output for relu, its input for silu) */
 int dimo_grouped_linear_dgrad(int dtype, int R, int E, int K, int N, const void *g, const int32_t *offsets, const void *w,
-                              void *gx, void *stream);
+                              int act, const void *saved, void *gx, void *stream);
 /* gw[e] = sum of g[r]^T x[src(r)], gb[e] = sum of g[r] (gb may be NULL) over the rows of the group */
 size_t dimo_grouped_linear_wgrad_workspace_bytes(int dtype, int R, int E, int K, int N);
-int dimo_grouped_linear_wgrad(int dtype, int R, int E, int K, int N, const void *g, const void *x, int64_t ldx, int places,
-                              const int32_t *order, const int32_t *offsets, void *gw, void *gb, void *workspace,
+int dimo_grouped_linear_wgrad(int dtype, int R, int E, int K, int N, const void *g, const void *x, int64_t ldx,
+                              const int32_t *rows, const int32_t *offsets, void *gw, void *gb, void *workspace,
                               size_t workspace_bytes, void *stream);
 /* out = g * act'(saved): saved = the activation's output for relu, its input for silu; n elements */
 int dimo_activation_backward(int dtype, int act, int64_t n, const void *g, const void *saved, void *out, void *stream);
@@ -494,11 +495,28 @@ int dimo_combine_rows_forward(int T, int k, int N, int64_t S, int dtype, const v
 int dimo_combine_rows_backward(int T, int k, int N, int64_t S, int E, int dtype, const void *g_out, int64_t ldg,
                                const void *y, int64_t ldy, const float *weights, const int32_t *position,
                                const int32_t *offsets, void *g_y, float *g_weights, void *stream);
+/* The expert block in one call per direction: out = x + sum over a row's k experts of weight * (w2 act(w1 x + b1) + b2),
+ * weights normalised over the chosen.  x [T, K] at ld_x, logits [T, E] at ld_logits, w1 [E, F, K], b1 [E, F] or NULL,
+ * w2 [E, K, F], b2 [E, K] or NULL, row_mask [T] or NULL (rows with 0: out = x).  keep: the workspace will be handed to the
+ * backward, which reads it (and x, logits, the weights) unchanged; any gradient may be NULL (g_b* only with their g_w*). */
+typedef struct dimo_expert_mlp_desc {
+  int dtype, T, K, F, E, k, act;
+  int64_t ld_x, ld_logits;
+  const void *x, *logits, *w1, *b1, *w2, *b2;
+  const uint8_t *row_mask;
+} dimo_expert_mlp_desc;
+size_t dimo_expert_mlp_workspace_bytes(const dimo_expert_mlp_desc *desc, int keep);
+size_t dimo_expert_mlp_scratch_bytes(const dimo_expert_mlp_desc *desc);
+int dimo_expert_mlp_forward(const dimo_expert_mlp_desc *desc, int keep, void *out, void *workspace, size_t workspace_bytes,
+                            void *stream);
+int dimo_expert_mlp_backward(const dimo_expert_mlp_desc *desc, const void *g_out, int64_t ld_g, const void *workspace,
+                             void *scratch, size_t scratch_bytes, void *g_x, void *g_logits, void *g_w1, void *g_b1,
+                             void *g_w2, void *g_b2, void *stream);
 /* Microscaled 4-bit floating point: e2m1 elements in blocks of 32 along a row, one scale byte (2^(byte - 127), 255 = NaN)
  * per block.  codes [rows, 16 ceil(K / 32)] (two to a byte, low four bits first), scales [rows, ceil(K / 32)].
- * x: rows at ldx; places > 0: row r is order[r] / places of x, zeros where order[r] is negative. */
-int dimo_mx4_quantize(int dtype, int64_t rows, int K, const void *x, int64_t ldx, int places, const int32_t *order,
-                      uint8_t *codes, uint8_t *scales, void *stream);
+ * x: rows at ldx; from [rows] or NULL: row r is x's row from[r], zeros where that is negative. */
+int dimo_mx4_quantize(int dtype, int64_t rows, int K, const void *x, int64_t ldx, const int32_t *from, uint8_t *codes,
+                      uint8_t *scales, void *stream);
 int dimo_mx4_dequantize(int dtype, int64_t rows, int K, const uint8_t *codes, const uint8_t *scales, void *out, void *stream);
 /* y[r] = act(w[e] x[r] + bias[e]) of quantised x [R, K] and w [E, N, K]; offsets as in dimo_grouped_linear_forward, or NULL
  * with E = 1; dtype: of y and bias.  Both code arrays on 16-byte boundaries. */

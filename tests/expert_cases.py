@@ -278,6 +278,34 @@ def check_combine(ex, device, T, k, E, N, dtype, weighted=True, residual=True, p
 
 
 # ------------------------------------------------------------------------------------------------------ used together
+def check_layer_is_its_parts(ex, device, T, K, F, E, k, dtype, act, biases=True, seed=0):
+    """expert_mlp gives what its operators give one by one: the forward bit by bit, the gradients within one more rounding
+    of the hidden gradient (the slope is applied behind its rounding in the one, in a pass of its own in the other)."""
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s, scale=1.0: (scale * torch.randn(*s, generator=g)).to(dtype).to(device).requires_grad_(True)
+    x, z, w1, w2 = r(T, K), r(T, E), r(E, F, K, scale=K ** -0.5), r(E, K, F, scale=F ** -0.5)
+    b1, b2 = (r(E, F), r(E, K)) if biases else (None, None)
+    mask = (torch.rand(T, generator=g) > 0.25).to(device)
+    go = torch.randn(T, K, generator=g).to(dtype).to(device)
+    leaves = [t for t in (x, z, w1, b1, w2, b2) if t is not None]
+    one = ex.expert_mlp(x, z, w1, b1, w2, b2, k, act, mask)
+    with torch.no_grad():
+        assert torch.equal(ex.expert_mlp(x, z, w1, b1, w2, b2, k, act, mask), one)
+    g_one = torch.autograd.grad(one, leaves, go)
+    weights, experts, _ = ex.route_topk(z, k, mask)
+    groups = ex.group_rows(experts, E)
+    h = ex.grouped_linear(x, w1, groups, b1, act, gather=True)
+    two = ex.combine_rows(ex.grouped_linear(h, w2, groups, b2), groups, weights, residual=x)
+    g_two = torch.autograd.grad(two, leaves, go)
+    assert torch.equal(one, two)
+    for a, b in zip(g_one, g_two):
+        assert a.shape == b.shape and a.dtype == b.dtype
+        if b.numel():
+            assert float((a - b).float().abs().max()) <= 8 * HALF_STEP[dtype] * max(float(b.float().abs().max()), 1e-6)
+    some = torch.autograd.grad(ex.expert_mlp(x, z, w1, b1, w2, b2, k, act, mask), [z, w1], go)
+    assert torch.equal(some[0], g_one[1]) and torch.equal(some[1], g_one[2])
+
+
 def check_layer(ex, device, T, K, F, E, k, act, seed=0):
     """expert_mlp in fp32, masked rows among them: output and every gradient against float64 autograd, and the gradient
     against differences of the float64 form along a random direction."""

@@ -135,11 +135,12 @@ SUBST["wave_ops.hpp"] = [
      '                 DIMO_RA1(7) DIMO_RTAIL DIMO_ROPS);', "simt_wave_reduce16<10>(v);"),
 ]
 # the expert operators: routing, grouping, grouped products, 4-bit products
-TARGETS["experts"] = (["experts.hip", "grouped.hip", "mx4.hip"], "experts_emu.cpp")
+TARGETS["experts"] = (["experts.hip", "grouped.hip", "expert_mlp.hip", "mx4.hip"], "experts_emu.cpp")
 SEPARATE.add("experts")
 SUBST["experts.hip"] = []
 SUBST["grouped.hip"] = []
 SUBST["mx4.hip"] = []
+SUBST["expert_mlp.hip"] = []
 SUBST["row_tiles.hpp"] = []
 SUBST["tile_product.hpp"] = [  # (an empty statement that pins registers)
     ('asm volatile("" : "+v"(v[j][i]));', ";"),

@@ -79,6 +79,13 @@ def test_layer(emulated, T, K, F, E, k, act):
     cases.check_layer(ex, "cpu", T, K, F, E, k, act)
 
 
+@pytest.mark.parametrize("T,K,F,E,k,dtype,act,biases", [
+    (0, 8, 8, 3, 2, F32, "relu", True), (1, 8, 24, 3, 1, BF16, "silu", True), (70, 40, 33, 4, 2, F32, "silu", True),
+    (50, 64, 40, 4, 2, BF16, "relu", True), (50, 33, 40, 4, 3, F16, "silu", False), (33, 16, 16, 2, 2, BF16, None, False)])
+def test_layer_is_its_parts(emulated, T, K, F, E, k, dtype, act, biases):
+    cases.check_layer_is_its_parts(ex, "cpu", T, K, F, E, k, dtype, act, biases, seed=T)
+
+
 def test_bad_offsets_stay_inside(emulated):
     """Offsets that the caller got wrong give wrong rows, never an address outside (run under AddressSanitizer too)."""
     x, w = torch.randn(40, 8), torch.randn(3, 4, 8)
@@ -121,6 +128,15 @@ def test_refusals():
     lambda: ex.grouped_linear(torch.zeros(4, 8), torch.zeros(6, 5, 8), ex.group_rows(torch.zeros(3, 2, dtype=torch.int32), 6),
                               gather=True),
     lambda: ex.grouped_linear(torch.zeros(4, 8), torch.zeros(6, 5, 8), ex.group_rows(torch.zeros(4, 2, dtype=torch.int32), 6)),
+    lambda: ex.expert_mlp(torch.zeros(4, 8), torch.zeros(4, 3), torch.zeros(3, 5, 8), None, torch.zeros(3, 8, 5), None, 4),
+    lambda: ex.expert_mlp(torch.zeros(4, 8), torch.zeros(5, 3), torch.zeros(3, 5, 8), None, torch.zeros(3, 8, 5), None, 2),
+    lambda: ex.expert_mlp(torch.zeros(4, 8), torch.zeros(4, 3), torch.zeros(3, 5, 8), None, torch.zeros(3, 8, 6), None, 2),
+    lambda: ex.expert_mlp(torch.zeros(4, 8), torch.zeros(4, 3).half(), torch.zeros(3, 5, 8), None, torch.zeros(3, 8, 5), None, 2),
+    lambda: ex.expert_mlp(torch.zeros(4, 8), torch.zeros(4, 3), torch.zeros(3, 5, 8), None, torch.zeros(3, 8, 5),
+                          torch.zeros(3, 5), 2),
+    lambda: ex.expert_mlp(torch.zeros(4, 8), torch.zeros(4, 3), torch.zeros(3, 5, 8), None, torch.zeros(3, 8, 5), None, 2, "tanh"),
+    lambda: ex.expert_mlp(torch.zeros(4, 8), torch.zeros(4, 3), torch.zeros(3, 5, 8), None, torch.zeros(3, 8, 5), None, 2,
+                          row_mask=torch.zeros(3, dtype=torch.bool)),
     lambda: ex.combine_rows(torch.zeros(4, 8), ex.RowGroups(torch.zeros(4, dtype=torch.int32))),
     lambda: ex.combine_rows(torch.zeros(4, 8), ex.group_rows(torch.zeros(4, 2, dtype=torch.int32), 6)),
     lambda: ex.combine_rows(torch.zeros(8, 8), ex.group_rows(torch.zeros(4, 2, dtype=torch.int32), 6),
@@ -141,15 +157,16 @@ def test_c_entry_points_refuse():
     assert L.dimo_route_topk_forward(4, 6, 2, 0, 1, 5, None, 1, 1, 1, None, None, 0, None) == -1
     assert L.dimo_route_topk_forward(4, 6, 2, 0, 1, 6, None, 1, 1, 1, 1, None, 0, None) == -3
     assert L.dimo_route_topk_forward(4, 6, 2, 0, None, 6, None, 1, 1, 1, None, None, 0, None) == -1
-    assert L.dimo_group_rows(10000, 6, 1, 1, 1, 1, None, 0, None) == -3
-    assert L.dimo_group_rows(-1, 6, 1, 1, 1, 1, None, 0, None) == -1
-    assert L.dimo_group_rows(4, 1025, 1, 1, 1, 1, None, 0, None) == -1
-    assert L.dimo_grouped_linear_forward(0, 4, 3, 8, 5, 1, 7, 0, None, 1, 1, None, 0, 1, None, None) == -1
-    assert L.dimo_grouped_linear_forward(0, 4, 3, 8, 5, 1, 8, 2, None, 1, 1, None, 0, 1, None, None) == -1
-    assert L.dimo_grouped_linear_forward(0, 4, 3, 8, 5, 1, 8, 0, None, 1, 1, None, 3, 1, None, None) == -1
-    assert L.dimo_grouped_linear_dgrad(0, 4, 0, 8, 5, 1, 1, 1, 1, None) == -1
-    assert L.dimo_grouped_linear_wgrad(0, 4, 3, 8, 5, 1, 1, 8, 0, None, None, 1, None, None, 0, None) == -1
-    assert L.dimo_grouped_linear_wgrad(1, 4096, 2, 64, 64, 1, 1, 64, 0, None, 1, 1, None, None, 0, None) == -3
+    assert L.dimo_group_rows(10000, 6, 2, 1, 1, 1, 1, None, None, 0, None) == -3
+    assert L.dimo_group_rows(-1, 6, 2, 1, 1, 1, 1, None, None, 0, None) == -1
+    assert L.dimo_group_rows(4, 6, 0, 1, 1, 1, 1, None, None, 0, None) == -1
+    assert L.dimo_group_rows(4, 1025, 1, 1, 1, 1, 1, None, None, 0, None) == -1
+    assert L.dimo_grouped_linear_forward(0, 4, 3, 8, 5, 1, 7, None, 1, 1, None, 0, 1, None, None) == -1
+    assert L.dimo_grouped_linear_forward(0, 4, 3, 8, 5, 1, 8, None, 1, 1, None, 3, 1, None, None) == -1
+    assert L.dimo_grouped_linear_dgrad(0, 4, 0, 8, 5, 1, 1, 1, 0, None, 1, None) == -1
+    assert L.dimo_grouped_linear_dgrad(0, 4, 3, 8, 5, 1, 1, 1, 1, None, 1, None) == -1
+    assert L.dimo_grouped_linear_wgrad(0, 4, 3, 8, 5, 1, 1, 8, None, None, 1, None, None, 0, None) == -1
+    assert L.dimo_grouped_linear_wgrad(1, 4096, 2, 64, 64, 1, 1, 64, None, 1, 1, None, None, 0, None) == -3
     assert L.dimo_activation_backward(0, 0, 8, 1, 1, 1, None) == -1
     assert L.dimo_combine_rows_forward(4, 2, 8, 8, 0, 1, 7, None, 1, None, 0, 1, None) == -1
     assert L.dimo_combine_rows_backward(4, 2, 8, 9, 3, 0, 1, 8, 1, 8, 1, 1, 1, 1, 1, None) == -1

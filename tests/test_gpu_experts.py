@@ -91,6 +91,13 @@ def test_layer(ex, T, K, F, E, k, act):
     cases.check_layer(ex, "cuda", T, K, F, E, k, act)
 
 
+@pytest.mark.parametrize("T,K,F,E,k,dtype,act,biases", [
+    (0, 8, 8, 3, 2, F32, "relu", True), (1, 256, 512, 3, 1, BF16, "silu", True), (700, 256, 256, 8, 2, F32, "silu", True),
+    (3000, 256, 512, 8, 2, BF16, "relu", True), (50, 33, 40, 4, 3, F16, "silu", False), (333, 16, 16, 2, 2, BF16, None, False)])
+def test_layer_is_its_parts(ex, T, K, F, E, k, dtype, act, biases):
+    cases.check_layer_is_its_parts(ex, "cuda", T, K, F, E, k, dtype, act, biases, seed=T)
+
+
 def _layer_leaves(T, K, F, E, dtype, seed):
     g = torch.Generator(device="cuda").manual_seed(seed)
     r = lambda *s: torch.randn(*s, generator=g, device="cuda")

@@ -83,10 +83,10 @@ def test_bad_arguments(emulated, call):
 
 def test_c_entry_points_refuse():
     L = expert_emulation.emulated_library()
-    assert L.dimo_mx4_quantize(0, 4, 0, 1, 8, 0, None, 1, 1, None) == -1
-    assert L.dimo_mx4_quantize(0, 4, 8, 1, 7, 0, None, 1, 1, None) == -1
-    assert L.dimo_mx4_quantize(0, 4, 8, 1, 8, 2, None, 4, 1, None) == -1
-    assert L.dimo_mx4_quantize(3, 4, 8, 1, 8, 0, None, 4, 1, None) == -1
+    assert L.dimo_mx4_quantize(0, 4, 0, 1, 8, None, 4, 1, None) == -1
+    assert L.dimo_mx4_quantize(0, 4, 8, 1, 7, None, 4, 1, None) == -1
+    assert L.dimo_mx4_quantize(0, 4, 8, 1, 8, None, 2, 1, None) == -1
+    assert L.dimo_mx4_quantize(3, 4, 8, 1, 8, None, 4, 1, None) == -1
     assert L.dimo_mx4_dequantize(0, 4, 8, 4, 1, None, None) == -1
     assert L.dimo_mx4_linear(0, 4, 2, 32, 8, 16, 1, None, 16, 1, None, 0, 16, None) == -1
     assert L.dimo_mx4_linear(0, 4, 1, 32, 8, 8, 1, None, 16, 1, None, 0, 16, None) == -1
