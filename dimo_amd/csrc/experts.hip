@@ -11,6 +11,8 @@
 // atomics, so results do not depend on the schedule.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "numeric.hpp"
 
 using namespace dimo;
@@ -22,11 +24,12 @@ constexpr int ROUTE_MAX_E = DIMO_MAX_EXPERTS;
 constexpr int ROUTE_MAX_BLOCKS = 512;  // workgroups of a routing launch that also sums the load: one row of partial sums each
 
 // ---- routing ---------------------------------------------------------------------------------------------------
-// L lanes per row (a power of two, so that the butterflies stay inside the row's lanes), V values per lane: element
-// c * L + lane.  Rows with 4 E <= 256 take L = E / 4 lanes: the cost of a selection round is log2(L) exchanges, which
-// outweighs the V comparisons before it.
+// A row lies in L neighbouring lanes (a power of two up to 64), V consecutive logits in each: sixteen-byte loads, and few
+// exchanges -- a selection round is V comparisons in a lane and log2(L) exchanges of (value, index) between lanes, most of
+// them DPP moves.  V = 16 from 9 experts on: 131072 rows of 128, k = 8, took 215 us with V = 4 (five exchanges a round,
+// through LDS) and 52 us this way.
 struct RouteArgs {
-  int T, E, k, normalize;
+  int T, E, k, normalize, wide;
   const void *logits;
   int64_t ld;
   const uint8_t *row_mask;
@@ -36,33 +39,60 @@ struct RouteArgs {
   float load_scale;
 };
 
+// The value of a lane of the other half of 2 M lanes whose halves are each uniform (the M-th step of a reduction).
+template <int M>
+__device__ __forceinline__ int from_other_half(int v) {
+  if constexpr (M == 1) return __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, false);   // quad_perm [1, 0, 3, 2]
+  else if constexpr (M == 2) return __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, false);   // quad_perm [2, 3, 0, 1]
+  else if constexpr (M == 4) return __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, false);  // row_half_mirror
+  else if constexpr (M == 8) return __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, false);  // row_mirror
+  else return __shfl_xor(v, M);
+}
+template <int M>
+__device__ __forceinline__ float from_other_half(float v) {
+  return __int_as_float(from_other_half<M>(__float_as_int(v)));
+}
+template <int L, int M = 1, class F>
+__device__ __forceinline__ void halving_steps(F &&f) {
+  if constexpr (M < L) {
+    f(std::integral_constant<int, M>{});
+    halving_steps<L, 2 * M>(f);
+  }
+}
 template <int L>
 __device__ __forceinline__ float row_sum(float v) {
-#pragma unroll
-  for (int m = 1; m < L; m *= 2) v += __shfl_xor(v, m);
+  halving_steps<L>([&](auto m) { v += from_other_half<decltype(m)::value>(v); });
   return v;
 }
 template <int L>
 __device__ __forceinline__ float row_max(float v) {
-#pragma unroll
-  for (int m = 1; m < L; m *= 2) v = fmaxf(v, __shfl_xor(v, m));
+  halving_steps<L>([&](auto m) { v = fmaxf(v, from_other_half<decltype(m)::value>(v)); });
   return v;
 }
 
+// this lane's V logits (first .. first + V - 1 of the row at `src`), -inf where there are none
 template <class T, int V>
-__device__ __forceinline__ void load_row(const void *logits, int64_t at, int E, int L, int lane, bool live, float (&z)[V]) {
-  const typename T::store *src = static_cast<const typename T::store *>(logits) + at;
+__device__ __forceinline__ void load_row(const typename T::store *src, int first, int E, bool live, bool wide, float (&z)[V]) {
+  if (wide) {
+    constexpr int N = Vec16<T>::N, G = V < N ? 1 : V / N;
 #pragma unroll
-  for (int c = 0; c < V; ++c) {
-    const int e = c * L + lane;
-    z[c] = (live && e < E) ? T::load(src[e]) : -INFINITY;
+    for (int g = 0; g < G; ++g) {
+      float q[N];
+      const bool in = live && first + g * N < E;
+      load_vec<T, N>(src + (in ? first + g * N : 0), q);
+#pragma unroll
+      for (int e = 0; e < N && g * N + e < V; ++e) z[g * N + e] = in ? q[e] : -INFINITY;
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < V; ++c) z[c] = (live && first + c < E) ? T::load(src[first + c]) : -INFINITY;
   }
 }
 
 template <class T, int L, int V>
 __global__ __launch_bounds__(ROUTE_THREADS) void route_forward_kernel(RouteArgs a) {
   constexpr int ROWS = ROUTE_THREADS / L;
-  const int lane = threadIdx.x % L, sub = threadIdx.x / L;
+  const int lane = threadIdx.x % L, sub = threadIdx.x / L, first = lane * V;
   float mine[V];  // sums of p over this lane's rows
 #pragma unroll
   for (int c = 0; c < V; ++c) mine[c] = 0.f;
@@ -72,38 +102,39 @@ __global__ __launch_bounds__(ROUTE_THREADS) void route_forward_kernel(RouteArgs 
     const bool in = row < a.T;
     const bool live = in && (!a.row_mask || a.row_mask[in ? row : 0] != 0);
     float z[V];
-    load_row<T, V>(a.logits, (in ? row : 0) * a.ld, a.E, L, lane, live, z);
+    load_row<T, V>(static_cast<const typename T::store *>(a.logits) + (in ? row : 0) * a.ld, first, a.E, live, a.wide, z);
     bool nan = false;
 #pragma unroll
     for (int c = 0; c < V; ++c) nan |= z[c] != z[c];
     // a NaN is never chosen; the row's weights and probabilities are NaN by the formula
     const float poison = row_max<L>(nan ? 1.f : 0.f) > 0.f ? NAN : 0.f;
-    int slot[V];
+    uint32_t left = (1u << V) - 1u;  // (V <= 16) this lane's logits that are not chosen yet
     float top = 0.f;      // the row's largest logit
     float chosen = 0.f;   // sum of exp over the chosen
     int count = 0;
-#pragma unroll
-    for (int c = 0; c < V; ++c) slot[c] = -1;
     for (int j = 0; j < a.k; ++j) {
       float best = -INFINITY;
       int at = ROUTE_MAX_E;
 #pragma unroll
       for (int c = 0; c < V; ++c)  // (ascending index: the first of equals stays)
-        if (slot[c] < 0 && z[c] > best) best = z[c], at = c * L + lane;
-#pragma unroll
-      for (int m = 1; m < L; m *= 2) {
-        const float ob = __shfl_xor(best, m);
-        const int oa = __shfl_xor(at, m);
+        if (((left >> c) & 1u) && z[c] > best) best = z[c], at = first + c;
+      halving_steps<L>([&](auto m) {
+        const float ob = from_other_half<decltype(m)::value>(best);
+        const int oa = from_other_half<decltype(m)::value>(at);
         if (ob > best || (ob == best && oa < at)) best = ob, at = oa;
+      });
+      const bool found = best > -INFINITY;
+      if (j == 0) top = found ? best : 0.f;
+      const float share = found ? expf(best - top) : 0.f;
+      chosen += share;
+      count += found;
+      const int own = at - first;
+      if (found && own >= 0 && own < V) left &= ~(1u << own);
+      // (the lane of place j keeps it; the sum is not known yet: the weight follows below)
+      if (in && j % L == lane) {
+        a.weights[row * a.k + j] = share;
+        a.experts[row * a.k + j] = found ? at : -1;
       }
-      if (j == 0) top = best > -INFINITY ? best : 0.f;
-      if (best > -INFINITY) {
-        chosen += expf(best - top);
-        ++count;
-      }
-#pragma unroll
-      for (int c = 0; c < V; ++c)
-        if (at == c * L + lane && best > -INFINITY) slot[c] = j;
     }
     float all = 0.f, p[V];
 #pragma unroll
@@ -111,27 +142,17 @@ __global__ __launch_bounds__(ROUTE_THREADS) void route_forward_kernel(RouteArgs 
     all = row_sum<L>(all);
     const float inv_all = (all > 0.f ? 1.f / all : 0.f) + poison;
     const float inv = a.normalize ? (count ? 1.f / chosen : 0.f) + poison : inv_all;
-    if (in) {
+    if (in)
+      for (int j = lane; j < a.k; j += L) a.weights[row * a.k + j] = j < count ? a.weights[row * a.k + j] * inv : 0.f;
+    if (live)
 #pragma unroll
-      for (int c = 0; c < V; ++c)
-        if (slot[c] >= 0) {
-          a.weights[row * a.k + slot[c]] = p[c] * inv;
-          a.experts[row * a.k + slot[c]] = c * L + lane;
-        }
-      for (int j = count + lane; j < a.k; j += L) {
-        a.weights[row * a.k + j] = 0.f;
-        a.experts[row * a.k + j] = -1;
-      }
-      if (live)
-#pragma unroll
-        for (int c = 0; c < V; ++c) mine[c] += p[c] * inv_all;
-    }
+      for (int c = 0; c < V; ++c) mine[c] += p[c] * inv_all;
   }
   if (!a.partial) return;
   // the workgroup's rows one after the other, in a fixed order
   __shared__ float sums[ROUTE_THREADS * V];
 #pragma unroll
-  for (int c = 0; c < V; ++c) sums[sub * (L * V) + c * L + lane] = mine[c];
+  for (int c = 0; c < V; ++c) sums[sub * (L * V) + first + c] = mine[c];
   __syncthreads();
   for (int e = threadIdx.x; e < a.E; e += ROUTE_THREADS) {
     float s = 0.f;
@@ -140,24 +161,30 @@ __global__ __launch_bounds__(ROUTE_THREADS) void route_forward_kernel(RouteArgs 
   }
 }
 
-// load[e] = sum over the workgroups' partial sums, in their order
+// load[e] = sum over the workgroups' partial sums: sixteen threads per expert, theirs summed in a fixed order
 __global__ __launch_bounds__(256) void route_load_kernel(int E, int blocks, const float *__restrict__ partial,
                                                          float *__restrict__ load) {
-  __shared__ float s[4][64];
-  const int e = blockIdx.x * 64 + (threadIdx.x & 63), part = threadIdx.x >> 6;
+  __shared__ float s[16][17];
+  const int e = blockIdx.x * 16 + (threadIdx.x & 15), part = threadIdx.x >> 4;
   float v = 0.f;
   if (e < E)
-    for (int b = part; b < blocks; b += 4) v += partial[(size_t)b * E + e];
-  s[part][threadIdx.x & 63] = v;
+#pragma unroll 8
+    for (int b = part; b < blocks; b += 16) v += partial[(size_t)b * E + e];
+  s[part][threadIdx.x & 15] = v;
   __syncthreads();
-  if (part == 0 && e < E) load[e] = (s[0][threadIdx.x] + s[1][threadIdx.x]) + (s[2][threadIdx.x] + s[3][threadIdx.x]);
+  if (part == 0 && e < E) {
+    float sum = 0.f;
+#pragma unroll
+    for (int q = 0; q < 16; ++q) sum += s[q][threadIdx.x];
+    load[e] = sum;
+  }
 }
 
 // Backward: the chosen experts' share arrives in LDS (one row of E per row of logits), the rest is per element.
 //   normalize:  g_ej = w_j (gw_j - sum_i w_i gw_i)         otherwise  p_e (g_e - sum p g), g_ej = gw_j
 //   load:       + p_e (gl_e - sum p gl) / T
 struct RouteBwdArgs {
-  int T, E, k, normalize;
+  int T, E, k, normalize, wide;
   const void *logits;
   int64_t ld;
   const uint8_t *row_mask;
@@ -170,15 +197,15 @@ struct RouteBwdArgs {
 
 template <class T, int L, int V>
 __global__ __launch_bounds__(ROUTE_THREADS) void route_backward_kernel(RouteBwdArgs a) {
-  constexpr int ROWS = ROUTE_THREADS / L;
-  __shared__ float sparse[ROUTE_THREADS * V];
-  const int lane = threadIdx.x % L, sub = threadIdx.x / L;
+  constexpr int ROWS = ROUTE_THREADS / L, PAD = 1;  // (rows of L V + 1 words: a lane's V words then lie on other banks)
+  __shared__ float sparse[ROWS * (L * V + PAD)];
+  const int lane = threadIdx.x % L, sub = threadIdx.x / L, first = lane * V;
   const int64_t row = (int64_t)blockIdx.x * ROWS + sub;
   const bool in = row < a.T;
   const bool live = in && (!a.row_mask || a.row_mask[in ? row : 0] != 0);
-  float *g_row = sparse + sub * (L * V);
+  float *g_row = sparse + sub * (L * V + PAD);
 #pragma unroll
-  for (int c = 0; c < V; ++c) g_row[c * L + lane] = 0.f;
+  for (int c = 0; c < V; ++c) g_row[first + c] = 0.f;
   __syncthreads();
   float inner = 0.f;
   if (live && a.g_weights && a.normalize)
@@ -195,10 +222,10 @@ __global__ __launch_bounds__(ROUTE_THREADS) void route_backward_kernel(RouteBwdA
   __syncthreads();
   float out[V];
 #pragma unroll
-  for (int c = 0; c < V; ++c) out[c] = g_row[c * L + lane];
+  for (int c = 0; c < V; ++c) out[c] = g_row[first + c];
   if (a.g_load || !a.normalize) {
     float z[V], p[V], g[V];
-    load_row<T, V>(a.logits, (in ? row : 0) * a.ld, a.E, L, lane, live, z);
+    load_row<T, V>(static_cast<const typename T::store *>(a.logits) + (in ? row : 0) * a.ld, first, a.E, live, a.wide, z);
     float m = -INFINITY, all = 0.f;
 #pragma unroll
     for (int c = 0; c < V; ++c) m = fmaxf(m, z[c]);
@@ -211,7 +238,7 @@ __global__ __launch_bounds__(ROUTE_THREADS) void route_backward_kernel(RouteBwdA
     float dot = 0.f;
 #pragma unroll
     for (int c = 0; c < V; ++c) {
-      const int e = c * L + lane;
+      const int e = first + c;
       p[c] *= inv;
       g[c] = (a.g_load && e < a.E) ? a.g_load[e] * a.load_scale : 0.f;
       if (!a.normalize) g[c] += out[c], out[c] = 0.f;
@@ -221,56 +248,58 @@ __global__ __launch_bounds__(ROUTE_THREADS) void route_backward_kernel(RouteBwdA
 #pragma unroll
     for (int c = 0; c < V; ++c) out[c] += p[c] * (g[c] - dot);
   }
-  if (in) {
-    typename T::store *dst = static_cast<typename T::store *>(a.g_logits) + row * a.E;
+  if (!in) return;
+#pragma unroll
+  for (int c = 0; c < V; ++c) out[c] = live ? out[c] : 0.f;
+  typename T::store *dst = static_cast<typename T::store *>(a.g_logits) + row * a.E;
+  constexpr int N = Vec16<T>::N;
+  if (V >= N && a.wide) {
+#pragma unroll
+    for (int g = 0; g < V / N; ++g) {
+      float q[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) q[e] = out[(g * N + e) % V];
+      if (first + g * N < a.E) store_vec<T, N>(dst + first + g * N, q);
+    }
+  } else {
 #pragma unroll
     for (int c = 0; c < V; ++c)
-      if (c * L + lane < a.E) dst[c * L + lane] = T::save(live ? out[c] : 0.f);
+      if (first + c < a.E) dst[first + c] = T::save(out[c]);
   }
 }
 
 // lanes per row and values per lane for E experts
+inline int route_values(int E) { return E <= 4 ? 4 : E <= 8 ? 8 : 16; }
 inline int route_lanes(int E) {
   int L = 1;
-  while (L < 64 && 4 * L < E) L *= 2;
+  while (L * route_values(E) < E) L *= 2;
   return L;
 }
 inline int route_blocks(int T, int E) {
   const int rows = ROUTE_THREADS / route_lanes(E);
   return (T + rows - 1) / rows;
 }
-
-template <class T>
-void launch_route_forward(const RouteArgs &a, int grid, hipStream_t s) {
-  switch (route_lanes(a.E)) {
-    case 1: hipLaunchKernelGGL((route_forward_kernel<T, 1, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a); break;
-    case 2: hipLaunchKernelGGL((route_forward_kernel<T, 2, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a); break;
-    case 4: hipLaunchKernelGGL((route_forward_kernel<T, 4, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a); break;
-    case 8: hipLaunchKernelGGL((route_forward_kernel<T, 8, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a); break;
-    case 16: hipLaunchKernelGGL((route_forward_kernel<T, 16, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a); break;
-    case 32: hipLaunchKernelGGL((route_forward_kernel<T, 32, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a); break;
-    default:
-      if (a.E <= 256)
-        hipLaunchKernelGGL((route_forward_kernel<T, 64, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a);
-      else
-        hipLaunchKernelGGL((route_forward_kernel<T, 64, 16>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a);
-  }
+// rows that sixteen-byte loads can take: whole, and on their boundaries
+inline bool route_wide(int dtype, int E, const void *p, int64_t ld) {
+  const int64_t n = 16 / (int64_t)dtype_bytes(dtype);
+  return E % n == 0 && ld % n == 0 && aligned16(p);
 }
-template <class T>
-void launch_route_backward(const RouteBwdArgs &a, int grid, hipStream_t s) {
-  switch (route_lanes(a.E)) {
-    case 1: hipLaunchKernelGGL((route_backward_kernel<T, 1, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a); break;
-    case 2: hipLaunchKernelGGL((route_backward_kernel<T, 2, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a); break;
-    case 4: hipLaunchKernelGGL((route_backward_kernel<T, 4, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a); break;
-    case 8: hipLaunchKernelGGL((route_backward_kernel<T, 8, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a); break;
-    case 16: hipLaunchKernelGGL((route_backward_kernel<T, 16, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a); break;
-    case 32: hipLaunchKernelGGL((route_backward_kernel<T, 32, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a); break;
-    default:
-      if (a.E <= 256)
-        hipLaunchKernelGGL((route_backward_kernel<T, 64, 4>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a);
-      else
-        hipLaunchKernelGGL((route_backward_kernel<T, 64, 16>), dim3(grid), dim3(ROUTE_THREADS), 0, s, a);
-  }
+
+// f(lanes, values) as constants
+template <class F>
+void with_route_shape(int E, F &&f) {
+  const auto go = [&](auto l, auto v) { f(l, v); };
+#define DIMO_ROUTE_SHAPE(l, v) go(std::integral_constant<int, l>{}, std::integral_constant<int, v>{})
+  if (E <= 4) DIMO_ROUTE_SHAPE(1, 4);
+  else if (E <= 8) DIMO_ROUTE_SHAPE(1, 8);
+  else if (E <= 16) DIMO_ROUTE_SHAPE(1, 16);
+  else if (E <= 32) DIMO_ROUTE_SHAPE(2, 16);
+  else if (E <= 64) DIMO_ROUTE_SHAPE(4, 16);
+  else if (E <= 128) DIMO_ROUTE_SHAPE(8, 16);
+  else if (E <= 256) DIMO_ROUTE_SHAPE(16, 16);
+  else if (E <= 512) DIMO_ROUTE_SHAPE(32, 16);
+  else DIMO_ROUTE_SHAPE(64, 16);
+#undef DIMO_ROUTE_SHAPE
 }
 
 // ---- grouping --------------------------------------------------------------------------------------------------
@@ -309,7 +338,7 @@ __global__ __launch_bounds__(GROUP_THREADS) void group_place_kernel(int64_t S, i
                                                                     int32_t *__restrict__ position, int places,
                                                                     int32_t *__restrict__ rows) {
   HIP_DYNAMIC_SHARED(int, base)  // [GROUP_WAVES][E + 1]
-  __shared__ int wave_total[GROUP_WAVES];
+  __shared__ int wave_total[GROUP_WAVES], tallies[2 * (ROUTE_MAX_E + 1)];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, E1 = E + 1;
   for (int i = t; i < GROUP_WAVES * E1; i += GROUP_THREADS) base[i] = 0;
   __syncthreads();
@@ -321,6 +350,26 @@ __global__ __launch_bounds__(GROUP_THREADS) void group_place_kernel(int64_t S, i
     if (key[r] >= 0) atomicAdd(&base[wave * E1 + key[r]], 1);
   }
   __syncthreads();
+  if (counts) {
+    // the workgroups' counts: `parts` threads per expert, eight loads in flight each
+    for (int i = t; i < 2 * E1; i += GROUP_THREADS) tallies[i] = 0;
+    __syncthreads();
+    int wide = 64;
+    while (wide < E1) wide *= 2;
+    const int parts = wide < GROUP_THREADS ? GROUP_THREADS / wide : 1, part = t / wide;
+    for (int e = t % wide; e < E1 && part < parts; e += (wide < GROUP_THREADS ? wide : GROUP_THREADS)) {
+      int before = 0, total = 0;
+#pragma unroll 8
+      for (int b = part; b < blocks; b += parts) {
+        const int n = counts[(size_t)b * E1 + e];
+        total += n;
+        before += b < (int)blockIdx.x ? n : 0;
+      }
+      atomicAdd(&tallies[e], before);
+      atomicAdd(&tallies[E1 + e], total);
+    }
+    __syncthreads();
+  }
   // exclusive scan over the experts: thread t owns expert t (the last thread's round also the places without one)
   int running = 0;
   for (int e0 = 0; e0 < E1; e0 += GROUP_THREADS) {
@@ -328,11 +377,7 @@ __global__ __launch_bounds__(GROUP_THREADS) void group_place_kernel(int64_t S, i
     int before = 0, total = 0;
     if (e < E1) {
       if (counts)
-        for (int b = 0; b < blocks; ++b) {
-          const int n = counts[(size_t)b * E1 + e];
-          if (b < (int)blockIdx.x) before += n;
-          total += n;
-        }
+        before = tallies[e], total = tallies[E1 + e];
       else
         for (int w = 0; w < GROUP_WAVES; ++w) total += base[w * E1 + e];
     }
@@ -500,12 +545,17 @@ extern "C" int dimo_route_topk_forward(int T, int E, int k, int dtype, const voi
   }
   float *partial = static_cast<float *>(workspace);
   if (T > 0) {
-    const RouteArgs a{T, E, k, normalize, logits, ld, row_mask, weights, experts,
+    const RouteArgs a{T, E, k, normalize, route_wide(dtype, E, logits, ld), logits, ld, row_mask, weights, experts,
                       load ? (grid == 1 ? load : partial) : nullptr, 1.0f / (float)T};
-    with_dtype(dtype, [&](auto tag) { launch_route_forward<decltype(tag)>(a, grid, s); });
+    with_dtype(dtype, [&](auto tag) {
+      with_route_shape(E, [&](auto l, auto v) {
+        hipLaunchKernelGGL((route_forward_kernel<decltype(tag), decltype(l)::value, decltype(v)::value>), dim3(grid),
+                           dim3(ROUTE_THREADS), 0, s, a);
+      });
+    });
   }
   if (load && grid != 1)
-    hipLaunchKernelGGL(route_load_kernel, dim3((E + 63) / 64), dim3(256), 0, s, E, grid, partial, load);
+    hipLaunchKernelGGL(route_load_kernel, dim3((E + 15) / 16), dim3(256), 0, s, E, grid, partial, load);
   return check_launch();
 }
 
@@ -519,8 +569,14 @@ extern "C" int dimo_route_topk_backward(int T, int E, int k, int dtype, const vo
   hipStream_t s = (hipStream_t)stream;
   clear_errors();
   ScopedTimer timer(T_ROUTE, s);
-  const RouteBwdArgs a{T, E, k, normalize, logits, ld, row_mask, weights, experts, g_weights, g_load, g_logits, 1.0f / (float)T};
-  with_dtype(dtype, [&](auto tag) { launch_route_backward<decltype(tag)>(a, route_blocks(T, E), s); });
+  const RouteBwdArgs a{T, E, k, normalize, route_wide(dtype, E, logits, ld) && route_wide(dtype, E, g_logits, E), logits, ld,
+                       row_mask, weights, experts, g_weights, g_load, g_logits, 1.0f / (float)T};
+  with_dtype(dtype, [&](auto tag) {
+    with_route_shape(E, [&](auto l, auto v) {
+      hipLaunchKernelGGL((route_backward_kernel<decltype(tag), decltype(l)::value, decltype(v)::value>),
+                         dim3(route_blocks(T, E)), dim3(ROUTE_THREADS), 0, s, a);
+    });
+  });
   return check_launch();
 }
 
@@ -544,7 +600,7 @@ extern "C" int dimo_group_rows(int64_t S, int E, int places, const int32_t *expe
   if (counts)
     hipLaunchKernelGGL(group_count_kernel, dim3(blocks), dim3(GROUP_THREADS), 0, s, S, E, experts, counts);
   const size_t lds = (size_t)GROUP_WAVES * (E + 1) * sizeof(int);
-  if (lds > 65536 - 1024) {  // (1024 experts: 65 600 bytes; a workgroup has 160 KB)
+  if (lds > 32768) {  // (1024 experts: 65 600 bytes and 8 KB of tallies; a workgroup has 160 KB)
     if (hipFuncSetAttribute(reinterpret_cast<const void *>(group_place_kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                             (int)lds) != hipSuccess)
       return check_launch();
