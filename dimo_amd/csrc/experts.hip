@@ -59,6 +59,11 @@ __device__ __forceinline__ void halving_steps(F &&f) {
     halving_steps<L, 2 * M>(f);
   }
 }
+// exp on the hardware's exponential: off by 2^-23 and the argument's rounding, |v| 2^-24 (logits within 30 of the row's
+// largest: 2e-6 of a probability of 1e-13; what is small is off most).  expf's sixteen instructions times V values were a
+// third of the kernel.
+__device__ __forceinline__ float exp_fast(float v) { return __builtin_amdgcn_exp2f(v * 1.44269504088896340736f); }
+
 template <int L>
 __device__ __forceinline__ float row_sum(float v) {
   halving_steps<L>([&](auto m) { v += from_other_half<decltype(m)::value>(v); });
@@ -125,7 +130,7 @@ __global__ __launch_bounds__(ROUTE_THREADS) void route_forward_kernel(RouteArgs 
       });
       const bool found = best > -INFINITY;
       if (j == 0) top = found ? best : 0.f;
-      const float share = found ? expf(best - top) : 0.f;
+      const float share = found ? exp_fast(best - top) : 0.f;
       chosen += share;
       count += found;
       const int own = at - first;
@@ -138,7 +143,7 @@ __global__ __launch_bounds__(ROUTE_THREADS) void route_forward_kernel(RouteArgs 
     }
     float all = 0.f, p[V];
 #pragma unroll
-    for (int c = 0; c < V; ++c) p[c] = expf(z[c] - top), all += z[c] == z[c] ? p[c] : 0.f;
+    for (int c = 0; c < V; ++c) p[c] = exp_fast(z[c] - top), all += z[c] == z[c] ? p[c] : 0.f;
     all = row_sum<L>(all);
     const float inv_all = (all > 0.f ? 1.f / all : 0.f) + poison;
     const float inv = a.normalize ? (count ? 1.f / chosen : 0.f) + poison : inv_all;
@@ -232,7 +237,7 @@ __global__ __launch_bounds__(ROUTE_THREADS) void route_backward_kernel(RouteBwdA
     m = row_max<L>(m);
     if (!(m > -INFINITY)) m = 0.f;
 #pragma unroll
-    for (int c = 0; c < V; ++c) p[c] = expf(z[c] - m), all += p[c];
+    for (int c = 0; c < V; ++c) p[c] = exp_fast(z[c] - m), all += p[c];
     all = row_sum<L>(all);
     const float inv = all > 0.f ? 1.f / all : (all == 0.f ? 0.f : all);  // (NaN stays NaN)
     float dot = 0.f;
@@ -438,7 +443,8 @@ __global__ __launch_bounds__(GROUP_THREADS) void group_place_kernel(int64_t S, i
 // out[t] = residual[t] + sum_j w[t, j] y[position[t, j]]: VEC consecutive elements per thread, the k loads of a thread
 // independent of each other.
 struct CombineArgs {
-  int T, k, N, chunks;  // chunks = N / VEC
+  int T, k, N;
+  Divide chunks;  // N / VEC
   int64_t S;
   const void *y;
   int64_t ldy;
@@ -447,14 +453,15 @@ struct CombineArgs {
   const void *residual;      // [T, N] rows at ld_res, or null
   int64_t ld_res;
   void *out;                 // [T, N]
+  int64_t first;             // first row of this launch
 };
 template <class T, int VEC>
 __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a) {
   typedef typename T::store E;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (int64_t)a.T * a.chunks) return;
-  const int64_t t = i / a.chunks;
-  const int n = (int)(i % a.chunks) * VEC;
+  const uint32_t i = blockIdx.x * 256u + threadIdx.x, local = a.chunks(i);
+  const int64_t t = a.first + local;
+  if (t >= a.T) return;
+  const int n = (int)(i - local * a.chunks.d) * VEC;
   float acc[VEC];
 #pragma unroll
   for (int v = 0; v < VEC; ++v) acc[v] = 0.f;
@@ -527,6 +534,7 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(CombineBwdArgs a)
 extern "C" size_t dimo_route_workspace_bytes(int T, int E) {
   if (T <= 0 || E <= 0) return 0;
   const int blocks = route_blocks(T, E);
+  if (blocks == 1) return 0;  // (one workgroup's sums are the load)
   return align_up((size_t)(blocks < ROUTE_MAX_BLOCKS ? blocks : ROUTE_MAX_BLOCKS) * E * sizeof(float));
 }
 
@@ -540,7 +548,8 @@ extern "C" int dimo_route_topk_forward(int T, int E, int k, int dtype, const voi
   ScopedTimer timer(T_ROUTE, s);
   int grid = T > 0 ? route_blocks(T, E) : 0;
   if (load) {
-    if (workspace_bytes < dimo_route_workspace_bytes(T, E) || (T > 0 && !workspace)) return DIMO_E_WORKSPACE;
+    const size_t need = dimo_route_workspace_bytes(T, E);
+    if (workspace_bytes < need || (need && !workspace)) return DIMO_E_WORKSPACE;
     if (grid > ROUTE_MAX_BLOCKS) grid = ROUTE_MAX_BLOCKS;
   }
   float *partial = static_cast<float *>(workspace);
@@ -613,7 +622,8 @@ extern "C" int dimo_group_rows(int64_t S, int E, int places, const int32_t *expe
 extern "C" int dimo_combine_rows_forward(int T, int k, int N, int64_t S, int dtype, const void *y, int64_t ldy,
                                          const float *weights, const int32_t *position, const void *residual,
                                          int64_t ld_residual, void *out, void *stream) {
-  if (T < 0 || k < 1 || N < 0 || S < 0 || !known_dtype(dtype) || ldy < N || (residual && ld_residual < N)) return DIMO_E_ARG;
+  if (T < 0 || k < 1 || N < 0 || N > (1 << 30) || S < 0 || !known_dtype(dtype) || ldy < N || (residual && ld_residual < N))
+    return DIMO_E_ARG;
   if (T == 0 || N == 0) return DIMO_OK;
   if ((S > 0 && !y) || !position || !out) return DIMO_E_ARG;
   hipStream_t s = (hipStream_t)stream;
@@ -622,17 +632,22 @@ extern "C" int dimo_combine_rows_forward(int T, int k, int N, int64_t S, int dty
   const int vec = 16 / (int)dtype_bytes(dtype);
   const bool wide = N % vec == 0 && ldy % vec == 0 && aligned16(y) && aligned16(out) &&
                     (!residual || (ld_residual % vec == 0 && aligned16(residual)));
-  CombineArgs a{T, k, N, wide ? N / vec : N, S, y, ldy, weights, position, residual, ld_residual, out};
-  const int64_t blocks = ((int64_t)T * a.chunks + 255) / 256;
-  if (blocks > 0x7fffffffLL) return DIMO_E_ARG;
-  with_dtype(dtype, [&](auto tag) {
-    typedef decltype(tag) Tag;
-    if (wide)
-      hipLaunchKernelGGL((combine_kernel<Tag, Vec16<Tag>::N>), dim3((unsigned)blocks), dim3(256), 0, s, a);
-    else
-      hipLaunchKernelGGL((combine_kernel<Tag, 1>), dim3((unsigned)blocks), dim3(256), 0, s, a);
-  });
-  return check_launch();
+  CombineArgs a{T, k, N, Divide((uint32_t)(wide ? N / vec : N)), S, y, ldy, weights, position, residual, ld_residual, out, 0};
+  // (bands of rows whose chunks a launch can count in 31 bits)
+  const int64_t most = (0x7fffffffLL - 255) / a.chunks.d;
+  for (; a.first < T; a.first += most) {
+    const int64_t units = (T - a.first < most ? T - a.first : most) * a.chunks.d;
+    with_dtype(dtype, [&](auto tag) {
+      typedef decltype(tag) Tag;
+      if (wide)
+        hipLaunchKernelGGL((combine_kernel<Tag, Vec16<Tag>::N>), dim3((unsigned)((units + 255) / 256)), dim3(256), 0, s, a);
+      else
+        hipLaunchKernelGGL((combine_kernel<Tag, 1>), dim3((unsigned)((units + 255) / 256)), dim3(256), 0, s, a);
+    });
+    const int rc = check_launch();
+    if (rc) return rc;
+  }
+  return DIMO_OK;
 }
 
 extern "C" int dimo_combine_rows_backward(int T, int k, int N, int64_t S, int E, int dtype, const void *g_out,

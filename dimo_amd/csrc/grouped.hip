@@ -41,7 +41,7 @@ __device__ __forceinline__ int64_t source_row(const GroupedArgs &a, int r) {
 
 enum { FORWARD = 0, DGRAD = 1 };
 
-template <class T, int MODE, bool DIRECT, class C>
+template <class T, int MODE, int HOW, class C>
 __global__ __launch_bounds__(C::THREADS, 2) void grouped_rows_kernel(GroupedArgs a) {
   typedef typename T::store E;
   constexpr int BK = Planes<T>::DEPTH;
@@ -76,8 +76,8 @@ __global__ __launch_bounds__(C::THREADS, 2) void grouped_rows_kernel(GroupedArgs
   Accumulators<C::NJ, C::NI> acc;
   acc.clear();
   const auto same = [](int r) { return (int64_t)r; };
-  DIMO_STAGE_BUFFERS(T, C, DIRECT);
-  run_stages<T, C, LINES, MODE == FORWARD ? LINES : COLUMNS, DIRECT, false>(sj, si, 0, reduction, same, same, acc, false, SJ0,
+  DIMO_STAGE_BUFFERS(T, C, HOW);
+  run_stages<T, C, LINES, MODE == FORWARD ? LINES : COLUMNS, HOW, false>(sj, si, 0, reduction, same, same, acc, false, SJ0,
                                                                             SI0, SJ1, SI1);
   __syncthreads();
   const E *bias = MODE == FORWARD && a.bias ? static_cast<const E *>(a.bias) + (int64_t)tile.expert * a.N : nullptr;
@@ -105,10 +105,91 @@ __global__ __launch_bounds__(C::THREADS, 2) void grouped_rows_kernel(GroupedArgs
   }
 }
 
+// WHOLE: the reduction is whole chunks of eight (then no load needs a branch: what is behind the end is read from the last
+// chunk and cleared)
+template <class T, bool WHOLE>
+__device__ __forceinline__ void thin_chunk(const typename T::store *line, int k, int K, typename T::store (&v)[8]) {
+  typedef typename T::store E;
+  if constexpr (WHOLE) {
+    __builtin_memcpy(v, line + min(k, K - 8), sizeof(v));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = k < K ? v[e] : E(0);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = k + e < K ? line[k + e] : E(0);
+  }
+}
+template <class T>
+__device__ __forceinline__ void thin_operand(const typename T::store (&v)[8], uint4 (&out)[Planes<T>::N]) {
+  if constexpr (Planes<T>::N == 1) {
+    __builtin_memcpy(&out[0], v, 16);
+  } else {
+    uint32_t w[3][4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const Split3 a = split3(v[2 * e]), b = split3(v[2 * e + 1]);
+      w[0][e] = a.hi | (uint32_t)b.hi << 16, w[1][e] = a.mid | (uint32_t)b.mid << 16, w[2][e] = a.lo | (uint32_t)b.lo << 16;
+    }
+#pragma unroll
+    for (int p = 0; p < 3; ++p) out[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+  }
+}
+
+template <class T, bool WHOLE>
+__global__ __launch_bounds__(64 * THIN_WAVES) void grouped_thin_kernel(GroupedArgs a) {
+  typedef typename T::store E;
+  constexpr int P = Planes<T>::N, STEPS = 128 / (16 * (int)sizeof(E));  // sixteens of the reduction in a line of memory
+  typedef typename Planes<T>::Tag Tag;
+  __shared__ float4 buffer[THIN_WAVES][4][64];
+  int ct = 0;
+  const RowTile tile = find_row_tile(a.offsets, a.E, a.R, 32, (a.N + 31) / 32, (int)blockIdx.x, &ct);
+  if (tile.expert < 0) return;
+  const int lane = threadIdx.x & 63, c0 = 32 * ct;
+  E *out = static_cast<E *>(a.y);
+  f32x16 acc;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+  const bool behind = tile.expert == a.E;  // the last group: zeros
+  if (!behind) {
+    const E *w = static_cast<const E *>(a.w) + ((int64_t)tile.expert * a.N + min(c0 + (lane & 31), a.N - 1)) * a.K;
+    const E *x = static_cast<const E *>(a.x) + source_row(a, min(tile.begin + (lane & 31), tile.end - 1)) * a.ldx;
+    for (int k1 = 0; k1 < a.K; k1 += 16 * STEPS * THIN_WAVES) {  // (the same count for every wave: behind the end are zeros)
+      const int k0 = k1 + 16 * STEPS * wave_number();
+      E vw[STEPS][8], vx[STEPS][8];
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        thin_chunk<T, WHOLE>(w, k0 + 16 * s + 8 * (lane >> 5), a.K, vw[s]);
+        thin_chunk<T, WHOLE>(x, k0 + 16 * s + 8 * (lane >> 5), a.K, vx[s]);
+      }
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        uint4 ow[P], ox[P];
+        thin_operand<T>(vw[s], ow);
+        thin_operand<T>(vx[s], ox);
+#pragma unroll
+        for (int d = P - 1; d >= 0; --d)
+#pragma unroll
+          for (int p = 0; p <= d; ++p) acc = mfma_32x32x16(Tag{}, ow[p], ox[d - p], acc);
+      }
+    }
+  }
+  sum_over_waves(acc, buffer, [&](float (&v)[4], int j, int i) {
+    const int r = tile.begin + j, c = c0 + i;
+    if (r >= tile.end || c >= a.N) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (a.bias && !behind) v[e] += T::load(static_cast<const E *>(a.bias)[(int64_t)tile.expert * a.N + min(c + e, a.N - 1)]);
+    if (a.z) store_quad<T>(static_cast<E *>(a.z) + (int64_t)r * a.N, c, a.N, a.wide, v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = behind ? 0.f : activate(v[e], a.act);
+    store_quad<T>(out + (int64_t)r * a.N, c, a.N, a.wide, v);
+  });
+}
+
 // gW[e]: rows n (from g) x columns k (from x), summed over the group's rows -- all of them, or split_rows of them into a
 // slice of `partial` (few experts with narrow weights would leave most of the chip idle otherwise; the slices are summed
 // in their order by the next kernel, so the result does not depend on the schedule)
-template <class T, bool DIRECT, class C>
+template <class T, int HOW, class C>
 __global__ __launch_bounds__(C::THREADS, 2) void grouped_wgrad_kernel(GroupedArgs a) {
   typedef typename T::store E;
   constexpr int BK = Planes<T>::DEPTH;
@@ -131,9 +212,9 @@ __global__ __launch_bounds__(C::THREADS, 2) void grouped_wgrad_kernel(GroupedArg
   Accumulators<C::NJ, C::NI> acc;
   acc.clear();
   const bool sums = a.gb && k0 == 0 && wave_number() % C::WI == 0;  // (one of the waves that read a row)
-  DIMO_STAGE_BUFFERS(T, C, DIRECT);
+  DIMO_STAGE_BUFFERS(T, C, HOW);
   if (begin < end)
-    run_stages<T, C, COLUMNS, COLUMNS, DIRECT, true>(sj, si, begin, end, [](int r) { return (int64_t)r; },
+    run_stages<T, C, COLUMNS, COLUMNS, HOW, true>(sj, si, begin, end, [](int r) { return (int64_t)r; },
                                                      [&](int r) { return source_row(a, r); }, acc, sums, SJ0, SI0, SJ1, SI1);
   __syncthreads();
   const int lane = threadIdx.x & 63, wave = wave_number();
@@ -166,10 +247,12 @@ __global__ __launch_bounds__(256) void grouped_wgrad_sum_kernel(GroupedArgs a) {
   typedef typename T::store E;
   const int e = blockIdx.y;
   int first = 0, count = 0;  // the expert's chunks: those of the experts before it come first
-  for (int i = 0; i <= e; ++i) {
-    const int lo = clamp_offset(a.offsets, i, a.R), hi = max(lo, clamp_offset(a.offsets, i + 1, a.R));
-    first += count;
-    count = (hi - lo + a.split_rows - 1) / a.split_rows;
+  for (int e0 = 0; e0 <= e; e0 += 64) {
+    RowTileScan s;
+    s.step(a.offsets, a.E, a.R, a.split_rows, e0);
+    const int upto = min(e - e0, 63);
+    count = __shfl(s.mine, upto);
+    first += __shfl(s.scan, upto) - (e0 + 63 < e ? 0 : count);
   }
   count = min(count, max(0, a.chunks - first));
   const int64_t size = (int64_t)a.N * a.K, all = size + (a.gb ? a.N : 0);
@@ -178,6 +261,7 @@ __global__ __launch_bounds__(256) void grouped_wgrad_sum_kernel(GroupedArgs a) {
                               : a.partial + (int64_t)a.chunks * size + (int64_t)first * a.N + (i - size);
     const int64_t step = i < size ? size : a.N;
     float s = 0.f;
+#pragma unroll 4
     for (int c = 0; c < count; ++c) s += p[c * step];
     if (i < size)
       static_cast<E *>(a.gw)[(int64_t)e * size + i] = T::save(s);
@@ -209,46 +293,64 @@ typedef Tile<64, 64, 2, 2> Small;
 typedef Tile<128, 128, 2, 2> Medium;
 typedef Tile<256, 256, 2, 4> Large;
 
-// rows on 16-byte boundaries whose ends are too
+// rows on 16-byte boundaries, their ends on whole chunks
 bool whole_chunks(int dtype, const void *p, int64_t ld, int64_t width) {
-  const int64_t per = 16 / (int64_t)dtype_bytes(dtype);
-  return dtype != DIMO_F32 && aligned16(p) && ld % per == 0 && width % per == 0;
+  return aligned16(p) && ld % (16 / (int64_t)dtype_bytes(dtype)) == 0 && width % 8 == 0;
 }
 bool wide_output(int dtype, const void *p, int64_t columns) {
   return columns % (16 / (int64_t)dtype_bytes(dtype)) == 0 && aligned16(p);
 }
 
-template <class T, int MODE, bool DIRECT, class C>
+template <class T, int MODE, int HOW, class C>
 int launch_rows(const GroupedArgs &a, hipStream_t s) {
   const int64_t groups = row_tile_workgroups(row_tile_count(a.R, a.E, C::TJ), ((MODE == FORWARD ? a.N : a.K) + C::TI - 1) / C::TI);
   if (groups > 0x7fffffffLL) return DIMO_E_ARG;
-  hipLaunchKernelGGL((grouped_rows_kernel<T, MODE, DIRECT, C>), dim3((unsigned)groups), dim3(C::THREADS), 0, s, a);
+  hipLaunchKernelGGL((grouped_rows_kernel<T, MODE, HOW, C>), dim3((unsigned)groups), dim3(C::THREADS), 0, s, a);
   return check_launch();
 }
-template <class T, bool DIRECT, class C>
+template <class T, int HOW, class C>
 int launch_wgrad(const GroupedArgs &a, hipStream_t s) {
   const int64_t tiles = (int64_t)((a.N + C::TJ - 1) / C::TJ) * ((a.K + C::TI - 1) / C::TI);
   const int64_t groups = a.split_rows ? row_tile_workgroups(row_tile_count(a.R, a.E, a.split_rows), tiles) : tiles * a.E;
   if (groups > 0x7fffffffLL || tiles > 0x7fffffffLL) return DIMO_E_ARG;
-  hipLaunchKernelGGL((grouped_wgrad_kernel<T, DIRECT, C>), dim3((unsigned)groups), dim3(C::THREADS), 0, s, a);
+  hipLaunchKernelGGL((grouped_wgrad_kernel<T, HOW, C>), dim3((unsigned)groups), dim3(C::THREADS), 0, s, a);
   return check_launch();
 }
 
+// Up to this many rows in all a forward takes the thin kernel: it reads each weight once per 32 rows of a group like the
+// tiles, but spreads the reduction over a workgroup's waves (one row, 2 x 2048 x 2048 of 16 experts in bf16: 5 us, the
+// 64 x 64 tile 18; 64 rows are a draw).
+constexpr int THIN_ROWS = 64;
+
 template <int MODE>
-int run_rows(int dtype, const GroupedArgs &a, bool direct, hipStream_t s) {
+int run_rows(int dtype, const GroupedArgs &a, bool whole, hipStream_t s) {
+  if (MODE == FORWARD && a.R <= THIN_ROWS) {
+    const int64_t groups = row_tile_workgroups(row_tile_count(a.R, a.E, 32), (a.N + 31) / 32);
+    if (groups > 0x7fffffffLL) return DIMO_E_ARG;
+    with_dtype(dtype, [&](auto tag) {
+      typedef decltype(tag) T;
+      if (a.K % 8 == 0)
+        hipLaunchKernelGGL((grouped_thin_kernel<T, true>), dim3((unsigned)groups), dim3(64 * THIN_WAVES), 0, s, a);
+      else
+        hipLaunchKernelGGL((grouped_thin_kernel<T, false>), dim3((unsigned)groups), dim3(64 * THIN_WAVES), 0, s, a);
+    });
+    return check_launch();
+  }
   const int64_t per_group = (a.R + a.E - 1) / a.E;
-  const int tile = choose_tile(per_group, (a.R + per_group - 1) / per_group, MODE == FORWARD ? a.N : a.K, direct);
+  const int tile = choose_tile(per_group, (a.R + per_group - 1) / per_group, MODE == FORWARD ? a.N : a.K,
+                               whole && dtype != DIMO_F32);
   int rc = DIMO_OK;
   with_dtype(dtype, [&](auto tag) {
     typedef decltype(tag) T;
-    if constexpr (sizeof(typename T::store) == 2) {
-      if (direct) {
-        rc = tile == LARGE ? launch_rows<T, MODE, true, Large>(a, s) : tile == MEDIUM ? launch_rows<T, MODE, true, Medium>(a, s)
-                                                                               : launch_rows<T, MODE, true, Small>(a, s);
-        return;
-      }
-    }
-    rc = tile == SMALL ? launch_rows<T, MODE, false, Small>(a, s) : launch_rows<T, MODE, false, Medium>(a, s);
+    constexpr int BEST = sizeof(typename T::store) == 2 ? DIRECT : WHOLE;
+    if (!whole)
+      rc = tile == SMALL ? launch_rows<T, MODE, ANY, Small>(a, s) : launch_rows<T, MODE, ANY, Medium>(a, s);
+    else if (tile == SMALL)
+      rc = launch_rows<T, MODE, BEST, Small>(a, s);
+    else if (tile == MEDIUM)
+      rc = launch_rows<T, MODE, BEST, Medium>(a, s);
+    else if constexpr (BEST == DIRECT)
+      rc = launch_rows<T, MODE, BEST, Large>(a, s);
   });
   return rc;
 }
@@ -263,7 +365,7 @@ WgradPlan wgrad_plan(int dtype, int R, int E, int K, int N) {
   const int64_t per_group = R > 0 ? (R + E - 1) / E : 1;
   const auto blocks = [&](int64_t t) { return (int64_t)E * ((N + t - 1) / t) * ((K + t - 1) / t); };
   const bool narrow = dtype == DIMO_F32;
-  p.tile = !narrow && blocks(256) >= 224 ? LARGE : N >= 96 && K >= 96 ? MEDIUM : SMALL;
+  p.tile = !narrow && blocks(256) >= 224 ? LARGE : N >= 96 && K >= 96 && (!narrow || blocks(128) >= 128) ? MEDIUM : SMALL;
   const int64_t have = blocks(p.tile == LARGE ? 256 : p.tile == MEDIUM ? 128 : 64);
   if (have < 512 && per_group >= 256) {
     const int64_t splits = (512 + have - 1) / have;
@@ -325,19 +427,19 @@ extern "C" int dimo_grouped_linear_wgrad(int dtype, int R, int E, int K, int N, 
   a.R = R, a.E = E, a.K = K, a.N = N, a.x = x, a.ldx = ldx, a.rows = rows, a.offsets = offsets;
   a.g = g, a.gw = gw, a.gb = gb, a.wide = wide_output(dtype, gw, K);
   a.split_rows = plan.split_rows, a.chunks = plan.chunks, a.partial = static_cast<float *>(workspace);
-  const bool direct = whole_chunks(dtype, g, N, N) && whole_chunks(dtype, x, ldx, K);
+  const bool whole = whole_chunks(dtype, g, N, N) && whole_chunks(dtype, x, ldx, K);
   int rc = DIMO_OK;
   with_dtype(dtype, [&](auto tag) {
     typedef decltype(tag) T;
-    bool done = false;
-    if constexpr (sizeof(typename T::store) == 2) {
-      if (direct) {
-        rc = plan.tile == LARGE ? launch_wgrad<T, true, Large>(a, s) : plan.tile == MEDIUM ? launch_wgrad<T, true, Medium>(a, s)
-                                                                                   : launch_wgrad<T, true, Small>(a, s);
-        done = true;
-      }
-    }
-    if (!done) rc = plan.tile == SMALL ? launch_wgrad<T, false, Small>(a, s) : launch_wgrad<T, false, Medium>(a, s);
+    constexpr int BEST = sizeof(typename T::store) == 2 ? DIRECT : WHOLE;
+    if (!whole)
+      rc = plan.tile == SMALL ? launch_wgrad<T, ANY, Small>(a, s) : launch_wgrad<T, ANY, Medium>(a, s);
+    else if (plan.tile == SMALL)
+      rc = launch_wgrad<T, BEST, Small>(a, s);
+    else if (plan.tile == MEDIUM)
+      rc = launch_wgrad<T, BEST, Medium>(a, s);
+    else if constexpr (BEST == DIRECT)
+      rc = launch_wgrad<T, BEST, Large>(a, s);
     if (!rc && a.split_rows) {
       const int64_t blocks = ((int64_t)N * K + (gb ? N : 0) + 255) / 256;
       hipLaunchKernelGGL((grouped_wgrad_sum_kernel<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096), E), dim3(256), 0, s, a);

@@ -24,6 +24,12 @@ __device__ __forceinline__ void load_to_lds(const void *from, uint16_t *S) {
   __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void *)from,
                                    (__attribute__((address_space(3))) void *)S, 16, 0, 0);
 }
+// Sixteen bytes from device memory by an address that may be a constant's: said to be global, or the compiler loads it as
+// "flat", which counts as an LDS access too.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ uint4 load_global(const void *p) {
+  return __builtin_bit_cast(uint4, *(const __attribute__((address_space(1))) u32x4 *)p);
+}
 // Eight bytes per lane from LDS, transposed among 16 lanes: lane j of them names four 16-bit values of row j / 4 (columns
 // 4 (j % 4) ..+ 3 of a 4 x 16 block) and gets column j of the block, rows 0 .. 3.
 typedef short s16x4 __attribute__((ext_vector_type(4)));

@@ -20,8 +20,8 @@ constexpr bool LINES = true, COLUMNS = false;
 // (a scalar: what it leads to stays out of the vector registers)
 __device__ __forceinline__ int wave_number() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
 
-// sixteen zero bytes: what lies behind the end of the reduction is read from here
-__device__ const uint4 zero_chunk = {0u, 0u, 0u, 0u};
+// a chunk of zeros: what lies behind the end of the reduction is read from here
+__device__ const uint4 zero_chunk[2] = {{0u, 0u, 0u, 0u}, {0u, 0u, 0u, 0u}};
 
 // Place (in chunks) of logical chunk c of LDS row `row`; `per_row` chunks in a row.  Eight neighbouring rows' chunk c
 // fall on eight different 16-byte columns of the banks, sixteen on sixteen of a bank row twice as wide.
@@ -115,11 +115,11 @@ struct Staging {
   template <class F>
   __device__ __forceinline__ const E *address(int q, int k0, int end, F &&row) const {
     if constexpr (ORDER == LINES) {
-      return k0 + col < end ? base[q] + k0 : reinterpret_cast<const E *>(&zero_chunk);
+      return k0 + col < end ? base[q] + k0 : reinterpret_cast<const E *>(zero_chunk);
     } else {
       const int r = k0 + lds_row(q);
       const E *p = base[0] + row(min(r, end - 1)) * ld;
-      return r < end ? p : reinterpret_cast<const E *>(&zero_chunk);
+      return r < end ? p : reinterpret_cast<const E *>(zero_chunk);
     }
   }
   // straight into LDS (16-bit elements, everything on 16-byte boundaries and the rows' ends too)
@@ -129,12 +129,20 @@ struct Staging {
     for (int q = 0; q < CHUNKS; ++q)
       load_to_lds(address(q, k0, end, row), S + (q * THREADS + 64 * wave_number()) * 8);
   }
-  // through registers: any alignment, any end
+  // through registers; whole: chunks are inside or outside as a whole, so that no load needs a branch
   typedef E Chunk[8];
-  template <class F>
+  template <bool WHOLE, class F>
   __device__ __forceinline__ void load(Chunk (&v)[CHUNKS], int k0, int end, F &&row) const {
 #pragma unroll
     for (int q = 0; q < CHUNKS; ++q) {
+      if constexpr (WHOLE) {
+        const char *from = reinterpret_cast<const char *>(address(q, k0, end, row));
+        uint4 w[sizeof(Chunk) / 16];
+#pragma unroll
+        for (int h = 0; h < (int)sizeof(Chunk) / 16; ++h) w[h] = load_global(from + 16 * h);
+        __builtin_memcpy(v[q], w, sizeof(Chunk));
+        continue;
+      }
       const E *p;
       int ok;
       if constexpr (ORDER == LINES) {
@@ -278,15 +286,19 @@ __device__ __forceinline__ void multiply_stage(const uint16_t *SJ, const uint16_
 
 // The LDS of a product's stages: separate arrays, so that the compiler knows that what is on its way into one is not what is
 // read from another (it would wait for every load in flight before each read otherwise).
-#define DIMO_STAGE_BUFFERS(T, C, DIRECT)                                                                                       \
+#define DIMO_STAGE_BUFFERS(T, C, HOW)                                                                                          \
   __shared__ __attribute__((aligned(1024))) uint16_t SJ0[Planes<T>::N * C::TJ * Planes<T>::DEPTH],                             \
-      SI0[Planes<T>::N * C::TI * Planes<T>::DEPTH], SJ1[DIRECT ? C::TJ * Planes<T>::DEPTH : 8],                                \
-      SI1[DIRECT ? C::TI * Planes<T>::DEPTH : 8]
+      SI0[Planes<T>::N * C::TI * Planes<T>::DEPTH], SJ1[HOW == DIRECT ? C::TJ * Planes<T>::DEPTH : 8],                                \
+      SI1[HOW == DIRECT ? C::TI * Planes<T>::DEPTH : 8]
 
-// The stages of a product, one after the other.  DIRECT: two LDS buffers, the next stage's loads go straight into the one
-// while the other is multiplied, one barrier per stage.  Otherwise (fp32, odd ends, odd alignment): the next stage waits in
-// registers, one buffer, two barriers.
-template <class T, class C, bool ORDER_J, bool ORDER_I, bool DIRECT, bool SUMS, class RowJ, class RowI>
+// How a stage gets into LDS.  DIRECT (16-bit, everything on 16-byte boundaries): two buffers, the next stage's loads go
+// straight into the one while the other is multiplied, one barrier per stage.  WHOLE (fp32 on such boundaries) and ANY: the
+// next stages wait in registers, one buffer, two barriers; a 64 x 64 tile has registers for two stages ahead, and needs
+// them: its stage is multiplied in a fraction of a load's round trip.
+enum Staged { ANY = 0, DIRECT = 1, WHOLE = 2 };
+
+// The stages of a product, one after the other.
+template <class T, class C, bool ORDER_J, bool ORDER_I, int HOW, bool SUMS, class RowJ, class RowI>
 __device__ __forceinline__ void run_stages(const Staging<T, ORDER_J, C::TJ, Planes<T>::DEPTH, C::THREADS> &sj,
                                            const Staging<T, ORDER_I, C::TI, Planes<T>::DEPTH, C::THREADS> &si, int begin,
                                            int end, RowJ &&row_j, RowI &&row_i, Accumulators<C::NJ, C::NI> &acc,
@@ -295,7 +307,7 @@ __device__ __forceinline__ void run_stages(const Staging<T, ORDER_J, C::TJ, Plan
   const int wave = wave_number();
   const Reader<ORDER_J, C::TJ, BK, C::NJ> rj((wave / C::WI) * 32 * C::NJ);
   const Reader<ORDER_I, C::TI, BK, C::NI> ri((wave % C::WI) * 32 * C::NI);
-  if constexpr (DIRECT) {
+  if constexpr (HOW == DIRECT) {
     const int stages = (end - begin + BK - 1) / BK;
     sj.load_direct(SJ0, begin, end, row_j);
     si.load_direct(SI0, begin, end, row_i);
@@ -321,21 +333,31 @@ __device__ __forceinline__ void run_stages(const Staging<T, ORDER_J, C::TJ, Plan
   } else {
     typedef Staging<T, ORDER_J, C::TJ, BK, C::THREADS> LJ;
     typedef Staging<T, ORDER_I, C::TI, BK, C::THREADS> LI;
-    typename LJ::Chunk vj[LJ::CHUNKS];
-    typename LI::Chunk vi[LI::CHUNKS];
-    sj.load(vj, begin, end, row_j);
-    si.load(vi, begin, end, row_i);
-    for (int k0 = begin; k0 < end; k0 += BK) {
-      __syncthreads();  // everyone is done with the last stage
-      sj.store(vj, SJ0, C::TJ * BK);
-      si.store(vi, SI0, C::TI * BK);
-      __syncthreads();
-      if (k0 + BK < end) {
-        sj.load(vj, k0 + BK, end, row_j);
-        si.load(vi, k0 + BK, end, row_i);
+    constexpr int AHEAD = HOW == WHOLE && C::NJ * C::NI == 1 ? 3 : 1;
+    typename LJ::Chunk vj[AHEAD][LJ::CHUNKS];
+    typename LI::Chunk vi[AHEAD][LI::CHUNKS];
+#pragma unroll
+    for (int d = 0; d < AHEAD; ++d) {
+      sj.template load<HOW == WHOLE>(vj[d], begin + d * BK, end, row_j);
+      si.template load<HOW == WHOLE>(vi[d], begin + d * BK, end, row_i);
+    }
+    for (int k1 = begin; k1 < end; k1 += AHEAD * BK) {
+#pragma unroll
+      for (int d = 0; d < AHEAD; ++d) {
+        const int k0 = k1 + d * BK;
+        if (k0 >= end) break;
+        __syncthreads();  // everyone is done with the last stage
+        sj.store(vj[d], SJ0, C::TJ * BK);
+        si.store(vi[d], SI0, C::TI * BK);
+        __syncthreads();
+        if (HOW == WHOLE || k0 + BK < end) {
+          sj.template load<HOW == WHOLE>(vj[d], k0 + AHEAD * BK, end, row_j);
+          si.template load<HOW == WHOLE>(vi[d], k0 + AHEAD * BK, end, row_i);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        multiply_stage<T, C, BK, SUMS>(SJ0, SI0, rj, ri, acc, with_sums);
+        acc.hold();
       }
-      __builtin_amdgcn_sched_barrier(0);
-      multiply_stage<T, C, BK, SUMS>(SJ0, SI0, rj, ri, acc, with_sums);
     }
   }
 }
@@ -379,80 +401,84 @@ __device__ __forceinline__ void write_outputs(const Accumulators<C::NJ, C::NI> &
   typedef typename T::store E;
   const int lane = threadIdx.x & 63, wave = wave_number();
   const int j0 = (wave / C::WI) * 32 * C::NJ, i0 = (wave % C::WI) * 32 * C::NI;
-  constexpr int SLAB_ROW = sizeof(E) * 32 * C::NI < 128 ? sizeof(E) * 32 * C::NI : 128;  // bytes of a row that go together
-  constexpr int CHUNKS = SLAB_ROW / 16, PER = 16 / (int)sizeof(E), SLABS = (int)sizeof(E) * 32 * C::NI / SLAB_ROW;
-  constexpr int BLOCKS = C::NI / SLABS;  // 32-column blocks per slab
-  if constexpr (C::WJ * C::WI * 32 * SLAB_ROW > BYTES) {
+  constexpr int ROW_BYTES = (int)sizeof(E) * 32 * C::NI, MOST = C::WJ * C::WI * 32 * 128 <= BYTES ? 128 : 64;
+  constexpr int SLAB_ROW = ROW_BYTES < MOST ? ROW_BYTES : MOST;  // bytes of a row that go together
+  constexpr int CHUNKS = SLAB_ROW / 16, PER = 16 / (int)sizeof(E), SLABS = ROW_BYTES / SLAB_ROW;
+  constexpr int EIGHTS = 4 * C::NI / SLABS;  // eights of columns per slab (a quad from each half of the wave)
+  static_assert(C::WJ * C::WI * 32 * SLAB_ROW <= BYTES, "4 KB (2 KB) per wave");
+  char *own = reinterpret_cast<char *>(buffer) + wave * 32 * SLAB_ROW;
 #pragma unroll
-    for (int i = 0; i < C::NI; ++i)
+  for (int j = 0; j < C::NJ; ++j)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
+    for (int s = 0; s < SLABS; ++s) {
+      __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int j = 0; j < C::NJ; ++j) {
-          const int c = i0 + 32 * i + 8 * q + 4 * (lane >> 5);
-          float v[4] = {acc.v[j][i][4 * q], acc.v[j][i][4 * q + 1], acc.v[j][i][4 * q + 2], acc.v[j][i][4 * q + 3]};
-          value(c, v);
-          E *row = at(j0 + 32 * j + (lane & 31));
-          if (!row || first_column + c >= columns) continue;
-          if constexpr (Out::ON)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (first_column + c + e < columns) v[e] *= activation_slope(T::load(row[first_column + c + e + slope.away]), slope.act);
-          store_quad<T>(row, first_column + c, columns, wide, v);
-        }
-  } else {
-    char *own = reinterpret_cast<char *>(buffer) + wave * 32 * SLAB_ROW;
-#pragma unroll
-    for (int j = 0; j < C::NJ; ++j)
-#pragma unroll
-      for (int s = 0; s < SLABS; ++s) {
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int i = 0; i < BLOCKS; ++i)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int in = 32 * i + 8 * q + 4 * (lane >> 5), b = s * BLOCKS + i;  // column inside the slab
-            float v[4] = {acc.v[j][b][4 * q], acc.v[j][b][4 * q + 1], acc.v[j][b][4 * q + 2], acc.v[j][b][4 * q + 3]};
-            value(i0 + 32 * b + 8 * q + 4 * (lane >> 5), v);
-            const int place = (in / PER) ^ (lane & (CHUNKS - 1));
-            store_quad<T>(reinterpret_cast<E *>(own + (lane & 31) * SLAB_ROW + 16 * place) + in % PER, 0, 4, true, v);
-          }
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int r = 0; r < 32; r += 64 / CHUNKS) {
-          const int row = r + lane / CHUNKS, chunk = lane % CHUNKS;
-          const uint4 v = *reinterpret_cast<const uint4 *>(own + row * SLAB_ROW + 16 * (chunk ^ (row & (CHUNKS - 1))));
-          E *dst = at(j0 + 32 * j + row);
-          const int c = first_column + i0 + 32 * BLOCKS * s + PER * chunk;
-          if (!dst || c >= columns) continue;
-          if (wide && c + PER <= columns) {
-            if constexpr (Out::ON) {
-              float f[PER], at_saved[PER];
-              Vec16<T> q{v};
-              q.get(f);
-              load_vec<T, PER>(dst + c + slope.away, at_saved);
-#pragma unroll
-              for (int k = 0; k < PER; ++k) f[k] *= activation_slope(at_saved[k], slope.act);
-              store_vec<T, PER>(dst + c, f);
-            } else {
-              *reinterpret_cast<uint4 *>(dst + c) = v;
-            }
-          } else {
-            E e[PER];
-            __builtin_memcpy(e, &v, 16);
-#pragma unroll
-            for (int k = 0; k < PER; ++k) {
-              if (c + k >= columns) continue;
-              if constexpr (Out::ON)
-                dst[c + k] = T::save(T::load(e[k]) * activation_slope(T::load(dst[c + k + slope.away]), slope.act));
-              else
-                dst[c + k] = e[k];
-            }
-          }
-        }
-        __builtin_amdgcn_sched_barrier(0);  // (block by block: all of them at once would not fit the registers)
+      for (int eight = 0; eight < EIGHTS; ++eight) {
+        const int in = 8 * eight + 4 * (lane >> 5), b = (s * EIGHTS + eight) / 4, q = (s * EIGHTS + eight) % 4;
+        float v[4] = {acc.v[j][b][4 * q], acc.v[j][b][4 * q + 1], acc.v[j][b][4 * q + 2], acc.v[j][b][4 * q + 3]};
+        value(i0 + 32 * b + 8 * q + 4 * (lane >> 5), v);
+        const int place = (in / PER) ^ (lane & (CHUNKS - 1));  // (in: the column inside the slab)
+        store_quad<T>(reinterpret_cast<E *>(own + (lane & 31) * SLAB_ROW + 16 * place) + in % PER, 0, 4, true, v);
       }
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int r = 0; r < 32; r += 64 / CHUNKS) {
+        const int row = r + lane / CHUNKS, chunk = lane % CHUNKS;
+        const uint4 v = *reinterpret_cast<const uint4 *>(own + row * SLAB_ROW + 16 * (chunk ^ (row & (CHUNKS - 1))));
+        E *dst = at(j0 + 32 * j + row);
+        const int c = first_column + i0 + 8 * EIGHTS * s + PER * chunk;
+        if (!dst || c >= columns) continue;
+        if (wide && c + PER <= columns) {
+          if constexpr (Out::ON) {
+            float f[PER], at_saved[PER];
+            Vec16<T> q{v};
+            q.get(f);
+            load_vec<T, PER>(dst + c + slope.away, at_saved);
+#pragma unroll
+            for (int k = 0; k < PER; ++k) f[k] *= activation_slope(at_saved[k], slope.act);
+            store_vec<T, PER>(dst + c, f);
+          } else {
+            *reinterpret_cast<uint4 *>(dst + c) = v;
+          }
+        } else {
+          E e[PER];
+          __builtin_memcpy(e, &v, 16);
+#pragma unroll
+          for (int k = 0; k < PER; ++k) {
+            if (c + k >= columns) continue;
+            if constexpr (Out::ON)
+              dst[c + k] = T::save(T::load(e[k]) * activation_slope(T::load(dst[c + k + slope.away]), slope.act));
+            else
+              dst[c + k] = e[k];
+          }
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);  // (block by block: all of them at once would not fit the registers)
+    }
+}
+
+// ---- few rows ------------------------------------------------------------------------------------------------------
+// A product of a handful of rows reads weights and does little else.  32 rows x 32 columns per workgroup: its THIN_WAVES
+// waves take the reduction in turn, a line (128 bytes) of every column at a time, straight from memory into the matrix
+// instruction's registers -- nothing is used twice, so nothing goes through LDS --, and add up their sums at the end.
+constexpr int THIN_WAVES = 8;
+
+// f(quad's sums, row of the tile, first of its four columns) for the workgroup's sums over its waves; `buffer`: 4 KB a wave
+template <class F>
+__device__ __forceinline__ void sum_over_waves(const f32x16 &acc, float4 (*buffer)[4][64], F &&f) {
+  const int lane = threadIdx.x & 63, wave = wave_number();
+#pragma unroll
+  for (int q = 0; q < 4; ++q) buffer[wave][q][lane] = make_float4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
+  __syncthreads();
+  const int t = threadIdx.x;
+  if (t >= 256) return;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int w = 0; w < THIN_WAVES; ++w) {
+    const float4 s = buffer[w][t >> 6][t & 63];
+    v[0] += s.x, v[1] += s.y, v[2] += s.z, v[3] += s.w;
   }
+  f(v, t & 31, 8 * (t >> 6) + 4 * ((t >> 5) & 1));
 }
 
 // Which tile: a workgroup's tile is worth its size only where there are enough of them.
@@ -460,7 +486,7 @@ enum { SMALL = 0, MEDIUM = 1, LARGE = 2 };
 inline int choose_tile(int64_t rows_per_group, int64_t groups, int64_t columns, bool direct) {
   const auto blocks = [&](int64_t t) { return groups * ((rows_per_group + t - 1) / t) * ((columns + t - 1) / t); };
   if (direct && rows_per_group >= 192 && columns >= 192 && blocks(256) >= 224) return LARGE;
-  if (rows_per_group >= 48 && columns >= 96 && blocks(128) >= 128) return MEDIUM;
+  if (rows_per_group >= 48 && columns >= 96 && blocks(128) >= 256) return MEDIUM;
   return SMALL;
 }
 

@@ -35,29 +35,30 @@ def _dtype(t, what):
 
 def _gpu(*tensors):
     """The tensors' common device (a GPU), or an error."""
-    device = tensors[0].device
+    first = tensors[0]
+    if not first.is_cuda:
+        raise RuntimeError("the expert operators need GPU tensors (no CPU fallback in the product path)")
+    device = first.device
     for t in tensors:
         if t is not None and t.device != device:
             raise ValueError(f"tensors on different devices ({device}, {t.device})")
-    if device.type != "cuda":
-        raise RuntimeError("the expert operators need GPU tensors (no CPU fallback in the product path)")
     return device
 
 
-class _on:
-    """Makes a tensor's device current for a launch (nothing to do when it is)."""
-
-    def __init__(self, device):
-        self.index = device.index
-
+class _Nothing:
     def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
+        pass
 
     def __exit__(self, *_):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
+        pass
+
+
+_HERE = _Nothing()
+
+
+def _on(device):
+    """Makes a tensor's device current for a launch (nothing to do when it is: one query of the runtime)."""
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def _rows(t):
@@ -83,10 +84,11 @@ def _route_forward(logits, k, row_mask, normalize):
     experts = torch.empty(T, k, dtype=torch.int32, device=logits.device)
     load = torch.empty(E, dtype=torch.float32, device=logits.device)
     with _on(logits.device):
-        ws = torch.empty(L.dimo_route_workspace_bytes(T, E), dtype=torch.uint8, device=logits.device)
+        nbytes = L.dimo_route_workspace_bytes(T, E)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device) if nbytes else None
         _lib.check(L.dimo_route_topk_forward(T, E, k, _DTYPES[logits.dtype], logits.data_ptr(), _ld(logits),
                                              _lib.ptr(row_mask), int(normalize), weights.data_ptr(), experts.data_ptr(),
-                                             load.data_ptr(), ws.data_ptr(), ws.numel(), _lib.current_stream()),
+                                             load.data_ptr(), _lib.ptr(ws), nbytes, _lib.current_stream()),
                    "dimo_route_topk_forward")
     return weights, experts, load
 

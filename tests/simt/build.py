@@ -139,7 +139,9 @@ TARGETS["experts"] = (["experts.hip", "grouped.hip", "expert_mlp.hip", "mx4.hip"
 SEPARATE.add("experts")
 SUBST["experts.hip"] = []
 SUBST["grouped.hip"] = []
-SUBST["mx4.hip"] = []
+SUBST["mx4.hip"] = [
+    ("typedef float f32x2 __attribute__((ext_vector_type(2)));", "typedef float f32x2 __attribute__((vector_size(8)));"),
+]
 SUBST["expert_mlp.hip"] = []
 SUBST["row_tiles.hpp"] = []
 SUBST["tile_product.hpp"] = [  # (an empty statement that pins registers)
@@ -162,6 +164,8 @@ SUBST["matrix_ops.hpp"] = [
      "simt_mfma_32x32x16(a, b, c, simt_from_bf16)"),
     ("__builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0)",
      "simt_mfma_32x32x16(a, b, c, simt_from_f16)"),
+    ("typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));", ""),
+    ("__builtin_bit_cast(uint4, *(const __attribute__((address_space(1))) u32x4 *)p)", "*reinterpret_cast<const uint4 *>(p)"),
     ("typedef short s16x4 __attribute__((ext_vector_type(4)));", ""),
     ("""__builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void *)from,
                                    (__attribute__((address_space(3))) void *)S, 16, 0, 0);""", "simt_load_to_lds(from, S);"),

@@ -363,6 +363,28 @@ struct SimtOperands {
     }
   }
 };
+static inline uint32_t __umulhi(uint32_t a, uint32_t b) { return (uint32_t)(((uint64_t)a * b) >> 32); }
+// v_cvt_scalef32_pk_fp4_f32: byte `sel` of the result = the e2m1 codes of a / scale (low four bits) and b / scale, to nearest,
+// ties to the even code, beyond 6 to 6
+static inline uint32_t simt_fp4_code(float v, float scale) {
+  const double a = fabs((double)v) / scale;
+  if (!(a == a)) return 7u;
+  return (uint32_t)((a > .25) + (a >= .75) + (a > 1.25) + (a >= 1.75) + (a > 2.5) + (a >= 3.5) + (a > 5.)) | (signbit(v) ? 8u : 0u);
+}
+static inline uint32_t simt_cvt_pk_fp4(uint32_t old, float a, float b, float scale, int sel) {
+  const uint32_t byte = simt_fp4_code(a, scale) | simt_fp4_code(b, scale) << 4;
+  return (old & ~(255u << (8 * sel))) | byte << (8 * sel);
+}
+#define __builtin_amdgcn_cvt_scalef32_pk_fp4_f32 simt_cvt_pk_fp4
+// v_cvt_scalef32_pk_f32_fp4: the two values of byte `sel`
+typedef float simt_f32x2 __attribute__((vector_size(8)));
+static inline simt_f32x2 simt_cvt_pk_f32_fp4(uint32_t w, float scale, int sel) {
+  static const float mag[8] = {0.f, .5f, 1.f, 1.5f, 2.f, 3.f, 4.f, 6.f};
+  const uint32_t b = w >> (8 * sel);
+  const float lo = (b & 8 ? -1.f : 1.f) * mag[b & 7] * scale, hi = (b & 128 ? -1.f : 1.f) * mag[(b >> 4) & 7] * scale;
+  return simt_f32x2{lo, hi};
+}
+#define __builtin_amdgcn_cvt_scalef32_pk_f32_fp4 simt_cvt_pk_f32_fp4
 // v_perm_b32: byte i of the result = byte (sel >> 8 i) & 7 of the eight bytes lo, hi
 static inline uint32_t simt_perm(uint32_t hi, uint32_t lo, uint32_t sel) {
   const uint64_t v = ((uint64_t)hi << 32) | lo;

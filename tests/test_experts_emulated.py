@@ -155,7 +155,7 @@ def test_c_entry_points_refuse():
     assert L.dimo_route_topk_forward(4, 6, 7, 0, 1, 6, None, 1, 1, 1, None, None, 0, None) == -1
     assert L.dimo_route_topk_forward(4, 6, 2, 3, 1, 6, None, 1, 1, 1, None, None, 0, None) == -1
     assert L.dimo_route_topk_forward(4, 6, 2, 0, 1, 5, None, 1, 1, 1, None, None, 0, None) == -1
-    assert L.dimo_route_topk_forward(4, 6, 2, 0, 1, 6, None, 1, 1, 1, 1, None, 0, None) == -3
+    assert L.dimo_route_topk_forward(4096, 6, 2, 0, 1, 6, None, 1, 1, 1, 1, None, 0, None) == -3
     assert L.dimo_route_topk_forward(4, 6, 2, 0, None, 6, None, 1, 1, 1, None, None, 0, None) == -1
     assert L.dimo_group_rows(10000, 6, 2, 1, 1, 1, 1, None, None, 0, None) == -3
     assert L.dimo_group_rows(-1, 6, 2, 1, 1, 1, 1, None, None, 0, None) == -1
