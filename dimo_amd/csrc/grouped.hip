@@ -201,7 +201,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void grouped_wgrad_kernel(GroupedArg
     if (t.expert < 0 || t.expert == a.E || t.number >= a.chunks) return;
     expert = t.expert, begin = t.begin, end = t.end, chunk = t.number, block = column;
   } else {
-    expert = blockIdx.x / (tiles_k * tiles_n), block = blockIdx.x % (tiles_k * tiles_n);
+    expert = largest_first(a.offsets, a.E, a.R, blockIdx.x / (tiles_k * tiles_n)), block = blockIdx.x % (tiles_k * tiles_n);
     begin = clamp_offset(a.offsets, expert, a.R), end = max(begin, clamp_offset(a.offsets, expert + 1, a.R));
   }
   const int n0 = block / tiles_k * C::TJ, k0 = block % tiles_k * C::TI;
@@ -355,7 +355,14 @@ int run_rows(int dtype, const GroupedArgs &a, bool whole, hipStream_t s) {
   return rc;
 }
 
-// wgrad: the tile, and rows per slice (0: no split): enough workgroups for two on every CU
+// wgrad: the tile, and rows per slice (0: no split).  Measured on equal groups (rows, groups, N x K; us):
+//                            fp32: 64 / 128 tiles           bf16: 64 / 128 / 256 tiles
+//   8192, 8, 256 x 256       22 / 24 (split), 61 unsplit    9 / 17 / 30 unsplit, 14 / 16 split
+//   65536, 4, 256 x 256      78 / 60 (split)                26 / 26 (split)
+//   32768, 16, 1024 x 256    139 / 116                      - / 36 / 52
+//   16384, 8, 1024 x 1024    257 / 182                      66 / 50 / 59
+// A split costs writing and reading the slices in fp32: it pays where fewer than half of the CUs would have a workgroup
+// (16-bit), or two (fp32, whose stages take six times as long), and slices stay at 256 rows or more.
 struct WgradPlan {
   int tile, split_rows, chunks;
   size_t bytes;
@@ -364,13 +371,16 @@ WgradPlan wgrad_plan(int dtype, int R, int E, int K, int N) {
   WgradPlan p{SMALL, 0, 0, 0};
   const int64_t per_group = R > 0 ? (R + E - 1) / E : 1;
   const auto blocks = [&](int64_t t) { return (int64_t)E * ((N + t - 1) / t) * ((K + t - 1) / t); };
-  const bool narrow = dtype == DIMO_F32;
-  p.tile = !narrow && blocks(256) >= 224 ? LARGE : N >= 96 && K >= 96 && (!narrow || blocks(128) >= 128) ? MEDIUM : SMALL;
-  const int64_t have = blocks(p.tile == LARGE ? 256 : p.tile == MEDIUM ? 128 : 64);
-  if (have < 512 && per_group >= 256) {
-    const int64_t splits = (512 + have - 1) / have;
+  const bool f32 = dtype == DIMO_F32;
+  if (!f32 && blocks(256) >= 512)
+    p.tile = LARGE;
+  else if (N >= 96 && K >= 96 && (f32 ? blocks(128) * per_group >= 128 * 1024 : blocks(128) >= 128))
+    p.tile = MEDIUM;
+  const int64_t have = blocks(p.tile == LARGE ? 256 : p.tile == MEDIUM ? 128 : 64), enough = f32 ? 512 : 128;
+  if (have < enough && per_group >= 512) {
+    const int64_t want = f32 ? 512 : 256, splits = (want + have - 1) / have;
     int64_t rows = (per_group + splits - 1) / splits;
-    rows = rows < 128 ? 128 : (rows + 63) / 64 * 64;
+    rows = rows < 256 ? 256 : (rows + 63) / 64 * 64;
     p.split_rows = (int)rows, p.chunks = row_tile_count(R, E, (int)rows);
     p.bytes = align_up((size_t)p.chunks * ((size_t)N * K + N) * sizeof(float));
   }

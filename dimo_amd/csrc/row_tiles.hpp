@@ -83,6 +83,21 @@ __device__ __forceinline__ RowTile find_row_tile(const int32_t *__restrict__ off
   }
   return t;
 }
+// The expert with the n-th most rows (up to 64 experts; otherwise n itself): work that is unequal from expert to expert is
+// handed out largest first, so that no large piece is left for the end.
+__device__ __forceinline__ int largest_first(const int32_t *__restrict__ offsets, int E, int R, int n) {
+  if (E > 64) return n;
+  const int lane = threadIdx.x & 63;
+  const int lo = lane < E ? clamp_offset(offsets, lane, R) : 0, hi = lane < E ? max(lo, clamp_offset(offsets, lane + 1, R)) : -1;
+  const int mine = hi - lo;  // (-1 behind the last expert)
+  int rank = 0;
+  for (int e = 0; e < E; ++e) {
+    const int other = __builtin_amdgcn_readlane(mine, e);
+    rank += other > mine || (other == mine && e < lane);
+  }
+  const unsigned long long it = __ballot(lane < E && rank == n);
+  return it ? __ffsll((long long)it) - 1 : n;
+}
 // workgroups for up to `tiles` x `columns` blocks: every XCD's share rounded up
 inline int64_t row_tile_workgroups(int64_t tiles, int64_t columns) { return (tiles * columns + 7) / 8 * 8; }
 
