@@ -75,9 +75,8 @@ __global__ __launch_bounds__(C::THREADS, 2) void grouped_rows_kernel(GroupedArgs
     si.init_columns(W + c0, a.K, a.K - c0);
   Accumulators<C::NJ, C::NI> acc;
   acc.clear();
-  const auto same = [](int r) { return (int64_t)r; };
   DIMO_STAGE_BUFFERS(T, C, HOW);
-  run_stages<T, C, LINES, MODE == FORWARD ? LINES : COLUMNS, HOW, false>(sj, si, 0, reduction, same, same, acc, false, SJ0,
+  run_stages<T, C, LINES, MODE == FORWARD ? LINES : COLUMNS, HOW, false>(sj, si, 0, reduction, SameRow{}, SameRow{}, acc, false, SJ0,
                                                                             SI0, SJ1, SI1);
   __syncthreads();
   const E *bias = MODE == FORWARD && a.bias ? static_cast<const E *>(a.bias) + (int64_t)tile.expert * a.N : nullptr;
@@ -186,20 +185,69 @@ __global__ __launch_bounds__(64 * THIN_WAVES) void grouped_thin_kernel(GroupedAr
   });
 }
 
-// gW[e]: rows n (from g) x columns k (from x), summed over the group's rows -- all of them, or split_rows of them into a
-// slice of `partial` (few experts with narrow weights would leave most of the chip idle otherwise; the slices are summed
-// in their order by the next kernel, so the result does not depend on the schedule)
-template <class T, int HOW, class C>
+// gW[e]: rows n (from g) x columns k (from x), summed over the group's rows -- all of them, or split_rows of them at a time:
+// a group of more rows than that is cut into slices, whose sums go to `partial` and are added in their order by the next
+// kernel (the result does not depend on the schedule).
+//
+// Slices of the expert's group (0 or 1: it is not cut) and the number of slices of cut groups before it.
+__device__ __forceinline__ int cut_slices(const GroupedArgs &a, int expert, int *before) {
+  int count = 0;
+  *before = 0;
+  for (int e0 = 0; e0 <= expert; e0 += 64) {
+    RowTileScan s;
+    s.step(a.offsets, a.E, a.R, a.split_rows, e0);
+    const int lane = threadIdx.x & 63;
+    int cut = e0 + lane < expert && s.mine > 1 ? s.mine : 0;
+#pragma unroll
+    for (int d = 32; d; d /= 2) cut += __shfl_xor(cut, d);
+    *before += cut;
+    if (expert - e0 < 64) count = __shfl(s.mine, expert - e0);
+  }
+  return __builtin_amdgcn_readfirstlane(count);
+}
+// The n-th slice of all groups, whole ones first, so that no long piece of work is left for the end; -1: there are fewer.
+__device__ __forceinline__ int find_slice(const GroupedArgs &a, int n, int *begin, int *end) {
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int rest = 0; rest < 2; ++rest)
+    for (int e0 = 0; e0 < a.E; e0 += 64) {
+      const int e = e0 + lane;
+      const int lo = e < a.E ? clamp_offset(a.offsets, e, a.R) : 0;
+      const int size = e < a.E ? max(lo, clamp_offset(a.offsets, e + 1, a.R)) - lo : 0, whole = size / a.split_rows;
+      const int mine = rest ? size > whole * a.split_rows : whole;
+      int scan = mine;
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) {
+        const int o = __shfl_up(scan, d);
+        if (lane >= d) scan += o;
+      }
+      const unsigned long long past = __ballot(before + scan > n);
+      if (past) {
+        const int f = __ffsll((long long)past) - 1;
+        const int at = rest ? whole : n - (before + scan - mine);
+        *begin = __builtin_amdgcn_readlane(lo + (lane == f ? at : 0) * a.split_rows, f);
+        *end = min(*begin + a.split_rows, __builtin_amdgcn_readlane(lo + size, f));
+        return e0 + f;
+      }
+      before += __builtin_amdgcn_readlane(scan, 63);
+    }
+  return -1;
+}
+template <class T, int HOW, class C, class Row>
 __global__ __launch_bounds__(C::THREADS, 2) void grouped_wgrad_kernel(GroupedArgs a) {
   typedef typename T::store E;
   constexpr int BK = Planes<T>::DEPTH;
   const int tiles_k = (a.K + C::TI - 1) / C::TI, tiles_n = (a.N + C::TJ - 1) / C::TJ;
-  int expert, begin, end, chunk = 0, block;
+  int expert, begin, end, chunk = -1, block;  // chunk: the slice's place in `partial`
   if (a.split_rows) {
-    int column = 0;
-    const RowTile t = find_row_tile(a.offsets, a.E, a.R, a.split_rows, tiles_k * tiles_n, (int)blockIdx.x, &column);
-    if (t.expert < 0 || t.expert == a.E || t.number >= a.chunks) return;
-    expert = t.expert, begin = t.begin, end = t.end, chunk = t.number, block = column;
+    int before = 0;
+    block = blockIdx.x % (tiles_k * tiles_n);
+    expert = find_slice(a, blockIdx.x / (tiles_k * tiles_n), &begin, &end);
+    if (expert < 0) return;
+    if (cut_slices(a, expert, &before) > 1) {
+      chunk = __builtin_amdgcn_readfirstlane(before) + (begin - clamp_offset(a.offsets, expert, a.R)) / a.split_rows;
+      if (chunk >= a.chunks) return;  // (only where bad offsets make the groups overlap)
+    }
   } else {
     expert = largest_first(a.offsets, a.E, a.R, blockIdx.x / (tiles_k * tiles_n)), block = blockIdx.x % (tiles_k * tiles_n);
     begin = clamp_offset(a.offsets, expert, a.R), end = max(begin, clamp_offset(a.offsets, expert + 1, a.R));
@@ -213,15 +261,16 @@ __global__ __launch_bounds__(C::THREADS, 2) void grouped_wgrad_kernel(GroupedArg
   acc.clear();
   const bool sums = a.gb && k0 == 0 && wave_number() % C::WI == 0;  // (one of the waves that read a row)
   DIMO_STAGE_BUFFERS(T, C, HOW);
+  Row row;
+  if constexpr (Row::AHEAD) row.rows = a.rows;
   if (begin < end)
-    run_stages<T, C, COLUMNS, COLUMNS, HOW, true>(sj, si, begin, end, [](int r) { return (int64_t)r; },
-                                                     [&](int r) { return source_row(a, r); }, acc, sums, SJ0, SI0, SJ1, SI1);
+    run_stages<T, C, COLUMNS, COLUMNS, HOW, true>(sj, si, begin, end, SameRow{}, row, acc, sums, SJ0, SI0, SJ1, SI1);
   __syncthreads();
   const int lane = threadIdx.x & 63, wave = wave_number();
   float *pw = a.partial + (int64_t)chunk * a.N * a.K, *pb = a.partial + (int64_t)a.chunks * a.N * a.K + (int64_t)chunk * a.N;
   E *gw = static_cast<E *>(a.gw) + (int64_t)expert * a.N * a.K, *gb = static_cast<E *>(a.gb) + (int64_t)expert * a.N;
   const auto as_it_is = [](int, float (&)[4]) {};
-  if (a.split_rows)
+  if (chunk >= 0)
     write_outputs<F32, C, (int)sizeof(SJ0)>(acc, SJ0, k0, a.K, a.wide,
                                             [&](int j) { return n0 + j < a.N ? pw + (int64_t)(n0 + j) * a.K : nullptr; }, as_it_is, NoSlope{});
   else
@@ -233,7 +282,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void grouped_wgrad_kernel(GroupedArg
       const float v = acc.sums[j] + __shfl_xor(acc.sums[j], 32);
       const int n = n0 + (wave / C::WI) * 32 * C::NJ + 32 * j + lane;
       if (lane >= 32 || n >= a.N) continue;
-      if (a.split_rows)
+      if (chunk >= 0)
         pb[n] = v;
       else
         gb[n] = T::save(v);
@@ -241,33 +290,37 @@ __global__ __launch_bounds__(C::THREADS, 2) void grouped_wgrad_kernel(GroupedArg
   }
 }
 
-// gW[e], gb[e] = the sums of the expert's slices, in their order (zeros without any)
+// gW[e], gb[e] of the experts whose group is cut (the sums of its slices) or empty (zeros)
 template <class T>
 __global__ __launch_bounds__(256) void grouped_wgrad_sum_kernel(GroupedArgs a) {
   typedef typename T::store E;
   const int e = blockIdx.y;
-  int first = 0, count = 0;  // the expert's chunks: those of the experts before it come first
-  for (int e0 = 0; e0 <= e; e0 += 64) {
-    RowTileScan s;
-    s.step(a.offsets, a.E, a.R, a.split_rows, e0);
-    const int upto = min(e - e0, 63);
-    count = __shfl(s.mine, upto);
-    first += __shfl(s.scan, upto) - (e0 + 63 < e ? 0 : count);
-  }
+  int first;
+  int count = cut_slices(a, e, &first);
+  if (count == 1) return;
   count = min(count, max(0, a.chunks - first));
-  const int64_t size = (int64_t)a.N * a.K, all = size + (a.gb ? a.N : 0);
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
-    const float *p = i < size ? a.partial + (int64_t)first * size + i
-                              : a.partial + (int64_t)a.chunks * size + (int64_t)first * a.N + (i - size);
-    const int64_t step = i < size ? size : a.N;
-    float s = 0.f;
+  const int64_t size = (int64_t)a.N * a.K, stride = (int64_t)gridDim.x * 256, t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const float *pw = a.partial + (int64_t)first * size, *pb = a.partial + (int64_t)a.chunks * size + (int64_t)first * a.N;
+  E *gw = static_cast<E *>(a.gw) + (int64_t)e * size, *gb = static_cast<E *>(a.gb) + (int64_t)e * a.N;
+  const int64_t quads = a.wide ? size / 4 : 0;
+  for (int64_t i = 4 * t; i < 4 * quads; i += 4 * stride) {
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int c = 0; c < count; ++c) s += p[c * step];
-    if (i < size)
-      static_cast<E *>(a.gw)[(int64_t)e * size + i] = T::save(s);
-    else
-      static_cast<E *>(a.gb)[(int64_t)e * a.N + (i - size)] = T::save(s);
+    for (int c = 0; c < count; ++c) {
+      const float4 p = *reinterpret_cast<const float4 *>(pw + c * size + i);
+      v[0] += p.x, v[1] += p.y, v[2] += p.z, v[3] += p.w;
+    }
+    store_quad<T>(gw + i, 0, 4, true, v);
   }
+  const auto sum = [&](const float *p, int64_t step) {
+    float v = 0.f;
+#pragma unroll 4
+    for (int c = 0; c < count; ++c) v += p[c * step];
+    return T::save(v);
+  };
+  for (int64_t i = 4 * quads + t; i < size; i += stride) gw[i] = sum(pw + i, size);
+  if (a.gb)
+    for (int64_t i = t; i < a.N; i += stride) gb[i] = sum(pb + i, a.N);
 }
 
 // gz = gy act'(s): s is the activation's output for relu (positive exactly where its input is) and its input for silu
@@ -311,9 +364,12 @@ int launch_rows(const GroupedArgs &a, hipStream_t s) {
 template <class T, int HOW, class C>
 int launch_wgrad(const GroupedArgs &a, hipStream_t s) {
   const int64_t tiles = (int64_t)((a.N + C::TJ - 1) / C::TJ) * ((a.K + C::TI - 1) / C::TI);
-  const int64_t groups = a.split_rows ? row_tile_workgroups(row_tile_count(a.R, a.E, a.split_rows), tiles) : tiles * a.E;
+  const int64_t groups = tiles * (a.split_rows ? row_tile_count(a.R, a.E, a.split_rows) : a.E);
   if (groups > 0x7fffffffLL || tiles > 0x7fffffffLL) return DIMO_E_ARG;
-  hipLaunchKernelGGL((grouped_wgrad_kernel<T, HOW, C>), dim3((unsigned)groups), dim3(C::THREADS), 0, s, a);
+  if (a.rows)
+    hipLaunchKernelGGL((grouped_wgrad_kernel<T, HOW, C, SourceRow>), dim3((unsigned)groups), dim3(C::THREADS), 0, s, a);
+  else
+    hipLaunchKernelGGL((grouped_wgrad_kernel<T, HOW, C, SameRow>), dim3((unsigned)groups), dim3(C::THREADS), 0, s, a);
   return check_launch();
 }
 
@@ -355,14 +411,23 @@ int run_rows(int dtype, const GroupedArgs &a, bool whole, hipStream_t s) {
   return rc;
 }
 
-// wgrad: the tile, and rows per slice (0: no split).  Measured on equal groups (rows, groups, N x K; us):
-//                            fp32: 64 / 128 tiles           bf16: 64 / 128 / 256 tiles
-//   8192, 8, 256 x 256       22 / 24 (split), 61 unsplit    9 / 17 / 30 unsplit, 14 / 16 split
-//   65536, 4, 256 x 256      78 / 60 (split)                26 / 26 (split)
-//   32768, 16, 1024 x 256    139 / 116                      - / 36 / 52
-//   16384, 8, 1024 x 1024    257 / 182                      66 / 50 / 59
-// A split costs writing and reading the slices in fp32: it pays where fewer than half of the CUs would have a workgroup
-// (16-bit), or two (fp32, whose stages take six times as long), and slices stay at 256 rows or more.
+// wgrad: the tile, and rows per slice (0: groups stay whole).  Measured in bf16 / fp32, uneven groups drawn from a
+// lognormal distribution (rows, groups, N x K; us; "cut at 2": groups of more than twice the mean are cut):
+//                                  64 tile          128 tile                      256 tile
+//   8192, 8, 256 x 256     even    10 / 23          17 / 27                       -       the 64s whole; 14 cut to 256 slices
+//                          uneven  15 / 25          18 / 27                       -       the 64s cut to 256 / 512; > 18 whole
+//   65536, 4, 256 x 256    even    38 / 89          33 / 65                       39      256 / 512 slices; 128s whole 61 / -
+//   65536, 1, 2048 x 256   even    154 / 590        122 / 402                     107     cut to 256 / 512; 64s whole 684 / -
+//   32768, 8, 1024 x 1024  even    131 / 532        96 whole, 101 cut at 2 / 380  99
+//                          uneven  150 / 552        181, 117 / 847, 519           133
+//   32768, 32, 1024 x 512  uneven  99 / 280         82, 82 / 350, 267             98
+//   4096, 8, 2048 x 512    uneven  29 / 76          29, 28 / 115, 79              -
+//   32768, 16, 4096 x 1024 even    - / -            401 / -                       313 whole, 330 cut at 2
+//                          uneven  - / -            393 / -                       306 whole, 366 cut at 2
+// So: the largest tile whose products last long enough to fill the chip in slices; slices where there are fewer workgroups
+// than CUs (fp32, whose stages take six times as long: than twice that), of 256 rows or more; with as many
+// 128 tiles as that, the groups of more than twice the mean are cut; with as many 256 tiles, taking the largest groups first
+// serves better, because slices are written and read once more in fp32.
 struct WgradPlan {
   int tile, split_rows, chunks;
   size_t bytes;
@@ -372,16 +437,25 @@ WgradPlan wgrad_plan(int dtype, int R, int E, int K, int N) {
   const int64_t per_group = R > 0 ? (R + E - 1) / E : 1;
   const auto blocks = [&](int64_t t) { return (int64_t)E * ((N + t - 1) / t) * ((K + t - 1) / t); };
   const bool f32 = dtype == DIMO_F32;
-  if (!f32 && blocks(256) >= 512)
+  if (!f32 && N >= 192 && K >= 192 && blocks(256) * per_group >= 512 * 1024)
     p.tile = LARGE;
-  else if (N >= 96 && K >= 96 && (f32 ? blocks(128) * per_group >= 128 * 1024 : blocks(128) >= 128))
+  else if (N >= 96 && K >= 96 && blocks(128) * per_group >= (f32 ? 128 : 256) * 1024)
     p.tile = MEDIUM;
-  const int64_t have = blocks(p.tile == LARGE ? 256 : p.tile == MEDIUM ? 128 : 64), enough = f32 ? 512 : 128;
-  if (have < enough && per_group >= 512) {
-    const int64_t want = f32 ? 512 : 256, splits = (want + have - 1) / have;
-    int64_t rows = (per_group + splits - 1) / splits;
-    rows = rows < 256 ? 256 : (rows + 63) / 64 * 64;
-    p.split_rows = (int)rows, p.chunks = row_tile_count(R, E, (int)rows);
+  const int64_t have = blocks(p.tile == LARGE ? 256 : p.tile == MEDIUM ? 128 : 64), enough = f32 ? 512 : 256;
+  int64_t rows = 0;
+  if (per_group >= 512) {
+    if (have < enough) {
+      const int64_t splits = (enough + have - 1) / have;
+      rows = (per_group + splits - 1) / splits;
+      rows = rows < 256 ? 256 : (rows + 63) / 64 * 64;
+    } else if (p.tile == MEDIUM) {
+      rows = (2 * per_group + 63) / 64 * 64;
+    }
+  }
+  if (rows && rows < R) {
+    // a group of r > rows rows is cut into fewer than 2 r / rows slices
+    const int64_t cut = 2 * (int64_t)R / rows, slices = row_tile_count(R, E, (int)rows);
+    p.split_rows = (int)rows, p.chunks = (int)(cut < slices ? cut : slices);
     p.bytes = align_up((size_t)p.chunks * ((size_t)N * K + N) * sizeof(float));
   }
   return p;
@@ -451,8 +525,9 @@ extern "C" int dimo_grouped_linear_wgrad(int dtype, int R, int E, int K, int N, 
     else if constexpr (BEST == DIRECT)
       rc = launch_wgrad<T, BEST, Large>(a, s);
     if (!rc && a.split_rows) {
-      const int64_t blocks = ((int64_t)N * K + (gb ? N : 0) + 255) / 256;
-      hipLaunchKernelGGL((grouped_wgrad_sum_kernel<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096), E), dim3(256), 0, s, a);
+      // (most experts' workgroups may find nothing to do: few each, unless there are few experts)
+      const int64_t blocks = ((int64_t)N * K / (a.wide ? 4 : 1) + 255) / 256, most = E < 16 ? 4096 / E : 256;
+      hipLaunchKernelGGL((grouped_wgrad_sum_kernel<T>), dim3((unsigned)(blocks < most ? blocks : most), E), dim3(256), 0, s, a);
       rc = check_launch();
     }
   });

@@ -30,6 +30,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ uint4 load_global(const void *p) {
   return __builtin_bit_cast(uint4, *(const __attribute__((address_space(1))) u32x4 *)p);
 }
+__device__ __forceinline__ int32_t load_global(const int32_t *p) { return *(const __attribute__((address_space(1))) int32_t *)p; }
 // Eight bytes per lane from LDS, transposed among 16 lanes: lane j of them names four 16-bit values of row j / 4 (columns
 // 4 (j % 4) ..+ 3 of a 4 x 16 block) and gets column j of the block, rows 0 .. 3.
 typedef short s16x4 __attribute__((ext_vector_type(4)));

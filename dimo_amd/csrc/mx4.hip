@@ -225,7 +225,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx4_rows_kernel(Mx4Args a) {
   Accumulators<C::NJ, C::NI> acc;
   acc.clear();
   uint32_t cj[C::NJ], ci[C::NI];
-  const auto same = [](int r) { return (int64_t)r; };
+  const SameRow same;
   const auto request = [&](uint16_t *SJ, uint16_t *SI, int k0) {
     sj.load_direct(SJ, k0, end, same);
     si.load_direct(SI, k0, end, same);

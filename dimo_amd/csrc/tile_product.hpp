@@ -13,6 +13,8 @@
 #pragma once
 #include "matrix_ops.hpp"
 
+#include <type_traits>
+
 namespace dimo {
 
 constexpr bool LINES = true, COLUMNS = false;
@@ -71,6 +73,21 @@ struct Reader {
   }
 };
 
+// Which memory row a step of the reduction is (COLUMNS).  AHEAD: finding it takes a load, done a stage early -- behind it the
+// operand's own load would wait out two round trips per stage (a weight gradient of 32768 gathered rows, 16 x 4096 x 1024 in
+// bf16: 515 us, so 375; of rows in their order 330).
+struct SameRow {
+  static constexpr bool AHEAD = false;
+  __device__ __forceinline__ int operator()(int r) const { return r; }
+};
+struct SourceRow {
+  static constexpr bool AHEAD = true;
+  const int32_t *rows;
+  __device__ __forceinline__ int load(int r) const { return load_global(rows + r); }
+  // (nothing is done with what was loaded before it is needed: it would be waited for)
+  __device__ __forceinline__ uint32_t operator()(int, int loaded) const { return max(loaded, 0); }
+};
+
 // ---- staging -----------------------------------------------------------------------------------------------------
 // A thread brings CHUNKS chunks of 8 elements of an operand per stage.  Chunk q of thread t is number q * THREADS + t of the
 // stage in LDS order, so that the 64 lanes of a wave write 1024 consecutive bytes (what a load straight into LDS does).
@@ -87,6 +104,7 @@ struct Staging {
   int64_t ld;                                  // COLUMNS: elements between two steps
   int col;                                     // this thread's first element: LINES along the reduction, COLUMNS across
   int limit;                                   // COLUMNS: elements of a row from `col` on that exist (<= 0: none)
+  int ahead[ORDER == LINES ? 1 : CHUNKS];      // COLUMNS, rows AHEAD: what row.load() gave for the stage that is loaded next
 
   static __device__ __forceinline__ int lds_row(int q) { return (int)threadIdx.x / PER_ROW + q * ROW_STEP; }
   // (the permutations are their own inverse: the logical chunk at this thread's place)
@@ -110,6 +128,20 @@ struct Staging {
     ld = ld_, limit = columns - col;
     base[0] = p + (limit > 0 ? col : 0);
   }
+  // the stage that begins at step k0 is loaded next
+  template <class F>
+  __device__ __forceinline__ void look_ahead(int k0, int end, F &&row) {
+    if constexpr (ORDER == COLUMNS && std::decay_t<F>::AHEAD)
+#pragma unroll
+      for (int q = 0; q < CHUNKS; ++q) ahead[q] = row.load(min(k0 + lds_row(q), end - 1));
+  }
+  template <class F>
+  __device__ __forceinline__ auto memory_row(int q, int r, F &&row) const {
+    if constexpr (std::decay_t<F>::AHEAD)
+      return row(r, ahead[q]);
+    else
+      return row(r);
+  }
   // address of chunk q of the stage that begins at step k0 (the reduction ends at `end`), row(r) -> memory row of step r;
   // what lies behind the end comes from the zero chunk
   template <class F>
@@ -118,7 +150,7 @@ struct Staging {
       return k0 + col < end ? base[q] + k0 : reinterpret_cast<const E *>(zero_chunk);
     } else {
       const int r = k0 + lds_row(q);
-      const E *p = base[0] + row(min(r, end - 1)) * ld;
+      const E *p = base[0] + memory_row(q, min(r, end - 1), row) * ld;
       return r < end ? p : reinterpret_cast<const E *>(zero_chunk);
     }
   }
@@ -149,7 +181,7 @@ struct Staging {
         ok = end - k0 - col, p = base[q] + (ok > 0 ? k0 : 0);
       } else {
         const int r = k0 + lds_row(q);
-        ok = r < end ? limit : 0, p = base[0] + (r < end ? row(r) : 0) * ld;
+        ok = r < end ? limit : 0, p = base[0] + memory_row(q, min(r, end - 1), row) * ld;
       }
       if (ok >= 8) {
         __builtin_memcpy(v[q], p, sizeof(Chunk));  // (one or two 16-byte loads; the hardware takes any alignment)
@@ -299,8 +331,8 @@ enum Staged { ANY = 0, DIRECT = 1, WHOLE = 2 };
 
 // The stages of a product, one after the other.
 template <class T, class C, bool ORDER_J, bool ORDER_I, int HOW, bool SUMS, class RowJ, class RowI>
-__device__ __forceinline__ void run_stages(const Staging<T, ORDER_J, C::TJ, Planes<T>::DEPTH, C::THREADS> &sj,
-                                           const Staging<T, ORDER_I, C::TI, Planes<T>::DEPTH, C::THREADS> &si, int begin,
+__device__ __forceinline__ void run_stages(Staging<T, ORDER_J, C::TJ, Planes<T>::DEPTH, C::THREADS> &sj,
+                                           Staging<T, ORDER_I, C::TI, Planes<T>::DEPTH, C::THREADS> &si, int begin,
                                            int end, RowJ &&row_j, RowI &&row_i, Accumulators<C::NJ, C::NI> &acc,
                                            bool with_sums, uint16_t *SJ0, uint16_t *SI0, uint16_t *SJ1, uint16_t *SI1) {
   constexpr int BK = Planes<T>::DEPTH;
@@ -309,19 +341,24 @@ __device__ __forceinline__ void run_stages(const Staging<T, ORDER_J, C::TJ, Plan
   const Reader<ORDER_I, C::TI, BK, C::NI> ri((wave % C::WI) * 32 * C::NI);
   if constexpr (HOW == DIRECT) {
     const int stages = (end - begin + BK - 1) / BK;
-    sj.load_direct(SJ0, begin, end, row_j);
-    si.load_direct(SI0, begin, end, row_i);
+    const auto load = [&](uint16_t *SJ, uint16_t *SI, int k0) {
+      sj.load_direct(SJ, k0, end, row_j);
+      si.load_direct(SI, k0, end, row_i);
+      sj.look_ahead(k0 + BK, end, row_j);
+      si.look_ahead(k0 + BK, end, row_i);
+    };
+    sj.look_ahead(begin, end, row_j);
+    si.look_ahead(begin, end, row_i);
+    load(SJ0, SI0, begin);
     int k0 = begin;
     for (int n = 1; n < stages; n += 2, k0 += 2 * BK) {
       __syncthreads();  // this stage is there, and everyone is done with the other buffer
-      sj.load_direct(SJ1, k0 + BK, end, row_j);
-      si.load_direct(SI1, k0 + BK, end, row_i);
+      load(SJ1, SI1, k0 + BK);
       __builtin_amdgcn_sched_barrier(0);  // (the loads first: they have this stage's products to arrive under)
       multiply_stage<T, C, BK, SUMS>(SJ0, SI0, rj, ri, acc, with_sums);
       acc.hold();
       __syncthreads();
-      sj.load_direct(SJ0, k0 + 2 * BK, end, row_j);  // (behind the end: zeros; a branch would split the stage)
-      si.load_direct(SI0, k0 + 2 * BK, end, row_i);
+      load(SJ0, SI0, k0 + 2 * BK);  // (behind the end: zeros; a branch would split the stage)
       __builtin_amdgcn_sched_barrier(0);
       multiply_stage<T, C, BK, SUMS>(SJ1, SI1, rj, ri, acc, with_sums);
       acc.hold();
@@ -336,11 +373,16 @@ __device__ __forceinline__ void run_stages(const Staging<T, ORDER_J, C::TJ, Plan
     constexpr int AHEAD = HOW == WHOLE && C::NJ * C::NI == 1 ? 3 : 1;
     typename LJ::Chunk vj[AHEAD][LJ::CHUNKS];
     typename LI::Chunk vi[AHEAD][LI::CHUNKS];
+    const auto load = [&](int d, int k0) {
+      sj.template load<HOW == WHOLE>(vj[d], k0, end, row_j);
+      si.template load<HOW == WHOLE>(vi[d], k0, end, row_i);
+      sj.look_ahead(k0 + BK, end, row_j);
+      si.look_ahead(k0 + BK, end, row_i);
+    };
+    sj.look_ahead(begin, end, row_j);
+    si.look_ahead(begin, end, row_i);
 #pragma unroll
-    for (int d = 0; d < AHEAD; ++d) {
-      sj.template load<HOW == WHOLE>(vj[d], begin + d * BK, end, row_j);
-      si.template load<HOW == WHOLE>(vi[d], begin + d * BK, end, row_i);
-    }
+    for (int d = 0; d < AHEAD; ++d) load(d, begin + d * BK);
     for (int k1 = begin; k1 < end; k1 += AHEAD * BK) {
 #pragma unroll
       for (int d = 0; d < AHEAD; ++d) {
@@ -350,10 +392,7 @@ __device__ __forceinline__ void run_stages(const Staging<T, ORDER_J, C::TJ, Plan
         sj.store(vj[d], SJ0, C::TJ * BK);
         si.store(vi[d], SI0, C::TI * BK);
         __syncthreads();
-        if (HOW == WHOLE || k0 + BK < end) {
-          sj.template load<HOW == WHOLE>(vj[d], k0 + AHEAD * BK, end, row_j);
-          si.template load<HOW == WHOLE>(vi[d], k0 + AHEAD * BK, end, row_i);
-        }
+        if (HOW == WHOLE || k0 + BK < end) load(d, k0 + AHEAD * BK);
         __builtin_amdgcn_sched_barrier(0);
         multiply_stage<T, C, BK, SUMS>(SJ0, SI0, rj, ri, acc, with_sums);
         acc.hold();
