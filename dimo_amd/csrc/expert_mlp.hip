@@ -51,7 +51,7 @@ struct ScratchLayout {
 
 bool bad(const dimo_expert_mlp_desc *d) {
   return !d || !known_dtype(d->dtype) || d->T < 0 || d->K < 1 || d->F < 1 || d->E < 1 || d->E > DIMO_MAX_EXPERTS || d->k < 1 ||
-         d->k > d->E || (int64_t)d->T * d->k > 0x7fffffffLL || d->act < DIMO_ACT_NONE || d->act > DIMO_ACT_SILU ||
+         d->k > d->E || (int64_t)d->T * d->k > DIMO_MAX_SIZE || d->K > DIMO_MAX_SIZE || d->F > DIMO_MAX_SIZE || d->act < DIMO_ACT_NONE || d->act > DIMO_ACT_SILU ||
          d->ld_x < d->K || d->ld_logits < d->E;
 }
 

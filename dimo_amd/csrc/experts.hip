@@ -541,7 +541,7 @@ extern "C" size_t dimo_route_workspace_bytes(int T, int E) {
 extern "C" int dimo_route_topk_forward(int T, int E, int k, int dtype, const void *logits, int64_t ld,
                                        const uint8_t *row_mask, int normalize, float *weights, int32_t *experts,
                                        float *load, void *workspace, size_t workspace_bytes, void *stream) {
-  if (T < 0 || E < 1 || E > ROUTE_MAX_E || k < 1 || k > E || !known_dtype(dtype) || ld < E) return DIMO_E_ARG;
+  if (T < 0 || T > DIMO_MAX_SIZE || E < 1 || E > ROUTE_MAX_E || k < 1 || k > E || !known_dtype(dtype) || ld < E) return DIMO_E_ARG;
   if (T > 0 && (!logits || !weights || !experts)) return DIMO_E_ARG;
   hipStream_t s = (hipStream_t)stream;
   clear_errors();
@@ -572,7 +572,7 @@ extern "C" int dimo_route_topk_backward(int T, int E, int k, int dtype, const vo
                                         const uint8_t *row_mask, int normalize, const float *weights,
                                         const int32_t *experts, const float *g_weights, const float *g_load,
                                         void *g_logits, void *stream) {
-  if (T < 0 || E < 1 || E > ROUTE_MAX_E || k < 1 || k > E || !known_dtype(dtype) || ld < E) return DIMO_E_ARG;
+  if (T < 0 || T > DIMO_MAX_SIZE || E < 1 || E > ROUTE_MAX_E || k < 1 || k > E || !known_dtype(dtype) || ld < E) return DIMO_E_ARG;
   if (T == 0) return DIMO_OK;
   if (!logits || !weights || !experts || !g_logits) return DIMO_E_ARG;
   hipStream_t s = (hipStream_t)stream;
@@ -596,7 +596,7 @@ extern "C" size_t dimo_group_rows_workspace_bytes(int64_t S, int E) {
 
 extern "C" int dimo_group_rows(int64_t S, int E, int places, const int32_t *experts, int32_t *offsets, int32_t *order,
                                int32_t *position, int32_t *rows, void *workspace, size_t workspace_bytes, void *stream) {
-  if (S < 0 || S > 0x7fffffffLL || E < 1 || E > ROUTE_MAX_E || places < 1 || !offsets) return DIMO_E_ARG;
+  if (S < 0 || S > DIMO_MAX_SIZE || E < 1 || E > ROUTE_MAX_E || places < 1 || !offsets) return DIMO_E_ARG;
   if (S > 0 && (!experts || !order || !position)) return DIMO_E_ARG;
   if (workspace_bytes < dimo_group_rows_workspace_bytes(S, E) || (S > GROUP_CHUNK && !workspace)) return DIMO_E_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
@@ -622,7 +622,7 @@ extern "C" int dimo_group_rows(int64_t S, int E, int places, const int32_t *expe
 extern "C" int dimo_combine_rows_forward(int T, int k, int N, int64_t S, int dtype, const void *y, int64_t ldy,
                                          const float *weights, const int32_t *position, const void *residual,
                                          int64_t ld_residual, void *out, void *stream) {
-  if (T < 0 || k < 1 || N < 0 || N > (1 << 30) || S < 0 || !known_dtype(dtype) || ldy < N || (residual && ld_residual < N))
+  if (T < 0 || T > DIMO_MAX_SIZE || k < 1 || N < 0 || N > DIMO_MAX_SIZE || S < 0 || S > DIMO_MAX_SIZE || !known_dtype(dtype) || ldy < N || (residual && ld_residual < N))
     return DIMO_E_ARG;
   if (T == 0 || N == 0) return DIMO_OK;
   if ((S > 0 && !y) || !position || !out) return DIMO_E_ARG;
@@ -654,7 +654,7 @@ extern "C" int dimo_combine_rows_backward(int T, int k, int N, int64_t S, int E,
                                           int64_t ldg, const void *y, int64_t ldy, const float *weights,
                                           const int32_t *position, const int32_t *offsets, void *g_y,
                                           float *g_weights, void *stream) {
-  if (T < 0 || k < 1 || N < 0 || E < 1 || S != (int64_t)T * k || !known_dtype(dtype) || ldg < N || (g_weights && ldy < N))
+  if (T < 0 || k < 1 || N < 0 || N > DIMO_MAX_SIZE || E < 1 || S != (int64_t)T * k || S > DIMO_MAX_SIZE || !known_dtype(dtype) || ldg < N || (g_weights && ldy < N))
     return DIMO_E_ARG;
   if (T == 0) return DIMO_OK;
   if ((N > 0 && (!g_out || (g_weights && !y))) || !position || !offsets) return DIMO_E_ARG;

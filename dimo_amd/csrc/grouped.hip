@@ -339,7 +339,8 @@ __global__ __launch_bounds__(256) void activation_backward_kernel(int64_t n, int
 }
 
 bool bad_shape(int dtype, int R, int E, int K, int N) {
-  return !known_dtype(dtype) || R < 0 || E < 1 || E > DIMO_MAX_EXPERTS || K < 1 || N < 1;
+  return !known_dtype(dtype) || R < 0 || R > DIMO_MAX_SIZE || E < 1 || E > DIMO_MAX_EXPERTS || K < 1 ||
+         K > DIMO_MAX_SIZE || N < 1 || N > DIMO_MAX_SIZE;
 }
 
 typedef Tile<64, 64, 2, 2> Small;

@@ -338,7 +338,7 @@ int launch_mx4(const Mx4Args &a, hipStream_t s) {
 // 31 bits
 template <class F>
 int for_row_bands(int64_t rows, uint32_t per_row, F &&launch) {
-  const int64_t most = (0x7fffffffLL - 255) / per_row;  // (K < 2^31: at least 7 rows)
+  const int64_t most = (0x7fffffffLL - 255) / per_row;  // (K <= 2^30: at least 15 rows)
   for (int64_t first = 0; first < rows; first += most) {
     const int64_t units = (rows - first < most ? rows - first : most) * per_row;
     launch(first, (unsigned)((units + 255) / 256));
@@ -352,7 +352,7 @@ int for_row_bands(int64_t rows, uint32_t per_row, F &&launch) {
 
 extern "C" int dimo_mx4_quantize(int dtype, int64_t rows, int K, const void *x, int64_t ldx,
                                  const int32_t *from, uint8_t *codes, uint8_t *scales, void *stream) {
-  if (!known_dtype(dtype) || rows < 0 || K < 1 || ldx < K) return DIMO_E_ARG;
+  if (!known_dtype(dtype) || rows < 0 || K < 1 || K > DIMO_MAX_SIZE || ldx < K) return DIMO_E_ARG;
   if (rows == 0) return DIMO_OK;
   if (!x || !codes || !scales || (reinterpret_cast<uintptr_t>(codes) & 3)) return DIMO_E_ARG;
   hipStream_t s = (hipStream_t)stream;
@@ -373,7 +373,7 @@ extern "C" int dimo_mx4_quantize(int dtype, int64_t rows, int K, const void *x, 
 
 extern "C" int dimo_mx4_dequantize(int dtype, int64_t rows, int K, const uint8_t *codes, const uint8_t *scales, void *out,
                                    void *stream) {
-  if (!known_dtype(dtype) || rows < 0 || K < 1) return DIMO_E_ARG;
+  if (!known_dtype(dtype) || rows < 0 || K < 1 || K > DIMO_MAX_SIZE) return DIMO_E_ARG;
   if (rows == 0) return DIMO_OK;
   if (!codes || !scales || !out || (reinterpret_cast<uintptr_t>(codes) & 3)) return DIMO_E_ARG;
   hipStream_t s = (hipStream_t)stream;
@@ -393,8 +393,8 @@ extern "C" int dimo_mx4_dequantize(int dtype, int64_t rows, int K, const uint8_t
 extern "C" int dimo_mx4_linear(int dtype, int R, int E, int K, int N, const uint8_t *x_codes, const uint8_t *x_scales,
                                const int32_t *offsets, const uint8_t *w_codes, const uint8_t *w_scales, const void *bias,
                                int act, void *y, void *stream) {
-  if (!known_dtype(dtype) || R < 0 || E < 1 || E > DIMO_MAX_EXPERTS || K < 1 || N < 1 || act < DIMO_ACT_NONE ||
-      act > DIMO_ACT_SILU || (!offsets && E != 1))
+  if (!known_dtype(dtype) || R < 0 || R > DIMO_MAX_SIZE || E < 1 || E > DIMO_MAX_EXPERTS || K < 1 || K > DIMO_MAX_SIZE ||
+      N < 1 || N > DIMO_MAX_SIZE || act < DIMO_ACT_NONE || act > DIMO_ACT_SILU || (!offsets && E != 1))
     return DIMO_E_ARG;
   if (R == 0) return DIMO_OK;
   if (!x_codes || !x_scales || !w_codes || !w_scales || !y || !aligned16(x_codes) || !aligned16(w_codes)) return DIMO_E_ARG;

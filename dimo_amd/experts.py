@@ -23,6 +23,7 @@ from torch import nn
 from . import _lib
 
 MAX_EXPERTS = 1024
+MAX_SIZE = 1 << 30  # rows, places and columns of a call
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTIVATIONS = {None: 0, "relu": 1, "silu": 2}
 
@@ -66,6 +67,11 @@ def _rows(t):
     if t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]):
         return t
     return t.contiguous()
+
+
+def _check_sizes(*sizes):
+    if max(sizes) > MAX_SIZE:
+        raise ValueError(f"up to {MAX_SIZE} rows, places and columns expected, got {max(sizes)}")
 
 
 def _ld(t):
@@ -133,6 +139,7 @@ def route_topk(logits, k, row_mask=None, normalize=True):
         raise ValueError("logits: [T, E] expected")
     _gpu(logits, row_mask)
     _dtype(logits, "logits")
+    _check_sizes(logits.shape[0])
     if not 1 <= logits.shape[1] <= MAX_EXPERTS or not 1 <= k <= logits.shape[1]:
         raise ValueError(f"1 <= k <= E <= {MAX_EXPERTS} expected, got k = {k}, E = {logits.shape[1]}")
     if row_mask is not None:
@@ -172,13 +179,13 @@ def group_rows(experts, num_experts):
     if not 1 <= num_experts <= MAX_EXPERTS or experts.shape[1] < 1:
         raise ValueError(f"1 to {MAX_EXPERTS} experts and k >= 1 expected")
     device = _gpu(experts)
-    experts = experts.contiguous()
     S = experts.numel()
-    if S > 0x7FFFFFFF:
-        raise ValueError("more than 2^31 - 1 places")
+    _check_sizes(S)
+    experts = experts.contiguous()
     L = _lib.lib()
     groups = RowGroups(torch.empty(num_experts + 1, dtype=torch.int32, device=device))
-    groups.order, groups.rows = torch.empty(2, S, dtype=torch.int32, device=device)
+    groups.order = torch.empty(S, dtype=torch.int32, device=device)
+    groups.rows = torch.empty(S, dtype=torch.int32, device=device)
     groups.position = torch.empty(experts.shape, dtype=torch.int32, device=device)
     with _on(device):
         nbytes = L.dimo_group_rows_workspace_bytes(S, num_experts)
@@ -300,6 +307,7 @@ def _check_linear(x, weight, bias, groups, activation, gather):
     if weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
         raise ValueError("x, weight and bias must have one type")
     E, N, K = weight.shape
+    _check_sizes(x.shape[0], N, K)
     if x.shape[1] != K or K < 1 or N < 1:
         raise ValueError(f"x has {x.shape[1]} columns, weight takes {K}")
     if bias is not None and bias.shape != (E, N):
@@ -356,6 +364,7 @@ def combine_rows(y, groups, weights=None, residual=None):
         raise ValueError(f"y: [{groups.order.shape[0]}, N] expected")
     _gpu(y, weights, residual, groups.offsets)
     _dtype(y, "y")
+    _check_sizes(y.shape[1])
     if weights is not None and (weights.shape != groups.position.shape or weights.dtype != torch.float32):
         raise ValueError("weights: fp32 [T, k] expected")
     if residual is not None and (residual.dtype != y.dtype or residual.shape != (groups.position.shape[0], y.shape[1])):
@@ -434,8 +443,9 @@ def expert_mlp(x, logits, w1, b1, w2, b2, k, activation="relu", row_mask=None):
                            (b1, (E, F), "b1: [E, F]"), (b2, (E, K), "b2: [E, K]")):
         if t is not None and (t.shape != shape or t.dtype != x.dtype):
             raise ValueError(f"{what} of x's type expected")
-    if not 1 <= k <= E <= MAX_EXPERTS or K < 1 or F < 1 or T * k > 0x7FFFFFFF:
-        raise ValueError(f"1 <= k <= E <= {MAX_EXPERTS} and fewer than 2^31 places expected")
+    if not 1 <= k <= E <= MAX_EXPERTS or K < 1 or F < 1:
+        raise ValueError(f"1 <= k <= E <= {MAX_EXPERTS} and at least one column expected")
+    _check_sizes(T * k, K, F)
     if activation not in _ACTIVATIONS:
         raise ValueError(f"activation: one of {list(_ACTIVATIONS)} expected")
     if row_mask is not None:

@@ -11,7 +11,7 @@ every element.  No gradients.  GPU only."""
 import torch
 
 from . import _lib
-from .experts import _ACTIVATIONS, _DTYPES, _check_linear_groups, _dtype, _gpu, _ld, _on, _rows
+from .experts import _ACTIVATIONS, _DTYPES, _check_linear_groups, _check_sizes, _dtype, _gpu, _ld, _on, _rows
 
 
 class MX4:
@@ -61,6 +61,7 @@ def quantize_mx4(x, groups=None):
     dtype = _dtype(x, "x")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("x: [..., K] with K >= 1 expected")
+    _check_sizes(x.shape[-1])
     x = x.detach()
     K, lead = x.shape[-1], x.shape[:-1]
     flat = _rows(x) if x.dim() == 2 else x.contiguous().view(-1, K)
@@ -95,6 +96,7 @@ def mx4_linear(x, weight, bias=None, groups=None, activation=None, out_dtype=tor
     R, N, E = x.shape[0], weight.shape[-2], 1
     if N < 1:
         raise ValueError("weight without rows")
+    _check_sizes(R, N, x.columns)
     _gpu(x.codes, weight.codes, bias, None if groups is None else groups.offsets)
     if groups is not None:
         E = weight.shape[0]

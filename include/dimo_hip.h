@@ -443,12 +443,13 @@ int dimo_executor_backward_accumulate(void *executor, const dimo_step_common *co
                                       const dimo_render_desc *renders, void *main_stream);
 
 /* ---- expert operators (no reference counterpart: the reference's deformation network is one dense MLP) ------------
- * Element types: DIMO_F32, DIMO_BF16, DIMO_F16; statistics, weights and sums are fp32.  Up to DIMO_MAX_EXPERTS experts.
- * Sizes of groups stay on the device; nothing synchronises, every launch may be captured. */
+ * Element types: DIMO_F32, DIMO_BF16, DIMO_F16; statistics, weights and sums are fp32.  Up to DIMO_MAX_EXPERTS experts,
+ * DIMO_MAX_SIZE rows (or places: rows times choices) and columns.  Sizes of groups stay on the device; nothing synchronises, every launch may be captured. */
 #define DIMO_F32 0
 #define DIMO_BF16 1
 #define DIMO_F16 2
 #define DIMO_MAX_EXPERTS 1024
+#define DIMO_MAX_SIZE (1 << 30) /* (indices of rows and columns, tiles added, stay 32-bit integers) */
 #define DIMO_ACT_NONE 0
 #define DIMO_ACT_RELU 1
 #define DIMO_ACT_SILU 2

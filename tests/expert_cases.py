@@ -245,6 +245,28 @@ def check_gather(ex, device, T, k, E, K, N, dtype, seed=0, pad=0):
 
 
 # ---------------------------------------------------------------------------------------------------- bringing together
+def check_wanted(ex, device, wanted, seed=0):
+    """A call that needs some of the gradients gets the ones (bit for bit) that it would get with all of them."""
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g).to(device)
+    z = r(60, 4)
+
+    def some(fn, tensors, pick):
+        leaves = [t.clone().requires_grad_(i in pick) for i, t in enumerate(tensors)]
+        out = fn(*leaves)
+        return torch.autograd.grad(out, [leaves[i] for i in pick], torch.ones_like(out))
+    _, experts, _ = ex.route_topk(z, 2)
+    groups = ex.group_rows(experts, 4)
+    calls = [(lambda x, w, b: ex.grouped_linear(x, w, groups, b, "silu", gather=True), (r(60, 24), r(4, 16, 24), r(4, 16))),
+             (lambda y, w, x: ex.combine_rows(y, groups, w, x), (r(120, 24), r(60, 2), r(60, 24))),
+             (lambda x, w1, b2: ex.expert_mlp(x, z, w1, None, w1.mT.contiguous(), b2, 2), (r(60, 24), r(4, 16, 24), r(4, 24))),
+             (lambda logits, b1, w2: ex.expert_mlp(z, logits, w2.mT.contiguous(), b1, w2, None, 2, None), (r(60, 3), r(3, 8), r(3, 4, 8)))]
+    for fn, tensors in calls:
+        every = some(fn, tensors, (0, 1, 2))
+        for i, got in zip(wanted, some(fn, tensors, wanted)):
+            assert torch.equal(got, every[i])
+
+
 def check_combine(ex, device, T, k, E, N, dtype, weighted=True, residual=True, pad=0, seed=0):
     g = torch.Generator().manual_seed(seed)
     e = torch.randint(-1, E, (T, k), generator=g, dtype=torch.int32)

@@ -86,6 +86,38 @@ def test_layer_is_its_parts(emulated, T, K, F, E, k, dtype, act, biases):
     cases.check_layer_is_its_parts(ex, "cpu", T, K, F, E, k, dtype, act, biases, seed=T)
 
 
+@pytest.mark.parametrize("counts,K,N,dtype,tail", [
+    ([0, 1500, 100, 0, 960], 24, 40, BF16, 5),   # cut into slices of 256 rows, whole, empty
+    ([0, 1500, 100, 0, 960], 23, 41, F32, 0),
+    ([256, 512, 257, 1, 1600], 16, 8, F16, 3),   # at the borders of a slice
+])
+def test_weight_gradients_of_cut_groups(emulated, counts, K, N, dtype, tail):
+    cases.check_products(ex, "cpu", counts, K, N, dtype, None, tail, 0, seed=K)
+
+
+def test_weight_gradients_of_cut_groups_gathered(emulated):
+    cases.check_gather(ex, "cpu", 1100, 2, 4, 24, 16, BF16, seed=5, pad=0)
+    cases.check_gather(ex, "cpu", 700, 2, 2, 9, 7, F32, seed=6, pad=1)
+
+
+@pytest.mark.parametrize("wanted", [(0,), (1,), (2,), (1, 2), (0, 2)])
+def test_only_the_gradients_that_are_wanted(emulated, wanted):
+    cases.check_wanted(ex, "cpu", wanted)
+
+
+def test_bad_offsets_stay_inside_the_weight_gradients(emulated):
+    for R, bad in ((40, [0, 100, -5, 40]), (1600, [0, 1600, 10, 1600]), (1600, [7, 2 ** 31 - 1, -2 ** 31, 3]),
+                   (1600, [0, 1600, 0, 1600])):
+        x, g = torch.randn(R, 8), torch.randn(R, 4)
+        w = torch.randn(3, 4, 8, requires_grad=True)
+        b = torch.randn(3, 4, requires_grad=True)
+        for rows in (None, torch.arange(R, dtype=torch.int32)):
+            groups = ex.RowGroups(torch.tensor(bad, dtype=torch.int32))
+            if rows is not None:
+                groups.order, groups.rows, groups.position = rows, rows, rows[:, None]
+            torch.autograd.grad(ex.grouped_linear(x, w, groups, b, gather=rows is not None), (w, b), g)
+
+
 def test_bad_offsets_stay_inside(emulated):
     """Offsets that the caller got wrong give wrong rows, never an address outside (run under AddressSanitizer too)."""
     x, w = torch.randn(40, 8), torch.randn(3, 4, 8)
@@ -147,6 +179,33 @@ def test_refusals():
 def test_bad_arguments(emulated, call):
     with pytest.raises(ValueError):
         call()
+
+
+@pytest.mark.parametrize("call", [
+    lambda many: ex.route_topk(torch.zeros(1).expand(many, 2), 1),
+    lambda many: ex.group_rows(torch.zeros(1, dtype=torch.int32).expand(many // 2 + 1, 2), 2),
+    lambda many: ex.grouped_linear(torch.zeros(1).expand(many, 1), torch.zeros(1, 1, 1), ex.RowGroups(torch.zeros(2, dtype=torch.int32))),
+    lambda many: ex.grouped_linear(torch.zeros(1, 1), torch.zeros(1).expand(1, many, 1), ex.RowGroups(torch.zeros(2, dtype=torch.int32))),
+    lambda many: ex.expert_mlp(torch.zeros(1).expand(many // 2 + 1, 1), torch.zeros(1).expand(many // 2 + 1, 2), torch.zeros(2, 1, 1),
+                               None, torch.zeros(2, 1, 1), None, k=2),
+])
+def test_sizes_beyond_the_indices(emulated, call):
+    with pytest.raises(ValueError, match="rows, places and columns"):
+        call(ex.MAX_SIZE + 1)
+
+
+def test_c_entry_points_refuse_sizes():
+    L, many = expert_emulation.emulated_library(), (1 << 30) + 1
+    assert L.dimo_route_topk_forward(many, 6, 2, 0, 1, 6, None, 1, 1, 1, None, None, 0, None) == -1
+    assert L.dimo_route_topk_backward(many, 6, 2, 0, 1, 6, None, 1, 1, 1, 1, None, 1, None) == -1
+    assert L.dimo_group_rows(many, 6, 2, 1, 1, 1, 1, None, 1, 1 << 60, None) == -1
+    for sizes in ((many, 3, 8, 5), (4, 3, many, 5), (4, 3, 8, many)):
+        assert L.dimo_grouped_linear_forward(0, *sizes, 1, 1 << 40, None, 1, 1, None, 0, 1, None, None) == -1
+        assert L.dimo_grouped_linear_dgrad(0, *sizes, 1, 1, 1, 0, None, 1, None) == -1
+        assert L.dimo_grouped_linear_wgrad(0, *sizes, 1, 1, 1 << 40, None, 1, 1, None, 1, 1 << 60, None) == -1
+        assert L.dimo_grouped_linear_wgrad_workspace_bytes(0, *sizes) == 0
+    assert L.dimo_combine_rows_forward(many, 1, 8, 8, 0, 1, 8, None, 1, None, 0, 1, None) == -1
+    assert L.dimo_combine_rows_backward(many, 1, 8, many, 3, 0, 1, 8, 1, 8, 1, 1, 1, 1, 1, None) == -1
 
 
 def test_c_entry_points_refuse():

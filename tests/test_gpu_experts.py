@@ -98,6 +98,36 @@ def test_layer_is_its_parts(ex, T, K, F, E, k, dtype, act, biases):
     cases.check_layer_is_its_parts(ex, "cuda", T, K, F, E, k, dtype, act, biases, seed=T)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("counts,K,N,tail", [
+    ([0, 1500, 100, 0, 960], 24, 40, 5),    # cut into slices of 256 rows, whole, empty
+    ([0, 1500, 100, 0, 960], 23, 41, 0),
+    ([256, 512, 257, 1, 1600], 16, 8, 3),   # at the borders of a slice
+    ([0] * 30 + [26000] + [500] * 20 + [17] * 19, 16, 24, 0),  # more than 64 groups
+    ([6000], 264, 520, 0),                  # one group, wide
+])
+def test_weight_gradients_of_cut_groups(ex, counts, K, N, dtype, tail):
+    cases.check_products(ex, "cuda", counts, K, N, dtype, None, tail, 0, seed=K)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_weight_gradients_of_groups_beyond_twice_the_mean(ex, dtype):
+    """128 x 128 tiles enough for the chip: only the groups of more than twice the mean are cut."""
+    counts = [512] * 120 + [4000, 0, 1100, 30, 1, 1500, 0, 2000]
+    cases.check_products(ex, "cuda", counts, 256, 256, dtype, None, 0, 0, seed=8)
+
+
+def test_weight_gradients_of_cut_groups_gathered(ex):
+    cases.check_gather(ex, "cuda", 1100, 2, 4, 24, 16, BF16, seed=5, pad=0)
+    cases.check_gather(ex, "cuda", 1100, 2, 4, 200, 136, F16, seed=7, pad=8)
+    cases.check_gather(ex, "cuda", 700, 2, 2, 9, 7, F32, seed=6, pad=1)
+
+
+@pytest.mark.parametrize("wanted", [(0,), (1,), (2,), (1, 2), (0, 2)])
+def test_only_the_gradients_that_are_wanted(ex, wanted):
+    cases.check_wanted(ex, "cuda", wanted)
+
+
 def _layer_leaves(T, K, F, E, dtype, seed):
     g = torch.Generator(device="cuda").manual_seed(seed)
     r = lambda *s: torch.randn(*s, generator=g, device="cuda")

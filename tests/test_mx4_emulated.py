@@ -81,6 +81,14 @@ def test_bad_arguments(emulated, call):
         call()
 
 
+def test_c_entry_points_refuse_sizes():
+    L, many = expert_emulation.emulated_library(), (1 << 30) + 1
+    assert L.dimo_mx4_quantize(0, 4, many, 16, many, None, 16, 16, None) == -1
+    assert L.dimo_mx4_dequantize(0, 4, many, 16, 16, 16, None) == -1
+    for sizes in ((many, 1, 8, 8), (4, 1, many, 8), (4, 1, 8, many)):
+        assert L.dimo_mx4_linear(0, *sizes, 16, 16, None, 16, 16, None, 0, 16, None) == -1
+
+
 def test_c_entry_points_refuse():
     L = expert_emulation.emulated_library()
     assert L.dimo_mx4_quantize(0, 4, 0, 1, 8, None, 4, 1, None) == -1
