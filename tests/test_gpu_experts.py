@@ -128,6 +128,37 @@ def test_only_the_gradients_that_are_wanted(ex, wanted):
     cases.check_wanted(ex, "cuda", wanted)
 
 
+def test_offsets_beyond_32_bits(ex):
+    """Rows whose elements lie more than 2^31 behind their matrix' first: products, their gradients, sums and routing of
+    the last rows against float64."""
+    R, K, N, n = 1_100_000, 2048, 8, 70
+    g = torch.Generator(device="cuda").manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda", dtype=torch.bfloat16)
+    x, w, gy = r(R, K), (r(2, N, K) / 64).requires_grad_(True), r(R, N)
+    x.requires_grad_(True)
+    groups = ex.RowGroups(torch.tensor([0, 1000, R], dtype=torch.int32, device="cuda"))
+    y = ex.grouped_linear(x, w, groups)
+    gx, = torch.autograd.grad(y, x, gy)
+    X, W, G = x[-n:].detach().double().cpu(), w[1].detach().double().cpu(), gy[-n:].double().cpu()
+    cases.near(y[-n:], X @ W.T, BF16, cases.product_slack(K, X.abs() @ W.abs().T), "y")
+    cases.near(gx[-n:], G @ W, BF16, cases.product_slack(N, G.abs() @ W.abs()), "g_x")
+    del y, gx
+    # the weight gradient of a group that lies behind 2^31 elements
+    late = ex.RowGroups(torch.tensor([0, R - n, R], dtype=torch.int32, device="cuda"))
+    gw, _ = ex._linear_wgrad(gy, x.detach(), (2, N, K), late, False, False)
+    cases.near(gw[1], G.T @ X, BF16, cases.product_slack(n, G.abs().T @ X.abs()), "g_w")
+    # the last rows brought back to the first places, the first to the last
+    position = torch.arange(R - 1, -1, -1, dtype=torch.int32, device="cuda")[:, None]
+    late.order, late.position, late.rows = position[:, 0], position, position[:, 0]
+    out = ex.combine_rows(x.detach(), late)
+    assert torch.equal(out[:n], x[-n:].flip(0)) and torch.equal(out[-n:], x[:n].flip(0))
+    del out, x
+    z = r(2 ** 21 + 77, 1024)
+    weights, experts, _ = ex.route_topk(z, 3)
+    some, which, _ = ex.route_topk(z[-n:].clone(), 3)
+    assert torch.equal(weights[-n:], some) and torch.equal(experts[-n:], which)
+
+
 def _layer_leaves(T, K, F, E, dtype, seed):
     g = torch.Generator(device="cuda").manual_seed(seed)
     r = lambda *s: torch.randn(*s, generator=g, device="cuda")

@@ -44,6 +44,22 @@ def test_layer(ops, T, k, E, K, F):
     cases.check_mx4_layer(*ops, "cuda", T, k, E, K, F)
 
 
+def test_offsets_beyond_32_bits(ops):
+    """Rows whose values lie more than 2^31 behind their matrix' first, and whose codes lie more than 2^32 bytes behind:
+    the same as those rows alone."""
+    mx4, _ = ops
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.randn(2_100_000, 4096, generator=g, device="cuda", dtype=torch.bfloat16)
+    q, alone = mx4.quantize_mx4(x), mx4.quantize_mx4(x[-90:])
+    assert torch.equal(q.codes[-90:], alone.codes) and torch.equal(q.scales[-90:], alone.scales)
+    del x
+    w = mx4.quantize_mx4(torch.randn(40, 4096, generator=g, device="cuda"))
+    X, W = alone.dequantize().double().cpu(), w.dequantize().double().cpu()
+    cases.near(mx4.mx4_linear(q, w)[-90:], X @ W.T, BF16, cases.product_slack(4096, X.abs() @ W.abs().T), "y")
+    tail = mx4.MX4(q.codes[-90:], q.scales[-90:], 4096).dequantize(torch.bfloat16)
+    assert torch.equal(q.dequantize(torch.bfloat16)[-90:], tail)
+
+
 def test_nan_block_makes_its_row_nan(ops):
     mx4, _ = ops
     x = torch.randn(300, 256, device="cuda")
