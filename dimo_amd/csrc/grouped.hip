@@ -375,13 +375,20 @@ int launch_wgrad(const GroupedArgs &a, hipStream_t s) {
 }
 
 // Up to this many rows in all a forward takes the thin kernel: it reads each weight once per 32 rows of a group like the
-// tiles, but spreads the reduction over a workgroup's waves (one row, 2 x 2048 x 2048 of 16 experts in bf16: 5 us, the
-// 64 x 64 tile 18; 64 rows are a draw).
-constexpr int THIN_ROWS = 64;
+// tiles, but spreads the reduction over a workgroup's waves.  Measured, thin / 64 x 64 tile (experts, N x K; us):
+//                        1 row        8           16          32          256         512
+//   bf16  8, 2048^2      9.5 / 11.7   15 / 19     16 / 19     17 / 19     28 / 18
+//        16, 2048^2      8.7 / 11.4   15 / 19     15 / 19     22 / 19     30 / 20
+//        64,  512^2      6.4 / 6.9    6.5 / 7.0   6.8 / 7.2   7.9 / 7.3   13 / 9
+//   fp32 16, 2048^2      17 / 47      30 / 52     31 / 52     43 / 63     58 / 63     102 / 69
+//         1, 1024^2      10 / 26      11 / 26     11 / 26     12 / 26     13 / 27     23 / 27
+//        64,  512^2      8.5 / 17     8.6 / 17    8.9 / 17    12 / 18     22 / 24     23 / 24
+// (fp32: the tile's stages are long and few workgroups run them)
+inline int thin_rows(int dtype) { return dtype == DIMO_F32 ? 256 : 16; }
 
 template <int MODE>
 int run_rows(int dtype, const GroupedArgs &a, bool whole, hipStream_t s) {
-  if (MODE == FORWARD && a.R <= THIN_ROWS) {
+  if (MODE == FORWARD && a.R <= thin_rows(dtype)) {
     const int64_t groups = row_tile_workgroups(row_tile_count(a.R, a.E, 32), (a.N + 31) / 32);
     if (groups > 0x7fffffffLL) return DIMO_E_ARG;
     with_dtype(dtype, [&](auto tag) {

@@ -52,6 +52,7 @@ def test_group(emulated, T, k, E, skew):
     ([70, 0, 5, 64], 40, 66, BF16, None, 3, 8),
     ([70, 0, 5, 64], 37, 65, F16, "relu", 0, 3),
     ([33, 130], 72, 64, F32, "silu", 1, 0),
+    ([233, 130], 72, 64, F32, "silu", 1, 0),  # (more rows than the kernel for few of them takes)
     ([0, 0], 16, 16, BF16, None, 5, 0),
     ([65], 129, 33, BF16, "silu", 0, 0),
     ([300, 0, 600], 24, 40, BF16, None, 0, 0),     # weight gradients from slices of the rows

@@ -62,6 +62,8 @@ def test_group(ex, T, k, E, skew):
     ([513, 0, 1, 255, 128], 360, 257, None, 0, 8),
     ([0, 0], 16, 16, None, 5, 0),
     ([65], 129, 33, "silu", 0, 0),
+    ([16], 264, 72, "silu", 0, 0), ([17], 264, 72, "silu", 0, 0),        # at the borders of the kernel for few rows
+    ([200, 56], 264, 72, None, 0, 0), ([200, 57], 264, 72, None, 0, 0),
     ([700], 512, 136, "relu", 60, 8),
     ([3] * 150, 72, 96, "silu", 0, 0),
     ([300, 0, 600], 24, 40, None, 0, 0),
