@@ -47,7 +47,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void grouped_rows_kernel(GroupedArgs
   constexpr int BK = Planes<T>::DEPTH;
   const int columns = MODE == FORWARD ? a.N : a.K, reduction = MODE == FORWARD ? a.K : a.N;
   int ct = 0;
-  const RowTile tile = find_row_tile(a.offsets, a.E, a.R, C::TJ, (columns + C::TI - 1) / C::TI, (int)blockIdx.x, &ct);
+  const RowTile tile = find_row_tile<HALVES<C>>(a.offsets, a.E, a.R, C::TJ, (columns + C::TI - 1) / C::TI, (int)blockIdx.x, &ct);
   if (tile.expert < 0) return;
   const int c0 = ct * C::TI;
   E *out = static_cast<E *>(MODE == FORWARD ? a.y : a.gx);
@@ -77,7 +77,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void grouped_rows_kernel(GroupedArgs
   acc.clear();
   DIMO_STAGE_BUFFERS(T, C, HOW);
   run_stages<T, C, LINES, MODE == FORWARD ? LINES : COLUMNS, HOW, false>(sj, si, 0, reduction, SameRow{}, SameRow{}, acc, false, SJ0,
-                                                                            SI0, SJ1, SI1);
+                                                                            SI0, SJ1, SI1, idle_wave<C>(tile));
   __syncthreads();
   const E *bias = MODE == FORWARD && a.bias ? static_cast<const E *>(a.bias) + (int64_t)tile.expert * a.N : nullptr;
   const auto add_bias = [&](int i, float (&v)[4]) {
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(64 * THIN_WAVES) void grouped_thin_kernel(GroupedAr
   typedef typename Planes<T>::Tag Tag;
   __shared__ float4 buffer[THIN_WAVES][4][64];
   int ct = 0;
-  const RowTile tile = find_row_tile(a.offsets, a.E, a.R, 32, (a.N + 31) / 32, (int)blockIdx.x, &ct);
+  const RowTile tile = find_row_tile<false>(a.offsets, a.E, a.R, 32, (a.N + 31) / 32, (int)blockIdx.x, &ct);
   if (tile.expert < 0) return;
   const int lane = threadIdx.x & 63, c0 = 32 * ct;
   E *out = static_cast<E *>(a.y);
@@ -357,7 +357,7 @@ bool wide_output(int dtype, const void *p, int64_t columns) {
 
 template <class T, int MODE, int HOW, class C>
 int launch_rows(const GroupedArgs &a, hipStream_t s) {
-  const int64_t groups = row_tile_workgroups(row_tile_count(a.R, a.E, C::TJ), ((MODE == FORWARD ? a.N : a.K) + C::TI - 1) / C::TI);
+  const int64_t groups = row_tile_workgroups<HALVES<C>>(row_tile_count<HALVES<C>>(a.R, a.E, C::TJ), ((MODE == FORWARD ? a.N : a.K) + C::TI - 1) / C::TI);
   if (groups > 0x7fffffffLL) return DIMO_E_ARG;
   hipLaunchKernelGGL((grouped_rows_kernel<T, MODE, HOW, C>), dim3((unsigned)groups), dim3(C::THREADS), 0, s, a);
   return check_launch();

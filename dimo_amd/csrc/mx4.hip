@@ -193,7 +193,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx4_rows_kernel(Mx4Args a) {
   __shared__ __attribute__((aligned(1024))) uint16_t SJ0[C::TJ * BK], SI0[C::TI * BK], SJ1[C::TJ * BK], SI1[C::TI * BK];
   __shared__ uint2 scales[2][C::TJ + C::TI][2];  // [pairs of stages in turn][line][stage of the pair]
   int ct = 0;
-  const RowTile tile = find_row_tile(a.offsets, a.E, a.R, C::TJ, (a.N + C::TI - 1) / C::TI, (int)blockIdx.x, &ct);
+  const RowTile tile = find_row_tile<HALVES<C>>(a.offsets, a.E, a.R, C::TJ, (a.N + C::TI - 1) / C::TI, (int)blockIdx.x, &ct);
   if (tile.expert < 0) return;
   const int c0 = ct * C::TI;
   E *out = static_cast<E *>(a.y);
@@ -244,7 +244,19 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx4_rows_kernel(Mx4Args a) {
   put(scales[0], fetch(0));
   uint4 next = fetch(16);
   int k0 = 0;
-  for (int n = 1; n < stages; n += 2, k0 += 2 * BK) {
+  const bool idle = idle_wave<C>(tile);
+  if (idle) {  // (as in run_stages)
+    for (int n = 1; n < stages; n += 2, k0 += 2 * BK) {
+      __syncthreads();
+      request(SJ1, SI1, k0 + BK);
+      __syncthreads();
+      put(scales[((n >> 1) + 1) & 1], next);
+      next = fetch((k0 + 4 * BK) / 8);
+      request(SJ0, SI0, k0 + 2 * BK);
+    }
+    if (stages & 1) __syncthreads();
+  }
+  for (int n = idle ? stages : 1; n < stages; n += 2, k0 += 2 * BK) {
     __syncthreads();  // this stage is there, and everyone is done with the other buffer
     take(scales[(n >> 1) & 1], 0);
     request(SJ1, SI1, k0 + BK);
@@ -260,7 +272,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx4_rows_kernel(Mx4Args a) {
     multiply_codes<C>(SJ1, SI1, rj, ri, cj, ci, acc);
     acc.hold();
   }
-  if (stages & 1) {
+  if (!idle && (stages & 1)) {
     __syncthreads();
     take(scales[(stages >> 1) & 1], 0);
     multiply_codes<C>(SJ0, SI0, rj, ri, cj, ci, acc);
@@ -282,7 +294,7 @@ __global__ __launch_bounds__(64 * THIN_WAVES) void mx4_thin_kernel(Mx4Args a) {
   typedef typename T::store E;
   __shared__ float4 buffer[THIN_WAVES][4][64];
   int ct = 0;
-  const RowTile tile = find_row_tile(a.offsets, a.E, a.R, 32, (a.N + 31) / 32, (int)blockIdx.x, &ct);
+  const RowTile tile = find_row_tile<false>(a.offsets, a.E, a.R, 32, (a.N + 31) / 32, (int)blockIdx.x, &ct);
   if (tile.expert < 0) return;
   const int lane = threadIdx.x & 63, half = lane >> 5, c0 = 32 * ct;
   E *out = static_cast<E *>(a.y);
@@ -328,7 +340,7 @@ typedef Tile<256, 256, 2, 4> Large;
 
 template <class T, class C, bool SHORT>
 int launch_mx4(const Mx4Args &a, hipStream_t s) {
-  const int64_t groups = row_tile_workgroups(row_tile_count(a.R, a.E, C::TJ), (a.N + C::TI - 1) / C::TI);
+  const int64_t groups = row_tile_workgroups<HALVES<C>>(row_tile_count<HALVES<C>>(a.R, a.E, C::TJ), (a.N + C::TI - 1) / C::TI);
   if (groups > 0x7fffffffLL) return DIMO_E_ARG;
   hipLaunchKernelGGL((mx4_rows_kernel<T, C, SHORT>), dim3((unsigned)groups), dim3(C::THREADS), 0, s, a);
   return check_launch();

@@ -12,6 +12,7 @@
 // LINES, the transposing ds_read_b64_tr_b16 for COLUMNS) spread over all banks (`lines_place`, `columns_place`).
 #pragma once
 #include "matrix_ops.hpp"
+#include "row_tiles.hpp"
 
 #include <type_traits>
 
@@ -334,7 +335,8 @@ template <class T, class C, bool ORDER_J, bool ORDER_I, int HOW, bool SUMS, clas
 __device__ __forceinline__ void run_stages(Staging<T, ORDER_J, C::TJ, Planes<T>::DEPTH, C::THREADS> &sj,
                                            Staging<T, ORDER_I, C::TI, Planes<T>::DEPTH, C::THREADS> &si, int begin,
                                            int end, RowJ &&row_j, RowI &&row_i, Accumulators<C::NJ, C::NI> &acc,
-                                           bool with_sums, uint16_t *SJ0, uint16_t *SI0, uint16_t *SJ1, uint16_t *SI1) {
+                                           bool with_sums, uint16_t *SJ0, uint16_t *SI0, uint16_t *SJ1, uint16_t *SI1,
+                                           bool idle = false) {
   constexpr int BK = Planes<T>::DEPTH;
   const int wave = wave_number();
   const Reader<ORDER_J, C::TJ, BK, C::NJ> rj((wave / C::WI) * 32 * C::NJ);
@@ -351,6 +353,16 @@ __device__ __forceinline__ void run_stages(Staging<T, ORDER_J, C::TJ, Planes<T>:
     si.look_ahead(begin, end, row_i);
     load(SJ0, SI0, begin);
     int k0 = begin;
+    if (idle) {  // a wave whose rows are not there: its share of the loads, at the same barriers
+      for (int n = 1; n < stages; n += 2, k0 += 2 * BK) {
+        __syncthreads();
+        load(SJ1, SI1, k0 + BK);
+        __syncthreads();
+        load(SJ0, SI0, k0 + 2 * BK);
+      }
+      if (stages & 1) __syncthreads();
+      return;
+    }
     for (int n = 1; n < stages; n += 2, k0 += 2 * BK) {
       __syncthreads();  // this stage is there, and everyone is done with the other buffer
       load(SJ1, SI1, k0 + BK);
@@ -518,6 +530,14 @@ __device__ __forceinline__ void sum_over_waves(const f32x16 &acc, float4 (*buffe
     v[0] += s.x, v[1] += s.y, v[2] += s.z, v[3] += s.w;
   }
   f(v, t & 31, 8 * (t >> 6) + 4 * ((t >> 5) & 1));
+}
+
+// 256 rows: the last tiles are halves (row_tiles.hpp), in which half of the waves have no rows
+template <class C>
+constexpr bool HALVES = C::TJ == 256;
+template <class C>
+__device__ __forceinline__ bool idle_wave(const RowTile &t) {
+  return HALVES<C> && (wave_number() / C::WI) * 32 * C::NJ >= t.end - t.begin;
 }
 
 // Which tile: a workgroup's tile is worth its size only where there are enough of them.

@@ -70,6 +70,9 @@ def test_group(ex, T, k, E, skew):
     ([2000, 3, 1500], 264, 136, "silu", 9, 0),
     ([48 + i % 7 for i in range(128)], 40, 104, None, 3, 8),
     ([200 + i % 5 for i in range(225)], 200, 200, None, 0, 0),  # 256 x 256 tiles
+    ([300, 0, 513, 128, 129, 256, 1, 700], 136, 7200, None, 5, 0),      # ... whole ones, one and two halves (forward)
+    ([300, 0, 513, 128, 129, 256, 1, 700], 7200, 72, "silu", 130, 0),   # (gradient of x)
+    ([1024] * 8, 136, 1800, "relu", 0, 0),                              # (no halves)
 ])
 def test_products(ex, counts, K, N, dtype, act, tail, pad):
     cases.check_products(ex, "cuda", counts, K, N, dtype, act, tail, pad, seed=K)

@@ -34,6 +34,7 @@ def test_quantize(ops, R, K, dtype, kind, pad):
     ([300, 513, 0, 129], 512, 257, None, True, 5, True),
     ([1000], 1024, 640, "silu", True, 0, False),
     ([3], 4096, 1000, None, True, 0, False),
+    ([300, 0, 513, 128, 129, 256, 1, 700], 520, 7200, None, True, 300, True),  # 256 x 256 tiles, their halves
     ([7, 0, 9], 288, 72, "silu", True, 0, True), ([7, 1, 9], 288, 72, "silu", True, 0, True),  # at the kernel for few rows's border
 ])
 def test_linear(ops, counts, K, N, dtype, act, bias, tail, grouped):
