@@ -27,7 +27,7 @@ constexpr int ROUTE_MAX_BLOCKS = 512;  // workgroups of a routing launch that al
 // A row lies in L neighbouring lanes (a power of two up to 64), V consecutive logits in each: sixteen-byte loads, and few
 // exchanges -- a selection round is V comparisons in a lane and log2(L) exchanges of (value, index) between lanes, most of
 // them DPP moves.  V = 16 from 9 experts on: 131072 rows of 128, k = 8, took 215 us with V = 4 (five exchanges a round,
-// through LDS) and 52 us this way.
+// through LDS) and 54 us this way.
 struct RouteArgs {
   int T, E, k, normalize, wide;
   const void *logits;

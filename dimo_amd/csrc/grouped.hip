@@ -435,7 +435,12 @@ int run_rows(int dtype, const GroupedArgs &a, bool whole, hipStream_t s) {
 // So: the largest tile whose products last long enough to fill the chip in slices; slices where there are fewer workgroups
 // than CUs (fp32, whose stages take six times as long: than twice that), of 256 rows or more; with as many
 // 128 tiles as that, the groups of more than twice the mean are cut; with as many 256 tiles, taking the largest groups first
-// serves better, because slices are written and read once more in fp32.
+// serves better, because slices are written and read once more in fp32.  64 tiles whose stages go through registers (fp32;
+// 16-bit rows that are no whole chunks) take a microsecond or two per stage, and the largest group's are one chain: groups of
+// more than the mean are cut (whole / cut at 1; us):
+//    5003, 13, 257 x 360   uneven 62 / 28, fp16 35 / 21        5008, 13, 256 x 360   uneven 41 / 28, even 23 / 26
+//    4096, 16, 256 x 256   uneven 43 / 21                      2048, 16, 512 x 256   uneven 27 / 20, even 12 / 15
+//    8192, 32, 256 x 256   uneven 45 / 27, fp16 in whole chunks 14 / 17
 struct WgradPlan {
   int tile, split_rows, chunks;
   size_t bytes;
@@ -451,15 +456,15 @@ WgradPlan wgrad_plan(int dtype, int R, int E, int K, int N) {
     p.tile = MEDIUM;
   const int64_t have = blocks(p.tile == LARGE ? 256 : p.tile == MEDIUM ? 128 : 64), enough = f32 ? 512 : 256;
   int64_t rows = 0;
-  if (per_group >= 512) {
-    if (have < enough) {
-      const int64_t splits = (enough + have - 1) / have;
-      rows = (per_group + splits - 1) / splits;
-      rows = rows < 256 ? 256 : (rows + 63) / 64 * 64;
-    } else if (p.tile == MEDIUM) {
-      rows = (2 * per_group + 63) / 64 * 64;
-    }
+  if (per_group >= 512 && have < enough) {
+    const int64_t splits = (enough + have - 1) / have;
+    rows = (per_group + splits - 1) / splits;
+  } else if (per_group >= 512 && p.tile == MEDIUM) {
+    rows = 2 * per_group;
+  } else if (per_group >= 128 && p.tile == SMALL && (f32 || N % 8 || K % 8)) {
+    rows = per_group;
   }
+  if (rows) rows = rows < 256 ? 256 : (rows + 63) / 64 * 64;
   if (rows && rows < R) {
     // a group of r > rows rows is cut into fewer than 2 r / rows slices
     const int64_t cut = 2 * (int64_t)R / rows, slices = row_tile_count(R, E, (int)rows);

@@ -540,7 +540,15 @@ __device__ __forceinline__ bool idle_wave(const RowTile &t) {
   return HALVES<C> && (wave_number() / C::WI) * 32 * C::NJ >= t.end - t.begin;
 }
 
-// Which tile: a workgroup's tile is worth its size only where there are enough of them.
+// Which tile: its size pays where there are enough of them.  Forward on 64 / 128 / 256 tiles, us (rows, groups, N x K; the
+// gradient of x is within a few per cent):
+//                                 bf16                              fp32
+//   65536, 32, 2048 x 1024        538 / 373 / 307
+//   16384,  8, 1024 x 1024        61 / 46 / 40, uneven 67 / 55 / 54   255 / 183, uneven 262 / 234
+//   16384, 64, 1024 x 1024        uneven 76 / 62 / 59                 uneven 288 / 253
+//    8192, 64,  512 x 512         uneven 19 / 17 / 22                 uneven 48 / 46
+//    4096,  8,  512 x 2048        19 / 24 / 50                        73 / 112
+//    2048, 16, 1024 x 1024        uneven 15 / 17 / 29                 uneven 52 / 61
 enum { SMALL = 0, MEDIUM = 1, LARGE = 2 };
 inline int choose_tile(int64_t rows_per_group, int64_t groups, int64_t columns, bool direct) {
   const auto blocks = [&](int64_t t) { return groups * ((rows_per_group + t - 1) / t) * ((columns + t - 1) / t); };
