@@ -2,10 +2,10 @@
 // the launches of experts.hip and grouped.hip in order on one stream, intermediates in a workspace of the caller's.  (One
 // by one from Python the same launches cost more host time than a step of 4096 rows costs the GPU.)
 //   forward   w, e = route(logits);  h = act(W1 x[rows] + b1);  y = W2 h + b2;  out = x + sum_j w_j y[position_j]
+//   backward  gy = w g, gw = <g, y>;  gz = (gy W2) act';  gx = g + sum_j (gz W1)[position_j];  g_logits from gw
 // h, z, y, gy, gz and gx of the places have the tensors' type: each is an operand of the next product in that type (y and gx:
 // read once, by a sum), and 32 bits would double their traffic and take the products off the 16-bit instructions.  Against
 // one rounding at the end the weight gradients' error is 1.7 times as large (bf16, rms: 0.0029 of the value, 0.0017).
-//   backward  gy = w g, gw = <g, y>;  gz = (gy W2) act';  gx = g + sum_j (gz W1)[position_j];  g_logits from gw
 #include <hip/hip_runtime.h>
 
 #include "numeric.hpp"
