@@ -21,13 +21,15 @@ namespace {
 
 constexpr int ROUTE_THREADS = 256;
 constexpr int ROUTE_MAX_E = DIMO_MAX_EXPERTS;
-constexpr int ROUTE_MAX_BLOCKS = 512;  // workgroups of a routing launch that also sums the load: one row of partial sums each
+// Workgroups of a routing launch that also sums the load (a row of partial sums each): 131072 rows of 128 take 38 us in 512
+// of them, 32 in 1024, 29 in 2048, the sums of the rows 4.0, 4.3, 7.3.
+constexpr int ROUTE_MAX_BLOCKS = 1024;
 
 // ---- routing ---------------------------------------------------------------------------------------------------
 // A row lies in L neighbouring lanes (a power of two up to 64), V consecutive logits in each: sixteen-byte loads, and few
 // exchanges -- a selection round is V comparisons in a lane and log2(L) exchanges of (value, index) between lanes, most of
 // them DPP moves.  V = 16 from 9 experts on: 131072 rows of 128, k = 8, took 215 us with V = 4 (five exchanges a round,
-// through LDS) and 54 us this way.
+// through LDS) and 54 us this way (bf16; less since: `Keys`).
 struct RouteArgs {
   int T, E, k, normalize, wide;
   const void *logits;
@@ -94,9 +96,74 @@ __device__ __forceinline__ void load_row(const typename T::store *src, int first
   }
 }
 
+// A lane's V logits that are not chosen yet; next() finds the row's largest of them (ties: the lowest index) and takes it out;
+// at = -1: a row without any (-inf and NaN never are).
+// fp32: comparisons of (value, index).
+template <class T, int V>
+struct Candidates {
+  float z[V];
+  int first;
+  uint32_t left = (1u << V) - 1u;  // (V <= 16)
+  __device__ __forceinline__ Candidates(const float (&v)[V], int first_) : first(first_) {
+#pragma unroll
+    for (int c = 0; c < V; ++c) z[c] = v[c];
+  }
+  template <int L>
+  __device__ __forceinline__ float next(int &at) {
+    float best = -INFINITY;
+    at = ROUTE_MAX_E;
+#pragma unroll
+    for (int c = 0; c < V; ++c)  // (ascending index: the first of equals stays)
+      if (((left >> c) & 1u) && z[c] > best) best = z[c], at = first + c;
+    halving_steps<L>([&](auto m) {
+      const float ob = from_other_half<decltype(m)::value>(best);
+      const int oa = from_other_half<decltype(m)::value>(at);
+      if (ob > best || (ob == best && oa < at)) best = ob, at = oa;
+    });
+    const int own = at - first;
+    if (own >= 0 && own < V) left &= ~(1u << own);
+    if (!(best > -INFINITY)) at = -1;
+    return best;
+  }
+};
+// 16 bits: value and index fit one word that sorts like the pair -- the value's bits in ascending order, behind them the
+// index, the lowest largest; 0 = none -- so a choice is a maximum (two values per instruction) and an equality.  131072 rows of
+// 128 in bf16, k = 8: 54 us by comparisons, 38 this way.
+template <class T, int V>
+struct Keys {
+  uint32_t key[V];
+  __device__ __forceinline__ Keys(const float (&v)[V], int first) {
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+      const uint32_t bits = (uint32_t)T::save(v[c] + 0.f) << 16;  // (-0 counts as 0)
+      const uint32_t up = bits ^ ((uint32_t)((int32_t)bits >> 31) | 0x80000000u);
+      key[c] = v[c] > -INFINITY ? (up & 0xffff0000u) | (0xffffu - (uint32_t)(first + c)) : 0u;
+    }
+  }
+  template <int L>
+  __device__ __forceinline__ float next(int &at) {
+    uint32_t best = 0u;
+#pragma unroll
+    for (int c = 0; c < V; ++c) best = max(best, key[c]);
+    halving_steps<L>([&](auto m) { best = max(best, (uint32_t)from_other_half<decltype(m)::value>((int)best)); });
+#pragma unroll
+    for (int c = 0; c < V; ++c) key[c] = key[c] == best ? 0u : key[c];
+    at = best ? (int)(0xffffu - (best & 0xffffu)) : -1;
+    return T::load((typename T::store)((best >> 16) ^ (best >> 31 ? 0x8000u : 0xffffu)));
+  }
+};
+template <int V>
+struct Candidates<BF16, V> : Keys<BF16, V> {
+  using Keys<BF16, V>::Keys;
+};
+template <int V>
+struct Candidates<F16, V> : Keys<F16, V> {
+  using Keys<F16, V>::Keys;
+};
+
 template <class T, int L, int V>
 __global__ __launch_bounds__(ROUTE_THREADS) void route_forward_kernel(RouteArgs a) {
-  constexpr int ROWS = ROUTE_THREADS / L;
+  constexpr int ROWS = ROUTE_THREADS / L, KEPT = L < 8 ? 8 / L : 1;
   const int lane = threadIdx.x % L, sub = threadIdx.x / L, first = lane * V;
   float mine[V];  // sums of p over this lane's rows
 #pragma unroll
@@ -113,32 +180,24 @@ __global__ __launch_bounds__(ROUTE_THREADS) void route_forward_kernel(RouteArgs 
     for (int c = 0; c < V; ++c) nan |= z[c] != z[c];
     // a NaN is never chosen; the row's weights and probabilities are NaN by the formula
     const float poison = row_max<L>(nan ? 1.f : 0.f) > 0.f ? NAN : 0.f;
-    uint32_t left = (1u << V) - 1u;  // (V <= 16) this lane's logits that are not chosen yet
+    Candidates<T, V> candidates(z, first);
     float top = 0.f;      // the row's largest logit
     float chosen = 0.f;   // sum of exp over the chosen
+    float kept[KEPT] = {};  // the lane of place j keeps its share until the sum is known (place j: kept[j / L]) ...
     int count = 0;
     for (int j = 0; j < a.k; ++j) {
-      float best = -INFINITY;
-      int at = ROUTE_MAX_E;
-#pragma unroll
-      for (int c = 0; c < V; ++c)  // (ascending index: the first of equals stays)
-        if (((left >> c) & 1u) && z[c] > best) best = z[c], at = first + c;
-      halving_steps<L>([&](auto m) {
-        const float ob = from_other_half<decltype(m)::value>(best);
-        const int oa = from_other_half<decltype(m)::value>(at);
-        if (ob > best || (ob == best && oa < at)) best = ob, at = oa;
-      });
-      const bool found = best > -INFINITY;
+      int at;
+      const float best = candidates.template next<L>(at);
+      const bool found = at >= 0;
       if (j == 0) top = found ? best : 0.f;
       const float share = found ? exp_fast(best - top) : 0.f;
       chosen += share;
       count += found;
-      const int own = at - first;
-      if (found && own >= 0 && own < V) left &= ~(1u << own);
-      // (the lane of place j keeps it; the sum is not known yet: the weight follows below)
       if (in && j % L == lane) {
-        a.weights[row * a.k + j] = share;
-        a.experts[row * a.k + j] = found ? at : -1;
+#pragma unroll
+        for (int i = 0; i < KEPT; ++i) kept[i] = j / L == i ? share : kept[i];
+        if (j >= KEPT * L) a.weights[row * a.k + j] = share;  // ... or writes it and reads it again
+        a.experts[row * a.k + j] = at;
       }
     }
     float all = 0.f, p[V];
@@ -147,8 +206,12 @@ __global__ __launch_bounds__(ROUTE_THREADS) void route_forward_kernel(RouteArgs 
     all = row_sum<L>(all);
     const float inv_all = (all > 0.f ? 1.f / all : 0.f) + poison;
     const float inv = a.normalize ? (count ? 1.f / chosen : 0.f) + poison : inv_all;
-    if (in)
-      for (int j = lane; j < a.k; j += L) a.weights[row * a.k + j] = j < count ? a.weights[row * a.k + j] * inv : 0.f;
+    if (in) {
+#pragma unroll
+      for (int i = 0; i < KEPT; ++i)
+        if (i * L + lane < a.k) a.weights[row * a.k + i * L + lane] = i * L + lane < count ? kept[i] * inv : 0.f;
+      for (int j = KEPT * L + lane; j < a.k; j += L) a.weights[row * a.k + j] = j < count ? a.weights[row * a.k + j] * inv : 0.f;
+    }
     if (live)
 #pragma unroll
       for (int c = 0; c < V; ++c) mine[c] += p[c] * inv_all;

@@ -267,7 +267,8 @@ __global__ __launch_bounds__(C::THREADS, 2) void grouped_wgrad_kernel(GroupedArg
     run_stages<T, C, COLUMNS, COLUMNS, HOW, true>(sj, si, begin, end, SameRow{}, row, acc, sums, SJ0, SI0, SJ1, SI1);
   __syncthreads();
   const int lane = threadIdx.x & 63, wave = wave_number();
-  float *pw = a.partial + (int64_t)chunk * a.N * a.K, *pb = a.partial + (int64_t)a.chunks * a.N * a.K + (int64_t)chunk * a.N;
+  const int64_t slice = max(chunk, 0);
+  float *pw = a.partial + slice * a.N * a.K, *pb = a.partial + (int64_t)a.chunks * a.N * a.K + slice * a.N;
   E *gw = static_cast<E *>(a.gw) + (int64_t)expert * a.N * a.K, *gb = static_cast<E *>(a.gb) + (int64_t)expert * a.N;
   const auto as_it_is = [](int, float (&)[4]) {};
   if (chunk >= 0)
