@@ -377,6 +377,9 @@ void with_route_shape(int E, F &&f) {
 // (any value outside 0 .. E-1) is sorted behind the last group and gets order = -1 there, position = -1.
 constexpr int GROUP_THREADS = 1024, GROUP_WAVES = GROUP_THREADS / 64, GROUP_CHUNK = 4096;
 constexpr int GROUP_ROUNDS = GROUP_CHUNK / GROUP_THREADS;
+// Up to twice that many places are one workgroup's, with twice the rounds and no counts to exchange: one launch instead of two
+// (8192 places, 8 experts: 11.3 us instead of 2.8 + 7.6, and 4 us less of the host's).
+constexpr int GROUP_ALONE = 2 * GROUP_CHUNK;
 
 __device__ __forceinline__ int group_key(const int32_t *experts, int64_t S, int64_t at, int E) {
   if (at >= S) return -1;
@@ -398,6 +401,7 @@ __global__ __launch_bounds__(GROUP_THREADS) void group_count_kernel(int64_t S, i
   for (int e = threadIdx.x; e <= E; e += GROUP_THREADS) counts[(size_t)blockIdx.x * (E + 1) + e] = hist[e];
 }
 
+template <int ROUNDS>
 __global__ __launch_bounds__(GROUP_THREADS) void group_place_kernel(int64_t S, int E, int bits,
                                                                     const int32_t *__restrict__ experts,
                                                                     const int32_t *__restrict__ counts, int blocks,
@@ -410,10 +414,10 @@ __global__ __launch_bounds__(GROUP_THREADS) void group_place_kernel(int64_t S, i
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, E1 = E + 1;
   for (int i = t; i < GROUP_WAVES * E1; i += GROUP_THREADS) base[i] = 0;
   __syncthreads();
-  int key[GROUP_ROUNDS];
-  const int64_t first = (int64_t)blockIdx.x * GROUP_CHUNK + wave * (64 * GROUP_ROUNDS) + lane;
+  int key[ROUNDS];
+  const int64_t first = (int64_t)blockIdx.x * (ROUNDS * GROUP_THREADS) + wave * (64 * ROUNDS) + lane;
 #pragma unroll
-  for (int r = 0; r < GROUP_ROUNDS; ++r) {
+  for (int r = 0; r < ROUNDS; ++r) {
     key[r] = group_key(experts, S, first + 64 * r, E);
     if (key[r] >= 0) atomicAdd(&base[wave * E1 + key[r]], 1);
   }
@@ -476,7 +480,7 @@ __global__ __launch_bounds__(GROUP_THREADS) void group_place_kernel(int64_t S, i
     __syncthreads();
   }
 #pragma unroll
-  for (int r = 0; r < GROUP_ROUNDS; ++r) {
+  for (int r = 0; r < ROUNDS; ++r) {
     unsigned long long peers = __ballot(key[r] >= 0);
     for (int b = 0; b < bits; ++b) {
       const bool bit = (key[r] >> b) & 1;
@@ -653,7 +657,7 @@ extern "C" int dimo_route_topk_backward(int T, int E, int k, int dtype, const vo
 }
 
 extern "C" size_t dimo_group_rows_workspace_bytes(int64_t S, int E) {
-  if (S <= GROUP_CHUNK || E <= 0) return 0;
+  if (S <= GROUP_ALONE || E <= 0) return 0;
   return align_up((size_t)((S + GROUP_CHUNK - 1) / GROUP_CHUNK) * (E + 1) * sizeof(int32_t));
 }
 
@@ -661,24 +665,25 @@ extern "C" int dimo_group_rows(int64_t S, int E, int places, const int32_t *expe
                                int32_t *position, int32_t *rows, void *workspace, size_t workspace_bytes, void *stream) {
   if (S < 0 || S > DIMO_MAX_SIZE || E < 1 || E > ROUTE_MAX_E || places < 1 || !offsets) return DIMO_E_ARG;
   if (S > 0 && (!experts || !order || !position)) return DIMO_E_ARG;
-  if (workspace_bytes < dimo_group_rows_workspace_bytes(S, E) || (S > GROUP_CHUNK && !workspace)) return DIMO_E_WORKSPACE;
+  if (workspace_bytes < dimo_group_rows_workspace_bytes(S, E) || (S > GROUP_ALONE && !workspace)) return DIMO_E_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
   clear_errors();
   ScopedTimer timer(T_ROUTE, s);
   int bits = 1;
   while ((1 << bits) <= E) ++bits;
-  const int blocks = S > 0 ? (int)((S + GROUP_CHUNK - 1) / GROUP_CHUNK) : 1;
+  const int blocks = S > GROUP_ALONE ? (int)((S + GROUP_CHUNK - 1) / GROUP_CHUNK) : 1;
   int32_t *counts = blocks > 1 ? static_cast<int32_t *>(workspace) : nullptr;
   if (counts)
     hipLaunchKernelGGL(group_count_kernel, dim3(blocks), dim3(GROUP_THREADS), 0, s, S, E, experts, counts);
   const size_t lds = (size_t)GROUP_WAVES * (E + 1) * sizeof(int);
+  auto place = S > GROUP_CHUNK && S <= GROUP_ALONE ? group_place_kernel<2 * GROUP_ROUNDS> : group_place_kernel<GROUP_ROUNDS>;
   if (lds > 32768) {  // (1024 experts: 65 600 bytes and 8 KB of tallies; a workgroup has 160 KB)
-    if (hipFuncSetAttribute(reinterpret_cast<const void *>(group_place_kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                            (int)lds) != hipSuccess)
+    if (hipFuncSetAttribute(reinterpret_cast<const void *>(place), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) !=
+        hipSuccess)
       return check_launch();
   }
-  hipLaunchKernelGGL(group_place_kernel, dim3(blocks), dim3(GROUP_THREADS), lds, s, S, E, bits, experts, counts, blocks,
-                     offsets, order, position, places, rows);
+  hipLaunchKernelGGL(place, dim3(blocks), dim3(GROUP_THREADS), lds, s, S, E, bits, experts, counts, blocks, offsets, order,
+                     position, places, rows);
   return check_launch();
 }
 

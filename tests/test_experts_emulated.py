@@ -41,7 +41,8 @@ def test_route_nan_and_infinities(emulated):
 
 
 @pytest.mark.parametrize("T,k,E,skew", [(0, 2, 3, False), (1, 1, 1, False), (1, 8, 64, False), (63, 1, 5, False),
-                                        (4096, 1, 7, True), (2049, 2, 64, False), (5000, 2, 3, True), (700, 2, 1024, False)])
+                                        (4096, 1, 7, True), (2049, 2, 64, False), (5000, 2, 3, True), (700, 2, 1024, False),
+                                        (4096, 2, 8, False), (2730, 3, 1024, True), (8193, 1, 5, True)])
 def test_group(emulated, T, k, E, skew):
     cases.check_group(ex, "cpu", T, k, E, seed=T + E, skew=skew)
 
