@@ -215,11 +215,12 @@ class Trainer:
 
     def _decide_direct(self):
         """Direct HIP pipeline: GPU, degree-0 colour (DIMO's configuration), product rasterizer; stage s2 (skinning by
-        <= 1800 control points, `_r` retired) or stage s1 (the TimeNet moves the Gaussians, shared (1, 1) radius `_r`)."""
+        <= 1800 control points, `_r` retired) or stage s1 (the TimeNet moves the Gaussians, shared (1, 1) radius `_r`).
+        Stage s1 needs the fused TimeNet there, which a network with experts is not: such a one trains s1 by autograd."""
         cfg, renderer, direct = self.cfg, self.renderer, self._direct_wanted
         g0 = renderer.gaussians
         stage_ok = (self.stage >= "s2" and len(g0._r) == 0 and g0._c_xyz.shape[0] <= 1800) or \
-                   (self.stage == "s1" and tuple(g0._r.shape) == (1, 1))
+                   (self.stage == "s1" and tuple(g0._r.shape) == (1, 1) and g0._timenet.experts is None)
         self.direct = (direct if direct is not None else True) and self.device.type == "cuda" \
             and stage_ok and cfg.sh_degree == 0 and renderer._rasterizer_factory is None
         if self.direct and not renderer.capacity:

@@ -1,0 +1,34 @@
+"""Networks with experts through the trainer on the GPU, on its default path."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def test_two_stages_with_experts():
+    """Renderer(timenet_experts=...) through Trainer.train_dynamic with the default pipeline: the block's parameters move in
+    stage s1 (autograd) and in stage s2 (direct)."""
+    from dimo_amd.renderer import Renderer
+    from dimo_amd.synth import init_synthetic_model
+    from dimo_amd.trainer import TrainConfig, Trainer
+    cfg = TrainConfig(num_pts=300, num_cpts=48, num_pts_per_cpt=10, num_motions=3, num_frames=4, num_views=4,
+                      motions_per_step=2, views_per_step=1, frames_per_step=2, resolution=64, stage="s1", FPS_iter=10 ** 6,
+                      density_end_iter=0, position_lr_max_steps=500)
+    rd = Renderer(sh_degree=0, num_latent_code=cfg.num_motions, add_normal=True, device="cuda", timenet_experts=4, timenet_top_k=2)
+    init_synthetic_model(rd, cfg.num_pts, cfg.num_cpts, seed=0, num_latent=cfg.num_motions)
+    g = rd.gaussians
+    g._r = torch.nn.Parameter(g._scaling.detach().mean() * torch.ones(1, 1, device="cuda"))
+    tr = Trainer(cfg, rd)
+    assert not tr.direct
+    values = lambda: {n: p.detach().clone() for n, p in g._timenet.experts.named_parameters()}
+    seen = [values()]
+
+    def note(t):
+        if (t.stage, t.step) in (("s1", 3), ("s2", 2)):
+            seen.append(values())
+    tr.train_dynamic(3, 2, on_step=note)
+    torch.cuda.synchronize()
+    assert tr.stage == "s2" and tr.direct and torch.isfinite(g.flat_params).all() and len(seen) == 3
+    for a, b in zip(seen, seen[1:]):
+        for n in a:
+            assert not torch.equal(a[n], b[n]), n
