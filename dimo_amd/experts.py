@@ -19,6 +19,7 @@ import ctypes as C
 
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -79,7 +80,17 @@ def _ld(t):
 
 
 def _tracked(*tensors):
+    """Whether a call goes through its autograd function: for gradients, and wherever a level of forward-mode derivatives is
+    open -- torch then refuses inputs with tangents, which would otherwise be dropped without a word."""
+    if forward_ad._current_level >= 0:
+        return True
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _refuse_tangents(*tensors):
+    """For calls without derivatives of either kind."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("no forward-mode derivative for the 4-bit operators")
 
 
 # ------------------------------------------------------------------------------------------------ routing

@@ -11,7 +11,7 @@ every element.  No gradients.  GPU only."""
 import torch
 
 from . import _lib
-from .experts import _ACTIVATIONS, _DTYPES, _check_linear_groups, _check_sizes, _dtype, _gpu, _ld, _on, _rows
+from .experts import _ACTIVATIONS, _DTYPES, _check_linear_groups, _check_sizes, _dtype, _gpu, _ld, _on, _refuse_tangents, _rows
 
 
 class MX4:
@@ -58,6 +58,7 @@ def quantize_mx4(x, groups=None):
     groups (from group_rows): x [T, K] is read through the grouping, the result is [T k, K] in the order of the groups
     (zeros behind the last one)."""
     _gpu(x)
+    _refuse_tangents(x)
     dtype = _dtype(x, "x")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("x: [..., K] with K >= 1 expected")
@@ -97,6 +98,7 @@ def mx4_linear(x, weight, bias=None, groups=None, activation=None, out_dtype=tor
     if N < 1:
         raise ValueError("weight without rows")
     _check_sizes(R, N, x.columns)
+    _refuse_tangents(bias)
     _gpu(x.codes, weight.codes, bias, None if groups is None else groups.offsets)
     if groups is not None:
         E = weight.shape[0]

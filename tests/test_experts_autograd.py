@@ -1,0 +1,61 @@
+"""How the expert operators stand to autograd beyond their gradients (tests/expert_cases.py): forward-mode derivatives are
+refused, never dropped."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from dimo_amd import experts as ex
+from dimo_amd import mx4
+from tests import expert_emulation
+
+
+@pytest.fixture
+def emulated(monkeypatch):
+    expert_emulation.use(monkeypatch, ex, mx4)
+
+
+def _inputs():
+    torch.manual_seed(0)
+    return torch.randn(6, 8), torch.randn(6, 3), torch.randn(3, 5, 8), torch.randn(3, 5), torch.randn(3, 8, 5), torch.randn(3, 8)
+
+
+CALLS = {
+    "route_topk": (lambda x, z, w1, b1, w2, b2, g: ex.route_topk(z, 2)[0], (1,)),
+    "grouped_linear": (lambda x, z, w1, b1, w2, b2, g: ex.grouped_linear(x, w1, g, b1, "silu", gather=True), (0, 2, 3)),
+    "combine_rows": (lambda x, z, w1, b1, w2, b2, g: ex.combine_rows(x.repeat(2, 1), g, z[:, :2].contiguous(), x), (0, 1)),
+    "expert_mlp": (lambda x, z, w1, b1, w2, b2, g: ex.expert_mlp(x, z, w1, b1, w2, b2, 2), (0, 1, 2, 3, 4, 5)),
+    "quantize_mx4": (lambda x, z, w1, b1, w2, b2, g: mx4.quantize_mx4(x).dequantize(), (0,)),
+    "mx4_linear": (lambda x, z, w1, b1, w2, b2, g: mx4.mx4_linear(mx4.quantize_mx4(w2[0]), mx4.quantize_mx4(w1), b1, g4(), None,
+                                                                  torch.float32), (3,)),
+}
+
+
+def g4():
+    return ex.RowGroups(torch.tensor([0, 4, 4, 8], dtype=torch.int32))
+
+
+def _call(name, tensors):
+    fn, _ = CALLS[name]
+    groups = ex.group_rows(ex.route_topk(_inputs()[1], 2)[1], 3)
+    if name == "mx4_linear":  # (w2[0] is [8, 5], w1 [3, 5, 8]: equal columns)
+        tensors = list(tensors)
+        tensors[2] = _inputs()[2][:, :, :5].contiguous()
+    return fn(*tensors, groups)
+
+
+@pytest.mark.parametrize("name,which", [(n, i) for n, (_, at) in CALLS.items() for i in at])
+@pytest.mark.parametrize("grad", [True, False])
+def test_tangents_are_refused(emulated, name, which, grad):
+    tensors = list(_inputs())
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        tensors[which] = forward_ad.make_dual(tensors[which], torch.ones_like(tensors[which]))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            _call(name, tensors)
+
+
+@pytest.mark.parametrize("name", list(CALLS))
+def test_an_open_level_changes_nothing_without_tangents(emulated, name):
+    want = _call(name, _inputs())
+    with forward_ad.dual_level():
+        got = _call(name, _inputs())
+    assert torch.equal(got, want)
