@@ -76,8 +76,8 @@ extern "C" int dimo_expert_mlp_forward(const dimo_expert_mlp_desc *d, int keep, 
   void *h = at<char>(workspace, L.h), *y = at<char>(workspace, L.y);
   void *z = keep && d->act == DIMO_ACT_SILU ? at<char>(workspace, L.z) : nullptr;
   const int R = (int)L.S;
-  int rc = dimo_route_topk_forward(d->T, d->E, d->k, d->dtype, d->logits, d->ld_logits, d->row_mask, 1, weights, experts,
-                                   nullptr, nullptr, 0, stream);
+  int rc = dimo_route_topk_forward(d->T, d->E, d->k, d->dtype, d->logits, d->ld_logits, d->row_mask, d->normalize, weights,
+                                   experts, nullptr, nullptr, 0, stream);
   if (!rc)
     rc = dimo_group_rows(L.S, d->E, d->k, experts, offsets, at<int32_t>(workspace, L.order), position, rows, h,
                          dimo_group_rows_workspace_bytes(L.S, d->E), stream);
@@ -110,8 +110,8 @@ extern "C" int dimo_expert_mlp_backward(const dimo_expert_mlp_desc *d, const voi
   int rc = dimo_combine_rows_backward(d->T, d->k, d->K, L.S, d->E, d->dtype, g_out, ld_g, y, d->K, weights, position, offsets,
                                       gy, g_logits ? gw : nullptr, stream);
   if (!rc && g_logits)
-    rc = dimo_route_topk_backward(d->T, d->E, d->k, d->dtype, d->logits, d->ld_logits, d->row_mask, 1, weights, experts, gw,
-                                  nullptr, g_logits, stream);
+    rc = dimo_route_topk_backward(d->T, d->E, d->k, d->dtype, d->logits, d->ld_logits, d->row_mask, d->normalize, weights,
+                                  experts, gw, nullptr, g_logits, stream);
   if (!rc && g_w2)
     rc = dimo_grouped_linear_wgrad(d->dtype, R, d->E, d->F, d->K, gy, h, d->F, nullptr, offsets, g_w2, g_b2, partial,
                                    P.partial_bytes, stream);

@@ -389,18 +389,18 @@ def combine_rows(y, groups, weights=None, residual=None):
 
 
 class _ExpertMlpDesc(C.Structure):
-    _fields_ = [(n, C.c_int) for n in ("dtype", "T", "K", "F", "E", "k", "act")] + [("ld_x", C.c_int64), ("ld_logits", C.c_int64)] \
+    _fields_ = [(n, C.c_int) for n in ("dtype", "T", "K", "F", "E", "k", "act", "normalize")] + [("ld_x", C.c_int64), ("ld_logits", C.c_int64)] \
         + [(n, C.c_void_p) for n in ("x", "logits", "w1", "b1", "w2", "b2", "row_mask")]
 
 
-def _expert_mlp_desc(x, logits, w1, b1, w2, b2, row_mask, k, act):
-    return _ExpertMlpDesc(_DTYPES[x.dtype], x.shape[0], x.shape[1], w1.shape[1], w1.shape[0], k, act, _ld(x), _ld(logits),
-                          x.data_ptr(), logits.data_ptr(), w1.data_ptr(), _lib.ptr(b1), w2.data_ptr(), _lib.ptr(b2),
+def _expert_mlp_desc(x, logits, w1, b1, w2, b2, row_mask, k, act, normalize):
+    return _ExpertMlpDesc(_DTYPES[x.dtype], x.shape[0], x.shape[1], w1.shape[1], w1.shape[0], k, act, normalize, _ld(x),
+                          _ld(logits), x.data_ptr(), logits.data_ptr(), w1.data_ptr(), _lib.ptr(b1), w2.data_ptr(), _lib.ptr(b2),
                           _lib.ptr(row_mask))
 
 
-def _expert_mlp_forward(x, logits, w1, b1, w2, b2, row_mask, k, act, keep):
-    L, d = _lib.lib(), _expert_mlp_desc(x, logits, w1, b1, w2, b2, row_mask, k, act)
+def _expert_mlp_forward(x, logits, w1, b1, w2, b2, row_mask, k, act, normalize, keep):
+    L, d = _lib.lib(), _expert_mlp_desc(x, logits, w1, b1, w2, b2, row_mask, k, act, normalize)
     at = C.addressof(d)
     out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     with _on(x.device):
@@ -413,10 +413,10 @@ def _expert_mlp_forward(x, logits, w1, b1, w2, b2, row_mask, k, act, keep):
 
 class _ExpertMlp(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, logits, w1, b1, w2, b2, row_mask, k, act):
-        out, ws = _expert_mlp_forward(x, logits, w1, b1, w2, b2, row_mask, k, act, True)
+    def forward(ctx, x, logits, w1, b1, w2, b2, row_mask, k, act, normalize):
+        out, ws = _expert_mlp_forward(x, logits, w1, b1, w2, b2, row_mask, k, act, normalize, True)
         ctx.save_for_backward(x, logits, w1, b1, w2, b2, row_mask, ws)
-        ctx.k, ctx.act = k, act
+        ctx.rest = k, act, normalize
         return out
 
     @staticmethod
@@ -424,7 +424,7 @@ class _ExpertMlp(torch.autograd.Function):
     def backward(ctx, g):
         *tensors, ws = ctx.saved_tensors
         x, logits, w1, b1, w2, b2, _ = tensors
-        L, d = _lib.lib(), _expert_mlp_desc(*tensors, ctx.k, ctx.act)
+        L, d = _lib.lib(), _expert_mlp_desc(*tensors, *ctx.rest)
         at, need = C.addressof(d), ctx.needs_input_grad
         g = _rows(g)
         # (a bias gradient comes with its weight's)
@@ -437,14 +437,15 @@ class _ExpertMlp(torch.autograd.Function):
             _lib.check(L.dimo_expert_mlp_backward(at, g.data_ptr(), _ld(g), ws.data_ptr(), scratch.data_ptr(), nbytes,
                                                   *[_lib.ptr(t) for t in grads], _lib.current_stream()),
                        "dimo_expert_mlp_backward")
-        return (*[t if on else None for t, on in zip(grads, need)], None, None, None)
+        return (*[t if on else None for t, on in zip(grads, need)], None, None, None, None)
 
 
-def expert_mlp(x, logits, w1, b1, w2, b2, k, activation="relu", row_mask=None):
+def expert_mlp(x, logits, w1, b1, w2, b2, k, activation="relu", row_mask=None, normalize=True):
     """x + sum over a row's k experts of weight * (w2 activation(w1 x + b1) + b2): routing (weights normalised over the
-    chosen), both products and the sum as one call per direction -- what route_topk, group_rows, grouped_linear (gathering,
+    chosen; normalize=False: softmax over all E), both products and the sum as one call per direction -- what route_topk, group_rows, grouped_linear (gathering,
     then plain) and combine_rows give one by one.  x [T, K], logits [T, E], w1 [E, F, K], b1 [E, F] or None, w2 [E, K, F],
-    b2 [E, K] or None; row_mask [T]: rows with False come back as they are.  Differentiable in x, logits and the weights."""
+    b2 [E, K] or None; row_mask [T]: rows with False come back as they are.  Differentiable in x, logits and the weights.
+    With k = 1 a normalised weight is the constant 1, and the logits' gradient zero."""
     if x.dim() != 2 or logits.dim() != 2 or w1.dim() != 3:
         raise ValueError("x: [T, K], logits: [T, E] and w1: [E, F, K] expected")
     _gpu(x, logits, w1, b1, w2, b2, row_mask)
@@ -466,13 +467,14 @@ def expert_mlp(x, logits, w1, b1, w2, b2, k, activation="relu", row_mask=None):
     x, logits, w1, w2 = _rows(x), _rows(logits), w1.contiguous(), w2.contiguous()
     b1, b2 = None if b1 is None else b1.contiguous(), None if b2 is None else b2.contiguous()
     if _tracked(x, logits, w1, b1, w2, b2):
-        return _ExpertMlp.apply(x, logits, w1, b1, w2, b2, row_mask, k, _ACTIVATIONS[activation])
-    return _expert_mlp_forward(x, logits, w1, b1, w2, b2, row_mask, k, _ACTIVATIONS[activation], False)[0]
+        return _ExpertMlp.apply(x, logits, w1, b1, w2, b2, row_mask, k, _ACTIVATIONS[activation], bool(normalize))
+    return _expert_mlp_forward(x, logits, w1, b1, w2, b2, row_mask, k, _ACTIVATIONS[activation], bool(normalize), False)[0]
 
 
 class ExpertMLP(nn.Module):
-    """h + the weighted sum of a row's k experts (each width -> hidden -> width), h [..., width].  The second products
-    start at zero, so a network that gets such a block starts as it was.  `quantized()`: the same block for evaluation
+    """h + the weighted sum of a row's k experts (each width -> hidden -> width), h [..., width].  The weights
+    are normalised over the chosen; with k = 1, where that would be the constant 1 and the router would not learn, they are
+    the softmax over all experts.  The second products start at zero, so a network that gets such a block starts as it was.  `quantized()`: the same block for evaluation
     only, its products in microscaled 4-bit form (dimo_amd/mx4.py)."""
 
     def __init__(self, width, num_experts, k=2, hidden=None, activation="relu", device=None):
@@ -482,7 +484,7 @@ class ExpertMLP(nn.Module):
             raise ValueError(f"1 <= k <= num_experts <= {MAX_EXPERTS} expected")
         if activation not in _ACTIVATIONS:
             raise ValueError(f"activation: one of {list(_ACTIVATIONS)} expected")
-        self.k, self.activation = k, activation
+        self.k, self.activation, self.normalize = k, activation, k > 1
         self.router = nn.Linear(width, num_experts, bias=False)
         self.w1 = nn.Parameter(torch.empty(num_experts, hidden, width))
         self.b1 = nn.Parameter(torch.zeros(num_experts, hidden))
@@ -495,7 +497,8 @@ class ExpertMLP(nn.Module):
 
     def forward(self, h):
         rows = h.reshape(-1, h.shape[-1])
-        out = expert_mlp(rows, self.router(rows), self.w1, self.b1, self.w2, self.b2, self.k, self.activation)
+        out = expert_mlp(rows, self.router(rows), self.w1, self.b1, self.w2, self.b2, self.k, self.activation,
+                         normalize=self.normalize)
         return out.view(h.shape)
 
     def quantized(self):
@@ -509,7 +512,7 @@ class QuantizedExpertMLP(nn.Module):
     def __init__(self, block):
         super().__init__()
         from .mx4 import quantize_mx4
-        self.k, self.activation, self.hidden = block.k, block.activation, block.w1.shape[1]
+        self.k, self.activation, self.normalize, self.hidden = block.k, block.activation, block.normalize, block.w1.shape[1]
         q1, q2 = quantize_mx4(block.w1), quantize_mx4(block.w2)
         for name, t in (("router", block.router.weight.detach().clone()), ("b1", block.b1.detach().clone()),
                         ("b2", block.b2.detach().clone()), ("w1_codes", q1.codes), ("w1_scales", q1.scales),
@@ -520,7 +523,7 @@ class QuantizedExpertMLP(nn.Module):
     def forward(self, h):
         from .mx4 import MX4, mx4_linear, quantize_mx4
         rows = h.reshape(-1, h.shape[-1])
-        weights, experts, _ = route_topk(rows @ self.router.T, self.k)
+        weights, experts, _ = route_topk(rows @ self.router.T, self.k, normalize=self.normalize)
         groups = group_rows(experts, self.router.shape[0])
         y = mx4_linear(quantize_mx4(rows, groups), MX4(self.w1_codes, self.w1_scales, rows.shape[1]), self.b1, groups,
                        self.activation, rows.dtype)

@@ -497,11 +497,11 @@ int dimo_combine_rows_backward(int T, int k, int N, int64_t S, int E, int dtype,
                                const void *y, int64_t ldy, const float *weights, const int32_t *position,
                                const int32_t *offsets, void *g_y, float *g_weights, void *stream);
 /* The expert block in one call per direction: out = x + sum over a row's k experts of weight * (w2 act(w1 x + b1) + b2),
- * weights normalised over the chosen.  x [T, K] at ld_x, logits [T, E] at ld_logits, w1 [E, F, K], b1 [E, F] or NULL,
+ * weights normalised over the chosen (normalize 0: softmax over all E).  x [T, K] at ld_x, logits [T, E] at ld_logits, w1 [E, F, K], b1 [E, F] or NULL,
  * w2 [E, K, F], b2 [E, K] or NULL, row_mask [T] or NULL (rows with 0: out = x).  keep: the workspace will be handed to the
  * backward, which reads it (and x, logits, the weights) unchanged; any gradient may be NULL (g_b* only with their g_w*). */
 typedef struct dimo_expert_mlp_desc {
-  int dtype, T, K, F, E, k, act;
+  int dtype, T, K, F, E, k, act, normalize;
   int64_t ld_x, ld_logits;
   const void *x, *logits, *w1, *b1, *w2, *b2;
   const uint8_t *row_mask;
