@@ -471,10 +471,20 @@ def expert_mlp(x, logits, w1, b1, w2, b2, k, activation="relu", row_mask=None, n
     return _expert_mlp_forward(x, logits, w1, b1, w2, b2, row_mask, k, _ACTIVATIONS[activation], bool(normalize), False)[0]
 
 
+def _without_autocast(block, h, dtype):
+    """block(h) in the type of its parameters where autocast is on (which would give the router's product another type than the
+    rows'), None elsewhere."""
+    if not torch.is_autocast_enabled(h.device.type):
+        return None
+    with torch.autocast(h.device.type, enabled=False):
+        return block(h.to(dtype))
+
+
 class ExpertMLP(nn.Module):
     """h + the weighted sum of a row's k experts (each width -> hidden -> width), h [..., width].  The weights
     are normalised over the chosen; with k = 1, where that would be the constant 1 and the router would not learn, they are
-    the softmax over all experts.  The second products start at zero, so a network that gets such a block starts as it was.  `quantized()`: the same block for evaluation
+    the softmax over all experts.  The second products start at zero, so a network that gets such a block starts as it was.
+    Under autocast the block works (and answers) in its parameters' type.  `quantized()`: the same block for evaluation
     only, its products in microscaled 4-bit form (dimo_amd/mx4.py)."""
 
     def __init__(self, width, num_experts, k=2, hidden=None, activation="relu", device=None):
@@ -496,6 +506,9 @@ class ExpertMLP(nn.Module):
             self.to(device)
 
     def forward(self, h):
+        out = _without_autocast(self, h, self.w1.dtype)
+        if out is not None:
+            return out
         rows = h.reshape(-1, h.shape[-1])
         out = expert_mlp(rows, self.router(rows), self.w1, self.b1, self.w2, self.b2, self.k, self.activation,
                          normalize=self.normalize)
@@ -522,6 +535,9 @@ class QuantizedExpertMLP(nn.Module):
     @torch.no_grad()
     def forward(self, h):
         from .mx4 import MX4, mx4_linear, quantize_mx4
+        out = _without_autocast(self, h, self.router.dtype)
+        if out is not None:
+            return out
         rows = h.reshape(-1, h.shape[-1])
         weights, experts, _ = route_topk(rows @ self.router.T, self.k, normalize=self.normalize)
         groups = group_rows(experts, self.router.shape[0])
