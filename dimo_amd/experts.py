@@ -182,6 +182,13 @@ class RowGroups:
         return self.offsets.shape[0] - 1
 
 
+def _saved_groups(offsets, rows, position):
+    """The grouping of a forward pass from tensors that autograd kept for its backward (and would miss if they had changed)."""
+    groups = RowGroups(offsets)
+    groups.rows, groups.position = rows, position
+    return groups
+
+
 def group_rows(experts, num_experts):
     """RowGroups of the places of experts [T, k] int32, stable: by expert, then by place.  A place whose value is outside
     0 .. num_experts - 1 belongs to nobody."""
@@ -281,15 +288,15 @@ class _GroupedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups, act, gather):
         y, z = _linear_forward(x, weight, bias, groups, act, gather, act == 2)
-        ctx.save_for_backward(x, weight, z if act == 2 else y if act == 1 else None)
-        ctx.groups, ctx.act, ctx.gather, ctx.bias = groups, act, gather, bias is not None
+        ctx.save_for_backward(x, weight, z if act == 2 else y if act == 1 else None, groups.offsets, groups.rows, groups.position)
+        ctx.act, ctx.gather, ctx.bias = act, gather, bias is not None
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        x, weight, saved = ctx.saved_tensors
-        groups = ctx.groups
+        x, weight, saved, *grouping = ctx.saved_tensors
+        groups = _saved_groups(*grouping)
         g = g.contiguous()
         if ctx.act:
             g = _activation_backward(g, saved, ctx.act)
@@ -351,17 +358,18 @@ def grouped_linear(x, weight, groups, bias=None, activation=None, gather=False):
 class _CombineRows(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, residual, groups):
-        ctx.save_for_backward(y if weights is not None and weights.requires_grad else None, weights)
-        ctx.groups = groups
+        ctx.save_for_backward(y if weights is not None and weights.requires_grad else None, weights, groups.offsets, groups.rows,
+                              groups.position)
         return _combine_forward(y, weights, groups, residual)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        y, weights = ctx.saved_tensors
+        y, weights, *grouping = ctx.saved_tensors
+        groups = _saved_groups(*grouping)
         g_y = g_w = None
         if ctx.needs_input_grad[0] or ctx.needs_input_grad[1]:
-            g_y, g_w = _combine_backward(_rows(g), y, weights, ctx.groups, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+            g_y, g_w = _combine_backward(_rows(g), y, weights, groups, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
         return g_y, g_w, g if ctx.needs_input_grad[2] else None, None
 
 

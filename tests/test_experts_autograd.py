@@ -1,5 +1,5 @@
 """How the expert operators stand to autograd beyond their gradients (tests/expert_cases.py): forward-mode derivatives are
-refused, never dropped."""
+refused, never dropped; a grouping that changes between a forward pass and its backward is an error, not another gradient."""
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -59,3 +59,26 @@ def test_an_open_level_changes_nothing_without_tangents(emulated, name):
     with forward_ad.dual_level():
         got = _call(name, _inputs())
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("name", ["offsets", "rows", "position"])
+def test_a_grouping_that_changed_is_an_error(emulated, name):
+    x, z, w1, b1, _, _ = (t.requires_grad_(True) for t in _inputs())
+    groups = ex.group_rows(ex.route_topk(z, 2)[1], 3)
+    y = ex.grouped_linear(x, w1, groups, b1, "relu", gather=True)
+    out = ex.combine_rows(y, groups, ex.route_topk(z, 2)[0])
+    getattr(groups, name).zero_()
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(out.sum(), (x, w1, z))
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(y.sum(), (x, w1))
+
+
+def test_a_grouping_that_was_replaced_keeps_the_gradient(emulated):
+    x, _, w1, _, _, _ = (t.requires_grad_(True) for t in _inputs())
+    groups = g4()
+    rows = x.repeat(2, 1)[:8]
+    y = ex.grouped_linear(rows, w1, groups)
+    want = torch.autograd.grad(y.sum(), w1, retain_graph=True)[0]
+    groups.offsets = torch.tensor([0, 0, 8, 8], dtype=torch.int32)
+    assert torch.equal(torch.autograd.grad(y.sum(), w1)[0], want)
