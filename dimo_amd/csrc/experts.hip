@@ -261,6 +261,7 @@ struct RouteBwdArgs {
   const float *g_weights, *g_load;
   void *g_logits;
   float load_scale;
+  int64_t first;  // first workgroup of this launch
 };
 
 template <class T, int L, int V>
@@ -268,7 +269,7 @@ __global__ __launch_bounds__(ROUTE_THREADS) void route_backward_kernel(RouteBwdA
   constexpr int ROWS = ROUTE_THREADS / L, PAD = 1;  // (rows of L V + 1 words: a lane's V words then lie on other banks)
   __shared__ float sparse[ROWS * (L * V + PAD)];
   const int lane = threadIdx.x % L, sub = threadIdx.x / L, first = lane * V;
-  const int64_t row = (int64_t)blockIdx.x * ROWS + sub;
+  const int64_t row = (a.first + blockIdx.x) * ROWS + sub;
   const bool in = row < a.T;
   const bool live = in && (!a.row_mask || a.row_mask[in ? row : 0] != 0);
   float *g_row = sparse + sub * (L * V + PAD);
@@ -556,12 +557,13 @@ struct CombineBwdArgs {
   const int32_t *position, *offsets;
   void *g_y;         // [S, N] or null
   float *g_weights;  // [T, k] or null
+  int64_t first;     // first workgroup of this launch
 };
 template <class T, int VEC>
 __global__ __launch_bounds__(256) void combine_backward_kernel(CombineBwdArgs a) {
   typedef typename T::store E;
   const int lane = threadIdx.x & 63;
-  const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t t = (a.first + blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (t >= a.T) return;
   for (int j = 0; j < a.k; ++j) {
     const int32_t p = a.position[t * a.k + j];
@@ -613,7 +615,9 @@ extern "C" int dimo_route_topk_forward(int T, int E, int k, int dtype, const voi
   hipStream_t s = (hipStream_t)stream;
   clear_errors();
   ScopedTimer timer(T_ROUTE, s);
+  const int64_t most = launch_groups(ROUTE_THREADS);  // (the kernel goes over the rows in rounds)
   int grid = T > 0 ? route_blocks(T, E) : 0;
+  if (grid > most) grid = (int)most;
   if (load) {
     const size_t need = dimo_route_workspace_bytes(T, E);
     if (workspace_bytes < need || (need && !workspace)) return DIMO_E_WORKSPACE;
@@ -645,15 +649,17 @@ extern "C" int dimo_route_topk_backward(int T, int E, int k, int dtype, const vo
   hipStream_t s = (hipStream_t)stream;
   clear_errors();
   ScopedTimer timer(T_ROUTE, s);
-  const RouteBwdArgs a{T, E, k, normalize, route_wide(dtype, E, logits, ld) && route_wide(dtype, E, g_logits, E), logits, ld,
-                       row_mask, weights, experts, g_weights, g_load, g_logits, 1.0f / (float)T};
-  with_dtype(dtype, [&](auto tag) {
-    with_route_shape(E, [&](auto l, auto v) {
-      hipLaunchKernelGGL((route_backward_kernel<decltype(tag), decltype(l)::value, decltype(v)::value>),
-                         dim3(route_blocks(T, E)), dim3(ROUTE_THREADS), 0, s, a);
+  RouteBwdArgs a{T, E, k, normalize, route_wide(dtype, E, logits, ld) && route_wide(dtype, E, g_logits, E), logits, ld,
+                 row_mask, weights, experts, g_weights, g_load, g_logits, 1.0f / (float)T, 0};
+  return for_launches(route_blocks(T, E), ROUTE_THREADS, [&](int64_t first, unsigned grid) {
+    a.first = first;
+    with_dtype(dtype, [&](auto tag) {
+      with_route_shape(E, [&](auto l, auto v) {
+        hipLaunchKernelGGL((route_backward_kernel<decltype(tag), decltype(l)::value, decltype(v)::value>), dim3(grid),
+                           dim3(ROUTE_THREADS), 0, s, a);
+      });
     });
   });
-  return check_launch();
 }
 
 extern "C" size_t dimo_group_rows_workspace_bytes(int64_t S, int E) {
@@ -732,14 +738,15 @@ extern "C" int dimo_combine_rows_backward(int T, int k, int N, int64_t S, int E,
   const int vec = 16 / (int)dtype_bytes(dtype);
   const bool wide = N % vec == 0 && ldg % vec == 0 && aligned16(g_out) && (!g_y || aligned16(g_y)) &&
                     (!g_weights || (ldy % vec == 0 && aligned16(y)));
-  const CombineBwdArgs a{T, k, N, E, S, g_out, y, ldg, ldy, weights, position, offsets, g_y, g_weights};
-  const int blocks = (T + 3) / 4;
-  with_dtype(dtype, [&](auto tag) {
-    typedef decltype(tag) Tag;
-    if (wide)
-      hipLaunchKernelGGL((combine_backward_kernel<Tag, Vec16<Tag>::N>), dim3(blocks), dim3(256), 0, s, a);
-    else
-      hipLaunchKernelGGL((combine_backward_kernel<Tag, 1>), dim3(blocks), dim3(256), 0, s, a);
+  CombineBwdArgs a{T, k, N, E, S, g_out, y, ldg, ldy, weights, position, offsets, g_y, g_weights, 0};
+  return for_launches(((int64_t)T + 3) / 4, 256, [&](int64_t first, unsigned grid) {
+    a.first = first;
+    with_dtype(dtype, [&](auto tag) {
+      typedef decltype(tag) Tag;
+      if (wide)
+        hipLaunchKernelGGL((combine_backward_kernel<Tag, Vec16<Tag>::N>), dim3(grid), dim3(256), 0, s, a);
+      else
+        hipLaunchKernelGGL((combine_backward_kernel<Tag, 1>), dim3(grid), dim3(256), 0, s, a);
+    });
   });
-  return check_launch();
 }

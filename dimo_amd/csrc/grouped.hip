@@ -33,6 +33,7 @@ struct GroupedArgs {
   int wide;                // sixteen bytes of an output row may be written at once
   int split_rows, chunks;  // wgrad: > 0: partial sums over that many rows at a time, `chunks` of them at most
   float *partial;          // [chunks, N, K], then [chunks, N]
+  int first;               // first workgroup of this launch
 };
 
 __device__ __forceinline__ int64_t source_row(const GroupedArgs &a, int r) {
@@ -47,7 +48,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void grouped_rows_kernel(GroupedArgs
   constexpr int BK = Planes<T>::DEPTH;
   const int columns = MODE == FORWARD ? a.N : a.K, reduction = MODE == FORWARD ? a.K : a.N;
   int ct = 0;
-  const RowTile tile = find_row_tile<HALVES<C>>(a.offsets, a.E, a.R, C::TJ, (columns + C::TI - 1) / C::TI, (int)blockIdx.x, &ct);
+  const RowTile tile = find_row_tile<HALVES<C>>(a.offsets, a.E, a.R, C::TJ, (columns + C::TI - 1) / C::TI, a.first + (int)blockIdx.x, &ct);
   if (tile.expert < 0) return;
   const int c0 = ct * C::TI;
   E *out = static_cast<E *>(MODE == FORWARD ? a.y : a.gx);
@@ -141,7 +142,7 @@ __global__ __launch_bounds__(64 * THIN_WAVES) void grouped_thin_kernel(GroupedAr
   typedef typename Planes<T>::Tag Tag;
   __shared__ float4 buffer[THIN_WAVES][4][64];
   int ct = 0;
-  const RowTile tile = find_row_tile<false>(a.offsets, a.E, a.R, 32, (a.N + 31) / 32, (int)blockIdx.x, &ct);
+  const RowTile tile = find_row_tile<false>(a.offsets, a.E, a.R, 32, (a.N + 31) / 32, a.first + (int)blockIdx.x, &ct);
   if (tile.expert < 0) return;
   const int lane = threadIdx.x & 63, c0 = 32 * ct;
   E *out = static_cast<E *>(a.y);
@@ -238,18 +239,19 @@ __global__ __launch_bounds__(C::THREADS, 2) void grouped_wgrad_kernel(GroupedArg
   typedef typename T::store E;
   constexpr int BK = Planes<T>::DEPTH;
   const int tiles_k = (a.K + C::TI - 1) / C::TI, tiles_n = (a.N + C::TJ - 1) / C::TJ;
+  const int workgroup = a.first + (int)blockIdx.x;
   int expert, begin, end, chunk = -1, block;  // chunk: the slice's place in `partial`
   if (a.split_rows) {
     int before = 0;
-    block = blockIdx.x % (tiles_k * tiles_n);
-    expert = find_slice(a, blockIdx.x / (tiles_k * tiles_n), &begin, &end);
+    block = workgroup % (tiles_k * tiles_n);
+    expert = find_slice(a, workgroup / (tiles_k * tiles_n), &begin, &end);
     if (expert < 0) return;
     if (cut_slices(a, expert, &before) > 1) {
       chunk = __builtin_amdgcn_readfirstlane(before) + (begin - clamp_offset(a.offsets, expert, a.R)) / a.split_rows;
       if (chunk >= a.chunks) return;  // (only where bad offsets make the groups overlap)
     }
   } else {
-    expert = largest_first(a.offsets, a.E, a.R, blockIdx.x / (tiles_k * tiles_n)), block = blockIdx.x % (tiles_k * tiles_n);
+    expert = largest_first(a.offsets, a.E, a.R, workgroup / (tiles_k * tiles_n)), block = workgroup % (tiles_k * tiles_n);
     begin = clamp_offset(a.offsets, expert, a.R), end = max(begin, clamp_offset(a.offsets, expert + 1, a.R));
   }
   const int n0 = block / tiles_k * C::TJ, k0 = block % tiles_k * C::TI;
@@ -328,8 +330,8 @@ __global__ __launch_bounds__(256) void grouped_wgrad_sum_kernel(GroupedArgs a) {
 template <class T, int VEC>
 __global__ __launch_bounds__(256) void activation_backward_kernel(int64_t n, int act, const typename T::store *__restrict__ g,
                                                                   const typename T::store *__restrict__ s,
-                                                                  typename T::store *__restrict__ out) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VEC;
+                                                                  typename T::store *__restrict__ out, int64_t first) {
+  const int64_t i = ((first + blockIdx.x) * 256 + threadIdx.x) * VEC;
   if (i >= n) return;
   float gv[VEC], sv[VEC];
   load_vec<T, VEC>(g + i, gv);
@@ -357,22 +359,26 @@ bool wide_output(int dtype, const void *p, int64_t columns) {
 }
 
 template <class T, int MODE, int HOW, class C>
-int launch_rows(const GroupedArgs &a, hipStream_t s) {
+int launch_rows(GroupedArgs a, hipStream_t s) {
   const int64_t groups = row_tile_workgroups<HALVES<C>>(row_tile_count<HALVES<C>>(a.R, a.E, C::TJ), ((MODE == FORWARD ? a.N : a.K) + C::TI - 1) / C::TI);
   if (groups > 0x7fffffffLL) return DIMO_E_ARG;
-  hipLaunchKernelGGL((grouped_rows_kernel<T, MODE, HOW, C>), dim3((unsigned)groups), dim3(C::THREADS), 0, s, a);
-  return check_launch();
+  return for_launches(groups, C::THREADS, [&](int64_t first, unsigned count) {
+    a.first = (int)first;
+    hipLaunchKernelGGL((grouped_rows_kernel<T, MODE, HOW, C>), dim3(count), dim3(C::THREADS), 0, s, a);
+  });
 }
 template <class T, int HOW, class C>
-int launch_wgrad(const GroupedArgs &a, hipStream_t s) {
+int launch_wgrad(GroupedArgs a, hipStream_t s) {
   const int64_t tiles = (int64_t)((a.N + C::TJ - 1) / C::TJ) * ((a.K + C::TI - 1) / C::TI);
   const int64_t groups = tiles * (a.split_rows ? row_tile_count(a.R, a.E, a.split_rows) : a.E);
   if (groups > 0x7fffffffLL || tiles > 0x7fffffffLL) return DIMO_E_ARG;
-  if (a.rows)
-    hipLaunchKernelGGL((grouped_wgrad_kernel<T, HOW, C, SourceRow>), dim3((unsigned)groups), dim3(C::THREADS), 0, s, a);
-  else
-    hipLaunchKernelGGL((grouped_wgrad_kernel<T, HOW, C, SameRow>), dim3((unsigned)groups), dim3(C::THREADS), 0, s, a);
-  return check_launch();
+  return for_launches(groups, C::THREADS, [&](int64_t first, unsigned count) {
+    a.first = (int)first;
+    if (a.rows)
+      hipLaunchKernelGGL((grouped_wgrad_kernel<T, HOW, C, SourceRow>), dim3(count), dim3(C::THREADS), 0, s, a);
+    else
+      hipLaunchKernelGGL((grouped_wgrad_kernel<T, HOW, C, SameRow>), dim3(count), dim3(C::THREADS), 0, s, a);
+  });
 }
 
 // Up to this many rows in all a forward takes the thin kernel: it reads each weight once per 32 rows of a group like the
@@ -388,18 +394,20 @@ int launch_wgrad(const GroupedArgs &a, hipStream_t s) {
 inline int thin_rows(int dtype) { return dtype == DIMO_F32 ? 256 : 16; }
 
 template <int MODE>
-int run_rows(int dtype, const GroupedArgs &a, bool whole, hipStream_t s) {
+int run_rows(int dtype, GroupedArgs a, bool whole, hipStream_t s) {
   if (MODE == FORWARD && a.R <= thin_rows(dtype)) {
     const int64_t groups = row_tile_workgroups(row_tile_count(a.R, a.E, 32), (a.N + 31) / 32);
     if (groups > 0x7fffffffLL) return DIMO_E_ARG;
-    with_dtype(dtype, [&](auto tag) {
-      typedef decltype(tag) T;
-      if (a.K % 8 == 0)
-        hipLaunchKernelGGL((grouped_thin_kernel<T, true>), dim3((unsigned)groups), dim3(64 * THIN_WAVES), 0, s, a);
-      else
-        hipLaunchKernelGGL((grouped_thin_kernel<T, false>), dim3((unsigned)groups), dim3(64 * THIN_WAVES), 0, s, a);
+    return for_launches(groups, 64 * THIN_WAVES, [&](int64_t first, unsigned count) {
+      a.first = (int)first;
+      with_dtype(dtype, [&](auto tag) {
+        typedef decltype(tag) T;
+        if (a.K % 8 == 0)
+          hipLaunchKernelGGL((grouped_thin_kernel<T, true>), dim3(count), dim3(64 * THIN_WAVES), 0, s, a);
+        else
+          hipLaunchKernelGGL((grouped_thin_kernel<T, false>), dim3(count), dim3(64 * THIN_WAVES), 0, s, a);
+      });
     });
-    return check_launch();
   }
   const int64_t per_group = (a.R + a.E - 1) / a.E;
   const int tile = choose_tile(per_group, (a.R + per_group - 1) / per_group, MODE == FORWARD ? a.N : a.K,
@@ -559,17 +567,16 @@ extern "C" int dimo_activation_backward(int dtype, int act, int64_t n, const voi
   const int vec = 16 / (int)dtype_bytes(dtype);
   const bool wide = n % vec == 0 && ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(saved) |
                                       reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-  const int64_t blocks = (n / (wide ? vec : 1) + 255) / 256;
-  if (blocks > 0x7fffffffLL) return DIMO_E_ARG;
-  with_dtype(dtype, [&](auto tag) {
-    typedef decltype(tag) Tag;
-    typedef typename Tag::store E;
-    if (wide)
-      hipLaunchKernelGGL((activation_backward_kernel<Tag, Vec16<Tag>::N>), dim3((unsigned)blocks), dim3(256), 0, s, n, act,
-                         static_cast<const E *>(g), static_cast<const E *>(saved), static_cast<E *>(out));
-    else
-      hipLaunchKernelGGL((activation_backward_kernel<Tag, 1>), dim3((unsigned)blocks), dim3(256), 0, s, n, act,
-                         static_cast<const E *>(g), static_cast<const E *>(saved), static_cast<E *>(out));
+  return for_launches((n / (wide ? vec : 1) + 255) / 256, 256, [&](int64_t first, unsigned count) {
+    with_dtype(dtype, [&](auto tag) {
+      typedef decltype(tag) Tag;
+      typedef typename Tag::store E;
+      if (wide)
+        hipLaunchKernelGGL((activation_backward_kernel<Tag, Vec16<Tag>::N>), dim3(count), dim3(256), 0, s, n, act,
+                           static_cast<const E *>(g), static_cast<const E *>(saved), static_cast<E *>(out), first);
+      else
+        hipLaunchKernelGGL((activation_backward_kernel<Tag, 1>), dim3(count), dim3(256), 0, s, n, act,
+                           static_cast<const E *>(g), static_cast<const E *>(saved), static_cast<E *>(out), first);
+    });
   });
-  return check_launch();
 }

@@ -126,6 +126,7 @@ struct Mx4Args {
   const void *bias;
   int act, wide;
   void *y;
+  int first;               // first workgroup of this launch
 };
 
 // Scale bytes of blocks b0 .. b0 + 7 of a line; what is behind its end counts as 2^0 (its codes are zero: a NaN scale must
@@ -193,7 +194,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx4_rows_kernel(Mx4Args a) {
   __shared__ __attribute__((aligned(1024))) uint16_t SJ0[C::TJ * BK], SI0[C::TI * BK], SJ1[C::TJ * BK], SI1[C::TI * BK];
   __shared__ uint2 scales[2][C::TJ + C::TI][2];  // [pairs of stages in turn][line][stage of the pair]
   int ct = 0;
-  const RowTile tile = find_row_tile<HALVES<C>>(a.offsets, a.E, a.R, C::TJ, (a.N + C::TI - 1) / C::TI, (int)blockIdx.x, &ct);
+  const RowTile tile = find_row_tile<HALVES<C>>(a.offsets, a.E, a.R, C::TJ, (a.N + C::TI - 1) / C::TI, a.first + (int)blockIdx.x, &ct);
   if (tile.expert < 0) return;
   const int c0 = ct * C::TI;
   E *out = static_cast<E *>(a.y);
@@ -294,7 +295,7 @@ __global__ __launch_bounds__(64 * THIN_WAVES) void mx4_thin_kernel(Mx4Args a) {
   typedef typename T::store E;
   __shared__ float4 buffer[THIN_WAVES][4][64];
   int ct = 0;
-  const RowTile tile = find_row_tile<false>(a.offsets, a.E, a.R, 32, (a.N + 31) / 32, (int)blockIdx.x, &ct);
+  const RowTile tile = find_row_tile<false>(a.offsets, a.E, a.R, 32, (a.N + 31) / 32, a.first + (int)blockIdx.x, &ct);
   if (tile.expert < 0) return;
   const int lane = threadIdx.x & 63, half = lane >> 5, c0 = 32 * ct;
   E *out = static_cast<E *>(a.y);
@@ -339,11 +340,13 @@ typedef Tile<128, 128, 2, 2> Medium;
 typedef Tile<256, 256, 2, 4> Large;
 
 template <class T, class C, bool SHORT>
-int launch_mx4(const Mx4Args &a, hipStream_t s) {
+int launch_mx4(Mx4Args a, hipStream_t s) {
   const int64_t groups = row_tile_workgroups<HALVES<C>>(row_tile_count<HALVES<C>>(a.R, a.E, C::TJ), (a.N + C::TI - 1) / C::TI);
   if (groups > 0x7fffffffLL) return DIMO_E_ARG;
-  hipLaunchKernelGGL((mx4_rows_kernel<T, C, SHORT>), dim3((unsigned)groups), dim3(C::THREADS), 0, s, a);
-  return check_launch();
+  return for_launches(groups, C::THREADS, [&](int64_t first, unsigned count) {
+    a.first = (int)first;
+    hipLaunchKernelGGL((mx4_rows_kernel<T, C, SHORT>), dim3(count), dim3(C::THREADS), 0, s, a);
+  });
 }
 
 // launch(first row, workgroups) for bands of rows whose units (`per_row` to a row, one per thread) a launch can count in
@@ -414,19 +417,21 @@ extern "C" int dimo_mx4_linear(int dtype, int R, int E, int K, int N, const uint
   clear_errors();
   ScopedTimer timer(T_MX4, s);
   const bool wide = N % (16 / (int)dtype_bytes(dtype)) == 0 && aligned16(y);
-  const Mx4Args a{R, E, K, N, (K + 31) / 32, x_codes, x_scales, w_codes, w_scales, offsets, bias, act, wide, y};
+  Mx4Args a{R, E, K, N, (K + 31) / 32, x_codes, x_scales, w_codes, w_scales, offsets, bias, act, wide, y, 0};
   // few rows, as in grouped.hip: 16 experts of 2048 x 2048, 1 / 8 / 16 / 32 / 256 rows: 6.2 / 7.5 / 7.6 / 9.4 / 12 us, the
   // 64 x 64 tile 8.1 / 8.4 / 8.4 / 9.5 / 9.7
   if (R <= 16) {
     const int64_t groups = row_tile_workgroups(row_tile_count(R, E, 32), (N + 31) / 32);
     if (groups > 0x7fffffffLL) return DIMO_E_ARG;
-    with_dtype(dtype, [&](auto tag) {
-      if (a.blocks < 8)
-        hipLaunchKernelGGL((mx4_thin_kernel<decltype(tag), true>), dim3((unsigned)groups), dim3(64 * THIN_WAVES), 0, s, a);
-      else
-        hipLaunchKernelGGL((mx4_thin_kernel<decltype(tag), false>), dim3((unsigned)groups), dim3(64 * THIN_WAVES), 0, s, a);
+    return for_launches(groups, 64 * THIN_WAVES, [&](int64_t first, unsigned count) {
+      a.first = (int)first;
+      with_dtype(dtype, [&](auto tag) {
+        if (a.blocks < 8)
+          hipLaunchKernelGGL((mx4_thin_kernel<decltype(tag), true>), dim3(count), dim3(64 * THIN_WAVES), 0, s, a);
+        else
+          hipLaunchKernelGGL((mx4_thin_kernel<decltype(tag), false>), dim3(count), dim3(64 * THIN_WAVES), 0, s, a);
+      });
     });
-    return check_launch();
   }
   const int64_t per_group = (R + E - 1) / E;
   const int tile = choose_tile(per_group, (R + per_group - 1) / per_group, N, true);

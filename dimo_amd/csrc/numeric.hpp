@@ -102,6 +102,20 @@ __device__ __forceinline__ void store_vec(typename T::store *dst, const float (&
   }
 }
 
+// A launch takes fewer than 2^32 threads: launch(first, count) for `total` workgroups of `threads`, as many at a time as fit
+// (a multiple of eight, so that every band begins on the first XCD).
+inline int64_t launch_groups(int threads) { return 0xffffffffLL / threads / 8 * 8; }
+template <class F>
+inline int for_launches(int64_t total, int threads, F &&launch) {
+  const int64_t most = launch_groups(threads);
+  for (int64_t first = 0; first < total; first += most) {
+    launch(first, (unsigned)(total - first < most ? total - first : most));
+    const int rc = check_launch();
+    if (rc) return rc;
+  }
+  return DIMO_OK;
+}
+
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // (relu keeps a NaN)

@@ -256,6 +256,33 @@ static int pool_size() {
   return n < 1 ? 1 : (n > 64 ? 64 : n);
 }
 
+static hipError_t last_error = hipSuccess;
+static bool dry = false;
+static std::vector<uint64_t> noted;  // threads of every launch since simt_dry_run(1)
+hipError_t take_error() {
+  const hipError_t e = last_error;
+  last_error = hipSuccess;
+  return e;
+}
+bool accept(dim3 grid, dim3 block) {
+  const uint64_t g[3] = {grid.x, grid.y, grid.z}, b[3] = {block.x, block.y, block.z};
+  for (int d = 0; d < 3; ++d)
+    if (g[d] * b[d] >= (1ull << 32)) {
+      last_error = hipErrorInvalidConfiguration;
+      return false;
+    }
+  if (dry) noted.push_back(g[0] * g[1] * g[2] * b[0] * b[1] * b[2]);
+  return !dry;
+}
+extern "C" void simt_dry_run(int on) {
+  dry = on != 0;
+  if (dry) noted.clear();
+}
+extern "C" int simt_launched(uint64_t *threads, int most) {  // how many launches were noted; the first `most` of them
+  for (int i = 0; i < most && i < (int)noted.size(); ++i) threads[i] = noted[i];
+  return (int)noted.size();
+}
+
 void launch(dim3 grid, dim3 block, size_t dynamic_lds_bytes, const std::function<void()> &body) {
   const size_t total = (size_t)grid.x * grid.y * grid.z;
   if (total == 0) return;

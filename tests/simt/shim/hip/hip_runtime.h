@@ -43,7 +43,7 @@ static inline float4 make_float4(float x, float y, float z, float w) { return fl
 
 typedef void *hipStream_t;
 typedef void *hipEvent_t;
-enum hipError_t { hipSuccess = 0, hipErrorUnknown = 999 };
+enum hipError_t { hipSuccess = 0, hipErrorInvalidConfiguration = 9, hipErrorUnknown = 999 };
 enum hipMemcpyKind { hipMemcpyHostToDevice = 1, hipMemcpyDeviceToHost = 2, hipMemcpyDeviceToDevice = 3 };
 enum { hipStreamNonBlocking = 1, hipEventDisableTiming = 2, hipStreamWaitValueGte = 0 };
 
@@ -64,8 +64,9 @@ void stream_wait_event(hipStream_t s, hipEvent_t e);
 void stream_write_value(hipStream_t s, uint32_t *p, uint32_t v);
 bool stream_wait_value(hipStream_t s, const uint32_t *p, uint32_t v, uint32_t mask);  // false: cannot ever hold (immediate mode)
 void synchronize();
+hipError_t take_error();  // the last launch error, forgotten by the call
 }  // namespace simt
-static inline hipError_t hipGetLastError() { return hipSuccess; }
+static inline hipError_t hipGetLastError() { return simt::take_error(); }
 static inline hipError_t hipDeviceSynchronize() { simt::synchronize(); return hipSuccess; }
 static inline hipError_t hipStreamSynchronize(hipStream_t) { simt::synchronize(); return hipSuccess; }
 static inline hipError_t hipMemsetAsync(void *p, int v, size_t n, hipStream_t s) {
@@ -116,6 +117,9 @@ void wg_barrier();
 int wg_barrier_or(int v);
 int wg_barrier_count(int v);
 void launch(dim3 grid, dim3 block, size_t dynamic_lds_bytes, const std::function<void()> &body);
+// Whether a launch of this shape is to run.  As on the device, one of 2^32 threads or more in a dimension is an error; with
+// simt_dry_run(1) (runtime.cpp) launches are noted, not run: what an entry point launches for sizes no emulation gets through.
+bool accept(dim3 grid, dim3 block);
 void *dynamic_lds();  // the workgroup's dynamically sized LDS (extern __shared__)
 }  // namespace simt
 
@@ -128,6 +132,7 @@ void *dynamic_lds();  // the workgroup's dynamically sized LDS (extern __shared_
   do {                                                                                        \
     const dim3 simt_grid_ = (grid), simt_block_ = (block);                                    \
     const size_t simt_lds_ = (size_t)(shmem);                                                 \
+    if (!simt::accept(simt_grid_, simt_block_)) break;                                        \
     simt::submit((stream), [=]() { simt::launch(simt_grid_, simt_block_, simt_lds_, [&]() { kernel(__VA_ARGS__); }); }); \
   } while (0)
 #define HIP_DYNAMIC_SHARED(type, var) type *var = reinterpret_cast<type *>(simt::dynamic_lds());
