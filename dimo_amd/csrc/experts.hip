@@ -381,6 +381,12 @@ constexpr int GROUP_ROUNDS = GROUP_CHUNK / GROUP_THREADS;
 // Up to twice that many places are one workgroup's, with twice the rounds and no counts to exchange: one launch instead of two
 // (8192 places, 8 experts: 11.3 us instead of 2.8 + 7.6, and 4 us less of the host's).
 constexpr int GROUP_ALONE = 2 * GROUP_CHUNK;
+// Few workgroups sum the counts of all of them each for itself; that work grows with the square of the places, so from some
+// number of them on a launch of its own does it once.  In-kernel sums / scan, us for all launches (workgroups, experts):
+//   8, 8     10.7 / 12.7      256, 8    13.5 / 15.6     1024, 8    49 / 39
+//   8, 128   12.7 / 14.7      128, 128  17.0 / 18.2     256, 128   22.9 / 23.0     1024, 128  117 / 60
+//   8, 1000  14.4 / 16.4      32, 1000  16.8 / 17.5      64, 1000  20.1 / 19.0      256, 1000  48 / 36
+inline bool group_scanned(int64_t blocks, int E) { return blocks > 256 || blocks * (E + 1) > 40000; }
 
 __device__ __forceinline__ int group_key(const int32_t *experts, int64_t S, int64_t at, int E) {
   if (at >= S) return -1;
@@ -402,10 +408,34 @@ __global__ __launch_bounds__(GROUP_THREADS) void group_count_kernel(int64_t S, i
   for (int e = threadIdx.x; e <= E; e += GROUP_THREADS) counts[(size_t)blockIdx.x * (E + 1) + e] = hist[e];
 }
 
+// Many workgroups: their counts become what lies before each (in place), and behind them the totals, once for all of them.
+// Sixteen experts per workgroup, 64 threads each over a contiguous share of the workgroups.
+__global__ __launch_bounds__(GROUP_THREADS) void group_scan_kernel(int E1, int blocks, int32_t *__restrict__ counts) {
+  __shared__ int sums[64][17];
+  const int col = threadIdx.x & 15, part = threadIdx.x >> 4, e = blockIdx.x * 16 + col;
+  const int share = (blocks + 63) / 64, begin = min(part * share, blocks), end = min(begin + share, blocks);
+  int sum = 0;
+  if (e < E1)
+#pragma unroll 8
+    for (int b = begin; b < end; ++b) sum += counts[(size_t)b * E1 + e];
+  sums[part][col] = sum;
+  __syncthreads();
+  int before = 0;
+  for (int p = 0; p < part; ++p) before += sums[p][col];
+  if (e >= E1) return;
+#pragma unroll 8
+  for (int b = begin; b < end; ++b) {
+    const int n = counts[(size_t)b * E1 + e];
+    counts[(size_t)b * E1 + e] = before;
+    before += n;
+  }
+  if (part == 63) counts[(size_t)blocks * E1 + e] = before;
+}
+
 template <int ROUNDS>
 __global__ __launch_bounds__(GROUP_THREADS) void group_place_kernel(int64_t S, int E, int bits,
                                                                     const int32_t *__restrict__ experts,
-                                                                    const int32_t *__restrict__ counts, int blocks,
+                                                                    const int32_t *__restrict__ counts, int blocks, int scanned,
                                                                     int32_t *__restrict__ offsets,
                                                                     int32_t *__restrict__ order,
                                                                     int32_t *__restrict__ position, int places,
@@ -423,7 +453,11 @@ __global__ __launch_bounds__(GROUP_THREADS) void group_place_kernel(int64_t S, i
     if (key[r] >= 0) atomicAdd(&base[wave * E1 + key[r]], 1);
   }
   __syncthreads();
-  if (counts) {
+  if (scanned) {
+    for (int e = t; e < E1; e += GROUP_THREADS)
+      tallies[e] = counts[(size_t)blockIdx.x * E1 + e], tallies[E1 + e] = counts[(size_t)blocks * E1 + e];
+    __syncthreads();
+  } else if (counts) {
     // the workgroups' counts: `parts` threads per expert, eight loads in flight each
     for (int i = t; i < 2 * E1; i += GROUP_THREADS) tallies[i] = 0;
     __syncthreads();
@@ -664,7 +698,8 @@ extern "C" int dimo_route_topk_backward(int T, int E, int k, int dtype, const vo
 
 extern "C" size_t dimo_group_rows_workspace_bytes(int64_t S, int E) {
   if (S <= GROUP_ALONE || E <= 0) return 0;
-  return align_up((size_t)((S + GROUP_CHUNK - 1) / GROUP_CHUNK) * (E + 1) * sizeof(int32_t));
+  const int64_t blocks = (S + GROUP_CHUNK - 1) / GROUP_CHUNK;
+  return align_up((size_t)(blocks + group_scanned(blocks, E)) * (E + 1) * sizeof(int32_t));
 }
 
 extern "C" int dimo_group_rows(int64_t S, int E, int places, const int32_t *experts, int32_t *offsets, int32_t *order,
@@ -679,8 +714,11 @@ extern "C" int dimo_group_rows(int64_t S, int E, int places, const int32_t *expe
   while ((1 << bits) <= E) ++bits;
   const int blocks = S > GROUP_ALONE ? (int)((S + GROUP_CHUNK - 1) / GROUP_CHUNK) : 1;
   int32_t *counts = blocks > 1 ? static_cast<int32_t *>(workspace) : nullptr;
+  const int scanned = group_scanned(blocks, E);
   if (counts)
     hipLaunchKernelGGL(group_count_kernel, dim3(blocks), dim3(GROUP_THREADS), 0, s, S, E, experts, counts);
+  if (scanned)
+    hipLaunchKernelGGL(group_scan_kernel, dim3((E + 16) / 16), dim3(GROUP_THREADS), 0, s, E + 1, blocks, counts);
   const size_t lds = (size_t)GROUP_WAVES * (E + 1) * sizeof(int);
   auto place = S > GROUP_CHUNK && S <= GROUP_ALONE ? group_place_kernel<2 * GROUP_ROUNDS> : group_place_kernel<GROUP_ROUNDS>;
   if (lds > 32768) {  // (1024 experts: 65 600 bytes and 8 KB of tallies; a workgroup has 160 KB)
@@ -688,8 +726,8 @@ extern "C" int dimo_group_rows(int64_t S, int E, int places, const int32_t *expe
         hipSuccess)
       return check_launch();
   }
-  hipLaunchKernelGGL(place, dim3(blocks), dim3(GROUP_THREADS), lds, s, S, E, bits, experts, counts, blocks, offsets, order,
-                     position, places, rows);
+  hipLaunchKernelGGL(place, dim3(blocks), dim3(GROUP_THREADS), lds, s, S, E, bits, experts, counts, blocks, scanned, offsets,
+                     order, position, places, rows);
   return check_launch();
 }
 

@@ -69,6 +69,11 @@ def test_4bit_products(launched, R, K, N):
     _whole(launched("dimo_mx4_linear", 1, R, 2, K, N, P, P, P, P, P, None, 0, P, None), 64 * (R * N // 65536))
 
 
-def test_grouping(launched):
-    rc, threads = launched("dimo_group_rows", MOST, 1024, 2, P, P, P, P, P, P, 1 << 60, None)
-    assert rc == 0 and max(threads) < 1 << 32
+@pytest.mark.parametrize("S,E,launches", [(8192, 1024, 1), (8193, 1024, 2), (256 * 4096, 128, 2), (257 * 4096, 2, 3), (41 * 4096, 1000, 3),
+                                          (MOST, 1024, 3)])
+def test_grouping(launched, S, E, launches):
+    """One launch, two, or (where every workgroup summing all workgroups' counts would be quadratic in the places) three."""
+    need = expert_emulation.emulated_library().dimo_group_rows_workspace_bytes(S, E)
+    rc, threads = launched("dimo_group_rows", S, E, 2, P, P, P, P, P, P, need, None)
+    assert rc == 0 and max(threads) < 1 << 32 and len(threads) == launches
+    assert need >= (0 if launches == 1 else (-(-S // 4096) + launches - 2) * (E + 1) * 4)

@@ -55,3 +55,27 @@ def test_products(ex):
     g = _random(R, 1)
     gx, = torch.autograd.grad(y, x, g)
     assert torch.equal(gx, g * w[0, 0, 0])
+
+
+def test_grouping_grows_with_its_places(ex):
+    """2^26 places: sorted as a stable sort does, in no more than twice the eightfold time of 2^23 (sums of all workgroups'
+    counts by every workgroup would take 64 times as long)."""
+    E, times = 128, []
+    for S in (1 << 23, 1 << 26):
+        experts = torch.randint(0, E, (S, 1), device="cuda", generator=torch.Generator(device="cuda").manual_seed(S), dtype=torch.int32)
+        groups = ex.group_rows(experts, E)
+        took = []
+        for _ in range(3):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            groups = ex.group_rows(experts, E)
+            b.record()
+            b.synchronize()
+            took.append(a.elapsed_time(b))
+        times.append(min(took))
+        key, order = torch.sort(experts[:, 0], stable=True)
+        assert torch.equal(groups.order, order.to(torch.int32)) and torch.equal(groups.rows, groups.order)
+        assert torch.equal(groups.offsets, torch.searchsorted(key, torch.arange(E + 1, device="cuda", dtype=torch.int32)).to(torch.int32))
+        assert torch.equal(groups.position[:, 0][order], torch.arange(S, device="cuda", dtype=torch.int32))
+    print(times)
+    assert times[1] <= 16 * times[0], times
