@@ -101,7 +101,10 @@ __global__ __launch_bounds__(C::THREADS, 2) void grouped_rows_kernel(GroupedArgs
     write_outputs<T, C, (int)sizeof(SJ0)>(acc, SJ0, c0, columns, a.wide, out_row(out), add_bias, NoSlope{});
   } else {
     const int64_t away = static_cast<const E *>(a.saved) - out;  // (both [R, K])
-    write_outputs<T, C, (int)sizeof(SJ0)>(acc, SJ0, c0, columns, a.wide, out_row(out), add_bias, Slope{a.act, away});
+    if (a.act == DIMO_ACT_RELU)
+      write_outputs<T, C, (int)sizeof(SJ0)>(acc, SJ0, c0, columns, a.wide, out_row(out), add_bias, ReluSlope{away});
+    else
+      write_outputs<T, C, (int)sizeof(SJ0)>(acc, SJ0, c0, columns, a.wide, out_row(out), add_bias, SiluSlope{away});
   }
 }
 
