@@ -453,6 +453,10 @@ int run_rows(int dtype, GroupedArgs a, bool whole, hipStream_t s) {
 //    5003, 13, 257 x 360   uneven 62 / 28, fp16 35 / 21        5008, 13, 256 x 360   uneven 41 / 28, even 23 / 26
 //    4096, 16, 256 x 256   uneven 43 / 21                      2048, 16, 512 x 256   uneven 27 / 20, even 12 / 15
 //    8192, 32, 256 x 256   uneven 45 / 27, fp16 in whole chunks 14 / 17
+// 16-bit rows that are no whole chunks, of sizes for which this asks 256 tiles, run 128 tiles in the slices of that plan, which
+// cuts them finer than a plan for 128 tiles does (256's / 128's slices, even; uneven; us):
+//    32768, 8, 1020 x 1020    265 / 271; 274 / 494         65536, 1, 2044 x 257    324 / 698
+//    32768, 32, 1020 x 516    150 / 150; 190 / 192         32768, 16, 1021 x 2043  409 / 412; 917 / 492 (whole / cut at 2)
 struct WgradPlan {
   int tile, split_rows, chunks;
   size_t bytes;
