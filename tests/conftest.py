@@ -20,15 +20,17 @@ def _build_oracle():
 
 # torch's conv2d backward -- the test's reference formula, no kernel of this package was in flight -- ended with a GPU memory
 # fault on this shape in a process that had run the expert operators' tests before it; the cause is not shown.  The shape is
-# tested against a reference on the host instead (test_gpu_ssim_host_reference.py).
-FAULTED = {"tests/test_gpu_ops.py::test_ssim_against_torch_conv[shape2]":
+# tested against a reference on the host instead (test_gpu_ssim_host_reference.py).  By file and test: the node id depends on the
+# directory the run starts in.
+FAULTED = {("test_gpu_ops.py", "test_ssim_against_torch_conv[shape2]"):
            "the reference's conv2d backward has faulted the GPU here; cause not shown"}
-# (their allocations of many gigabytes come behind everything else)
-LAST = ("test_gpu_experts.py", "test_gpu_mx4.py")
+# (their allocations of many gigabytes come behind everything else; an order that keeps apart what has failed together, no cure)
+LAST = ("test_gpu_experts", "test_gpu_mx4")
 
 
 def pytest_collection_modifyitems(items):
     for item in items:
-        if item.nodeid in FAULTED:
-            item.add_marker(pytest.mark.skip(reason=FAULTED[item.nodeid]))
-    items.sort(key=lambda item: item.path.name in LAST)
+        reason = FAULTED.get((item.path.name, item.name))
+        if reason:
+            item.add_marker(pytest.mark.skip(reason=reason))
+    items.sort(key=lambda item: item.path.name.startswith(LAST))
