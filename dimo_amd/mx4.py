@@ -6,8 +6,9 @@ that are only evaluated (render-only use, ExpertMLP.quantized()).
     y = mx4_linear(x4, w4, bias)             # [R, K] x [N, K] -> [R, N]; or grouped: w4 [E, N, K], groups=RowGroups
 
 Products of the quantised values are exact and summed in fp32, so what an `mx4_linear` loses against the product of its
-inputs is what `quantize_mx4` rounded: up to half a step of e2m1, 2^-2 relative at the coarsest (between 4 and 6), of
-every element.  No gradients.  GPU only."""
+inputs is what `quantize_mx4` rounded.  That is bounded against the block's scale s, not against the element: s / 4 up to 2 s,
+s / 2 up to 4 s, s up to 6 s, and |x| - 6 s (below 2 s) beyond, where elements saturate -- at most a quarter of the block's
+largest magnitude, and all of an element below s / 4.  No gradients.  GPU only."""
 import torch
 
 from . import _lib

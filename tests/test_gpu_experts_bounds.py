@@ -1,0 +1,14 @@
+"""Bounds that the documentation of the expert operators states, on the GPU."""
+import pytest
+import torch
+
+from dimo_amd import experts as ex
+from dimo_amd import mx4
+from tests import expert_bounds_cases as cases
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_4bit_error(dtype):
+    cases.check_4bit_error(mx4, "cuda", dtype)
