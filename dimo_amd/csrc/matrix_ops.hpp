@@ -51,8 +51,10 @@ __device__ __forceinline__ f32x16 mfma_mx4_32x32x64(uint4 a, uint32_t scale_a, u
 
 // fp32 = three bf16 pieces: the top eight significant bits (cut, so that no finite value becomes infinite), what is left
 // rounded to eight bits, and the rest, which eight bits hold exactly -- 24 bits in all.  Of the nine products of two
-// such sums the three smallest (below 2^-21 of the product, of random sign) are left out: the error of one product is
-// then of the size of one fp32 rounding, at 6 / 16 of an fp32 matrix instruction's issue time.
+// such sums the three smallest are left out (two of up to 2^-7 2^-16 of the product and one far below: 2^-22 in all, of random
+// sign), at 6 / 16 of an fp32 matrix instruction's issue time.  With the roundings of the sums a single product is off by up
+// to 6.1 x 2^-24 of it (measured: 4.9 at most, 0.44 in the middle), where an fp32 multiplication is off by 1.  From 2^-110
+// down the lowest piece leaves bf16's range (2^-133), and an operand is off by up to 2^-134.
 // An infinite value leaves NaN (inf - inf) and so shows up as NaN in its row of outputs.
 struct Split3 {
   uint16_t hi, mid, lo;

@@ -11,7 +11,9 @@ the experts' rows back together (dimo_amd/csrc/experts.hip, grouped.hip; include
 reference, whose deformation network (renderer/latent_gs_renderer.py:184-245) is one dense MLP for all motions: an
 expert block gives that network capacity of which every row uses k parts (`deform.TimeNet(experts=...)`).
 
-Types: fp32, bf16, fp16 (all tensors of a call alike; routing weights, load and their gradients are fp32).  The sizes of
+Types: fp32, bf16, fp16 (all tensors of a call alike; routing weights, load and their gradients are fp32).  Sums are fp32.
+fp32 products are made of bf16 ones: each is off by up to 6.1 x 2^-24 of its size (an fp32 multiplication: 1 x 2^-24) where its
+operands are 2^-110 or larger, by up to 2^-134 of the other operand where one is smaller; an infinite operand gives NaN.  The sizes of
 the groups stay on the device: no call synchronises, every call may be captured into a graph.  All calls run on the
 current stream of the tensors' device.  GPU only.
 """
