@@ -15,7 +15,7 @@ using namespace dimo;
 namespace {
 
 struct BlockLayout {
-  size_t weights, experts, offsets, order, position, rows, h, z, y, bytes;
+  size_t weights, experts, offsets, position, rows, h, z, y, bytes;
   int64_t S;
   __host__ BlockLayout(const dimo_expert_mlp_desc &d, bool keep) {
     S = (int64_t)d.T * d.k;
@@ -24,7 +24,6 @@ struct BlockLayout {
     weights = o, o = align_up(o + s * sizeof(float));
     experts = o, o = align_up(o + s * sizeof(int32_t));
     offsets = o, o = align_up(o + ((size_t)d.E + 1) * sizeof(int32_t));
-    order = o, o = align_up(o + s * sizeof(int32_t));
     position = o, o = align_up(o + s * sizeof(int32_t));
     rows = o, o = align_up(o + s * sizeof(int32_t));
     // h also holds the grouping's counts before it is written
@@ -79,7 +78,7 @@ extern "C" int dimo_expert_mlp_forward(const dimo_expert_mlp_desc *d, int keep, 
   int rc = dimo_route_topk_forward(d->T, d->E, d->k, d->dtype, d->logits, d->ld_logits, d->row_mask, d->normalize, weights,
                                    experts, nullptr, nullptr, 0, stream);
   if (!rc)
-    rc = dimo_group_rows(L.S, d->E, d->k, experts, offsets, at<int32_t>(workspace, L.order), position, rows, h,
+    rc = dimo_group_rows(L.S, d->E, d->k, experts, offsets, nullptr, position, rows, h,
                          dimo_group_rows_workspace_bytes(L.S, d->E), stream);
   if (!rc)
     rc = dimo_grouped_linear_forward(d->dtype, R, d->E, d->K, d->F, d->x, d->ld_x, rows, offsets, d->w1, d->b1, d->act, h, z,

@@ -534,7 +534,7 @@ __global__ __launch_bounds__(GROUP_THREADS) void group_place_kernel(int64_t S, i
     if (key[r] >= 0) {
       const int at = start + __popcll(peers & ((1ull << lane) - 1ull));
       const bool has = key[r] < E;
-      order[at] = has ? (int32_t)place : -1;
+      if (order) order[at] = has ? (int32_t)place : -1;
       if (rows) rows[at] = has ? (int32_t)place / places : -1;
       position[place] = has ? at : -1;
     }
@@ -705,7 +705,7 @@ extern "C" size_t dimo_group_rows_workspace_bytes(int64_t S, int E) {
 extern "C" int dimo_group_rows(int64_t S, int E, int places, const int32_t *experts, int32_t *offsets, int32_t *order,
                                int32_t *position, int32_t *rows, void *workspace, size_t workspace_bytes, void *stream) {
   if (S < 0 || S > DIMO_MAX_SIZE || E < 1 || E > ROUTE_MAX_E || places < 1 || !offsets) return DIMO_E_ARG;
-  if (S > 0 && (!experts || !order || !position)) return DIMO_E_ARG;
+  if (S > 0 && (!experts || !position)) return DIMO_E_ARG;
   if (workspace_bytes < dimo_group_rows_workspace_bytes(S, E) || (S > GROUP_ALONE && !workspace)) return DIMO_E_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
   clear_errors();

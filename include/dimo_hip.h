@@ -466,7 +466,7 @@ int dimo_route_topk_forward(int T, int E, int k, int dtype, const void *logits, 
 int dimo_route_topk_backward(int T, int E, int k, int dtype, const void *logits, int64_t ld, const uint8_t *row_mask,
                              int normalize, const float *weights, const int32_t *experts, const float *g_weights,
                              const float *g_load, void *g_logits, void *stream);
-/* Stable grouping of S places by expert: offsets [E + 1], order [S] (the places, group after group; -1 behind the last
+/* Stable grouping of S places by expert: offsets [E + 1], order [S] or NULL (the places, group after group; -1 behind the last
  * group), position [S] (its inverse; -1 for a place whose expert is outside 0 .. E-1), rows [S] or NULL: order / places. */
 size_t dimo_group_rows_workspace_bytes(int64_t S, int E);
 int dimo_group_rows(int64_t S, int E, int places, const int32_t *experts, int32_t *offsets, int32_t *order,

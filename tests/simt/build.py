@@ -156,7 +156,6 @@ SUBST["numeric.hpp"] = [  # gcc 11 has neither 16-bit floating type on x86-64, n
     ("__builtin_bit_cast(uint32_t, v[i % N])", "__float_as_uint(v[i % N])"),
 ]
 SUBST["matrix_ops.hpp"] = [
-    ("typedef float f32x4 __attribute__((ext_vector_type(4)));", "typedef float f32x4 __attribute__((vector_size(16)));"),
     ("typedef float f32x16 __attribute__((ext_vector_type(16)));", "typedef float f32x16 __attribute__((vector_size(64)));"),
     ("typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));", ""),
     ("typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));", ""),
