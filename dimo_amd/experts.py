@@ -529,8 +529,8 @@ class ExpertMLP(nn.Module):
 
 
 class QuantizedExpertMLP(nn.Module):
-    """An ExpertMLP's weights of this moment in 4-bit form, for evaluation: no parameters, no gradients; the router stays
-    as it is."""
+    """An ExpertMLP's weights of this moment in 4-bit form, for evaluation: no parameters, no gradients (a call that would have
+    to give any is refused: use torch.no_grad()); the router stays as it is."""
 
     def __init__(self, block):
         super().__init__()
@@ -542,9 +542,10 @@ class QuantizedExpertMLP(nn.Module):
                         ("w2_codes", q2.codes), ("w2_scales", q2.scales)):
             self.register_buffer(name, t)
 
-    @torch.no_grad()
     def forward(self, h):
         from .mx4 import MX4, mx4_linear, quantize_mx4
+        if torch.is_grad_enabled() and h.requires_grad:
+            raise RuntimeError("a quantized expert block has no gradients: evaluate it under torch.no_grad()")
         out = _without_autocast(self, h, self.router.dtype)
         if out is not None:
             return out

@@ -82,3 +82,16 @@ def test_a_grouping_that_was_replaced_keeps_the_gradient(emulated):
     want = torch.autograd.grad(y.sum(), w1, retain_graph=True)[0]
     groups.offsets = torch.tensor([0, 0, 8, 8], dtype=torch.int32)
     assert torch.equal(torch.autograd.grad(y.sum(), w1)[0], want)
+
+
+def test_a_quantized_block_is_not_trained_through(emulated):
+    """What lies before a quantized block would get no gradient, silently."""
+    torch.manual_seed(0)
+    block = ex.ExpertMLP(16, 3, 2)
+    q, h = block.quantized(), torch.randn(5, 16)
+    want = q(h)
+    assert not want.requires_grad
+    with pytest.raises(RuntimeError, match="no_grad"):
+        q(h.clone().requires_grad_(True))
+    with torch.no_grad():
+        assert torch.equal(q(h.clone().requires_grad_(True)), want)
