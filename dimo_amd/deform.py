@@ -70,6 +70,12 @@ class TimeNet(nn.Module):
         if device is not None:
             self.to(device)
 
+    def quantize_experts(self):
+        """For evaluation only: the expert block's products in microscaled 4-bit form from here on (dimo_amd/mx4.py)."""
+        if not hasattr(self.experts, "quantized"):
+            raise ValueError("a network with an expert block that is not quantized yet expected")
+        self.experts = self.experts.quantized()
+
     def forward(self, pts, t, latent_code, nobatch=False, t_apply=False):
         if pts.dim() == 2:
             nobatch = True

@@ -197,6 +197,11 @@ class GaussianModel(DensifyMixin, PlyMixin):
             self._c_radius = nn.Parameter(scales[: cpts.shape[0], :1].clone().requires_grad_(True))
             self._r = nn.Parameter((scales.mean() * torch.ones((1, 1), device=dev)).requires_grad_(True))
 
+    def quantize_experts(self):
+        """For render-only use of a trained or loaded model with experts: their products in microscaled 4-bit form from here
+        on.  The model renders under torch.no_grad() and is not trained any more."""
+        self._timenet.quantize_experts()
+
     # ------------------------------------------------------------------ optimizer
     def param_groups(self, a):
         """The reference's Adam groups, in order (latent_gs_renderer.py:460-473; VAE: gaussian_gs_renderer.py:478-479)."""

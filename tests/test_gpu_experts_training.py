@@ -32,3 +32,33 @@ def test_two_stages_with_experts():
     for a, b in zip(seen, seen[1:]):
         for n in a:
             assert not torch.equal(a[n], b[n]), n
+
+
+def test_renders_through_quantized_experts():
+    """Render-only use: a model with experts, quantized, through Renderer.render -- the image is the one of its quantized
+    network's deformation, handed to render as it is."""
+    from dimo_amd.experts import QuantizedExpertMLP
+    from dimo_amd.renderer import Renderer
+    from dimo_amd.synth import init_synthetic_model
+    from dimo_amd.trainer import TrainConfig, Trainer
+    cfg = TrainConfig(num_pts=2000, num_cpts=64, num_motions=2, resolution=96, motions_per_step=1, views_per_step=1, frames_per_step=1)
+    rd = Renderer(sh_degree=0, num_latent_code=2, add_normal=True, device="cuda", timenet_experts=4, timenet_top_k=2)
+    init_synthetic_model(rd, cfg.num_pts, cfg.num_cpts, seed=0, num_latent=2)
+    g = rd.gaussians
+    tr = Trainer(cfg, rd, direct=False)
+    tr.find_knn(k=4)
+    with torch.no_grad():
+        g._timenet.experts.w2.copy_(torch.randn(g._timenet.experts.w2.shape, device="cuda",
+                                                generator=torch.Generator(device="cuda").manual_seed(0)) / 16)
+    cam = tr.cams.get(0.0, 40.0, cfg.radius, 96, 96)
+    with torch.no_grad():
+        full = rd.render(cam, time=0.5, stage="s2", latent_index=1)["image"] + 0
+        g.quantize_experts()
+        assert isinstance(g._timenet.experts, QuantizedExpertMLP)
+        dx, dq = g._timenet(g._c_xyz, 0.5, g.latent_code(1))
+        image = rd.render(cam, time=0.5, stage="s2", latent_index=1)["image"] + 0
+        want = rd.render(cam, time=0.5, stage="s2", latent_index=1, deform=(dx, dq))["image"] + 0
+    assert torch.isfinite(image).all() and float((image - want).abs().max()) <= 1e-5  # (as batched and immediate renders agree)
+    assert float((image - full).abs().max()) > 1e-5  # (the block's products count, in the one form as in the other)
+    with pytest.raises(RuntimeError, match="no_grad"):
+        rd.render(cam, time=0.5, stage="s2", latent_index=1)
