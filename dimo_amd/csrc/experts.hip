@@ -378,8 +378,10 @@ void with_route_shape(int E, F &&f) {
 // (any value outside 0 .. E-1) is sorted behind the last group and gets order = -1 there, position = -1.
 constexpr int GROUP_THREADS = 1024, GROUP_WAVES = GROUP_THREADS / 64, GROUP_CHUNK = 4096;
 constexpr int GROUP_ROUNDS = GROUP_CHUNK / GROUP_THREADS;
-// Up to twice that many places are one workgroup's, with twice the rounds and no counts to exchange: one launch instead of two
-// (8192 places, 8 experts: 11.3 us instead of 2.8 + 7.6, and 4 us less of the host's).
+// Up to twice that many places are one workgroup's, with twice the rounds and no counts to exchange: one launch instead of two.
+// One / two launches (places, experts; us on the GPU, and a call from Python one after another):
+//   4098, 8    8.9, 12.8 / 10.0, 16.6      6000, 8    9.6, 13.0 / 10.2, 17.1      8192, 8     10.9, 13.0 / 10.5, 17.0
+//   4098, 128  11.1, 12.9 / 11.2, 17.2     8192, 128  13.1, 13.1 / 11.8, 17.2     8192, 1000  15.3, 14.7 / 13.6, 17.2
 constexpr int GROUP_ALONE = 2 * GROUP_CHUNK;
 // Few workgroups sum the counts of all of them each for itself; that work grows with the square of the places, so from some
 // number of them on a launch of its own does it once.  In-kernel sums / scan, us for all launches (workgroups, experts):

@@ -213,8 +213,8 @@ __global__ __launch_bounds__(C::THREADS, 2) void mx4_rows_kernel(Mx4Args a) {
   Staging<BF16, LINES, C::TI, BK, C::THREADS> si;
   sj.init_lines([&](int i) { return reinterpret_cast<const uint16_t *>(a.xc) + x_line(i) * end; });
   si.init_lines([&](int i) { return reinterpret_cast<const uint16_t *>(a.wc) + w_line(i) * end; });
-  // a thread brings one line's scales, two stages of them at a time, into LDS (each wave reading those of its lines from
-  // memory took three times the requests of the codes themselves)
+  // a thread brings one line's scales, two stages of them at a time, into LDS (as many requests as the codes themselves, since
+  // a request brings 16 bytes of a line; each wave reading those of its lines from memory took three times as many)
   const int mine = threadIdx.x % (C::TJ + C::TI);
   const uint8_t *line = mine < C::TJ ? a.xs + x_line(mine) * a.blocks : a.ws + w_line(mine - C::TJ) * a.blocks;
   const auto fetch = [&](int b0) {
