@@ -452,8 +452,8 @@ class _ExpertMlp(torch.autograd.Function):
 
 def expert_mlp(x, logits, w1, b1, w2, b2, k, activation="relu", row_mask=None, normalize=True):
     """x + sum over a row's k experts of weight * (w2 activation(w1 x + b1) + b2): routing (weights normalised over the
-    chosen; normalize=False: softmax over all E), both products and the sum as one call per direction -- what route_topk, group_rows, grouped_linear (gathering,
-    then plain) and combine_rows give one by one.  x [T, K], logits [T, E], w1 [E, F, K], b1 [E, F] or None, w2 [E, K, F],
+    chosen; normalize=False: softmax over all E), both products and the sum as one call per direction -- what route_topk,
+    group_rows, grouped_linear (gathering, then plain) and combine_rows give one by one.  x [T, K], logits [T, E], w1 [E, F, K], b1 [E, F] or None, w2 [E, K, F],
     b2 [E, K] or None; row_mask [T]: rows with False come back as they are.  Differentiable in x, logits and the weights.
     With k = 1 a normalised weight is the constant 1, and the logits' gradient zero."""
     if x.dim() != 2 or logits.dim() != 2 or w1.dim() != 3:
@@ -494,7 +494,8 @@ class ExpertMLP(nn.Module):
     """h + the weighted sum of a row's k experts (each width -> hidden -> width), h [..., width].  The weights
     are normalised over the chosen; with k = 1, where that would be the constant 1 and the router would not learn, they are
     the softmax over all experts.  The second products start at zero, so a network that gets such a block starts as it was.
-    Under autocast the block works (and answers) in its parameters' type.  `quantized()`: the same block for evaluation
+    Under autocast the block works (and answers) in its parameters' type.  Nothing here keeps the experts' load even: a balancing
+    term takes `load` of route_topk(block.router(rows), k), differentiable in the router.  `quantized()`: the same block for evaluation
     only, its products in microscaled 4-bit form (dimo_amd/mx4.py)."""
 
     def __init__(self, width, num_experts, k=2, hidden=None, activation="relu", device=None):

@@ -62,3 +62,36 @@ def test_renders_through_quantized_experts():
     assert float((image - full).abs().max()) > 1e-5  # (the block's products count, in the one form as in the other)
     with pytest.raises(RuntimeError, match="no_grad"):
         rd.render(cam, time=0.5, stage="s2", latent_index=1)
+
+
+def test_direct_pipeline_equals_autograd_pipeline_with_experts():
+    """Stage s2: the direct pipeline around the module's autograd gives the loss and the gradients -- the block's and the
+    router's among them -- of the reference-shaped autograd path."""
+    from dimo_amd.rasterizer import CapacityPolicy
+    from dimo_amd.renderer import Renderer
+    from dimo_amd.synth import init_synthetic_model
+    from dimo_amd.trainer import TrainConfig, Trainer
+    cfg = TrainConfig(num_pts=3000, num_cpts=48, num_motions=3, num_frames=5, num_views=4, motions_per_step=2, views_per_step=2,
+                      frames_per_step=2, resolution=128)
+    res = []
+    for direct in (False, True):
+        rd = Renderer(sh_degree=0, num_latent_code=cfg.num_motions, add_normal=True, device="cuda",
+                      capacity=CapacityPolicy(initial=1 << 19) if direct else None, timenet_experts=4, timenet_top_k=2)
+        init_synthetic_model(rd, cfg.num_pts, cfg.num_cpts, seed=0, num_latent=cfg.num_motions)
+        g = rd.gaussians
+        with torch.no_grad():
+            g._timenet.experts.w2.copy_(torch.randn(g._timenet.experts.w2.shape, device="cuda",
+                                                    generator=torch.Generator(device="cuda").manual_seed(0)) / 16)
+        tr = Trainer(cfg, rd, direct=direct)
+        assert tr.direct == direct
+        tr.optimizer.step = lambda *a, **k: None
+        g.zero_grad = lambda: None
+        tr.step = 298
+        tr.train_step(tr.sample())
+        torch.cuda.synchronize()
+        res.append((tr.last_loss.item(), g.flat_grads.clone(), {n: p.grad.clone() for n, p in g._timenet.experts.named_parameters()}))
+    (la, ga, ba), (lb, gb, bb) = res
+    assert abs(la - lb) <= 1e-5 * abs(la), (la, lb)
+    assert (ga - gb).abs().sum() / ga.abs().sum() < 1e-4
+    for n in ba:
+        assert float(ba[n].abs().sum()) > 0 and (ba[n] - bb[n]).abs().sum() / ba[n].abs().sum() < 1e-3, n
