@@ -79,3 +79,22 @@ def test_grouping_grows_with_its_places(ex):
         assert torch.equal(groups.position[:, 0][order], torch.arange(S, device="cuda", dtype=torch.int32))
     print(times)
     assert times[1] <= 16 * times[0], times
+
+
+def test_captured_grouping_of_many_places(ex):
+    """The three launches of a large grouping, captured once and replayed on other places: what the eager call gives."""
+    E, S = 128, 300 * 4096 - 7
+    experts = torch.zeros(S, 1, dtype=torch.int32, device="cuda")
+    draw = lambda seed: torch.randint(-1, E, (S, 1), device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed), dtype=torch.int32)
+    ex.group_rows(experts, E)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        groups = ex.group_rows(experts, E)
+    for seed in range(4):
+        experts.copy_(draw(seed))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = ex.group_rows(experts, E)
+        for name in ("offsets", "order", "position", "rows"):
+            assert torch.equal(getattr(groups, name), getattr(want, name)), (seed, name)
